@@ -7,7 +7,7 @@
  * drive them.  Plain C: host or device pointers, sizes, status codes; no C++
  * or framework types cross this boundary.
  *
- * Three layers, each citing the reference interface it replaces:
+ * Four layers, the first three citing the reference interface it replaces:
  *   1. runtime            iris_metal_init / iris_metal_available / iris_gpu_sync
  *                         (iris_metal.h:23-33, :309)
  *   2. model + sampler    iris_transformer_* (iris_transformer_flux.c:3939, :4579,
@@ -17,6 +17,8 @@
  *   3. tensor/op surface  the iris_gpu_* device-resident API of iris_metal.h
  *                         (:155-600), same names and signatures, so the
  *                         reference's bf16 block code can link against it.
+ *   4. language model     rotary positions into a paged key-value cache,
+ *                         attention over it, token log probabilities
  *
  * Conventions (same as the reference): latents are NCHW f32 [C, h, w] with
  * h, w in patches (image pixels / 16 for Flux); text embeddings are f32
@@ -664,6 +666,123 @@ void iris_metal_warmup_bf16_buffers_parallel(const uint16_t **ptrs, const size_t
  * that falls back to its CPU path when an op fails (as the reference does)
  * can check that the GPU path really ran. */
 unsigned long iris_gpu_op_failures(void);
+
+/* ------------------------------------------------------------------ 4. language-model operators
+ * What running the resident text model a token at a time needs beside the
+ * dense ops above: rotary positions written into a paged key-value cache,
+ * attention that reads the cache, and the answer side of a logits matrix.  No
+ * counterpart in the reference, whose text model only encodes prompts.
+ *
+ * Manner of iris_gpu_adaln_norm_bf16_noalloc: raw device pointers the caller
+ * owns and a cudaStream_t (void *, 0 = default stream); work is queued
+ * without synchronising, nothing is allocated, so the calls may be captured
+ * into a graph.  Pointers must be device memory of the library's device
+ * (iris_cuda_init).  Arguments are checked before anything is queued:
+ * IRIS_CUDA_ERR_ARG with the reason in iris_cuda_last_error(), counted by
+ * iris_gpu_op_failures().  Values in device memory (positions, sequence and
+ * page numbers, targets) can not be checked then; the kernels bound them and
+ * never read or write outside the tensors they are given.  A workspace is
+ * scratch of one call: calls that may overlap on the GPU (two streams, two
+ * graphs) need one each; its contents need not be set or kept. */
+
+/* A paged cache: keys and values of sequence s at position p lie in page
+ * table[s][p / page_size], slot p % page_size, of two pools laid out alike.
+ * Any order of slots and heads within a page: the strides say it.  Pages may
+ * be shared by sequences that only read them. */
+typedef struct {
+    void *k, *v;              /* bf16 page pools                                        */
+    const int32_t *table;     /* [num_seqs] rows of max_blocks page numbers             */
+    int num_pages;            /* pages in each pool                                     */
+    int page_size;            /* tokens a page holds, any number                        */
+    int kv_heads;
+    int head_dim;             /* 64, 128 or 256 contiguous columns                      */
+    int num_seqs;
+    int max_blocks;
+    int64_t table_stride;     /* page numbers between table rows                        */
+    int64_t page_stride;      /* elements between pages, slots and heads: multiples of  */
+    int64_t token_stride;     /*   8; the pools 16-byte aligned                         */
+    int64_t head_stride;
+} iris_gpu_kv_cache_t;
+
+/* A rotation of the first rot_dim columns of a head: pair i turns by
+ * position * turns[i] * 2^-64 of a full turn (64-bit fixed point: the product
+ * wraps where the angle does, so far positions lose nothing).  Plain data,
+ * filled on the host by one of the two functions below. */
+#define IRIS_ROPE_HALF 0         /* pairs (i, i + rot_dim / 2), as Qwen3                */
+#define IRIS_ROPE_INTERLEAVED 1  /* pairs (2i, 2i + 1), as the image transformers       */
+typedef struct {
+    int layout;
+    int rot_dim;              /* a multiple of 16, at most 256                          */
+    float amplitude;          /* factor of cos and sin                                  */
+    uint64_t turns[128];
+} iris_gpu_rope_t;
+
+/* Scaling for contexts longer than the trained one.  original_len 0: every
+ * frequency divided by factor.  Else by parts: pair i, which makes r =
+ * original_len * f_i / (2 pi) turns over the trained context, keeps f_i for
+ * r >= high, gets f_i / factor for r <= low, and the mix linear in r between. */
+typedef struct {
+    double factor;
+    double original_len;
+    double low, high;
+    double amplitude;
+} iris_gpu_rope_scaling_t;
+
+/* f_i = theta^(-2 i / rot_dim) radians per position; scaling may be NULL. */
+int iris_gpu_rope_init(iris_gpu_rope_t *rope, int layout, int rot_dim, double theta,
+                       const iris_gpu_rope_scaling_t *scaling);
+/* Frequencies [rot_dim / 2] of the caller's own, in radians per position. */
+int iris_gpu_rope_init_freqs(iris_gpu_rope_t *rope, int layout, int rot_dim, const double *freqs, double amplitude);
+
+/* New tokens into the cache.  Token t has query heads q[t] [heads, head_dim]
+ * and key / value heads k[t], v[t] [kv_heads, head_dim] (rows ldq / ldk / ldv
+ * elements apart, all bf16, or all f32 when f32 != 0: the three column ranges
+ * of one QKV projection, for instance) and belongs at position pos[t] of
+ * sequence seq[t].  Q and K: RMSNorm per head with q_norm / k_norm [head_dim]
+ * (each may be NULL: none), then the rotation (rope NULL: none); f32 inside,
+ * rounded once to bf16.  Q goes to q_out[t] [heads, head_dim] (bf16, rows
+ * ldq_out apart; may be q itself), K and V to their slots.  heads may be 0
+ * (q, q_out NULL).  A token with seq[t] outside [0, num_seqs) or pos[t] < 0 is
+ * padding: nothing of it is written.  One past the table's end or with a page
+ * number outside the pool gets its q_out and no slot.  Two tokens of one call
+ * must not share a slot (one of them, or a mix, is what stays).  Row strides
+ * multiples of 8 (f32: 4), pointers 16-byte aligned. */
+int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
+                         const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int f32,
+                         const float *q_norm, const float *k_norm, float eps, const int32_t *seq, const int32_t *pos,
+                         int tokens, int heads, void *stream);
+
+/* Attention over the cache.  Row t, query head h of q (bf16 [rows, heads,
+ * head_dim], rows ldq elements apart) sees the keys at positions 0 .. pos[t]
+ * of sequence seq[t] (seq NULL: row t is sequence t) and reads key-value head
+ * h / (heads / kv_heads):  out = softmax(scale * q K^T) V, bf16, rows ldo
+ * apart.  So the newest tokens of many sequences are one call, and a run of
+ * tokens of one sequence is causal.  A row that sees nothing (pos[t] < 0)
+ * gives zeros; a row with seq[t] outside [0, num_seqs) is left as it was.
+ * Positions past the table's end and pages outside the pool are not seen.
+ * The same call gives the same bits every time; among other rows a row's sum
+ * may be split elsewhere and differ in its last bits before rounding.
+ * Workspace: iris_gpu_attention_paged_workspace bytes, 16-byte aligned. */
+size_t iris_gpu_attention_paged_workspace(const iris_gpu_kv_cache_t *cache, int heads);
+int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const void *q, int64_t ldo, int64_t ldq,
+                             const int32_t *seq, const int32_t *pos, int rows, int heads, float scale,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* The answer side of a logits matrix [rows, vocab] (bf16, or f32 when f32 !=
+ * 0; rows ld elements apart, any alignment of the elements), in one pass over
+ * it.  Per row, each output optional (NULL):
+ *   logprob[r]       log softmax at targets[r] (outside [0, vocab): 0)
+ *   entropy[r]       -sum p log p, natural logarithm
+ *   top_ids[r], top_logprobs[r]  [top_k]: the top_k largest logits, largest
+ *                    first, equal ones by id (0 <= top_k <= min(32, vocab))
+ * A logit of -inf is a token that can not come: probability 0.  A row of
+ * nothing else gives logprob -inf and entropy 0.  A NaN or +inf makes the
+ * row's log probabilities and entropy NaN; NaN ranks first among the ids.
+ * Workspace: iris_gpu_token_logprobs_workspace bytes, 16-byte aligned. */
+size_t iris_gpu_token_logprobs_workspace(int rows, int vocab);
+int iris_gpu_token_logprobs(const void *logits, int f32, int64_t ld, int rows, int vocab, const int32_t *targets,
+                            float *logprob, float *entropy, int top_k, int32_t *top_ids, float *top_logprobs,
+                            void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

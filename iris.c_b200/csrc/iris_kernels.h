@@ -424,6 +424,46 @@ cudaError_t iris_launch_gated_add_f32(float *out, const float *gate, const float
 cudaError_t iris_launch_add_f32(float *out, const float *a, const float *b, long n, cudaStream_t stream);
 cudaError_t iris_launch_add_bf16(void *out, const void *a, const void *b, long n, cudaStream_t stream);
 
+/* ------------------------------------------------------------------ language-model operators (lm_kernels.cu)
+ * Arguments as the public entry points of the same names, already checked. */
+#include "iris_cuda.h"
+typedef struct {
+    iris_gpu_kv_cache_t cache;
+    iris_gpu_rope_t rope;     /* rot_dim 0: no rotation */
+    void *q_out;
+    const void *q, *k, *v;
+    int64_t ldq_out, ldq, ldk, ldv;
+    const float *q_norm, *k_norm;
+    float eps;
+    const int32_t *seq, *pos;
+    int tokens, heads;
+} IrisRopeAppend;
+cudaError_t iris_launch_rope_append(const IrisRopeAppend *a, int f32, int num_sms, cudaStream_t stream);
+typedef struct {
+    iris_gpu_kv_cache_t cache;
+    void *out;
+    const void *q;
+    int64_t ldo, ldq;
+    const int32_t *seq, *pos;
+    int rows, heads;
+    float scale;
+    float *ws;
+} IrisPagedAttention;
+size_t iris_paged_attention_ws_bytes(const iris_gpu_kv_cache_t *cache, int heads, int num_sms);
+/* *launches = kernels queued */
+cudaError_t iris_launch_paged_attention(const IrisPagedAttention *a, int num_sms, cudaStream_t stream, int *launches);
+typedef struct {
+    const void *logits;
+    int64_t ld;
+    int rows, vocab, top_k;
+    const int32_t *targets;
+    float *logprob, *entropy, *top_logprobs;
+    int32_t *top_ids;
+    void *ws;
+} IrisLogprobs;
+size_t iris_logprobs_ws_bytes(int rows, int vocab);
+cudaError_t iris_launch_logprobs(const IrisLogprobs *a, int f32, int num_sms, cudaStream_t stream, int *launches);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,59 @@ class Ref(C.Structure):
     _fields_ = [("latent", _fp), ("h", C.c_int), ("w", C.c_int), ("t_offset", C.c_int)]
 
 
+class RopeScaling(C.Structure):
+    """iris_gpu_rope_scaling_t."""
+    _fields_ = [("factor", C.c_double), ("original_len", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("amplitude", C.c_double)]
+
+
+class Rope(C.Structure):
+    """iris_gpu_rope_t: a rotation of the first rot_dim columns of each head."""
+    _fields_ = [("layout", C.c_int), ("rot_dim", C.c_int), ("amplitude", C.c_float), ("turns", C.c_uint64 * 128)]
+
+    @classmethod
+    def of(cls, rot_dim: int, theta: float, interleaved: bool = False, factor: float = 1.0, original_len: float = 0.0,
+           low: float = 1.0, high: float = 32.0, amplitude: float = 1.0) -> "Rope":
+        """Frequencies theta^(-2i / rot_dim), scaled for long contexts (iris_gpu_rope_scaling_t)."""
+        r = cls()
+        sc = RopeScaling(factor, original_len, low, high, amplitude)
+        _ok(lib().iris_gpu_rope_init(C.byref(r), int(interleaved), rot_dim, theta, C.byref(sc)))
+        return r
+
+    @classmethod
+    def of_freqs(cls, freqs, interleaved: bool = False, amplitude: float = 1.0) -> "Rope":
+        """Frequencies of the caller's own [rot_dim / 2], radians per position."""
+        r = cls()
+        f = np.ascontiguousarray(freqs, np.float64)
+        _ok(lib().iris_gpu_rope_init_freqs(C.byref(r), int(interleaved), 2 * f.size,
+                                           f.ctypes.data_as(C.POINTER(C.c_double)), amplitude))
+        return r
+
+
+class KvCache(C.Structure):
+    """iris_gpu_kv_cache_t: a paged key-value cache over the caller's own pools."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("num_pages", C.c_int),
+                ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("num_seqs", C.c_int),
+                ("max_blocks", C.c_int), ("table_stride", C.c_int64), ("page_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+    @classmethod
+    def of(cls, k, v, table) -> "KvCache":
+        """k, v: bf16 device tensors seen as [pages, slots, heads, columns] (any order of
+        slots and heads in memory, columns contiguous, both laid out alike); table:
+        int32 [sequences, blocks].  The tensors are kept alive."""
+        if _dtype(k) != "bfloat16" or _dtype(v) != "bfloat16" or _dtype(table) != "int32":
+            raise IrisCudaError("KvCache: pools are bfloat16, the page table int32")
+        if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()):
+            raise IrisCudaError("KvCache: pools [pages, slots, heads, columns] laid out alike")
+        if k.stride(3) != 1 or len(table.shape) != 2 or table.stride(1) != 1:
+            raise IrisCudaError("KvCache: columns and table rows are contiguous")
+        c = cls(k.data_ptr(), v.data_ptr(), table.data_ptr(), k.shape[0], k.shape[1], k.shape[2], k.shape[3],
+                table.shape[0], table.shape[1], table.stride(0), k.stride(0), k.stride(1), k.stride(2))
+        c.tensors = (k, v, table)
+        return c
+
+
 PROGRESS_CB = C.CFUNCTYPE(None, C.c_int, C.c_int)
 
 # name -> (restype, argtypes) for every exported entry point of include/iris_cuda.h
@@ -275,6 +328,20 @@ SIGNATURES = {
     "iris_metal_warmup_bf16_buffer": (None, [_u16p, C.c_size_t]),
     "iris_metal_warmup_bf16_buffers_parallel": (None, [C.POINTER(_u16p), C.POINTER(C.c_size_t), C.c_int]),
     "iris_gpu_op_failures": (C.c_ulong, []),
+    # language-model operators
+    "iris_gpu_rope_init": (C.c_int, [C.POINTER(Rope), C.c_int, C.c_int, C.c_double, C.POINTER(RopeScaling)]),
+    "iris_gpu_rope_init_freqs": (C.c_int, [C.POINTER(Rope), C.c_int, C.c_int, C.POINTER(C.c_double), C.c_double]),
+    "iris_gpu_rope_append": (C.c_int, [C.POINTER(KvCache), C.POINTER(Rope), C.c_void_p, C.c_int64, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
+                                       C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "iris_gpu_attention_paged_workspace": (C.c_size_t, [C.POINTER(KvCache), C.c_int]),
+    "iris_gpu_attention_paged": (C.c_int, [C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                           C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_void_p,
+                                           C.c_size_t, C.c_void_p]),
+    "iris_gpu_token_logprobs_workspace": (C.c_size_t, [C.c_int, C.c_int]),
+    "iris_gpu_token_logprobs": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                          C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                          C.c_void_p]),
 }
 
 _libc = C.CDLL(None)
@@ -730,3 +797,101 @@ class Qwen3:
         p = lib().iris_cuda_qwen3_forward(self.h, ids.ctypes.data_as(ip),
                                           None if m is None else m.ctypes.data_as(ip), len(ids))
         return _take_floats(p, len(ids) * self.text_dim(), (len(ids), self.text_dim()))
+
+
+# ---------------------------------------------------------------- language-model operators
+# Device tensors are anything with data_ptr(), shape, stride() and dtype (torch's
+# are); every call queues its work on `stream` (a cudaStream_t as an integer, 0:
+# the default stream) and raises IrisCudaError when it is refused.
+
+def _ok(rc: int) -> None:
+    if rc:
+        raise IrisCudaError(last_error())
+
+
+def _dtype(t) -> str:
+    return str(t.dtype).rpartition(".")[2]
+
+
+def _need(what: str, t, dtype: str, shape, optional: bool = False):
+    """Address of t after a check of its type, shape and contiguous last axis (None: 0)."""
+    if t is None and optional:
+        return None
+    if _dtype(t) != dtype or tuple(t.shape) != tuple(shape) or (shape and t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise IrisCudaError(f"{what}: needs {dtype} {tuple(shape)}, contiguous in the last axis; "
+                            f"got {_dtype(t)} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _heads_rows(what: str, t, dtype: str, rows: int, heads: int, head_dim: int):
+    """(address, row stride) of [rows, heads, head_dim] or [rows, heads * head_dim]."""
+    shape = tuple(t.shape)
+    if _dtype(t) != dtype or shape not in ((rows, heads, head_dim), (rows, heads * head_dim)) or \
+            t.stride(-1) != 1 or (len(shape) == 3 and heads > 1 and t.stride(1) != head_dim):
+        raise IrisCudaError(f"{what}: needs {dtype} [{rows}, {heads}, {head_dim}] with contiguous rows; "
+                            f"got {_dtype(t)} {shape}")
+    return t.data_ptr(), t.stride(0) if rows > 1 else heads * head_dim
+
+
+def rope_append(cache: KvCache, rope: Rope | None, q_out, q, k, v, seq, pos, *, heads: int, q_norm=None, k_norm=None,
+                eps: float = 1e-6, stream: int = 0) -> None:
+    """iris_gpu_rope_append: rotate the new tokens' Q and K, write K and V to the cache."""
+    n, d, nkv = seq.shape[0], cache.head_dim, cache.kv_heads
+    ty = _dtype(k)
+    if ty not in ("float32", "bfloat16"):
+        raise IrisCudaError(f"rope_append: k is {ty}")
+    kp, ldk = _heads_rows("k", k, ty, n, nkv, d)
+    vp, ldv = _heads_rows("v", v, ty, n, nkv, d)
+    qp = op = None
+    ldq = ldo = 0
+    if heads:
+        qp, ldq = _heads_rows("q", q, ty, n, heads, d)
+        op, ldo = _heads_rows("q_out", q_out, "bfloat16", n, heads, d)
+    _ok(lib().iris_gpu_rope_append(cache, rope, op, ldo, qp, kp, vp, ldq, ldk, ldv, ty == "float32",
+                                   _need("q_norm", q_norm, "float32", (d,), True),
+                                   _need("k_norm", k_norm, "float32", (d,), True), eps,
+                                   _need("seq", seq, "int32", (n,)), _need("pos", pos, "int32", (n,)), n, heads, stream))
+
+
+def attention_paged_workspace(cache: KvCache, heads: int) -> int:
+    n = lib().iris_gpu_attention_paged_workspace(cache, heads)
+    if not n:
+        raise IrisCudaError(last_error())
+    return n
+
+
+def attention_paged(cache: KvCache, out, q, seq, pos, *, scale: float, workspace, stream: int = 0) -> None:
+    """iris_gpu_attention_paged: q, out [rows, heads, head_dim]; seq None: row t is sequence t."""
+    n, d = pos.shape[0], cache.head_dim
+    heads = q.shape[1] if len(q.shape) == 3 else q.shape[1] // d
+    qp, ldq = _heads_rows("q", q, "bfloat16", n, heads, d)
+    op, ldo = _heads_rows("out", out, "bfloat16", n, heads, d)
+    _ok(lib().iris_gpu_attention_paged(cache, op, qp, ldo, ldq, _need("seq", seq, "int32", (n,), True),
+                                       _need("pos", pos, "int32", (n,)), n, heads, scale, workspace.data_ptr(),
+                                       workspace.numel() * workspace.element_size(), stream))
+
+
+def token_logprobs_workspace(rows: int, vocab: int) -> int:
+    n = lib().iris_gpu_token_logprobs_workspace(rows, vocab)
+    if not n:
+        raise IrisCudaError(last_error())
+    return n
+
+
+def token_logprobs(logits, targets, logprob, entropy, top_ids, top_logprobs, *, workspace, stream: int = 0) -> None:
+    """iris_gpu_token_logprobs: logits [rows, vocab]; the outputs may be None."""
+    rows, vocab = logits.shape
+    ty = _dtype(logits)
+    if ty not in ("float32", "bfloat16") or logits.stride(1) != 1:
+        raise IrisCudaError(f"token_logprobs: logits {ty}, stride {logits.stride(1)} between a row's values")
+    k = top_ids.shape[1] if top_ids is not None else top_logprobs.shape[1] if top_logprobs is not None else 0
+    if (top_ids is not None and k > 1 and rows > 1 and top_ids.stride(0) != k) or \
+            (top_logprobs is not None and k > 1 and rows > 1 and top_logprobs.stride(0) != k):
+        raise IrisCudaError("token_logprobs: the alternatives' rows lie one after the other")
+    _ok(lib().iris_gpu_token_logprobs(logits.data_ptr(), ty == "float32", logits.stride(0) if rows > 1 else vocab, rows,
+                                      vocab, _need("targets", targets, "int32", (rows,), True),
+                                      _need("logprob", logprob, "float32", (rows,), True),
+                                      _need("entropy", entropy, "float32", (rows,), True), k,
+                                      _need("top_ids", top_ids, "int32", (rows, k), True),
+                                      _need("top_logprobs", top_logprobs, "float32", (rows, k), True),
+                                      workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
