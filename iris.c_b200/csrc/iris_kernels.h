@@ -449,6 +449,8 @@ typedef struct {
     float scale;
     float *ws;
 } IrisPagedAttention;
+/* one-time kernel attribute setup, called at library init */
+cudaError_t iris_lm_init(void);
 size_t iris_paged_attention_ws_bytes(const iris_gpu_kv_cache_t *cache, int heads, int num_sms);
 /* *launches = kernels queued */
 cudaError_t iris_launch_paged_attention(const IrisPagedAttention *a, int num_sms, cudaStream_t stream, int *launches);

@@ -1,0 +1,110 @@
+/*
+ * Index arithmetic of the paged-cache attention, shared by the kernels
+ * (lm_kernels.cu) and by its host test: which keys a row sees, where a key
+ * lies, and how the key tiles of all rows are shared out.
+ *
+ * Work is counted in tiles of IRIS_PAGED_TILE keys.  A unit is one row, one
+ * key-value head and up to IRIS_PAGED_HEADS of the query heads on it; a row has
+ * `units` of them, each of as many tiles as the row's keys fill.  All tiles of
+ * all rows stand in one line (row by row, unit by unit, tile by tile) that is
+ * cut into equal shares, one per CTA, whatever the rows' lengths.  A unit cut
+ * by a share's border is summed in pieces: a CTA leaves at most two, slot 2 c
+ * for a piece whose unit began in an earlier share, slot 2 c + 1 for one that
+ * begins here and goes on.
+ */
+#ifndef IRIS_PAGED_H
+#define IRIS_PAGED_H
+
+#include <stdint.h>
+
+#include "iris_cuda.h"
+
+#ifdef __CUDACC__
+#define IRIS_HD __host__ __device__ __forceinline__
+#else
+#define IRIS_HD static inline
+#endif
+
+#define IRIS_PAGED_TILE 64
+#define IRIS_PAGED_HEADS 8
+
+/* units of a row */
+IRIS_HD int iris_paged_units(const iris_gpu_kv_cache_t *c, int heads) {
+    const int group = heads / c->kv_heads;
+    return c->kv_heads * ((group + IRIS_PAGED_HEADS - 1) / IRIS_PAGED_HEADS);
+}
+
+/* sequence of row t, or -1 */
+IRIS_HD int iris_paged_seq(const iris_gpu_kv_cache_t *c, const int32_t *seq, int t) {
+    const int s = seq ? seq[t] : t;
+    return s >= 0 && s < c->num_seqs ? s : -1;
+}
+
+/* keys that a row at position `pos` sees (no more than the table has room for) */
+IRIS_HD int iris_paged_len(const iris_gpu_kv_cache_t *c, int pos) {
+    const int64_t room = (int64_t)c->max_blocks * c->page_size;
+    const int64_t len = pos < 0 ? 0 : (int64_t)pos + 1;
+    const int64_t n = len < room ? len : room;
+    return n < 0x7FFFFFFF ? (int)n : 0x7FFFFFFF;
+}
+
+IRIS_HD int iris_paged_tiles(int len) { return len / IRIS_PAGED_TILE + (len % IRIS_PAGED_TILE != 0); }
+
+/* tiles of one unit of row t */
+IRIS_HD int iris_paged_row_tiles(const iris_gpu_kv_cache_t *c, const int32_t *seq, const int32_t *pos, int t) {
+    return iris_paged_seq(c, seq, t) < 0 ? 0 : iris_paged_tiles(iris_paged_len(c, pos[t]));
+}
+
+/* page of key p of sequence s, or -1 where the table or the pool has none */
+IRIS_HD int iris_paged_page(const iris_gpu_kv_cache_t *c, int s, int p) {
+    const int b = p / c->page_size;
+    if (b >= c->max_blocks) return -1;
+    const int page = c->table[(int64_t)s * c->table_stride + b];
+    return page >= 0 && page < c->num_pages ? page : -1;
+}
+
+/* element offset in the pools of key p (head 0) on `page` */
+IRIS_HD int64_t iris_paged_offset(const iris_gpu_kv_cache_t *c, int page, int p) {
+    return (int64_t)page * c->page_stride + (int64_t)(p % c->page_size) * c->token_stride;
+}
+
+/* tiles in a share */
+IRIS_HD int64_t iris_paged_share(int64_t total, int ctas) { return total <= ctas ? 1 : (total + ctas - 1) / ctas; }
+
+/* A place in the line of tiles. */
+typedef struct {
+    int t;        /* row                          */
+    int s, len;   /* its sequence and visible keys */
+    int n;        /* tiles of each of its units   */
+    int u;        /* unit                         */
+    int i;        /* tile of the unit             */
+} iris_paged_at_t;
+
+IRIS_HD void iris_paged_row(iris_paged_at_t *a, const iris_gpu_kv_cache_t *c, const int32_t *seq, const int32_t *pos) {
+    a->s = iris_paged_seq(c, seq, a->t);
+    a->len = a->s < 0 ? 0 : iris_paged_len(c, pos[a->t]);
+    a->n = iris_paged_tiles(a->len);
+}
+
+/* the next tile (there is one) */
+IRIS_HD void iris_paged_next(iris_paged_at_t *a, int units, const iris_gpu_kv_cache_t *c, const int32_t *seq,
+                             const int32_t *pos) {
+    if (++a->i < a->n) return;
+    a->i = 0;
+    if (++a->u < units) return;
+    a->u = 0;
+    do {
+        a->t++;
+        iris_paged_row(a, c, seq, pos);
+    } while (a->n == 0);
+}
+
+/* Share c begins at tile `at.i` of a unit.  The number of later shares that
+ * hold pieces of that unit when c is the first after the one it began in,
+ * else 0.  The pieces then are slot 2 (c - 1) + 1 and slots 2 c, 2 (c + 1), ... */
+IRIS_HD int iris_paged_join(const iris_paged_at_t *at, int64_t share) {
+    if (at->i == 0 || at->i > share) return 0;
+    return (int)((at->n - at->i + share - 1) / share);
+}
+
+#endif

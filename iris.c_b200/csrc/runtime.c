@@ -100,6 +100,7 @@ int iris_cuda_init(int device) {
     cudaStreamSynchronize(g_rt.stream);
     if ((e = iris_gemm_init()) != cudaSuccess) return iris_cuda_check(e, "gemm init");
     if ((e = iris_attention_tc_init()) != cudaSuccess) return iris_cuda_check(e, "attention init");
+    if ((e = iris_lm_init()) != cudaSuccess) return iris_cuda_check(e, "language-model operators init");
     iris_attention_set_status(g_rt.d_status);
     g_rt.initialized = 1;
     return IRIS_CUDA_OK;
