@@ -472,74 +472,368 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 }
 
 // ------------------------------------------------------------------ log probabilities
-__device__ __forceinline__ float value(const float* p, int64_t i) { return p[i]; }
-__device__ __forceinline__ float value(const __nv_bfloat16* p, int64_t i) { return __bfloat162float(p[i]); }
+// Bound by the logits' bytes, and close behind by the exponentials (16 a clock
+// and SM: 0.72 of the bf16 stream's rate).  One pass: a warp reads LP_BLOCK
+// values at a time and keeps, per lane, the running maximum m and
+//   s1 = sum e^(x - m),   s2 = sum (x - m) e^(x - m)
+// from which lse = m + log s1 and the entropy log s1 - s2 / s1.  A new maximum
+// m' turns them into f s1 and f (s2 + (m - m') s1), f = e^(m - m').  For the
+// alternatives it leaves the largest value of every block: the k largest
+// values of a row lie in the k blocks with the largest maxima (each of k blocks
+// ahead of another one holds a value ahead of all of the other's), so the second
+// kernel reads those k blocks again and nothing else.
+constexpr int LP_BLOCK = 512;  // values; k of them are read twice: 4 % of a bf16 row of 151936 at k = 20, in L2
+constexpr int LP_LOADS = 8;    // 16-byte loads of a lane in flight
+
+template <typename In>
+struct LpShape {
+  static constexpr int kVec = 16 / sizeof(In);                  // values of a load
+  static constexpr int kPer = LP_BLOCK / (32 * kVec);           // loads of a block
+  static constexpr int kBlocks = LP_LOADS / kPer;               // blocks in flight
+};
 
 // Order of the alternatives: larger values first, equal ones by id, NaN before
-// all; as one whole number a value, larger first.
+// all; as one whole number a value, larger first, 0 for none.
 __device__ __forceinline__ uint32_t rank_bits(float x) {
   if (x != x) return 0xFF800001u;  // one above +inf
   const uint32_t u = __float_as_uint(x + 0.0f);  // -0 counts as 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ uint64_t place(uint32_t rank, uint32_t id) { return (uint64_t)rank << 32 | (uint32_t)~id; }
 
-template <typename T, typename F>
-__device__ T block_reduce(T v, T* red, F f) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-  __syncthreads();
-  T t = red[0];
-  for (int w = 1; w < (int)blockDim.x / 32; w++) t = f(t, red[w]);
-  return t;
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 
-// One block per row: the maximum, the sums, then top_k rounds of the best
-// (value, id) below the one before.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+
+// Two values x0, x1 into two sums each: d = x - base, e = 2^(d log2 e).
+__device__ __forceinline__ void add_pair(uint64_t x, uint64_t neg_base, uint64_t log2e, uint64_t& s1, uint64_t& s2) {
+  asm("{\n\t"
+      ".reg .b64 d, y, e;\n\t.reg .f32 y0, y1, e0, e1;\n\t"
+      "add.rn.f32x2 d, %2, %3;\n\t"
+      "mul.rn.f32x2 y, d, %4;\n\t"
+      "mov.b64 {y0, y1}, y;\n\t"
+      "ex2.approx.ftz.f32 e0, y0;\n\t"
+      "ex2.approx.ftz.f32 e1, y1;\n\t"
+      "mov.b64 e, {e0, e1};\n\t"
+      "add.rn.f32x2 %0, %0, e;\n\t"
+      "fma.rn.f32x2 %1, d, e, %1;\n\t}"
+      : "+l"(s1), "+l"(s2)
+      : "l"(x), "l"(neg_base), "l"(log2e));
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Softmax sums against a reference m.
+struct LpSum {
+  float m, s1, s2;
+  // the same sums against mn >= m
+  __device__ __forceinline__ void raise(float mn) {
+    if (m != mn) {
+      if (m != -INFINITY) {
+        const float f = exp2_approx((m - mn) * kLog2e);
+        s2 = f == 0.f ? 0.f : f * (s2 + (m - mn) * s1);  // (m - mn) s1 may be infinite where f is 0
+        s1 = f * s1;
+      }
+      m = mn;
+    }
+  }
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_add(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The values at [e, e + kVec) of a row of `vocab` values, 16-byte aligned;
+// -inf where the row has none.  Nothing outside the row is read.
 template <typename In>
-__global__ void __launch_bounds__(256) logprobs_kernel(const __grid_constant__ IrisLogprobs a) {
-  __shared__ float redf[8];
-  __shared__ unsigned long long redu[8];
-  const int r = blockIdx.x;
-  const In* x = (const In*)a.logits + (int64_t)r * a.ld;
-  auto fmx = [](float u, float v) { return fmaxf(u, v); };
-  auto add = [](float u, float v) { return u + v; };
-  auto umx = [](unsigned long long u, unsigned long long v) { return u > v ? u : v; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < a.vocab; i += 256) m = fmaxf(m, value(x, i));
-  m = block_reduce(m, redf, fmx);
-  float s1 = 0.f, s2 = 0.f;
-  const bool none = m == -INFINITY;  // or nothing but NaN, which the sums then show
-  for (int i = threadIdx.x; i < a.vocab; i += 256) {
-    const float d = none ? value(x, i) : value(x, i) - m, e = expf(d);
-    s1 += e;
-    s2 += fmaxf(d, -1000.f) * e;  // a logit of -inf adds 0
+__device__ __forceinline__ uint4 row_vec(const In* x, int64_t e, int vocab) {
+  constexpr int VEC = 16 / sizeof(In);
+  if (e >= 0 && e + VEC <= vocab) return __ldg(reinterpret_cast<const uint4*>(x + e));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(In) == 4) {
+      w[i] = e + i >= 0 && e + i < vocab ? __float_as_uint(x[e + i]) : 0xFF800000u;
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+      const uint32_t lo = e + 2 * i >= 0 && e + 2 * i < vocab ? h[e + 2 * i] : 0xFF80u;
+      const uint32_t hi = e + 2 * i + 1 >= 0 && e + 2 * i + 1 < vocab ? h[e + 2 * i + 1] : 0xFF80u;
+      w[i] = lo | hi << 16;
+    }
   }
-  s1 = block_reduce(s1, redf, add);
-  s2 = block_reduce(s2, redf, add);
-  const float lse = s1 == 0.f ? 0.f : m + logf(s1);
-  if (threadIdx.x == 0) {
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename In>
+__device__ __forceinline__ void vec_values(uint4 u, float x[16 / sizeof(In)]) {
+  if constexpr (sizeof(In) == 4) {
+    x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
+  } else {
+    const float2 a = unpack2(u.x), b = unpack2(u.y), c = unpack2(u.z), d = unpack2(u.w);
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
+  }
+}
+
+// The largest of the values, NaN if one is.
+template <typename In>
+__device__ __forceinline__ float vec_max(uint4 u) {
+  if constexpr (sizeof(In) == 4) {
+    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)),
+                   max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else {
+    auto h = [](uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); };
+    const __nv_bfloat162 v = __hmax2_nan(__hmax2_nan(h(u.x), h(u.y)), __hmax2_nan(h(u.z), h(u.w)));
+    return max_nan(__low2float(v), __high2float(v));
+  }
+}
+
+struct LpPlan {
+  int nblk;    // blocks of a row
+  int rounds;  // of kBlocks blocks each, per warp
+  int warps;   // of a row
+  float4* sums;     // [rows][warps] m, s1, s2
+  uint32_t* maxima; // [rows][nblk] rank of each block's largest value, 0 for a block outside the row
+};
+
+// First value of block 0 before the row's first one: blocks are cut at 16-byte boundaries.
+template <typename In>
+__device__ __forceinline__ int row_offset(const In* x) {
+  return (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(In));
+}
+
+template <typename In>
+__global__ void __launch_bounds__(256) logprobs_stream_kernel(const __grid_constant__ IrisLogprobs a,
+                                                              const __grid_constant__ LpPlan plan) {
+  using Sh = LpShape<In>;
+  const int lane = threadIdx.x % 32;
+  const int64_t wid = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  const int64_t row = wid / plan.warps;
+  if (row >= a.rows) return;
+  const int w = (int)(wid - row * plan.warps);
+  const In* x = (const In*)a.logits + row * a.ld;
+  const int off = row_offset(x);
+  LpSum sum = {-INFINITY, 0.f, 0.f};
+  const uint64_t log2e = pair(kLog2e, kLog2e);
+  for (int r = 0; r < plan.rounds; r++) {
+    const int b0 = (w * plan.rounds + r) * Sh::kBlocks;
+    uint4 u[LP_LOADS];
+#pragma unroll
+    for (int j = 0; j < LP_LOADS; j++)
+      u[j] = row_vec(x, ((int64_t)b0 * LP_BLOCK - off) + (j * 32 + lane) * Sh::kVec, a.vocab);
+    uint32_t ranks = 0;
+#pragma unroll
+    for (int b = 0; b < Sh::kBlocks; b++) {
+      float cm = vec_max<In>(u[b * Sh::kPer]);
+#pragma unroll
+      for (int j = 1; j < Sh::kPer; j++) cm = max_nan(cm, vec_max<In>(u[b * Sh::kPer + j]));
+      if (a.top_k) {
+        const uint32_t best = __reduce_max_sync(0xffffffffu, rank_bits(cm));
+        if (lane == b) ranks = best;
+      }
+      if (cm > sum.m) sum.raise(cm);
+      const float base = sum.m == -INFINITY ? 0.f : sum.m;
+      const uint64_t nb = pair(-base, -base);
+      uint64_t s1 = 0, s2 = 0;  // two zeros each
+#pragma unroll
+      for (int j = 0; j < Sh::kPer; j++) {
+        float v[Sh::kVec];
+        vec_values<In>(u[b * Sh::kPer + j], v);
+#pragma unroll
+        for (int i = 0; i < Sh::kVec; i += 2) add_pair(pair(v[i], v[i + 1]), nb, log2e, s1, s2);
+      }
+      float p1, q1, p2, q2;
+      unpair(s1, p1, q1);
+      unpair(s2, p2, q2);
+      p2 += q2;
+      if (p2 != p2) {  // a value of -inf (0 times -inf), which adds 0, or one that spoils the row
+        p2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < Sh::kPer; j++) {
+          float v[Sh::kVec];
+          vec_values<In>(u[b * Sh::kPer + j], v);
+#pragma unroll
+          for (int i = 0; i < Sh::kVec; i++) {
+            const float d = v[i] - base;
+            p2 += d == -INFINITY ? 0.f : d * exp2_approx(d * kLog2e);
+          }
+        }
+      }
+      sum.s1 += p1 + q1;
+      sum.s2 += p2;
+    }
+    if (a.top_k && lane < Sh::kBlocks && b0 + lane < plan.nblk) {
+      const bool any = (int64_t)(b0 + lane) * LP_BLOCK - off < a.vocab;
+      plan.maxima[row * plan.nblk + b0 + lane] = any ? ranks : 0u;
+    }
+  }
+  sum.raise(warp_max(sum.m));
+  const float s1 = warp_add(sum.s1), s2 = warp_add(sum.s2);
+  if (lane == 0) plan.sums[row * plan.warps + w] = make_float4(sum.m, s1, s2, 0.f);
+}
+
+// The k largest of the places that items(f) hands to f (each thread its own
+// share of them, the same on every call; all different, 0 is none), largest
+// first, into best; returns how many there are.  A threshold that at least k
+// places reach is searched by halving over the threads' largest ones, which is
+// one barrier a step; the few places above it are then put in order by counting.
+struct TopK {
+  uint64_t list[1024], best[32];
+  int n;
+  unsigned sum;
+};
+
+template <typename Items>
+__device__ int select_top(TopK& s, int k, Items items) {
+  constexpr int FEW = 48;  // enough; over k = 32
+  uint64_t own = 0;
+  items([&](uint64_t p) { own = p > own ? p : own; });
+  uint64_t lo = 1, hi = 0xFF800002ull << 32;
+  if (__syncthreads_count(own >= lo) > FEW)
+    while (true) {
+      const uint64_t mid = lo + (hi - lo) / 2;
+      const int c = __syncthreads_count(own >= mid);
+      if (c < k) {
+        hi = mid;
+      } else {
+        lo = mid;
+        if (c <= FEW) break;
+      }
+    }
+  // the places >= lo; where one thread holds many of them the halving goes on over all places
+  hi = 0xFF800002ull << 32;
+  while (true) {
+    if (threadIdx.x == 0) s.n = 0, s.sum = 0;
+    __syncthreads();
+    items([&](uint64_t p) {
+      if (p >= lo) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < 1024) s.list[at] = p;
+      }
+    });
+    __syncthreads();
+    if (s.n <= 1024) break;
+    while (true) {
+      const uint64_t mid = lo + (hi - lo) / 2;
+      unsigned c = 0;
+      items([&](uint64_t p) { c += p >= mid; });
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (threadIdx.x % 32 == 0) atomicAdd(&s.sum, c);
+      __syncthreads();
+      c = s.sum;
+      __syncthreads();
+      if (threadIdx.x == 0) s.sum = 0;
+      __syncthreads();
+      if (c < (unsigned)k) {
+        hi = mid;
+      } else {
+        lo = mid;
+        if (c <= 1024) break;
+      }
+    }
+  }
+  const int n = s.n;
+  for (int c = threadIdx.x; c < n; c += 256) {
+    const uint64_t p = s.list[c];
+    int ahead = 0;
+    for (int j = 0; j < n; j++) ahead += s.list[j] > p;
+    if (ahead < k) s.best[ahead] = p;
+  }
+  __syncthreads();
+  return min(n, k);
+}
+
+// One block per row: the warps' sums joined, the outputs, the alternatives.
+template <typename In>
+__global__ void __launch_bounds__(256) logprobs_finish_kernel(const __grid_constant__ IrisLogprobs a,
+                                                              const __grid_constant__ LpPlan plan) {
+  using Sh = LpShape<In>;
+  __shared__ TopK top;
+  __shared__ uint64_t blocks[32];
+  __shared__ float red[3][8];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  const In* x = (const In*)a.logits + row * a.ld;
+  LpSum sum = {-INFINITY, 0.f, 0.f};
+  for (int w = tid; w < plan.warps; w += 256) {
+    const float4 v = plan.sums[row * plan.warps + w];
+    LpSum other = {v.x, v.y, v.z};
+    const float m = fmaxf(sum.m, other.m);
+    sum.raise(m);
+    other.raise(m);
+    sum.s1 += other.s1;
+    sum.s2 += other.s2;
+  }
+  float m = warp_max(sum.m);
+  if (tid % 32 == 0) red[0][tid / 32] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; w++) m = fmaxf(m, red[0][w]);
+  sum.raise(m);
+  float s1 = warp_add(sum.s1), s2 = warp_add(sum.s2);
+  if (tid % 32 == 0) red[1][tid / 32] = s1, red[2][tid / 32] = s2;
+  __syncthreads();
+  s1 = s2 = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; w++) s1 += red[1][w], s2 += red[2][w];
+  auto value = [&](int64_t i) {
+    if constexpr (sizeof(In) == 4) return x[i];
+    else return __bfloat162float(x[i]);
+  };
+  const float log_s1 = logf(s1), lse = s1 == 0.f ? 0.f : m + log_s1;
+  if (tid == 0) {
     if (a.logprob) {
-      const int t = a.targets[r];
-      a.logprob[r] = t >= 0 && t < a.vocab ? value(x, t) - lse : 0.f;
+      const int t = a.targets[row];
+      a.logprob[row] = t >= 0 && t < a.vocab ? value(t) - lse : 0.f;
     }
-    if (a.entropy) a.entropy[r] = s1 == 0.f ? 0.f : logf(s1) - s2 / s1;
+    if (a.entropy) a.entropy[row] = s1 == 0.f ? 0.f : log_s1 - s2 / s1;
   }
-  unsigned long long below = ~0ull;
-  for (int k = 0; k < a.top_k; k++) {
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += 256) {
-      const unsigned long long c = (unsigned long long)rank_bits(value(x, i)) << 32 | (uint32_t)~i;
-      if (c < below) best = umx(best, c);
+  if (!a.top_k) return;
+  const int nb = select_top(top, a.top_k, [&](auto f) {
+    for (int b = tid; b < plan.nblk; b += 256) {
+      const uint32_t r = plan.maxima[row * plan.nblk + b];
+      if (r) f(place(r, b));
     }
-    best = block_reduce(best, redu, umx);
-    below = best;
-    if (threadIdx.x == 0) {
-      const int id = (int)~(uint32_t)best;
-      if (a.top_ids) a.top_ids[(int64_t)r * a.top_k + k] = id;
-      if (a.top_logprobs) a.top_logprobs[(int64_t)r * a.top_k + k] = value(x, id) - lse;
+  });
+  if (tid < nb) blocks[tid] = top.best[tid];
+  __syncthreads();
+  const int off = row_offset(x);
+  select_top(top, a.top_k, [&](auto f) {
+    constexpr int VPB = LP_BLOCK / Sh::kVec;
+    for (int j = tid; j < nb * VPB; j += 256) {
+      const int64_t e = (int64_t)(uint32_t)~(uint32_t)blocks[j / VPB] * LP_BLOCK - off + (j % VPB) * Sh::kVec;
+      float v[Sh::kVec];
+      vec_values<In>(row_vec(x, e, a.vocab), v);
+#pragma unroll
+      for (int i = 0; i < Sh::kVec; i++)
+        if (e + i >= 0 && e + i < a.vocab) f(place(rank_bits(v[i]), (uint32_t)(e + i)));
     }
+  });
+  if (tid < a.top_k) {
+    const int id = (int)~(uint32_t)top.best[tid];
+    if (a.top_ids) a.top_ids[row * a.top_k + tid] = id;
+    if (a.top_logprobs) a.top_logprobs[row * a.top_k + tid] = value(id) - lse;
   }
 }
 
@@ -618,18 +912,34 @@ extern "C" cudaError_t iris_lm_init(void) {
   return e;
 }
 
+static int lp_blocks(int vocab) { return (int)(((int64_t)vocab + 7 + LP_BLOCK - 1) / LP_BLOCK); }  // 7: row_offset at most
+
+static size_t lp_align(size_t n) { return (n + 15) & ~(size_t)15; }
+
 extern "C" size_t iris_logprobs_ws_bytes(int rows, int vocab) {
-  (void)rows, (void)vocab;
-  return 16;
+  const size_t n = (size_t)lp_blocks(vocab);  // warps of a row: at most a block each
+  return 16 + (size_t)rows * n * sizeof(float4) + lp_align((size_t)rows * n * sizeof(uint32_t));
+}
+
+template <typename In>
+static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStream_t stream) {
+  LpPlan plan;
+  plan.nblk = lp_blocks(a->vocab);
+  constexpr int K = LpShape<In>::kBlocks;
+  // a warp's sums are joined once, so it takes two rounds of loads where that still leaves every SM some 64 warps
+  plan.rounds = (int64_t)a->rows * plan.nblk >= (int64_t)num_sms * 64 * 2 * K ? 2 : 1;
+  plan.warps = (plan.nblk + plan.rounds * K - 1) / (plan.rounds * K);
+  plan.sums = (float4*)a->ws;
+  plan.maxima = (uint32_t*)(plan.sums + (size_t)a->rows * plan.warps);
+  const int64_t ctas = ((int64_t)a->rows * plan.warps + 7) / 8;
+  if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  cudaError_t e = iris::launch_overlapped(logprobs_stream_kernel<In>, dim3((unsigned)ctas), dim3(256), 0, stream, *a, plan);
+  if (e != cudaSuccess) return e;
+  return iris::launch_overlapped(logprobs_finish_kernel<In>, dim3(a->rows), dim3(256), 0, stream, *a, plan);
 }
 
 extern "C" cudaError_t iris_launch_logprobs(const IrisLogprobs* a, int f32, int num_sms, cudaStream_t stream,
                                             int* launches) {
-  (void)num_sms;
-  *launches = 1;
-  if (f32)
-    logprobs_kernel<float><<<a->rows, 256, 0, stream>>>(*a);
-  else
-    logprobs_kernel<__nv_bfloat16><<<a->rows, 256, 0, stream>>>(*a);
-  return cudaGetLastError();
+  *launches = 2;
+  return f32 ? launch_logprobs<float>(a, num_sms, stream) : launch_logprobs<__nv_bfloat16>(a, num_sms, stream);
 }
