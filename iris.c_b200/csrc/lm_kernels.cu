@@ -482,7 +482,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 // values of a row lie in the k blocks with the largest maxima (each of k blocks
 // ahead of another one holds a value ahead of all of the other's), so the second
 // kernel reads those k blocks again and nothing else.
-constexpr int LP_BLOCK = 512;  // values; k of them are read twice: 4 % of a bf16 row of 151936 at k = 20, in L2
+// LP_BLOCK values a block: the second kernel reads vocab / LP_BLOCK maxima and k LP_BLOCK values, alike at
+// LP_BLOCK = sqrt(vocab / k), 87 for 151936 and k = 20; 256 is one load of the warp
+constexpr int LP_BLOCK = 256;
 constexpr int LP_LOADS = 8;    // 16-byte loads of a lane in flight
 
 template <typename In>
@@ -499,6 +501,7 @@ __device__ __forceinline__ uint32_t rank_bits(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);  // -0 counts as 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float rank_value(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r & 0x7FFFFFFFu : ~r); }
 __device__ __forceinline__ uint64_t place(uint32_t rank, uint32_t id) { return (uint64_t)rank << 32 | (uint32_t)~id; }
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
@@ -507,53 +510,39 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   return y;
 }
 
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  return v;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-
-// Two values x0, x1 into two sums each: d = x - base, e = 2^(d log2 e).
-__device__ __forceinline__ void add_pair(uint64_t x, uint64_t neg_base, uint64_t log2e, uint64_t& s1, uint64_t& s2) {
-  asm("{\n\t"
-      ".reg .b64 d, y, e;\n\t.reg .f32 y0, y1, e0, e1;\n\t"
-      "add.rn.f32x2 d, %2, %3;\n\t"
-      "mul.rn.f32x2 y, d, %4;\n\t"
-      "mov.b64 {y0, y1}, y;\n\t"
-      "ex2.approx.ftz.f32 e0, y0;\n\t"
-      "ex2.approx.ftz.f32 e1, y1;\n\t"
-      "mov.b64 e, {e0, e1};\n\t"
-      "add.rn.f32x2 %0, %0, e;\n\t"
-      "fma.rn.f32x2 %1, d, e, %1;\n\t}"
-      : "+l"(s1), "+l"(s2)
-      : "l"(x), "l"(neg_base), "l"(log2e));
-}
-
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Softmax sums against a reference m.
-struct LpSum {
-  float m, s1, s2;
-  // the same sums against mn >= m
-  __device__ __forceinline__ void raise(float mn) {
-    if (m != mn) {
-      if (m != -INFINITY) {
-        const float f = exp2_approx((m - mn) * kLog2e);
-        s2 = f == 0.f ? 0.f : f * (s2 + (m - mn) * s1);  // (m - mn) s1 may be infinite where f is 0
-        s1 = f * s1;
-      }
-      m = mn;
+// A value x into the sums: d = x - base, e = 2^(d log2 e).  In the second one d
+// is held at -1000 (e is 0 there), so that a value of -inf adds 0 and not 0 inf.
+// A NaN shows in the first.
+__device__ __forceinline__ void add_value(float x, float base, float& s1, float& s2) {
+  const float d = x - base, e = exp2_approx(d * kLog2e);
+  s1 += e;
+  s2 = fmaf(fmaxf(d, -1000.f), e, s2);
+}
+
+// Softmax sums against m, moved to mn >= m.
+__device__ __forceinline__ void raise(float& m, float& s1, float& s2, float mn) {
+  if (m != mn) {
+    if (m != -INFINITY) {
+      const float f = exp2_approx((m - mn) * kLog2e);
+      s2 = f == 0.f ? 0.f : f * (s2 + (m - mn) * s1);  // (m - mn) s1 may be infinite where f is 0
+      s1 = f * s1;
     }
+    m = mn;
   }
-};
+}
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
+}
+// over the warp, NaN if one is
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float y;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+  return y;
 }
 __device__ __forceinline__ float warp_add(float v) {
 #pragma unroll
@@ -561,13 +550,17 @@ __device__ __forceinline__ float warp_add(float v) {
   return v;
 }
 
-// The values at [e, e + kVec) of a row of `vocab` values, 16-byte aligned;
-// -inf where the row has none.  Nothing outside the row is read.
+// The values at [e, e + kVec) of a row of `vocab` <= 2^30 values, 16-byte
+// aligned; -inf where the row has none.  Nothing outside the row is read.
 template <typename In>
-__device__ __forceinline__ uint4 row_vec(const In* x, int64_t e, int vocab) {
+__device__ __forceinline__ uint4 row_vec(const In* x, int e, int vocab) {
   constexpr int VEC = 16 / sizeof(In);
   if (e >= 0 && e + VEC <= vocab) return __ldg(reinterpret_cast<const uint4*>(x + e));
   uint32_t w[4];
+  if (e >= vocab || e + VEC <= 0) {
+    w[0] = sizeof(In) == 4 ? 0xFF800000u : 0xFF80FF80u;
+    return make_uint4(w[0], w[0], w[0], w[0]);
+  }
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     if constexpr (sizeof(In) == 4) {
@@ -624,137 +617,134 @@ __global__ void __launch_bounds__(256) logprobs_stream_kernel(const __grid_const
                                                               const __grid_constant__ LpPlan plan) {
   using Sh = LpShape<In>;
   const int lane = threadIdx.x % 32;
-  const int64_t wid = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const uint32_t wid = blockIdx.x * 8 + threadIdx.x / 32;
   iris::grid_dep_wait();
   iris::grid_dep_launch();
-  const int64_t row = wid / plan.warps;
+  const int64_t row = wid / (uint32_t)plan.warps;
   if (row >= a.rows) return;
-  const int w = (int)(wid - row * plan.warps);
+  const int w = (int)(wid - (uint32_t)row * plan.warps);
   const In* x = (const In*)a.logits + row * a.ld;
   const int off = row_offset(x);
-  LpSum sum = {-INFINITY, 0.f, 0.f};
-  const uint64_t log2e = pair(kLog2e, kLog2e);
-  for (int r = 0; r < plan.rounds; r++) {
-    const int b0 = (w * plan.rounds + r) * Sh::kBlocks;
-    uint4 u[LP_LOADS];
-#pragma unroll
-    for (int j = 0; j < LP_LOADS; j++)
-      u[j] = row_vec(x, ((int64_t)b0 * LP_BLOCK - off) + (j * 32 + lane) * Sh::kVec, a.vocab);
-    uint32_t ranks = 0;
-#pragma unroll
-    for (int b = 0; b < Sh::kBlocks; b++) {
-      float cm = vec_max<In>(u[b * Sh::kPer]);
-#pragma unroll
-      for (int j = 1; j < Sh::kPer; j++) cm = max_nan(cm, vec_max<In>(u[b * Sh::kPer + j]));
-      if (a.top_k) {
-        const uint32_t best = __reduce_max_sync(0xffffffffu, rank_bits(cm));
-        if (lane == b) ranks = best;
-      }
-      if (cm > sum.m) sum.raise(cm);
-      const float base = sum.m == -INFINITY ? 0.f : sum.m;
-      const uint64_t nb = pair(-base, -base);
-      uint64_t s1 = 0, s2 = 0;  // two zeros each
-#pragma unroll
-      for (int j = 0; j < Sh::kPer; j++) {
-        float v[Sh::kVec];
-        vec_values<In>(u[b * Sh::kPer + j], v);
-#pragma unroll
-        for (int i = 0; i < Sh::kVec; i += 2) add_pair(pair(v[i], v[i + 1]), nb, log2e, s1, s2);
-      }
-      float p1, q1, p2, q2;
-      unpair(s1, p1, q1);
-      unpair(s2, p2, q2);
-      p2 += q2;
-      if (p2 != p2) {  // a value of -inf (0 times -inf), which adds 0, or one that spoils the row
-        p2 = 0.f;
-#pragma unroll
-        for (int j = 0; j < Sh::kPer; j++) {
-          float v[Sh::kVec];
-          vec_values<In>(u[b * Sh::kPer + j], v);
-#pragma unroll
-          for (int i = 0; i < Sh::kVec; i++) {
-            const float d = v[i] - base;
-            p2 += d == -INFINITY ? 0.f : d * exp2_approx(d * kLog2e);
-          }
-        }
-      }
-      sum.s1 += p1 + q1;
-      sum.s2 += p2;
+  float m = -INFINITY;                       // the warp's
+  float s1[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};  // the lane's
+  constexpr int STEP = LP_LOADS * 32 * Sh::kVec;  // values of a round
+  int b = w * plan.rounds * Sh::kBlocks + lane;   // the block whose maximum this lane writes
+  int e0 = w * plan.rounds * STEP - off;
+  uint32_t* maxima = plan.maxima + row * plan.nblk;
+  const bool keeps = a.top_k && lane < Sh::kBlocks;
+  for (int r = 0; r < plan.rounds; r++, b += Sh::kBlocks, e0 += STEP) {
+    if (e0 >= a.vocab) {  // blocks are counted for the row that begins furthest from a 16-byte boundary
+      if (keeps && b < plan.nblk) maxima[b] = 0u;
+      continue;
     }
-    if (a.top_k && lane < Sh::kBlocks && b0 + lane < plan.nblk) {
-      const bool any = (int64_t)(b0 + lane) * LP_BLOCK - off < a.vocab;
-      plan.maxima[row * plan.nblk + b0 + lane] = any ? ranks : 0u;
+    uint4 u[LP_LOADS];
+    if (e0 >= 0 && e0 + STEP <= a.vocab) {
+      const uint4* p = reinterpret_cast<const uint4*>(x + e0) + lane;
+#pragma unroll
+      for (int j = 0; j < LP_LOADS; j++) u[j] = __ldg(p + j * 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < LP_LOADS; j++) u[j] = row_vec(x, e0 + (j * 32 + lane) * Sh::kVec, a.vocab);
+    }
+    float best = 0.f, top = m;
+#pragma unroll
+    for (int i = 0; i < Sh::kBlocks; i++) {
+      float cm = vec_max<In>(u[i * Sh::kPer]);
+#pragma unroll
+      for (int j = 1; j < Sh::kPer; j++) cm = max_nan(cm, vec_max<In>(u[i * Sh::kPer + j]));
+      cm = warp_max_nan(cm);
+      if (lane == i) best = cm;
+      top = fmaxf(top, cm);
+    }
+    if (keeps && b < plan.nblk) maxima[b] = e0 + lane * LP_BLOCK < a.vocab ? rank_bits(best) : 0u;
+    if (top > m) {
+      float from = m;
+      raise(from, s1[0], s2[0], top);
+      raise(m, s1[1], s2[1], top);
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int j = 0; j < LP_LOADS; j++) {
+      float v[Sh::kVec];
+      vec_values<In>(u[j], v);
+#pragma unroll
+      for (int i = 0; i < Sh::kVec; i++) add_value(v[i], base, s1[i & 1], s2[i & 1]);
     }
   }
-  sum.raise(warp_max(sum.m));
-  const float s1 = warp_add(sum.s1), s2 = warp_add(sum.s2);
-  if (lane == 0) plan.sums[row * plan.warps + w] = make_float4(sum.m, s1, s2, 0.f);
+  const float t1 = warp_add(s1[0] + s1[1]), t2 = warp_add(s2[0] + s2[1]);
+  if (lane == 0) plan.sums[row * plan.warps + w] = make_float4(m, t1, t2, 0.f);
 }
 
 // The k largest of the places that items(f) hands to f (each thread its own
-// share of them, the same on every call; all different, 0 is none), largest
-// first, into best; returns how many there are.  A threshold that at least k
-// places reach is searched by halving over the threads' largest ones, which is
-// one barrier a step; the few places above it are then put in order by counting.
+// share of them, the same on every call; all different, none 0), largest first,
+// into best; returns how many there are.  `from`: where it is known that k
+// places reach it, else 0.  Without one the k-th largest of the threads' own
+// largest places is such a value (found by counting, as the order of the few
+// places that reach it).  Only where more than LP_LIST places do, many of the
+// largest in one thread's share, is a closer value searched by halving.
+constexpr int LP_LIST = 512, LP_THREADS = 128;
 struct TopK {
-  uint64_t list[1024], best[32];
+  __align__(16) uint64_t own[LP_THREADS];
+  uint64_t list[LP_LIST], best[32], from;
   int n;
   unsigned sum;
 };
 
 template <typename Items>
-__device__ int select_top(TopK& s, int k, Items items) {
-  constexpr int FEW = 48;  // enough; over k = 32
-  uint64_t own = 0;
-  items([&](uint64_t p) { own = p > own ? p : own; });
-  uint64_t lo = 1, hi = 0xFF800002ull << 32;
-  if (__syncthreads_count(own >= lo) > FEW)
-    while (true) {
-      const uint64_t mid = lo + (hi - lo) / 2;
-      const int c = __syncthreads_count(own >= mid);
-      if (c < k) {
-        hi = mid;
-      } else {
-        lo = mid;
-        if (c <= FEW) break;
-      }
+__device__ int select_top(TopK& s, int k, uint64_t from, Items items) {
+  const int tid = threadIdx.x;
+  if (!from) {
+    uint64_t own = 0;
+    items([&](uint64_t p) { own = p > own ? p : own; });
+    s.own[tid] = own;
+    if (tid == 0) s.from = 1;  // fewer than k threads have one
+    __syncthreads();
+    int ahead = 0;
+#pragma unroll 16
+    for (int j = 0; j < LP_THREADS; j += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&s.own[j]);
+      ahead += (two.x > own) + (two.y > own);
     }
-  // the places >= lo; where one thread holds many of them the halving goes on over all places
-  hi = 0xFF800002ull << 32;
+    if (own && ahead == k - 1) s.from = own;
+    __syncthreads();
+    from = s.from;
+  }
   while (true) {
-    if (threadIdx.x == 0) s.n = 0, s.sum = 0;
+    if (tid == 0) s.n = 0;
     __syncthreads();
     items([&](uint64_t p) {
-      if (p >= lo) {
+      if (p >= from) {
         const int at = atomicAdd(&s.n, 1);
-        if (at < 1024) s.list[at] = p;
+        if (at < LP_LIST) s.list[at] = p;
       }
     });
     __syncthreads();
-    if (s.n <= 1024) break;
+    if (s.n <= LP_LIST) break;
+    uint64_t hi = 0xFF800002ull << 32;  // over all places
     while (true) {
-      const uint64_t mid = lo + (hi - lo) / 2;
+      const uint64_t mid = from + (hi - from) / 2;
+      if (tid == 0) s.sum = 0;
+      __syncthreads();
       unsigned c = 0;
       items([&](uint64_t p) { c += p >= mid; });
       c = __reduce_add_sync(0xffffffffu, c);
-      if (threadIdx.x % 32 == 0) atomicAdd(&s.sum, c);
+      if (tid % 32 == 0) atomicAdd(&s.sum, c);
       __syncthreads();
       c = s.sum;
-      __syncthreads();
-      if (threadIdx.x == 0) s.sum = 0;
       __syncthreads();
       if (c < (unsigned)k) {
         hi = mid;
       } else {
-        lo = mid;
-        if (c <= 1024) break;
+        from = mid;
+        if (c <= LP_LIST) break;
       }
     }
   }
   const int n = s.n;
-  for (int c = threadIdx.x; c < n; c += 256) {
+  for (int c = tid; c < n; c += LP_THREADS) {
     const uint64_t p = s.list[c];
     int ahead = 0;
+#pragma unroll 8
     for (int j = 0; j < n; j++) ahead += s.list[j] > p;
     if (ahead < k) s.best[ahead] = p;
   }
@@ -763,77 +753,101 @@ __device__ int select_top(TopK& s, int k, Items items) {
 }
 
 // One block per row: the warps' sums joined, the outputs, the alternatives.
+// Bound by latency (a chain of three reads and some forty barriers).
 template <typename In>
-__global__ void __launch_bounds__(256) logprobs_finish_kernel(const __grid_constant__ IrisLogprobs a,
-                                                              const __grid_constant__ LpPlan plan) {
+__global__ void __launch_bounds__(LP_THREADS) logprobs_finish_kernel(const __grid_constant__ IrisLogprobs a,
+                                                                     const __grid_constant__ LpPlan plan) {
   using Sh = LpShape<In>;
+  constexpr int WARPS = LP_THREADS / 32, HELD = 5;
   __shared__ TopK top;
   __shared__ uint64_t blocks[32];
-  __shared__ float red[3][8];
+  __shared__ float red[3][WARPS];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   iris::grid_dep_wait();
   iris::grid_dep_launch();
   const In* x = (const In*)a.logits + row * a.ld;
-  LpSum sum = {-INFINITY, 0.f, 0.f};
-  for (int w = tid; w < plan.warps; w += 256) {
-    const float4 v = plan.sums[row * plan.warps + w];
-    LpSum other = {v.x, v.y, v.z};
-    const float m = fmaxf(sum.m, other.m);
-    sum.raise(m);
-    other.raise(m);
-    sum.s1 += other.s1;
-    sum.s2 += other.s2;
+  float given = 0.f;
+  bool has = false;
+  if (tid == 0 && a.logprob) {
+    const int t = a.targets[row];
+    has = t >= 0 && t < a.vocab;
+    if (has) {
+      if constexpr (sizeof(In) == 4) given = x[t];
+      else given = __bfloat162float(x[t]);
+    }
   }
-  float m = warp_max(sum.m);
-  if (tid % 32 == 0) red[0][tid / 32] = m;
+  uint32_t held[HELD];  // the first maxima, read with the sums
+  const uint32_t* maxima = plan.maxima + row * plan.nblk;
+#pragma unroll
+  for (int i = 0; i < HELD; i++) held[i] = a.top_k && tid + i * LP_THREADS < plan.nblk ? maxima[tid + i * LP_THREADS] : 0u;
+  float m = -INFINITY, s1 = 0.f, s2 = 0.f;
+  for (int w = tid; w < plan.warps; w += LP_THREADS) {
+    float4 v = plan.sums[row * plan.warps + w];
+    const float mn = fmaxf(m, v.x);
+    raise(m, s1, s2, mn);
+    raise(v.x, v.y, v.z, mn);
+    s1 += v.y;
+    s2 += v.z;
+  }
+  float mm = warp_max(m);
+  if (tid % 32 == 0) red[0][tid / 32] = mm;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; w++) m = fmaxf(m, red[0][w]);
-  sum.raise(m);
-  float s1 = warp_add(sum.s1), s2 = warp_add(sum.s2);
+  for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, red[0][w]);
+  raise(m, s1, s2, mm);
+  s1 = warp_add(s1), s2 = warp_add(s2);
   if (tid % 32 == 0) red[1][tid / 32] = s1, red[2][tid / 32] = s2;
   __syncthreads();
   s1 = s2 = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; w++) s1 += red[1][w], s2 += red[2][w];
-  auto value = [&](int64_t i) {
-    if constexpr (sizeof(In) == 4) return x[i];
-    else return __bfloat162float(x[i]);
-  };
+  for (int w = 0; w < WARPS; w++) s1 += red[1][w], s2 += red[2][w];
   const float log_s1 = logf(s1), lse = s1 == 0.f ? 0.f : m + log_s1;
   if (tid == 0) {
-    if (a.logprob) {
-      const int t = a.targets[row];
-      a.logprob[row] = t >= 0 && t < a.vocab ? value(t) - lse : 0.f;
-    }
+    if (a.logprob) a.logprob[row] = has ? given - lse : 0.f;
     if (a.entropy) a.entropy[row] = s1 == 0.f ? 0.f : log_s1 - s2 / s1;
   }
   if (!a.top_k) return;
-  const int nb = select_top(top, a.top_k, [&](auto f) {
-    for (int b = tid; b < plan.nblk; b += 256) {
-      const uint32_t r = plan.maxima[row * plan.nblk + b];
+  const int nb = select_top(top, a.top_k, 0, [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+      if (held[i]) f(place(held[i], tid + i * LP_THREADS));
+    for (int b = tid + HELD * LP_THREADS; b < plan.nblk; b += LP_THREADS) {
+      const uint32_t r = maxima[b];
       if (r) f(place(r, b));
     }
   });
   if (tid < nb) blocks[tid] = top.best[tid];
   __syncthreads();
+  // k blocks: each holds a value no less than the k-th maximum
+  const uint64_t from = nb == a.top_k ? blocks[nb - 1] >> 32 << 32 : 0;
   const int off = row_offset(x);
-  select_top(top, a.top_k, [&](auto f) {
-    constexpr int VPB = LP_BLOCK / Sh::kVec;
-    for (int j = tid; j < nb * VPB; j += 256) {
-      const int64_t e = (int64_t)(uint32_t)~(uint32_t)blocks[j / VPB] * LP_BLOCK - off + (j % VPB) * Sh::kVec;
-      float v[Sh::kVec];
-      vec_values<In>(row_vec(x, e, a.vocab), v);
+  select_top(top, a.top_k, from, [&](auto f) {
+    constexpr int VPB = LP_BLOCK / Sh::kVec, FLY = 5;
+    for (int j0 = tid; j0 < nb * VPB; j0 += FLY * LP_THREADS) {
+      uint4 u[FLY];
+      int e[FLY];
 #pragma unroll
-      for (int i = 0; i < Sh::kVec; i++)
-        if (e + i >= 0 && e + i < a.vocab) f(place(rank_bits(v[i]), (uint32_t)(e + i)));
+      for (int i = 0; i < FLY; i++) {
+        const int j = j0 + i * LP_THREADS;
+        e[i] = j < nb * VPB ? (int)~(uint32_t)blocks[j / VPB] * LP_BLOCK - off + j % VPB * Sh::kVec : a.vocab;
+        u[i] = row_vec(x, e[i], a.vocab);
+      }
+#pragma unroll
+      for (int i = 0; i < FLY; i++) {
+        if (rank_bits(vec_max<In>(u[i])) < (uint32_t)(from >> 32)) continue;
+        float v[Sh::kVec];
+        vec_values<In>(u[i], v);
+#pragma unroll
+        for (int q = 0; q < Sh::kVec; q++)
+          if (e[i] + q >= 0 && e[i] + q < a.vocab) f(place(rank_bits(v[q]), (uint32_t)(e[i] + q)));
+      }
     }
   });
   if (tid < a.top_k) {
-    const int id = (int)~(uint32_t)top.best[tid];
-    if (a.top_ids) a.top_ids[row * a.top_k + tid] = id;
-    if (a.top_logprobs) a.top_logprobs[row * a.top_k + tid] = value(id) - lse;
+    const uint64_t p = top.best[tid];
+    if (a.top_ids) a.top_ids[row * a.top_k + tid] = (int)~(uint32_t)p;
+    if (a.top_logprobs) a.top_logprobs[row * a.top_k + tid] = rank_value((uint32_t)(p >> 32)) - lse;
   }
 }
 
@@ -926,16 +940,18 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   LpPlan plan;
   plan.nblk = lp_blocks(a->vocab);
   constexpr int K = LpShape<In>::kBlocks;
-  // a warp's sums are joined once, so it takes two rounds of loads where that still leaves every SM some 64 warps
-  plan.rounds = (int64_t)a->rows * plan.nblk >= (int64_t)num_sms * 64 * 2 * K ? 2 : 1;
+  // a warp begins and ends with some 100 instructions, as many as 10 values of each lane: it takes up to 8 rounds
+  // of loads, as long as every SM is left three times the 32 warps that it holds
+  const int64_t rounds = (plan.nblk + K - 1) / K * (int64_t)a->rows / ((int64_t)num_sms * 32 * 3);
+  plan.rounds = rounds < 1 ? 1 : rounds > 8 ? 8 : (int)rounds;
   plan.warps = (plan.nblk + plan.rounds * K - 1) / (plan.rounds * K);
   plan.sums = (float4*)a->ws;
   plan.maxima = (uint32_t*)(plan.sums + (size_t)a->rows * plan.warps);
   const int64_t ctas = ((int64_t)a->rows * plan.warps + 7) / 8;
-  if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  if (ctas * 8 > 0xFFFFFFFFll) return cudaErrorInvalidConfiguration;  // more logits than any device holds
   cudaError_t e = iris::launch_overlapped(logprobs_stream_kernel<In>, dim3((unsigned)ctas), dim3(256), 0, stream, *a, plan);
   if (e != cudaSuccess) return e;
-  return iris::launch_overlapped(logprobs_finish_kernel<In>, dim3(a->rows), dim3(256), 0, stream, *a, plan);
+  return iris::launch_overlapped(logprobs_finish_kernel<In>, dim3(a->rows), dim3(LP_THREADS), 0, stream, *a, plan);
 }
 
 extern "C" cudaError_t iris_launch_logprobs(const IrisLogprobs* a, int f32, int num_sms, cudaStream_t stream,
