@@ -473,15 +473,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 
 // ------------------------------------------------------------------ log probabilities
 // Bound by the logits' bytes, and close behind by the exponentials (16 a clock
-// and SM: 0.72 of the bf16 stream's rate).  One pass: a warp reads LP_BLOCK
-// values at a time and keeps, per lane, the running maximum m and
+// and SM) and the instructions around them.  One pass, against the running
+// maximum m:
 //   s1 = sum e^(x - m),   s2 = sum (x - m) e^(x - m)
-// from which lse = m + log s1 and the entropy log s1 - s2 / s1.  A new maximum
-// m' turns them into f s1 and f (s2 + (m - m') s1), f = e^(m - m').  For the
-// alternatives it leaves the largest value of every block: the k largest
-// values of a row lie in the k blocks with the largest maxima (each of k blocks
-// ahead of another one holds a value ahead of all of the other's), so the second
-// kernel reads those k blocks again and nothing else.
+// from which log softmax x = (x - m) - log s1 and the entropy log s1 - s2 / s1.
+// A new maximum m' turns the sums into f s1 and f (s2 + (m - m') s1), f =
+// e^(m - m').  For the alternatives the pass leaves the largest value of every
+// block: the k largest values of a row lie in the k blocks with the largest
+// maxima (each of k blocks ahead of another one holds a value ahead of all of
+// the other's), so the second kernel reads those k blocks again and nothing else.
 // LP_BLOCK values a block: the second kernel reads vocab / LP_BLOCK maxima and k LP_BLOCK values, alike at
 // LP_BLOCK = sqrt(vocab / k), 87 for 151936 and k = 20; 256 is one load of the warp
 constexpr int LP_BLOCK = 256;
@@ -512,21 +512,40 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A value x into the sums: d = x - base, e = 2^(d log2 e).  In the second one d
-// is held at -1000 (e is 0 there), so that a value of -inf adds 0 and not 0 inf.
-// A NaN shows in the first.
-__device__ __forceinline__ void add_value(float x, float base, float& s1, float& s2) {
-  const float d = x - base, e = exp2_approx(d * kLog2e);
-  s1 += e;
-  s2 = fmaf(fmaxf(d, -1000.f), e, s2);
+// Two f32 in one register pair, for the packed instructions.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
-// Softmax sums against m, moved to mn >= m.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Sums against m, moved to mn >= m.
 __device__ __forceinline__ void raise(float& m, float& s1, float& s2, float mn) {
   if (m != mn) {
     if (m != -INFINITY) {
-      const float f = exp2_approx((m - mn) * kLog2e);
-      s2 = f == 0.f ? 0.f : f * (s2 + (m - mn) * s1);  // (m - mn) s1 may be infinite where f is 0
+      const float d = m - mn, f = exp2_approx(d * kLog2e);
+      s2 = f == 0.f ? 0.f : f * (s2 + d * s1);  // d s1 may be infinite where f is 0
       s1 = f * s1;
     }
     m = mn;
@@ -585,6 +604,25 @@ __device__ __forceinline__ void vec_values(uint4 u, float x[16 / sizeof(In)]) {
   }
 }
 
+// The same in pairs, -inf (and what is below it in f32's terms) as -1e37.
+template <typename In>
+__device__ __forceinline__ void vec_pairs(uint4 u, uint64_t x[8 / sizeof(In)]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (sizeof(In) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      x[i] = pair(max_nan(__uint_as_float(w[2 * i]), -1e37f), max_nan(__uint_as_float(w[2 * i + 1]), -1e37f));
+  } else {
+    const __nv_bfloat162 low = __floats2bfloat162_rn(-1e37f, -1e37f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const __nv_bfloat162 h = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), low);
+      const float2 f = unpack2(*reinterpret_cast<const uint32_t*>(&h));
+      x[i] = pair(f.x, f.y);
+    }
+  }
+}
+
 // The largest of the values, NaN if one is.
 template <typename In>
 __device__ __forceinline__ float vec_max(uint4 u) {
@@ -613,7 +651,7 @@ __device__ __forceinline__ int row_offset(const In* x) {
 }
 
 template <typename In>
-__global__ void __launch_bounds__(256) logprobs_stream_kernel(const __grid_constant__ IrisLogprobs a,
+__global__ void __launch_bounds__(256, 4) logprobs_stream_kernel(const __grid_constant__ IrisLogprobs a,
                                                               const __grid_constant__ LpPlan plan) {
   using Sh = LpShape<In>;
   const int lane = threadIdx.x % 32;
@@ -625,8 +663,8 @@ __global__ void __launch_bounds__(256) logprobs_stream_kernel(const __grid_const
   const int w = (int)(wid - (uint32_t)row * plan.warps);
   const In* x = (const In*)a.logits + row * a.ld;
   const int off = row_offset(x);
-  float m = -INFINITY;                       // the warp's
-  float s1[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};  // the lane's
+  float m = -INFINITY;                        // the warp's
+  uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};    // the lane's, two in each register pair
   constexpr int STEP = LP_LOADS * 32 * Sh::kVec;  // values of a round
   int b = w * plan.rounds * Sh::kBlocks + lane;   // the block whose maximum this lane writes
   int e0 = w * plan.rounds * STEP - off;
@@ -646,7 +684,7 @@ __global__ void __launch_bounds__(256) logprobs_stream_kernel(const __grid_const
 #pragma unroll
       for (int j = 0; j < LP_LOADS; j++) u[j] = row_vec(x, e0 + (j * 32 + lane) * Sh::kVec, a.vocab);
     }
-    float best = 0.f, top = m;
+    float best = 0.f, now = m;
 #pragma unroll
     for (int i = 0; i < Sh::kBlocks; i++) {
       float cm = vec_max<In>(u[i * Sh::kPer]);
@@ -654,60 +692,102 @@ __global__ void __launch_bounds__(256) logprobs_stream_kernel(const __grid_const
       for (int j = 1; j < Sh::kPer; j++) cm = max_nan(cm, vec_max<In>(u[i * Sh::kPer + j]));
       cm = warp_max_nan(cm);
       if (lane == i) best = cm;
-      top = fmaxf(top, cm);
+      now = fmaxf(now, cm);
     }
     if (keeps && b < plan.nblk) maxima[b] = e0 + lane * LP_BLOCK < a.vocab ? rank_bits(best) : 0u;
-    if (top > m) {
-      float from = m;
-      raise(from, s1[0], s2[0], top);
-      raise(m, s1[1], s2[1], top);
+    if (now > m) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        float2 u1 = halves(s1[i]), u2 = halves(s2[i]);
+        float from = m;
+        raise(from, u1.x, u2.x, now);
+        from = m;
+        raise(from, u1.y, u2.y, now);
+        s1[i] = pair(u1.x, u1.y), s2[i] = pair(u2.x, u2.y);
+      }
+      m = now;
     }
-    const float base = m == -INFINITY ? 0.f : m;
+    if (m > -1e36f) {
+      // 3 instructions a value and its exponential.  Values are held at -1e37 (under any such maximum e^(x - m) is 0
+      // there and below), so that one of -inf adds 0 and not 0 inf.
+      const uint64_t c = pair(kLog2e, kLog2e), nm = pair(-m, -m);
 #pragma unroll
-    for (int j = 0; j < LP_LOADS; j++) {
-      float v[Sh::kVec];
-      vec_values<In>(u[j], v);
+      for (int j = 0; j < LP_LOADS; j++) {
+        uint64_t x[Sh::kVec / 2];
+        vec_pairs<In>(u[j], x);
 #pragma unroll
-      for (int i = 0; i < Sh::kVec; i++) add_value(v[i], base, s1[i & 1], s2[i & 1]);
+        for (int i = 0; i < Sh::kVec / 2; i++) {
+          const uint64_t d = add2(x[i], nm);
+          const float2 y = halves(mul2(d, c));
+          const uint64_t e = pair(exp2_approx(y.x), exp2_approx(y.y));
+          s1[i & 1] = add2(s1[i & 1], e);
+          s2[i & 1] = fma2(d, e, s2[i & 1]);
+        }
+      }
+    } else {  // nothing but -inf and NaN so far, or next to the least value
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int j = 0; j < LP_LOADS; j++) {
+        float v[Sh::kVec];
+        vec_values<In>(u[j], v);
+        for (int i = 0; i < Sh::kVec; i++) {
+          const float d = v[i] - base, e = exp2_approx(d * kLog2e);
+          s1[0] = add2(s1[0], pair(e, 0.f));
+          s2[0] = add2(s2[0], pair(fmaxf(d, -1000.f) * e, 0.f));
+        }
+      }
     }
   }
-  const float t1 = warp_add(s1[0] + s1[1]), t2 = warp_add(s2[0] + s2[1]);
+  const float2 u1 = halves(add2(s1[0], s1[1])), u2 = halves(add2(s2[0], s2[1]));
+  const float t1 = warp_add(u1.x + u1.y), t2 = warp_add(u2.x + u2.y);
   if (lane == 0) plan.sums[row * plan.warps + w] = make_float4(m, t1, t2, 0.f);
 }
 
 // The k largest of the places that items(f) hands to f (each thread its own
 // share of them, the same on every call; all different, none 0), largest first,
 // into best; returns how many there are.  `from`: where it is known that k
-// places reach it, else 0.  Without one the k-th largest of the threads' own
-// largest places is such a value (found by counting, as the order of the few
-// places that reach it).  Only where more than LP_LIST places do, many of the
-// largest in one thread's share, is a closer value searched by halving.
-constexpr int LP_LIST = 512, LP_THREADS = 128;
+// places reach it, else 0.  Without one, every thread's largest place is ranked
+// against 32 of them, and the least of the 32 that k of them reach is such a
+// value.  The few places that reach it are put in order by counting.  Only
+// where more than LP_LIST do, many of the largest in one thread's share, is a
+// closer value searched by halving.
+constexpr int LP_LIST = 512;
+template <int THREADS>
 struct TopK {
-  __align__(16) uint64_t own[LP_THREADS];
-  uint64_t list[LP_LIST], best[32], from;
+  uint64_t own[THREADS], list[LP_LIST], best[32], pick[THREADS / 32];
+  int reach[THREADS / 32];
   int n;
   unsigned sum;
 };
 
-template <typename Items>
-__device__ int select_top(TopK& s, int k, uint64_t from, Items items) {
-  const int tid = threadIdx.x;
+template <int THREADS, typename Items>
+__device__ int select_top(TopK<THREADS>& s, int k, uint64_t from, Items items) {
+  constexpr int W = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   if (!from) {
     uint64_t own = 0;
     items([&](uint64_t p) { own = p > own ? p : own; });
     s.own[tid] = own;
-    if (tid == 0) s.from = 1;  // fewer than k threads have one
     __syncthreads();
-    int ahead = 0;
-#pragma unroll 16
-    for (int j = 0; j < LP_THREADS; j += 2) {
-      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&s.own[j]);
-      ahead += (two.x > own) + (two.y > own);
+    uint64_t o[W], pick = 1;  // 1: fewer than k threads have a place
+    int reach = THREADS + 1;
+#pragma unroll
+    for (int i = 0; i < W; i++) o[i] = s.own[i * 32 + lane];
+#pragma unroll
+    for (int j = 0; j < 32 / W; j++) {
+      const uint64_t c = s.own[(warp * (32 / W) + j) * W];
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < W; i++) n += o[i] >= c;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (c && n >= k && n < reach) pick = c, reach = n;
     }
-    if (own && ahead == k - 1) s.from = own;
+    if (lane == 0) s.pick[warp] = pick, s.reach[warp] = reach;
     __syncthreads();
-    from = s.from;
+    from = s.pick[0];
+    reach = s.reach[0];
+#pragma unroll
+    for (int i = 1; i < W; i++)
+      if (s.reach[i] < reach) from = s.pick[i], reach = s.reach[i];
   }
   while (true) {
     if (tid == 0) s.n = 0;
@@ -741,7 +821,7 @@ __device__ int select_top(TopK& s, int k, uint64_t from, Items items) {
     }
   }
   const int n = s.n;
-  for (int c = tid; c < n; c += LP_THREADS) {
+  for (int c = tid; c < n; c += THREADS) {
     const uint64_t p = s.list[c];
     int ahead = 0;
 #pragma unroll 8
@@ -754,12 +834,12 @@ __device__ int select_top(TopK& s, int k, uint64_t from, Items items) {
 
 // One block per row: the warps' sums joined, the outputs, the alternatives.
 // Bound by latency (a chain of three reads and some forty barriers).
-template <typename In>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_finish_kernel(const __grid_constant__ IrisLogprobs a,
+template <typename In, int THREADS>
+__global__ void __launch_bounds__(THREADS) logprobs_finish_kernel(const __grid_constant__ IrisLogprobs a,
                                                                      const __grid_constant__ LpPlan plan) {
   using Sh = LpShape<In>;
-  constexpr int WARPS = LP_THREADS / 32, HELD = 5;
-  __shared__ TopK top;
+  constexpr int WARPS = THREADS / 32, HELD = 5;
+  __shared__ TopK<THREADS> top;
   __shared__ uint64_t blocks[32];
   __shared__ float red[3][WARPS];
   const int64_t row = blockIdx.x;
@@ -780,9 +860,9 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_finish_kernel(const __gri
   uint32_t held[HELD];  // the first maxima, read with the sums
   const uint32_t* maxima = plan.maxima + row * plan.nblk;
 #pragma unroll
-  for (int i = 0; i < HELD; i++) held[i] = a.top_k && tid + i * LP_THREADS < plan.nblk ? maxima[tid + i * LP_THREADS] : 0u;
+  for (int i = 0; i < HELD; i++) held[i] = a.top_k && tid + i * THREADS < plan.nblk ? maxima[tid + i * THREADS] : 0u;
   float m = -INFINITY, s1 = 0.f, s2 = 0.f;
-  for (int w = tid; w < plan.warps; w += LP_THREADS) {
+  for (int w = tid; w < plan.warps; w += THREADS) {
     float4 v = plan.sums[row * plan.warps + w];
     const float mn = fmaxf(m, v.x);
     raise(m, s1, s2, mn);
@@ -802,17 +882,18 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_finish_kernel(const __gri
   s1 = s2 = 0.f;
 #pragma unroll
   for (int w = 0; w < WARPS; w++) s1 += red[1][w], s2 += red[2][w];
-  const float log_s1 = logf(s1), lse = s1 == 0.f ? 0.f : m + log_s1;
+  const float log_s1 = logf(s1);
+  auto log_softmax = [&](float x) { return s1 == 0.f ? -INFINITY : (x - m) - log_s1; };  // no sum: -inf alone
   if (tid == 0) {
-    if (a.logprob) a.logprob[row] = has ? given - lse : 0.f;
+    if (a.logprob) a.logprob[row] = has ? log_softmax(given) : 0.f;
     if (a.entropy) a.entropy[row] = s1 == 0.f ? 0.f : log_s1 - s2 / s1;
   }
   if (!a.top_k) return;
   const int nb = select_top(top, a.top_k, 0, [&](auto f) {
 #pragma unroll
     for (int i = 0; i < HELD; i++)
-      if (held[i]) f(place(held[i], tid + i * LP_THREADS));
-    for (int b = tid + HELD * LP_THREADS; b < plan.nblk; b += LP_THREADS) {
+      if (held[i]) f(place(held[i], tid + i * THREADS));
+    for (int b = tid + HELD * THREADS; b < plan.nblk; b += THREADS) {
       const uint32_t r = maxima[b];
       if (r) f(place(r, b));
     }
@@ -821,33 +902,34 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_finish_kernel(const __gri
   __syncthreads();
   // k blocks: each holds a value no less than the k-th maximum
   const uint64_t from = nb == a.top_k ? blocks[nb - 1] >> 32 << 32 : 0;
+  const float least = from ? rank_value((uint32_t)(from >> 32)) : -INFINITY;  // NaN: everything may reach it
   const int off = row_offset(x);
   select_top(top, a.top_k, from, [&](auto f) {
     constexpr int VPB = LP_BLOCK / Sh::kVec, FLY = 5;
-    for (int j0 = tid; j0 < nb * VPB; j0 += FLY * LP_THREADS) {
+    for (int j0 = tid; j0 < nb * VPB; j0 += FLY * THREADS) {
       uint4 u[FLY];
       int e[FLY];
 #pragma unroll
       for (int i = 0; i < FLY; i++) {
-        const int j = j0 + i * LP_THREADS;
+        const int j = j0 + i * THREADS;
         e[i] = j < nb * VPB ? (int)~(uint32_t)blocks[j / VPB] * LP_BLOCK - off + j % VPB * Sh::kVec : a.vocab;
         u[i] = row_vec(x, e[i], a.vocab);
       }
 #pragma unroll
       for (int i = 0; i < FLY; i++) {
-        if (rank_bits(vec_max<In>(u[i])) < (uint32_t)(from >> 32)) continue;
+        if (vec_max<In>(u[i]) < least) continue;
         float v[Sh::kVec];
         vec_values<In>(u[i], v);
 #pragma unroll
         for (int q = 0; q < Sh::kVec; q++)
-          if (e[i] + q >= 0 && e[i] + q < a.vocab) f(place(rank_bits(v[q]), (uint32_t)(e[i] + q)));
+          if (!(v[q] < least) && e[i] + q >= 0 && e[i] + q < a.vocab) f(place(rank_bits(v[q]), (uint32_t)(e[i] + q)));
       }
     }
   });
   if (tid < a.top_k) {
     const uint64_t p = top.best[tid];
     if (a.top_ids) a.top_ids[row * a.top_k + tid] = (int)~(uint32_t)p;
-    if (a.top_logprobs) a.top_logprobs[row * a.top_k + tid] = rank_value((uint32_t)(p >> 32)) - lse;
+    if (a.top_logprobs) a.top_logprobs[row * a.top_k + tid] = log_softmax(rank_value((uint32_t)(p >> 32)));
   }
 }
 
@@ -951,7 +1033,9 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   if (ctas * 8 > 0xFFFFFFFFll) return cudaErrorInvalidConfiguration;  // more logits than any device holds
   cudaError_t e = iris::launch_overlapped(logprobs_stream_kernel<In>, dim3((unsigned)ctas), dim3(256), 0, stream, *a, plan);
   if (e != cudaSuccess) return e;
-  return iris::launch_overlapped(logprobs_finish_kernel<In>, dim3(a->rows), dim3(LP_THREADS), 0, stream, *a, plan);
+  // 128 threads a row: 64 are 4 % faster at 2047 rows of 50021 and 8 alternatives, and at one row of 151936 and 20
+  // take 12.7 us for 8.6
+  return iris::launch_overlapped(logprobs_finish_kernel<In, 128>, dim3(a->rows), dim3(128), 0, stream, *a, plan);
 }
 
 extern "C" cudaError_t iris_launch_logprobs(const IrisLogprobs* a, int f32, int num_sms, cudaStream_t stream,
