@@ -426,7 +426,7 @@ cudaError_t iris_launch_add_bf16(void *out, const void *a, const void *b, long n
 
 /* ------------------------------------------------------------------ language-model operators (lm_kernels.cu)
  * Arguments as the public entry points of the same names, already checked. */
-#include "iris_cuda.h"
+#include "paged.h"
 typedef struct {
     iris_gpu_kv_cache_t cache;
     iris_gpu_rope_t rope;     /* rot_dim 0: no rotation */
@@ -448,12 +448,13 @@ typedef struct {
     int rows, heads;
     float scale;
     float *ws;
+    iris_paged_div_t div;     /* set by iris_launch_paged_attention */
 } IrisPagedAttention;
 /* one-time kernel attribute setup, called at library init */
 cudaError_t iris_lm_init(void);
 size_t iris_paged_attention_ws_bytes(const iris_gpu_kv_cache_t *cache, int heads, int num_sms);
 /* *launches = kernels queued */
-cudaError_t iris_launch_paged_attention(const IrisPagedAttention *a, int num_sms, cudaStream_t stream, int *launches);
+cudaError_t iris_launch_paged_attention(IrisPagedAttention *a, int num_sms, cudaStream_t stream, int *launches);
 typedef struct {
     const void *logits;
     int64_t ld;

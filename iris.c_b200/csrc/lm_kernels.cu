@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
   __syncthreads();
   const int nh = a.heads, nkv = a.cache.kv_heads, total = nh + 2 * nkv;
   const int lane = threadIdx.x % LPH, c0 = lane * 8;
-  const int page = iris_paged_page(&a.cache, seq, pos);
-  const int64_t slot = page < 0 ? -1 : iris_paged_offset(&a.cache, page, pos);
+  const int block = pos / a.cache.page_size, page = iris_paged_page(&a.cache, seq, block);
+  const int64_t slot = page < 0 ? -1 : iris_paged_offset(&a.cache, page, pos - block * a.cache.page_size);
   for (int h0 = blockIdx.y * GROUPS; h0 < total; h0 += gridDim.y * GROUPS) {
     const int h = h0 + threadIdx.x / LPH;
     const bool live = h < total, is_q = h < nh, is_k = !is_q && h < nh + nkv;
@@ -170,8 +170,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
 
 template <int HD>
 struct PagedShape {
-  static constexpr int kStages = HD == 64 ? 6 : 3;
-  static constexpr int kCtas = HD == 256 ? 1 : 2;                // resident per SM
+  static constexpr int kStages = HD == 64 ? 2 : 3;
+  static constexpr int kCtas = HD == 64 ? 4 : HD == 128 ? 2 : 1;  // resident per SM
   static constexpr int kStageBytes = 16 * HD * 2;                // 16 rows of K or of V
   static constexpr int kRing = kStages * 2 * kStageBytes;        // per warp
   static constexpr int kSlot = IRIS_PAGED_HEADS * (HD + 2);      // floats of a piece: m, l, then o
@@ -262,16 +262,20 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   // ---- loads, up to D - 1 stages ahead of the arithmetic
   iris_paged_at_t ld = at;
   int64_t to_load = count;
-  auto find_page = [&]() {  // of this lane's key (lanes 16-31 as lanes 0-15)
-    const int p = ld.i * IRIS_PAGED_TILE + warp * 16 + (lane & 15);
-    return p < ld.len ? iris_paged_page(&cache, ld.s, p) : -1;
+  int page, slot;                  // of this lane's key (lanes 16-31 as lanes 0-15) of the next tile to load
+  int64_t head = 0;                // its head's offset
+  auto find = [&]() {
+    const int p = ld.i * IRIS_PAGED_TILE + warp * 16 + (lane & 15), b = iris_paged_block(a.div, p);
+    slot = p - b * cache.page_size;
+    page = p < ld.len ? iris_paged_page(&cache, ld.s, b) : -1;
+    if (ld.i == 0) head = (int64_t)(ld.u / rtiles) * cache.head_stride;
   };
-  int page = find_page();
+  head = (int64_t)(ld.u / rtiles) * cache.head_stride;
+  find();
   auto issue = [&](int stage) {
     if (to_load > 0) {
-      const int p = ld.i * IRIS_PAGED_TILE + warp * 16 + (lane & 15);
       const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
-      const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, p) + (int64_t)(ld.u / rtiles) * cache.head_stride : 0;
+      const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
       if (lane == 0) seen[warp][stage] = have;
       const uint32_t kd = ring + stage * 2 * Sh::kStageBytes, vd = kd + Sh::kStageBytes;
       constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows one instruction of the warp covers
@@ -286,7 +290,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       }
       if (--to_load > 0) {
         iris_paged_next(&ld, units, &cache, a.seq, a.pos);
-        page = find_page();
+        find();
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -420,11 +424,11 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 // One block per (share border, query head of a unit): where the border is the
 // first inside its unit, the unit's pieces are added up, in order.
 template <int HD>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas) {
+__global__ void __launch_bounds__(HD * 2) paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas) {
   using Sh = PagedShape<HD>;
-  constexpr int COLS = HD / 4, PARTS = 256 / COLS;
+  constexpr int COLS = HD / 4, PARTS = 8;
   __shared__ float4 acc[PARTS][COLS];
-  __shared__ float wsum[PARTS], wmax[8];
+  __shared__ float wsum[PARTS], wmax[HD / 16];
   const int c = blockIdx.x + 1, h = blockIdx.y, tid = threadIdx.x;
   iris::grid_dep_wait();
   iris::grid_dep_launch();
@@ -437,13 +441,13 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   auto piece = [&](int p) { return slots + (size_t)(p == 0 ? 2 * c - 1 : 2 * (c + p - 1)) * Sh::kSlot; };
   const int n = join.z + 1;
   float mm = -INFINITY;
-  for (int p = tid; p < n; p += 256) mm = fmaxf(mm, piece(p)[2 * h]);
+  for (int p = tid; p < n; p += HD * 2) mm = fmaxf(mm, piece(p)[2 * h]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
   if (tid % 32 == 0) wmax[tid / 32] = mm;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; w++) mm = fmaxf(mm, wmax[w]);
+  for (int w = 0; w < HD / 16; w++) mm = fmaxf(mm, wmax[w]);
   const float base = mm == -INFINITY ? 0.f : mm;
   const int part = tid / COLS, col = tid % COLS;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -974,7 +978,7 @@ static cudaError_t launch_paged(const IrisPagedAttention* a, int num_sms, cudaSt
   const int group = a->heads / a->cache.kv_heads;
   *launches = 2;
   return iris::launch_overlapped(paged_join_kernel<HD>, dim3(ctas - 1, group < IRIS_PAGED_HEADS ? group : IRIS_PAGED_HEADS),
-                                 dim3(256), 0, stream, *a, ctas);
+                                 dim3(HD * 2), 0, stream, *a, ctas);
 }
 
 template <int HD>
@@ -988,8 +992,8 @@ extern "C" size_t iris_paged_attention_ws_bytes(const iris_gpu_kv_cache_t* cache
   return cache->head_dim == 64 ? paged_ws<64>(num_sms) : cache->head_dim == 128 ? paged_ws<128>(num_sms) : paged_ws<256>(num_sms);
 }
 
-extern "C" cudaError_t iris_launch_paged_attention(const IrisPagedAttention* a, int num_sms, cudaStream_t stream,
-                                                   int* launches) {
+extern "C" cudaError_t iris_launch_paged_attention(IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
+  a->div = iris_paged_div(a->cache.page_size);
   if (a->cache.head_dim == 64) return launch_paged<64>(a, num_sms, stream, launches);
   if (a->cache.head_dim == 128) return launch_paged<128>(a, num_sms, stream, launches);
   return launch_paged<256>(a, num_sms, stream, launches);

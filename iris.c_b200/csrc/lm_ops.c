@@ -212,7 +212,7 @@ int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const 
         lm_leave(&d, cudaSuccess, what, 0);
         return LM_FAIL("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
     }
-    IrisPagedAttention a = {*cache, out, q, ldo, ldq, seq, pos, rows, heads, scale, (float *)workspace};
+    IrisPagedAttention a = {*cache, out, q, ldo, ldq, seq, pos, rows, heads, scale, (float *)workspace, {0, 0}};
     int launches = 0;
     cudaError_t e = iris_launch_paged_attention(&a, g_rt.num_sms, (cudaStream_t)stream, &launches);
     return lm_leave(&d, e, what, launches);

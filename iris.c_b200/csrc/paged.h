@@ -55,17 +55,28 @@ IRIS_HD int iris_paged_row_tiles(const iris_gpu_kv_cache_t *c, const int32_t *se
     return iris_paged_seq(c, seq, t) < 0 ? 0 : iris_paged_tiles(iris_paged_len(c, pos[t]));
 }
 
-/* page of key p of sequence s, or -1 where the table or the pool has none */
-IRIS_HD int iris_paged_page(const iris_gpu_kv_cache_t *c, int s, int p) {
-    const int b = p / c->page_size;
+/* p / page_size for 0 <= p < 2^31 as p * mul >> shift: shift = 31 + ceil(log2 page_size), mul = ceil(2^shift /
+ * page_size) <= 2^32 - 1, and p (mul page_size - 2^shift) < 2^31 page_size <= 2^shift keeps the floor */
+typedef struct { uint32_t mul; int shift; } iris_paged_div_t;
+IRIS_HD iris_paged_div_t iris_paged_div(int page_size) {
+    iris_paged_div_t d;
+    d.shift = 31;
+    while (((uint64_t)1 << (d.shift - 31)) < (uint64_t)page_size) d.shift++;
+    d.mul = (uint32_t)((((uint64_t)1 << d.shift) + page_size - 1) / page_size);
+    return d;
+}
+IRIS_HD int iris_paged_block(iris_paged_div_t d, int p) { return (int)(((uint64_t)(uint32_t)p * d.mul) >> d.shift); }
+
+/* page of block b of sequence s, or -1 where the table or the pool has none */
+IRIS_HD int iris_paged_page(const iris_gpu_kv_cache_t *c, int s, int b) {
     if (b >= c->max_blocks) return -1;
     const int page = c->table[(int64_t)s * c->table_stride + b];
     return page >= 0 && page < c->num_pages ? page : -1;
 }
 
-/* element offset in the pools of key p (head 0) on `page` */
-IRIS_HD int64_t iris_paged_offset(const iris_gpu_kv_cache_t *c, int page, int p) {
-    return (int64_t)page * c->page_stride + (int64_t)(p % c->page_size) * c->token_stride;
+/* element offset in the pools of `slot` (head 0) of `page` */
+IRIS_HD int64_t iris_paged_offset(const iris_gpu_kv_cache_t *c, int page, int slot) {
+    return (int64_t)page * c->page_stride + (int64_t)slot * c->token_stride;
 }
 
 /* tiles in a share */

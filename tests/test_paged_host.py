@@ -118,10 +118,11 @@ static int pages(std::mt19937 &rng) {
     for (int j = 0; j < 400; j++) {
         const int s = pick(0, c.num_seqs - 1);
         const int p = j < 100 ? pick(0, (int)room + 200) : j == 100 ? 0x7FFFFFFF : pick(0, (int)room - 1);
-        const int page = iris_paged_page(&c, s, p);
+        const int block = iris_paged_block(iris_paged_div(c.page_size), p), page = iris_paged_page(&c, s, block);
+        CHECK(block == p / c.page_size);
         CHECK(page == (p < room ? good[s][p / c.page_size] : -1));
         if (page >= 0) {
-            const int64_t o = iris_paged_offset(&c, page, p);
+            const int64_t o = iris_paged_offset(&c, page, p - block * c.page_size);
             CHECK(o >= 0 && o < c.num_pages * c.page_stride && o % 512 == 0);
             CHECK(o == page * c.page_stride + (p % c.page_size) * c.token_stride);
         }
@@ -146,6 +147,17 @@ int main() {
     CHECK(iris_paged_len(&c, 0x7FFFFFFF) == 0x7FFFFFFF);
     CHECK(iris_paged_tiles(0x7FFFFFFF) == 33554432);
     CHECK(iris_paged_share((int64_t)33554432 * 4096, 296) * 296 >= (int64_t)33554432 * 4096);
+    // blocks of every position, pages of any size
+    for (int j = 0; j < 4000; j++) {
+        const int ps = j < 600 ? j + 1 : j < 660 ? (1 << (j - 600) / 2) - 1 + j % 2 : pick(1, 0x7FFFFFFF);
+        if (ps < 1) continue;
+        const iris_paged_div_t d = iris_paged_div(ps);
+        for (int i = 0; i < 60; i++) {
+            const int64_t m = (int64_t)ps * pick(0, 0x7FFFFFFF / ps) + (i % 3 - 1);
+            const int p = i == 0 ? 0x7FFFFFFF : i == 1 ? 0 : m < 0 || m > 0x7FFFFFFF ? pick(0, 0x7FFFFFFF) : (int)m;
+            CHECK(iris_paged_block(d, p) == p / ps);
+        }
+    }
     std::puts("ok");
     return 0;
 }
