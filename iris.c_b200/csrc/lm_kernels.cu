@@ -128,10 +128,12 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
 //   s = q k^T      mma m16n8k16, rows = up to 8 query heads of the head's group
 //   p = 2^(s c - m), c = scale log2(e);  l = l 2^(m_old - m) + sum p
 //   o = o 2^(m_old - m) + p v
-// The 8 unused rows of the second product carry what p loses to bf16: row g
-// holds bf16(p), row g + 8 holds bf16(p - bf16(p)), and the two halves of o are
-// added at the end, so that weights count with 16 bits at no extra instruction
-// (with 8 bits the result would be off by sqrt(2) of its own rounding).
+// p counts with 16 bits, bf16(p) + bf16(p - bf16(p)) (with 8 the result would be
+// off by sqrt(2) of its own rounding).  Up to 8 heads fill half of the product's
+// rows and the second parts the other half, at no extra instruction; the halves
+// of o are added at the end.  For 9 to 16 heads on a key-value head the second
+// part is a second product.  At head_dim 256 two warps share 16 keys and hold
+// half of o's columns each (all of them did not fit a warp's registers).
 // At a unit's end the four warps' sums are joined in shared memory and written,
 // or, where a share's border cuts the unit, left for the join kernel.
 
@@ -168,31 +170,47 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-template <int HD>
+// HD: head_dim.  MH: query heads of a unit (8 or 16).
+template <int HD, int MH>
 struct PagedShape {
-  static constexpr int kStages = HD == 64 ? 2 : 3;
-  static constexpr int kCtas = HD == 64 ? 4 : HD == 128 ? 2 : 1;  // resident per SM
+  static constexpr int kPair = HD / 128 ? HD / 128 : 1;          // warps on the same 16 keys, 128 columns of o each
+  static constexpr int kThreads = 128 * kPair;
+  // CTAs on an SM and stages of a ring, as measured on 256 rows of 0 to 2048 keys at head_dim 64 (14 heads on 2): 4 x 2
+  // 38 us, 3 x 4 40 us, 2 x 6 46 us (the arithmetic of 16 short keys is latency, and wants warps); at 128 and 256 a ring
+  // of three stages fills shared memory, with MH = 16 two
+  static constexpr int kCtas = HD == 64 ? 4 : HD == 128 ? 2 : 1;
+  static constexpr int kStages = HD == 64 || MH == 16 ? 2 : 3;
   static constexpr int kStageBytes = 16 * HD * 2;                // 16 rows of K or of V
-  static constexpr int kRing = kStages * 2 * kStageBytes;        // per warp
-  static constexpr int kSlot = IRIS_PAGED_HEADS * (HD + 2);      // floats of a piece: m, l, then o
+  static constexpr int kRing = kStages * 2 * kStageBytes;        // of 16 keys of a tile
+  static constexpr int kSlot = MH * (HD + 2);                    // floats of a piece: m, l, then o
   static constexpr int kSmem = 4 * kRing + 4 * kSlot * 4;
+  // column of o of head h in the sums of 16 keys in shared memory, which are laid out as a piece: the eight heads of a
+  // store's half warp fall into different banks
+  __device__ static int col(int h, int c) { return c ^ (h & 3) << 3; }
 };
 
 // Offset of the first slot in the workspace (floats), after the joins
 // {row, unit, later pieces, -} of every share
 __host__ __device__ __forceinline__ size_t paged_slots_at(int ctas) { return (size_t)ctas * 4; }
 
-template <int HD>
-__global__ void __launch_bounds__(128, PagedShape<HD>::kCtas)
+template <int HD, int MH>
+__global__ void __launch_bounds__(PagedShape<HD, MH>::kThreads, PagedShape<HD, MH>::kCtas)
 paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
-  using Sh = PagedShape<HD>;
+  using Sh = PagedShape<HD, MH>;
   constexpr int D = Sh::kStages, CH = HD / 8;  // CH: 16-byte chunks of a row
+  constexpr int PAIR = Sh::kPair, T = Sh::kThreads, W = T / 32, OC = HD / PAIR;  // OC: columns of o a warp holds
+  constexpr bool WIDE = MH == 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t scan[5];
+  __shared__ int64_t scan[W];
   __shared__ int64_t found_prefix;
   __shared__ int found_row;
-  __shared__ uint32_t seen[4][D];  // per warp and stage: which of its 16 keys exist
+  __shared__ uint32_t seen[4][D];  // of each 16 keys of a tile and stage: which exist
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, i4 = lane % 4;
+  const int kg = warp / PAIR, half = warp % PAIR;  // which 16 keys of a tile, which columns of o
+  auto sync_keys = [&]() {  // the warps on the same keys
+    if constexpr (PAIR == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * PAIR) : "memory");
+  };
   const iris_gpu_kv_cache_t& cache = a.cache;
   const int units = iris_paged_units(&cache, a.heads), group = a.heads / cache.kv_heads;
   iris::grid_dep_wait();
@@ -202,11 +220,11 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   for (int t = blockIdx.x; t < a.rows; t += gridDim.x)
     if (iris_paged_seq(&cache, a.seq, t) >= 0 && a.pos[t] < 0) {
       uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)t * a.ldo);
-      for (int c = tid; c < a.heads * CH; c += 128) o[c] = make_uint4(0u, 0u, 0u, 0u);
+      for (int c = tid; c < a.heads * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
     }
 
   // this share's first tile: prefix sums over the rows, a run of rows per thread
-  const int run = (a.rows + 127) / 128, r0 = min(a.rows, tid * run), r1 = min(a.rows, r0 + run);
+  const int run = (a.rows + T - 1) / T, r0 = min(a.rows, tid * run), r1 = min(a.rows, r0 + run);
   int64_t mine = 0;
   for (int t = r0; t < r1; t++) mine += iris_paged_row_tiles(&cache, a.seq, a.pos, t);
   int64_t incl = mine;
@@ -218,7 +236,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   if (lane == 31) scan[warp] = incl;
   __syncthreads();
   int64_t before = incl - mine, total = 0;
-  for (int w = 0; w < 4; w++) {
+  for (int w = 0; w < W; w++) {
     if (w < warp) before += scan[w];
     total += scan[w];
   }
@@ -256,7 +274,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   if (tid == 0) joins[blockIdx.x] = make_int4(at.t, at.u, iris_paged_join(&at, share), 0);
 
   const int rtiles = units / cache.kv_heads;
-  const uint32_t ring = iris::smem_u32(smem) + warp * Sh::kRing;
+  const uint32_t ring = iris::smem_u32(smem) + kg * Sh::kRing;
   float* red = reinterpret_cast<float*>(smem + 4 * Sh::kRing);
 
   // ---- loads, up to D - 1 stages ahead of the arithmetic
@@ -265,7 +283,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   int page, slot;                  // of this lane's key (lanes 16-31 as lanes 0-15) of the next tile to load
   int64_t head = 0;                // its head's offset
   auto find = [&]() {
-    const int p = ld.i * IRIS_PAGED_TILE + warp * 16 + (lane & 15), b = iris_paged_block(a.div, p);
+    const int p = ld.i * IRIS_PAGED_TILE + kg * 16 + (lane & 15), b = iris_paged_block(a.div, p);
     slot = p - b * cache.page_size;
     page = p < ld.len ? iris_paged_page(&cache, ld.s, b) : -1;
     if (ld.i == 0) head = (int64_t)(ld.u / rtiles) * cache.head_stride;
@@ -276,12 +294,12 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     if (to_load > 0) {
       const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
       const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
-      if (lane == 0) seen[warp][stage] = have;
+      if (half == 0 && lane == 0) seen[kg][stage] = have;
       const uint32_t kd = ring + stage * 2 * Sh::kStageBytes, vd = kd + Sh::kStageBytes;
       constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows one instruction of the warp covers
 #pragma unroll
-      for (int j = 0; j < 16 / RPI; j++) {
-        const int r = j * RPI + lane / CH, ch = lane % CH;
+      for (int j = 0; j < 16 / RPI / PAIR; j++) {
+        const int r = (j * PAIR + half) * RPI + lane / CH, ch = lane % CH;
         const int64_t o = __shfl_sync(0xffffffffu, off, r) + ch * 8;
         const int bytes = (have >> r) & 1 ? 16 : 0;
         const uint32_t d = r * (HD * 2) + ((ch ^ (r & 7)) << 4);
@@ -297,38 +315,45 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   };
   for (int s = 0; s < D - 1; s++) issue(s);
 
-  // ---- arithmetic
+  // ---- arithmetic.  Rows of the products: head g, and head g + 8 where MH is 16.
+  constexpr int R = WIDE ? 2 : 1;
   const float c = a.scale * 1.4426950408889634f;
-  uint32_t qf[HD / 16][2];
-  float o[HD / 8][4], m = -INFINITY, l = 0.f;
+  uint32_t qf[HD / 16][2 * R];
+  float o[OC / 8][4], m[R], l[R];
   int heads_here = 0, head0 = 0;
-  bool fresh = true, begun_here = false;
-  int stage = 0;
-  for (int64_t k = 0; k < count; k++) {
-    if (fresh) {
-      fresh = false;
-      begun_here = at.i == 0;
-      const int kvh = at.u / rtiles, r = at.u - kvh * rtiles;
-      head0 = kvh * group + r * IRIS_PAGED_HEADS;
-      heads_here = min(IRIS_PAGED_HEADS, group - r * IRIS_PAGED_HEADS);
-      const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)at.t * a.ldq + (int64_t)(head0 + g) * HD + 2 * i4;
+  auto begin_unit = [&]() {
+    const int kvh = at.u / rtiles, r = at.u - kvh * rtiles;
+    head0 = kvh * group + r * MH;
+    heads_here = min(MH, group - r * MH);
+    const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)at.t * a.ldq + (int64_t)(head0 + g) * HD + 2 * i4;
+#pragma unroll
+    for (int h = 0; h < R; h++) {
+      const bool live = g + 8 * h < heads_here;
 #pragma unroll
       for (int j = 0; j < HD / 16; j++) {
-        qf[j][0] = g < heads_here ? *reinterpret_cast<const uint32_t*>(q + j * 16) : 0u;
-        qf[j][1] = g < heads_here ? *reinterpret_cast<const uint32_t*>(q + j * 16 + 8) : 0u;
+        qf[j][h] = live ? *reinterpret_cast<const uint32_t*>(q + h * 8 * HD + j * 16) : 0u;
+        qf[j][R + h] = live ? *reinterpret_cast<const uint32_t*>(q + h * 8 * HD + j * 16 + 8) : 0u;
       }
-#pragma unroll
-      for (int j = 0; j < HD / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      m = -INFINITY;
-      l = 0.f;
+      m[h] = -INFINITY;
+      l[h] = 0.f;
     }
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (int j = 0; j < OC / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  };
+  begin_unit();
+  clear();
+  bool begun_here = at.i == 0;
+  int stage = 0;
+  for (int64_t k = 0; k < count; k++) {
     issue(stage == 0 ? D - 1 : stage - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
-    __syncwarp();
+    sync_keys();
     const uint32_t kd = ring + stage * 2 * Sh::kStageBytes, vd = kd + Sh::kStageBytes;
-    const uint32_t have = seen[warp][stage];
+    const uint32_t have = seen[kg][stage];
     if (have) {
-      // scores of 8 heads x 16 keys: s0 keys 2 i4, 2 i4 + 1, s1 the same + 8
+      // scores of a row and 16 keys: s0 keys 2 i4, 2 i4 + 1 (of head g, then of head g + 8), s1 the same + 8
       float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
       // matrices (keys 0-7, columns 0-7), (keys 0-7, 8-15), (keys 8-15, 0-7), (keys 8-15, 8-15) of each 16 columns
       const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
@@ -336,62 +361,96 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       for (int j = 0; j < HD / 16; j++) {
         uint32_t b[4];
         ldsm4(b, kd + kr * (HD * 2) + (((2 * j + kc) ^ (kr & 7)) << 4));
-        mma_bf16(s0, qf[j][0], 0u, qf[j][1], 0u, b[0], b[1]);
-        mma_bf16(s1, qf[j][0], 0u, qf[j][1], 0u, b[2], b[3]);
+        const uint32_t a1 = WIDE ? qf[j][1] : 0u, a3 = WIDE ? qf[j][2 * R - 1] : 0u;
+        mma_bf16(s0, qf[j][0], a1, qf[j][R], a3, b[0], b[1]);
+        mma_bf16(s1, qf[j][0], a1, qf[j][R], a3, b[2], b[3]);
       }
-      float x0 = s0[0] * c, x1 = s0[1] * c, x2 = s1[0] * c, x3 = s1[1] * c;
-      if (have != 0xFFFFu) {
-        const uint32_t hv = have >> (2 * i4);
-        if (!(hv & 1)) x0 = -INFINITY;
-        if (!(hv & 2)) x1 = -INFINITY;
-        if (!(hv & 0x100)) x2 = -INFINITY;
-        if (!(hv & 0x200)) x3 = -INFINITY;
-      }
-      float mn = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
-      mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
-      mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
-      mn = fmaxf(mn, m);
-      const float base = mn == -INFINITY ? 0.f : mn;  // scores of -inf weigh nothing
-      if (__any_sync(0xffffffffu, mn != m)) {
-        const float f = exp2_approx(m - base);
-        l *= f;
+      uint32_t hi[R][2], lo[R][2];
+      bool moved = false;
+      float f[R];
 #pragma unroll
-        for (int j = 0; j < HD / 8; j++) o[j][0] *= f, o[j][1] *= f, o[j][2] *= f, o[j][3] *= f;
-        m = mn;
+      for (int h = 0; h < R; h++) {
+        float x0 = s0[2 * h] * c, x1 = s0[2 * h + 1] * c, x2 = s1[2 * h] * c, x3 = s1[2 * h + 1] * c;
+        if (have != 0xFFFFu) {
+          const uint32_t hv = have >> (2 * i4);
+          if (!(hv & 1)) x0 = -INFINITY;
+          if (!(hv & 2)) x1 = -INFINITY;
+          if (!(hv & 0x100)) x2 = -INFINITY;
+          if (!(hv & 0x200)) x3 = -INFINITY;
+        }
+        float mn = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
+        mn = fmaxf(mn, m[h]);
+        const float base = mn == -INFINITY ? 0.f : mn;  // scores of -inf weigh nothing
+        f[h] = exp2_approx(m[h] - base);
+        moved |= mn != m[h];
+        m[h] = mn;
+        const float p0 = exp2_approx(x0 - base), p1 = exp2_approx(x1 - base), p2 = exp2_approx(x2 - base),
+                    p3 = exp2_approx(x3 - base);
+        l[h] = l[h] * f[h] + ((p0 + p1) + (p2 + p3));
+        hi[h][0] = pack2(p0, p1), hi[h][1] = pack2(p2, p3);
+        const float2 u0 = unpack2(hi[h][0]), u1 = unpack2(hi[h][1]);
+        lo[h][0] = pack2(p0 - u0.x, p1 - u0.y), lo[h][1] = pack2(p2 - u1.x, p3 - u1.y);
       }
-      const float p0 = exp2_approx(x0 - base), p1 = exp2_approx(x1 - base), p2 = exp2_approx(x2 - base),
-                  p3 = exp2_approx(x3 - base);
-      l += (p0 + p1) + (p2 + p3);
-      const uint32_t h0 = pack2(p0, p1), h1 = pack2(p2, p3);
-      const float2 u0 = unpack2(h0), u1 = unpack2(h1);
-      const uint32_t e0 = pack2(p0 - u0.x, p1 - u0.y), e1 = pack2(p2 - u1.x, p3 - u1.y);
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int j = 0; j < OC / 8; j++) {
+          o[j][0] *= f[0], o[j][1] *= f[0];
+          o[j][2] *= f[R - 1], o[j][3] *= f[R - 1];
+        }
+      }
       // transposed: (keys 0-7, columns 0-7), (keys 8-15, 0-7), (keys 0-7, 8-15), (keys 8-15, 8-15)
-      const int vr = lane & 15, vc = lane >> 4;
+      const int vr = lane & 15, vc = (lane >> 4) + half * (OC / 8);
 #pragma unroll
-      for (int j = 0; j < HD / 16; j++) {
+      for (int j = 0; j < OC / 16; j++) {
         uint32_t b[4];
         ldsm4t(b, vd + vr * (HD * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
-        mma_bf16(o[2 * j], h0, e0, h1, e1, b[0], b[1]);
-        mma_bf16(o[2 * j + 1], h0, e0, h1, e1, b[2], b[3]);
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          if constexpr (WIDE) {
+            mma_bf16(o[2 * j + n], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b[2 * n], b[2 * n + 1]);
+            mma_bf16(o[2 * j + n], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b[2 * n], b[2 * n + 1]);
+          } else {
+            mma_bf16(o[2 * j + n], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b[2 * n], b[2 * n + 1]);
+          }
+        }
       }
     }
-    __syncwarp();  // this stage is filled again by the next iteration's issue
+    sync_keys();  // this stage is filled again by the next iteration's issue
     stage = stage == D - 1 ? 0 : stage + 1;
     const bool ends = at.i == at.n - 1;
     if (ends || k == count - 1) {
-      // join the four warps' sums of this unit (or piece)
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      float* mine_f = red + warp * Sh::kSlot;
-      if (i4 == 0) mine_f[2 * g] = m, mine_f[2 * g + 1] = l;
+      // the sums of the tile's four key groups joined: this unit, or the piece of it that is here
+      float* mine_f = red + kg * Sh::kSlot;
 #pragma unroll
-      for (int j = 0; j < HD / 8; j++)
-        *reinterpret_cast<float2*>(mine_f + 2 * IRIS_PAGED_HEADS + g * HD + j * 8 + 2 * i4) =
-            make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
-      __syncthreads();
+      for (int h = 0; h < R; h++) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (half == 0 && i4 == 0) mine_f[2 * (g + 8 * h)] = m[h], mine_f[2 * (g + 8 * h) + 1] = l[h];
+      }
+      float* mine_o = mine_f + 2 * MH + g * HD;
+#pragma unroll
+      for (int j = 0; j < OC / 8; j++) {
+        float* to = mine_o + Sh::col(g, half * OC + j * 8 + 2 * i4);
+        if constexpr (WIDE) {
+          *reinterpret_cast<float2*>(to) = make_float2(o[j][0], o[j][1]);
+          *reinterpret_cast<float2*>(to + 8 * HD) = make_float2(o[j][2], o[j][3]);
+        } else {
+          *reinterpret_cast<float2*>(to) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
+        }
+      }
       const bool whole = ends && begun_here;
       float* slot = a.ws + paged_slots_at(gridDim.x) + (size_t)(2 * blockIdx.x + (begun_here ? 1 : 0)) * Sh::kSlot;
-      for (int e = tid; e < heads_here * (HD / 4); e += 128) {
+      __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)head0 * HD;
+      const int heads = heads_here;
+      if (k < count - 1) {  // the next unit's queries come while this one is joined
+        iris_paged_next(&at, units, &cache, a.seq, a.pos);
+        begin_unit();
+        begun_here = true;
+      }
+      __syncthreads();
+      for (int e = tid; e < heads * (HD / 4); e += T) {
         const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
         float mm = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -400,77 +459,78 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-          const float f = exp2_approx(red[w * Sh::kSlot + 2 * h] - base);
-          sum += f * red[w * Sh::kSlot + 2 * h + 1];
-          const float4 v = *reinterpret_cast<const float4*>(red + w * Sh::kSlot + 2 * IRIS_PAGED_HEADS + h * HD + col);
-          y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+          const float s = exp2_approx(red[w * Sh::kSlot + 2 * h] - base);
+          sum += s * red[w * Sh::kSlot + 2 * h + 1];
+          const float4 v = *reinterpret_cast<const float4*>(red + w * Sh::kSlot + 2 * MH + h * HD + Sh::col(h, col));
+          y.x += s * v.x, y.y += s * v.y, y.z += s * v.z, y.w += s * v.w;
         }
         if (whole) {
           const float r = sum == 0.f ? 0.f : 1.0f / sum;
-          *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)(head0 + h) * HD + col) =
-              make_uint2(pack2(y.x * r, y.y * r), pack2(y.z * r, y.w * r));
+          *reinterpret_cast<uint2*>(out + h * HD + col) = make_uint2(pack2(y.x * r, y.y * r), pack2(y.z * r, y.w * r));
         } else {
           if (col == 0) slot[2 * h] = mm, slot[2 * h + 1] = sum;
-          *reinterpret_cast<float4*>(slot + 2 * IRIS_PAGED_HEADS + h * HD + col) = y;
+          *reinterpret_cast<float4*>(slot + 2 * MH + h * HD + col) = y;
         }
       }
+      clear();
       __syncthreads();
-      fresh = true;
+    } else {
+      at.i++;
     }
-    if (k < count - 1) iris_paged_next(&at, units, &cache, a.seq, a.pos);
   }
 }
 
 // One block per (share border, query head of a unit): where the border is the
-// first inside its unit, the unit's pieces are added up, in order.
-template <int HD>
+// first inside its unit, the unit's pieces are added up, in order: piece p by
+// part p % PARTS of the block, the parts' sums at the end.  The first pieces are
+// read before it is known how many there are.
+template <int HD, int MH>
 __global__ void __launch_bounds__(HD * 2) paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas) {
-  using Sh = PagedShape<HD>;
+  using Sh = PagedShape<HD, MH>;
   constexpr int COLS = HD / 4, PARTS = 8;
   __shared__ float4 acc[PARTS][COLS];
-  __shared__ float wsum[PARTS], wmax[HD / 16];
-  const int c = blockIdx.x + 1, h = blockIdx.y, tid = threadIdx.x;
+  __shared__ float2 ml[PARTS];
+  const int c = blockIdx.x + 1, h = blockIdx.y, part = threadIdx.x / COLS, col = threadIdx.x % COLS;
+  const int units = iris_paged_units(&a.cache, a.heads), group = a.heads / a.cache.kv_heads;
   iris::grid_dep_wait();
   iris::grid_dep_launch();
+  const float* slots = a.ws + paged_slots_at(ctas);
+  auto place = [&](int p) { return slots + (size_t)(p == 0 ? 2 * c - 1 : min(2 * (c + p - 1), 2 * ctas - 1)) * Sh::kSlot; };
+  auto ml_of = [&](int p) { return *reinterpret_cast<const float2*>(place(p) + 2 * h); };
+  auto o_of = [&](int p) { return *reinterpret_cast<const float4*>(place(p) + 2 * MH + h * HD + col * 4); };
+  float m = -INFINITY, l = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float2 s, float4 v) {
+    const float mn = fmaxf(m, s.x), base = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2_approx(m - base), e = exp2_approx(s.x - base);
+    m = mn;
+    l = f * l + e * s.y;
+    y.x = f * y.x + e * v.x, y.y = f * y.y + e * v.y, y.z = f * y.z + e * v.z, y.w = f * y.w + e * v.w;
+  };
+  const float2 s0 = ml_of(part);
+  const float4 v0 = o_of(part);
   const int4 join = reinterpret_cast<const int4*>(a.ws)[c];
   if (join.z == 0) return;
-  const int units = iris_paged_units(&a.cache, a.heads), group = a.heads / a.cache.kv_heads;
   const int rtiles = units / a.cache.kv_heads, kvh = join.y / rtiles, r = join.y - kvh * rtiles;
-  if (h >= group - r * IRIS_PAGED_HEADS) return;
-  const float* slots = a.ws + paged_slots_at(ctas);
-  auto piece = [&](int p) { return slots + (size_t)(p == 0 ? 2 * c - 1 : 2 * (c + p - 1)) * Sh::kSlot; };
+  if (h >= group - r * MH) return;
   const int n = join.z + 1;
-  float mm = -INFINITY;
-  for (int p = tid; p < n; p += HD * 2) mm = fmaxf(mm, piece(p)[2 * h]);
+  if (part < n) add(s0, v0);
+  for (int p = part + PARTS; p < n; p += 4 * PARTS) {
+    float2 s[4];
+    float4 v[4];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  if (tid % 32 == 0) wmax[tid / 32] = mm;
-  __syncthreads();
+    for (int i = 0; i < 4; i++) s[i] = ml_of(min(p + i * PARTS, n - 1)), v[i] = o_of(min(p + i * PARTS, n - 1));
 #pragma unroll
-  for (int w = 0; w < HD / 16; w++) mm = fmaxf(mm, wmax[w]);
-  const float base = mm == -INFINITY ? 0.f : mm;
-  const int part = tid / COLS, col = tid % COLS;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-#pragma unroll 4
-  for (int p = part; p < n; p += PARTS) {
-    const float* s = piece(p);
-    const float f = exp2_approx(s[2 * h] - base);
-    const float4 v = *reinterpret_cast<const float4*>(s + 2 * IRIS_PAGED_HEADS + h * HD + col * 4);
-    sum += f * s[2 * h + 1];
-    y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+    for (int i = 0; i < 4; i++)
+      if (p + i * PARTS < n) add(s[i], v[i]);
   }
   acc[part][col] = y;
-  if (col == 0) wsum[part] = sum;
+  if (col == 0) ml[part] = make_float2(m, l);
   __syncthreads();
   if (part) return;
-  for (int p = 1; p < PARTS; p++) {
-    const float4 v = acc[p][col];
-    sum += wsum[p];
-    y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
-  }
-  const float f = sum == 0.f ? 0.f : 1.0f / sum;
-  const int head = kvh * group + r * IRIS_PAGED_HEADS + h;
+  for (int p = 1; p < PARTS; p++) add(ml[p], acc[p][col]);
+  const float f = l == 0.f ? 0.f : 1.0f / l;
+  const int head = kvh * group + r * MH + h;
   *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + (int64_t)join.x * a.ldo + (int64_t)head * HD + col * 4) =
       make_uint2(pack2(y.x * f, y.y * f), pack2(y.z * f, y.w * f));
 }
@@ -960,56 +1020,62 @@ extern "C" cudaError_t iris_launch_rope_append(const IrisRopeAppend* a, int f32,
 }
 
 // CTAs of an attention launch: as many as the device holds at once, no more than the tables have room for tiles
-template <int HD>
+template <int HD, int MH>
 static int paged_ctas(const iris_gpu_kv_cache_t* c, int heads, int64_t rows, int num_sms) {
-  const int64_t all = (int64_t)num_sms * PagedShape<HD>::kCtas;
+  const int64_t all = (int64_t)num_sms * PagedShape<HD, MH>::kCtas;
   const int64_t room = iris_paged_tiles(iris_paged_len(c, 0x7FFFFFFF));
   const int64_t most = rows * iris_paged_units(c, heads);
   return (int)(most >= all || most * room >= all ? all : most * room);
 }
 
-template <int HD>
-static cudaError_t launch_paged(const IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
-  const int ctas = paged_ctas<HD>(&a->cache, a->heads, a->rows, num_sms);
-  cudaError_t e = iris::launch_overlapped(paged_attention_kernel<HD>, dim3(ctas), dim3(128), PagedShape<HD>::kSmem,
-                                          stream, *a);
-  *launches = 1;
-  if (e != cudaSuccess || ctas == 1) return e;
-  const int group = a->heads / a->cache.kv_heads;
-  *launches = 2;
-  return iris::launch_overlapped(paged_join_kernel<HD>, dim3(ctas - 1, group < IRIS_PAGED_HEADS ? group : IRIS_PAGED_HEADS),
-                                 dim3(HD * 2), 0, stream, *a, ctas);
-}
+template <int HD, int MH>
+struct PagedLaunch {
+  using Sh = PagedShape<HD, MH>;
+  static size_t ws_bytes(int num_sms) {
+    const int ctas = num_sms * Sh::kCtas;
+    return (paged_slots_at(ctas) + (size_t)2 * ctas * Sh::kSlot) * sizeof(float);
+  }
+  static cudaError_t init() {
+    return cudaFuncSetAttribute(paged_attention_kernel<HD, MH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+  }
+  static cudaError_t launch(const IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
+    const int ctas = paged_ctas<HD, MH>(&a->cache, a->heads, a->rows, num_sms);
+    cudaError_t e = iris::launch_overlapped(paged_attention_kernel<HD, MH>, dim3(ctas), dim3(Sh::kThreads), Sh::kSmem,
+                                            stream, *a);
+    *launches = 1;
+    if (e != cudaSuccess || ctas == 1) return e;
+    const int group = a->heads / a->cache.kv_heads;
+    *launches = 2;
+    return iris::launch_overlapped(paged_join_kernel<HD, MH>, dim3(ctas - 1, group < MH ? group : MH), dim3(HD * 2), 0,
+                                   stream, *a, ctas);
+  }
+};
 
-template <int HD>
-static size_t paged_ws(int num_sms) {
-  const int ctas = num_sms * PagedShape<HD>::kCtas;
-  return (paged_slots_at(ctas) + (size_t)2 * ctas * PagedShape<HD>::kSlot) * sizeof(float);
+// f(PagedLaunch) of the variant for this cache and group of query heads
+template <typename F>
+static auto paged_variant(const iris_gpu_kv_cache_t* c, int heads, F f) {
+  const bool wide = iris_paged_heads(heads / c->kv_heads) == 16;
+  if (c->head_dim == 64) return wide ? f(PagedLaunch<64, 16>()) : f(PagedLaunch<64, 8>());
+  if (c->head_dim == 128) return wide ? f(PagedLaunch<128, 16>()) : f(PagedLaunch<128, 8>());
+  return wide ? f(PagedLaunch<256, 16>()) : f(PagedLaunch<256, 8>());
 }
 
 extern "C" size_t iris_paged_attention_ws_bytes(const iris_gpu_kv_cache_t* cache, int heads, int num_sms) {
-  (void)heads;
-  return cache->head_dim == 64 ? paged_ws<64>(num_sms) : cache->head_dim == 128 ? paged_ws<128>(num_sms) : paged_ws<256>(num_sms);
+  return paged_variant(cache, heads, [&](auto v) { return v.ws_bytes(num_sms); });
 }
 
 extern "C" cudaError_t iris_launch_paged_attention(IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
   a->div = iris_paged_div(a->cache.page_size);
-  if (a->cache.head_dim == 64) return launch_paged<64>(a, num_sms, stream, launches);
-  if (a->cache.head_dim == 128) return launch_paged<128>(a, num_sms, stream, launches);
-  return launch_paged<256>(a, num_sms, stream, launches);
+  return paged_variant(&a->cache, a->heads, [&](auto v) { return v.launch(a, num_sms, stream, launches); });
 }
 
 // dynamic shared memory limits, once per device, so that launches may be captured
 extern "C" cudaError_t iris_lm_init(void) {
-  cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       PagedShape<64>::kSmem);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(paged_attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             PagedShape<128>::kSmem);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(paged_attention_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             PagedShape<256>::kSmem);
-  return e;
+  const cudaError_t e[] = {PagedLaunch<64, 8>::init(),  PagedLaunch<64, 16>::init(),  PagedLaunch<128, 8>::init(),
+                           PagedLaunch<128, 16>::init(), PagedLaunch<256, 8>::init(), PagedLaunch<256, 16>::init()};
+  for (cudaError_t x : e)
+    if (x != cudaSuccess) return x;
+  return cudaSuccess;
 }
 
 static int lp_blocks(int vocab) { return (int)(((int64_t)vocab + 7 + LP_BLOCK - 1) / LP_BLOCK); }  // 7: row_offset at most

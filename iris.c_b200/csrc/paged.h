@@ -4,7 +4,7 @@
  * lies, and how the key tiles of all rows are shared out.
  *
  * Work is counted in tiles of IRIS_PAGED_TILE keys.  A unit is one row, one
- * key-value head and up to IRIS_PAGED_HEADS of the query heads on it; a row has
+ * key-value head and up to 8 or 16 of the query heads on it; a row has
  * `units` of them, each of as many tiles as the row's keys fill.  All tiles of
  * all rows stand in one line (row by row, unit by unit, tile by tile) that is
  * cut into equal shares, one per CTA, whatever the rows' lengths.  A unit cut
@@ -26,12 +26,15 @@
 #endif
 
 #define IRIS_PAGED_TILE 64
-#define IRIS_PAGED_HEADS 8
+
+/* query heads of a unit, where `group` of them share a key-value head: the 16 rows of a matrix instruction hold up to
+ * 8 heads twice (see the kernel) or up to 16 once, so that groups of up to 16 read the cache once */
+IRIS_HD int iris_paged_heads(int group) { return group > 8 ? 16 : 8; }
 
 /* units of a row */
 IRIS_HD int iris_paged_units(const iris_gpu_kv_cache_t *c, int heads) {
-    const int group = heads / c->kv_heads;
-    return c->kv_heads * ((group + IRIS_PAGED_HEADS - 1) / IRIS_PAGED_HEADS);
+    const int group = heads / c->kv_heads, n = iris_paged_heads(group);
+    return c->kv_heads * ((group + n - 1) / n);
 }
 
 /* sequence of row t, or -1 */

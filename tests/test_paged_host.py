@@ -32,7 +32,7 @@ static int shares(std::mt19937 &rng, int rows, int heads, int kv_heads, int long
         pos[t] = pick(0, 9) == 0 ? -pick(1, 3) : pick(0, 9) == 0 ? 0x7FFFFFFF : pick(0, longest);
     }
     const int units = iris_paged_units(&c, heads);
-    CHECK(units == kv_heads * ((heads / kv_heads + 7) / 8));
+    CHECK(units == kv_heads * (heads / kv_heads <= 16 ? 1 : (heads / kv_heads + 15) / 16));
     int64_t total = 0;
     std::vector<int> n(rows);
     for (int t = 0; t < rows; t++) {
