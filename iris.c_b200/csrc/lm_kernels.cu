@@ -223,10 +223,10 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       for (int c = tid; c < a.heads * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
     }
 
-  // this share's first tile: prefix sums over the rows, a run of rows per thread
+  // this share's first place: prefix sums over the rows, a run of rows per thread
   const int run = (a.rows + T - 1) / T, r0 = min(a.rows, tid * run), r1 = min(a.rows, r0 + run);
   int64_t mine = 0;
-  for (int t = r0; t < r1; t++) mine += iris_paged_row_tiles(&cache, a.seq, a.pos, t);
+  for (int t = r0; t < r1; t++) mine += iris_paged_row_places(&cache, a.seq, a.pos, t);
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -241,19 +241,21 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     total += scan[w];
   }
   total *= units;
-  const int64_t share = iris_paged_share(total, gridDim.x), start = blockIdx.x * share;
+  // (divisions in 32 bits where they do: 64-bit ones take a tenth of a microsecond each)
+  const int64_t share = total <= 0x7FFFFFFF ? iris_paged_share32((uint32_t)total, gridDim.x) : iris_paged_share(total, gridDim.x);
+  const int64_t start = blockIdx.x * share;
   int4* joins = reinterpret_cast<int4*>(a.ws);
   if (start >= total) {
     if (tid == 0) joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
   {
-    const int64_t x = start / units;  // before * units <= start < (before + mine) * units
+    const int64_t x = total <= 0x7FFFFFFF ? (uint32_t)start / (uint32_t)units : start / units;  // before * units <= start < (before + mine) * units
     if (before <= x && x < before + mine) {
       int t = r0;
       int64_t p = before;
       for (;; t++) {
-        const int n = iris_paged_row_tiles(&cache, a.seq, a.pos, t);
+        const int n = iris_paged_row_places(&cache, a.seq, a.pos, t);
         if (x < p + n) break;
         p += n;
       }
@@ -264,14 +266,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   __syncthreads();
   iris_paged_at_t at;
   at.t = found_row;
-  iris_paged_row(&at, &cache, a.seq, a.pos);
-  {
-    const int64_t rest = start - found_prefix * units;
-    at.u = (int)(rest / at.n);
-    at.i = (int)(rest - (int64_t)at.u * at.n);
-  }
-  const int64_t count = min(share, total - start);
-  if (tid == 0) joins[blockIdx.x] = make_int4(at.t, at.u, iris_paged_join(&at, share), 0);
+  const bool any = iris_paged_start(&at, start - found_prefix * units, min(share, total - start), units, &cache, a.seq, a.pos);
+  if (tid == 0) joins[blockIdx.x] = make_int4(at.t, at.u, any ? iris_paged_join(&at, share) : 0, 0);
+  if (!any) return;
 
   const int rtiles = units / cache.kv_heads;
   const uint32_t ring = iris::smem_u32(smem) + kg * Sh::kRing;
@@ -279,7 +276,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 
   // ---- loads, up to D - 1 stages ahead of the arithmetic
   iris_paged_at_t ld = at;
-  int64_t to_load = count;
+  bool loads = true;
   int page, slot;                  // of this lane's key (lanes 16-31 as lanes 0-15) of the next tile to load
   int64_t head = 0;                // its head's offset
   auto find = [&]() {
@@ -291,7 +288,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   head = (int64_t)(ld.u / rtiles) * cache.head_stride;
   find();
   auto issue = [&](int stage) {
-    if (to_load > 0) {
+    if (loads) {
       const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
       const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
       if (half == 0 && lane == 0) seen[kg][stage] = have;
@@ -306,7 +303,8 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         cp_async16(kd + d, (const __nv_bfloat16*)cache.k + o, bytes);
         cp_async16(vd + d, (const __nv_bfloat16*)cache.v + o, bytes);
       }
-      if (--to_load > 0) {
+      loads = iris_paged_more(&ld);
+      if (loads) {
         iris_paged_next(&ld, units, &cache, a.seq, a.pos);
         find();
       }
@@ -346,7 +344,8 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   clear();
   bool begun_here = at.i == 0;
   int stage = 0;
-  for (int64_t k = 0; k < count; k++) {
+  for (bool more = true; more;) {
+    more = iris_paged_more(&at);
     issue(stage == 0 ? D - 1 : stage - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
     sync_keys();
@@ -420,7 +419,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     sync_keys();  // this stage is filled again by the next iteration's issue
     stage = stage == D - 1 ? 0 : stage + 1;
     const bool ends = at.i == at.n - 1;
-    if (ends || k == count - 1) {
+    if (ends || !more) {
       // the sums of the tile's four key groups joined: this unit, or the piece of it that is here
       float* mine_f = red + kg * Sh::kSlot;
 #pragma unroll
@@ -444,7 +443,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       float* slot = a.ws + paged_slots_at(gridDim.x) + (size_t)(2 * blockIdx.x + (begun_here ? 1 : 0)) * Sh::kSlot;
       __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)head0 * HD;
       const int heads = heads_here;
-      if (k < count - 1) {  // the next unit's queries come while this one is joined
+      if (more) {  // the next unit's queries come while this one is joined
         iris_paged_next(&at, units, &cache, a.seq, a.pos);
         begin_unit();
         begun_here = true;
@@ -476,24 +475,51 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       __syncthreads();
     } else {
       at.i++;
+      at.left--;
     }
   }
 }
 
-// One block per (share border, query head of a unit): where the border is the
-// first inside its unit, the unit's pieces are added up, in order: piece p by
-// part p % PARTS of the block, the parts' sums at the end.  The first pieces are
-// read before it is known how many there are.
-template <int HD, int MH>
-__global__ void __launch_bounds__(HD * 2) paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas) {
+// Adds up the pieces of cut units.  A thread takes four columns of a head; where
+// those are fewer than the threads, the block has parts that take every
+// parts-th piece each and are added at the end.  Two ways to find the pieces:
+// many units, most of them in two pieces: a block per share border, which works
+// where its border is the first inside a unit, for all heads that fit, and
+// reads the first pieces before it knows how many there are; few units in many
+// pieces (FEW): a block per unit and head, which looks for the unit's first
+// border (one row, 16 heads on one of 128 and 131072 keys, 295 pieces: 63 us in
+// the first way).
+constexpr int JOIN_THREADS = 512;
+
+template <int HD, int MH, bool FEW>
+__global__ void __launch_bounds__(JOIN_THREADS)
+paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int per_block) {
   using Sh = PagedShape<HD, MH>;
-  constexpr int COLS = HD / 4, PARTS = 8;
-  __shared__ float4 acc[PARTS][COLS];
-  __shared__ float2 ml[PARTS];
-  const int c = blockIdx.x + 1, h = blockIdx.y, part = threadIdx.x / COLS, col = threadIdx.x % COLS;
+  constexpr int COLS = HD / 4;
+  __shared__ float4 acc[JOIN_THREADS];
+  __shared__ float2 ml[JOIN_THREADS / COLS];
+  __shared__ int border, pieces;
   const int units = iris_paged_units(&a.cache, a.heads), group = a.heads / a.cache.kv_heads;
+  const int width = per_block * COLS;  // threads of a part
+  const int parts = JOIN_THREADS / width, part = threadIdx.x / width, i = threadIdx.x - part * width;
+  const int h = blockIdx.y * per_block + i / COLS, col = i % COLS;
   iris::grid_dep_wait();
   iris::grid_dep_launch();
+  const bool works = part < parts && h < min(group, MH);
+  const int4* joins = reinterpret_cast<const int4*>(a.ws);
+  int c = blockIdx.x + 1, row = 0, unit = 0, n = 0;
+  if constexpr (FEW) {
+    row = blockIdx.x / units, unit = blockIdx.x - row * units;
+    if (threadIdx.x == 0) border = 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < ctas; b += JOIN_THREADS) {
+      const int4 j = joins[b];
+      if (j.z && j.x == row && j.y == unit) border = b, pieces = j.z + 1;
+    }
+    __syncthreads();
+    if (!border) return;
+    c = border, n = pieces;
+  }
   const float* slots = a.ws + paged_slots_at(ctas);
   auto place = [&](int p) { return slots + (size_t)(p == 0 ? 2 * c - 1 : min(2 * (c + p - 1), 2 * ctas - 1)) * Sh::kSlot; };
   auto ml_of = [&](int p) { return *reinterpret_cast<const float2*>(place(p) + 2 * h); };
@@ -507,31 +533,37 @@ __global__ void __launch_bounds__(HD * 2) paged_join_kernel(const __grid_constan
     l = f * l + e * s.y;
     y.x = f * y.x + e * v.x, y.y = f * y.y + e * v.y, y.z = f * y.z + e * v.z, y.w = f * y.w + e * v.w;
   };
-  const float2 s0 = ml_of(part);
-  const float4 v0 = o_of(part);
-  const int4 join = reinterpret_cast<const int4*>(a.ws)[c];
-  if (join.z == 0) return;
-  const int rtiles = units / a.cache.kv_heads, kvh = join.y / rtiles, r = join.y - kvh * rtiles;
-  if (h >= group - r * MH) return;
-  const int n = join.z + 1;
-  if (part < n) add(s0, v0);
-  for (int p = part + PARTS; p < n; p += 4 * PARTS) {
-    float2 s[4];
-    float4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) s[i] = ml_of(min(p + i * PARTS, n - 1)), v[i] = o_of(min(p + i * PARTS, n - 1));
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (p + i * PARTS < n) add(s[i], v[i]);
+  float2 s0 = make_float2(0.f, 0.f);
+  float4 v0 = y;
+  if (works) s0 = ml_of(part), v0 = o_of(part);
+  if constexpr (!FEW) {
+    const int4 j = joins[c];
+    if (j.z == 0) return;
+    row = j.x, unit = j.y, n = j.z + 1;
   }
-  acc[part][col] = y;
-  if (col == 0) ml[part] = make_float2(m, l);
-  __syncthreads();
-  if (part) return;
-  for (int p = 1; p < PARTS; p++) add(ml[p], acc[p][col]);
+  const int rtiles = units / a.cache.kv_heads, kvh = unit / rtiles, r = unit - kvh * rtiles;
+  const bool live = works && h < group - r * MH;
+  if (live && part < n) add(s0, v0);
+  if (live)
+    for (int p = part + parts; p < n; p += 4 * parts) {
+      float2 s[4];
+      float4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) s[j] = ml_of(min(p + j * parts, n - 1)), v[j] = o_of(min(p + j * parts, n - 1));
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (p + j * parts < n) add(s[j], v[j]);
+    }
+  if (parts > 1) {
+    acc[threadIdx.x] = y;
+    if (col == 0) ml[threadIdx.x / COLS] = make_float2(m, l);
+    __syncthreads();
+    for (int p = 1; part == 0 && p < parts && p < n; p++) add(ml[(p * width + i) / COLS], acc[p * width + i]);
+  }
+  if (part || !live) return;
   const float f = l == 0.f ? 0.f : 1.0f / l;
   const int head = kvh * group + r * MH + h;
-  *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + (int64_t)join.x * a.ldo + (int64_t)head * HD + col * 4) =
+  *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + (int64_t)row * a.ldo + (int64_t)head * HD + col * 4) =
       make_uint2(pack2(y.x * f, y.y * f), pack2(y.z * f, y.w * f));
 }
 
@@ -1023,7 +1055,7 @@ extern "C" cudaError_t iris_launch_rope_append(const IrisRopeAppend* a, int f32,
 template <int HD, int MH>
 static int paged_ctas(const iris_gpu_kv_cache_t* c, int heads, int64_t rows, int num_sms) {
   const int64_t all = (int64_t)num_sms * PagedShape<HD, MH>::kCtas;
-  const int64_t room = iris_paged_tiles(iris_paged_len(c, 0x7FFFFFFF));
+  const int64_t room = iris_paged_tiles(iris_paged_len(c, 0x7FFFFFFF)) + IRIS_PAGED_EXTRA;
   const int64_t most = rows * iris_paged_units(c, heads);
   return (int)(most >= all || most * room >= all ? all : most * room);
 }
@@ -1046,8 +1078,14 @@ struct PagedLaunch {
     if (e != cudaSuccess || ctas == 1) return e;
     const int group = a->heads / a->cache.kv_heads;
     *launches = 2;
-    return iris::launch_overlapped(paged_join_kernel<HD, MH>, dim3(ctas - 1, group < MH ? group : MH), dim3(HD * 2), 0,
-                                   stream, *a, ctas);
+    const int h = group < MH ? group : MH, fit = JOIN_THREADS / (HD / 4);
+    const int64_t all = (int64_t)a->rows * iris_paged_units(&a->cache, a->heads);
+    if (all * 8 <= ctas)
+      return iris::launch_overlapped(paged_join_kernel<HD, MH, true>, dim3((unsigned)all, h), dim3(JOIN_THREADS), 0, stream, *a,
+                                     ctas, 1);
+    const int per_block = h < fit ? h : fit;
+    return iris::launch_overlapped(paged_join_kernel<HD, MH, false>, dim3(ctas - 1, (h + per_block - 1) / per_block),
+                                   dim3(JOIN_THREADS), 0, stream, *a, ctas, per_block);
   }
 };
 

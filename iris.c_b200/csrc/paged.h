@@ -7,7 +7,9 @@
  * key-value head and up to 8 or 16 of the query heads on it; a row has
  * `units` of them, each of as many tiles as the row's keys fill.  All tiles of
  * all rows stand in one line (row by row, unit by unit, tile by tile) that is
- * cut into equal shares, one per CTA, whatever the rows' lengths.  A unit cut
+ * cut into equal shares, one per CTA, whatever the rows' lengths.  To begin and
+ * finish a unit takes a CTA about as long as a tile, so that every unit has one
+ * empty place in the line behind its tiles (IRIS_PAGED_EXTRA).  A unit cut
  * by a share's border is summed in pieces: a CTA leaves at most two, slot 2 c
  * for a piece whose unit began in an earlier share, slot 2 c + 1 for one that
  * begins here and goes on.
@@ -26,6 +28,7 @@
 #endif
 
 #define IRIS_PAGED_TILE 64
+#define IRIS_PAGED_EXTRA 1
 
 /* query heads of a unit, where `group` of them share a key-value head: the 16 rows of a matrix instruction hold up to
  * 8 heads twice (see the kernel) or up to 16 once, so that groups of up to 16 read the cache once */
@@ -53,9 +56,10 @@ IRIS_HD int iris_paged_len(const iris_gpu_kv_cache_t *c, int pos) {
 
 IRIS_HD int iris_paged_tiles(int len) { return len / IRIS_PAGED_TILE + (len % IRIS_PAGED_TILE != 0); }
 
-/* tiles of one unit of row t */
-IRIS_HD int iris_paged_row_tiles(const iris_gpu_kv_cache_t *c, const int32_t *seq, const int32_t *pos, int t) {
-    return iris_paged_seq(c, seq, t) < 0 ? 0 : iris_paged_tiles(iris_paged_len(c, pos[t]));
+/* places in the line of one unit of row t */
+IRIS_HD int iris_paged_row_places(const iris_gpu_kv_cache_t *c, const int32_t *seq, const int32_t *pos, int t) {
+    const int n = iris_paged_seq(c, seq, t) < 0 ? 0 : iris_paged_tiles(iris_paged_len(c, pos[t]));
+    return n ? n + IRIS_PAGED_EXTRA : 0;
 }
 
 /* p / page_size for 0 <= p < 2^31 as p * mul >> shift: shift = 31 + ceil(log2 page_size), mul = ceil(2^shift /
@@ -82,11 +86,13 @@ IRIS_HD int64_t iris_paged_offset(const iris_gpu_kv_cache_t *c, int page, int sl
     return (int64_t)page * c->page_stride + (int64_t)slot * c->token_stride;
 }
 
-/* tiles in a share */
+/* places in a share */
 IRIS_HD int64_t iris_paged_share(int64_t total, int ctas) { return total <= ctas ? 1 : (total + ctas - 1) / ctas; }
+IRIS_HD uint32_t iris_paged_share32(uint32_t total, uint32_t ctas) { return total <= ctas ? 1 : (total - 1) / ctas + 1; }
 
-/* A place in the line of tiles. */
+/* A place in the line. */
 typedef struct {
+    int64_t left; /* places of the share from this one on */
     int t;        /* row                          */
     int s, len;   /* its sequence and visible keys */
     int n;        /* tiles of each of its units   */
@@ -100,10 +106,12 @@ IRIS_HD void iris_paged_row(iris_paged_at_t *a, const iris_gpu_kv_cache_t *c, co
     a->n = iris_paged_tiles(a->len);
 }
 
-/* the next tile (there is one) */
-IRIS_HD void iris_paged_next(iris_paged_at_t *a, int units, const iris_gpu_kv_cache_t *c, const int32_t *seq,
+/* whether another tile of the share comes after this one, and which */
+IRIS_HD int iris_paged_more(const iris_paged_at_t *a) {
+    return a->i + 1 < a->n ? a->left > 1 : a->left > 1 + IRIS_PAGED_EXTRA;
+}
+IRIS_HD void iris_paged_unit(iris_paged_at_t *a, int units, const iris_gpu_kv_cache_t *c, const int32_t *seq,
                              const int32_t *pos) {
-    if (++a->i < a->n) return;
     a->i = 0;
     if (++a->u < units) return;
     a->u = 0;
@@ -111,6 +119,30 @@ IRIS_HD void iris_paged_next(iris_paged_at_t *a, int units, const iris_gpu_kv_ca
         a->t++;
         iris_paged_row(a, c, seq, pos);
     } while (a->n == 0);
+}
+IRIS_HD void iris_paged_next(iris_paged_at_t *a, int units, const iris_gpu_kv_cache_t *c, const int32_t *seq,
+                             const int32_t *pos) {
+    a->left--;
+    if (++a->i < a->n) return;
+    a->left -= IRIS_PAGED_EXTRA;
+    iris_paged_unit(a, units, c, seq, pos);
+}
+
+/* The first tile at or after place `rest` of row a->t's units, of a share of
+ * `left` places from there; 0 if the share has none. */
+IRIS_HD int iris_paged_start(iris_paged_at_t *a, int64_t rest, int64_t left, int units, const iris_gpu_kv_cache_t *c,
+                             const int32_t *seq, const int32_t *pos) {
+    iris_paged_row(a, c, seq, pos);
+    const int places = a->n + IRIS_PAGED_EXTRA;
+    a->u = rest <= 0x7FFFFFFF ? (int)((uint32_t)rest / (uint32_t)places) : (int)(rest / places);
+    a->i = (int)(rest - (int64_t)a->u * places);
+    a->left = left;
+    if (a->i < a->n) return 1;
+    const int skip = places - a->i;  /* empty places */
+    if (left <= skip) return 0;
+    a->left -= skip;
+    iris_paged_unit(a, units, c, seq, pos);
+    return 1;
 }
 
 /* Share c begins at tile `at.i` of a unit.  The number of later shares that

@@ -33,17 +33,19 @@ static int shares(std::mt19937 &rng, int rows, int heads, int kv_heads, int long
     }
     const int units = iris_paged_units(&c, heads);
     CHECK(units == kv_heads * (heads / kv_heads <= 16 ? 1 : (heads / kv_heads + 15) / 16));
-    int64_t total = 0;
+    int64_t total = 0, tiles = 0;
     std::vector<int> n(rows);
     for (int t = 0; t < rows; t++) {
-        n[t] = iris_paged_row_tiles(&c, seq.data(), pos.data(), t);
+        n[t] = iris_paged_row_places(&c, seq.data(), pos.data(), t);
         const bool live = seq[t] >= 0 && seq[t] < c.num_seqs && pos[t] >= 0;
         CHECK((n[t] > 0) == live);
-        CHECK(!live || (int64_t)(n[t] - 1) * IRIS_PAGED_TILE < (int64_t)c.max_blocks * c.page_size);
+        const int real = n[t] ? n[t] - IRIS_PAGED_EXTRA : 0;
+        CHECK(!live || (real > 0 && (int64_t)(real - 1) * IRIS_PAGED_TILE < (int64_t)c.max_blocks * c.page_size));
         total += (int64_t)n[t] * units;
+        tiles += (int64_t)real * units;
     }
     const int64_t share = iris_paged_share(total, ctas);
-    CHECK(share * ctas >= total);
+    CHECK(share * ctas >= total && share == iris_paged_share32((uint32_t)total, ctas));
     std::set<std::tuple<int, int, int>> done;                 // row, unit, tile
     std::map<std::pair<int, int>, std::set<int>> pieces;      // unit -> slots left
     std::map<std::pair<int, int>, int> whole, joined;
@@ -54,9 +56,8 @@ static int shares(std::mt19937 &rng, int rows, int heads, int kv_heads, int long
         iris_paged_at_t at = {};
         int64_t before = 0;
         while (start >= before + (int64_t)n[at.t] * units) before += (int64_t)n[at.t++] * units;
-        iris_paged_row(&at, &c, seq.data(), pos.data());
-        at.u = (int)((start - before) / at.n);
-        at.i = (int)((start - before) % at.n);
+        const int64_t mine = share < total - start ? share : total - start;
+        if (!iris_paged_start(&at, start - before, mine, units, &c, seq.data(), pos.data())) continue;
         if (const int later = iris_paged_join(&at, share)) {
             CHECK(cta > 0);
             joined[{at.t, at.u}]++;
@@ -64,22 +65,22 @@ static int shares(std::mt19937 &rng, int rows, int heads, int kv_heads, int long
             w.insert(2 * cta - 1);
             for (int p = 0; p < later; p++) w.insert(2 * (cta + p));
         }
-        const int64_t count = share < total - start ? share : total - start;
         bool fresh = true, begun = false;
-        for (int64_t k = 0; k < count; k++) {
-            CHECK(at.t < rows && at.u < units && at.i < at.n && at.s == seq[at.t]);
+        for (bool more = true; more;) {
+            more = iris_paged_more(&at);
+            CHECK(at.t < rows && at.u < units && at.i < at.n && at.s == seq[at.t] && at.left > 0);
             if (fresh) begun = at.i == 0, fresh = false;
             CHECK(done.insert({at.t, at.u, at.i}).second);
             const bool ends = at.i == at.n - 1;
-            if (ends || k == count - 1) {
+            if (ends || !more) {
                 if (ends && begun) whole[{at.t, at.u}]++;
                 else CHECK((pieces[{at.t, at.u}].insert(2 * cta + (begun ? 1 : 0)).second));
                 fresh = true;
             }
-            if (k < count - 1) iris_paged_next(&at, units, &c, seq.data(), pos.data());
+            if (more) iris_paged_next(&at, units, &c, seq.data(), pos.data());
         }
     }
-    CHECK((int64_t)done.size() == total);
+    CHECK((int64_t)done.size() == tiles);
     for (auto &p : pieces) {
         CHECK(whole.find(p.first) == whole.end());
         CHECK(joined[p.first] == 1);
