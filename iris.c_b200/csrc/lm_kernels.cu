@@ -216,15 +216,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   iris::grid_dep_wait();
   iris::grid_dep_launch();
 
-  // rows that see nothing give zeros
-  for (int t = blockIdx.x; t < a.rows; t += gridDim.x)
-    if (iris_paged_seq(&cache, a.seq, t) >= 0 && a.pos[t] < 0) {
-      uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)t * a.ldo);
-      for (int c = tid; c < a.heads * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
-    }
-
-  // this share's first place: prefix sums over the rows, a run of rows per thread
-  const int run = (a.rows + T - 1) / T, r0 = min(a.rows, tid * run), r1 = min(a.rows, r0 + run);
+  // this share's first place: prefix sums over the rows, a run of rows per thread (up to 32 rows: in each warp by itself)
+  const bool few = a.rows <= 32;
+  const int run = (a.rows + T - 1) / T, r0 = min(a.rows, (few ? lane : tid) * run), r1 = min(a.rows, r0 + run);
   int64_t mine = 0;
   for (int t = r0; t < r1; t++) mine += iris_paged_row_places(&cache, a.seq, a.pos, t);
   int64_t incl = mine;
@@ -233,40 +227,59 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) scan[warp] = incl;
-  __syncthreads();
   int64_t before = incl - mine, total = 0;
-  for (int w = 0; w < W; w++) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
+  if (few) {
+    total = __shfl_sync(0xffffffffu, incl, 31);
+  } else {
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    for (int w = 0; w < W; w++) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
   }
   total *= units;
   // (divisions in 32 bits where they do: 64-bit ones take a tenth of a microsecond each)
   const int64_t share = total <= 0x7FFFFFFF ? iris_paged_share32((uint32_t)total, gridDim.x) : iris_paged_share(total, gridDim.x);
   const int64_t start = blockIdx.x * share;
   int4* joins = reinterpret_cast<int4*>(a.ws);
+  // rows that see nothing give zeros
+  for (int t = blockIdx.x; t < a.rows; t += gridDim.x)
+    if (iris_paged_seq(&cache, a.seq, t) >= 0 && a.pos[t] < 0) {
+      uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)t * a.ldo);
+      for (int c = tid; c < a.heads * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
+    }
   if (start >= total) {
     if (tid == 0) joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
+  iris_paged_at_t at;
+  int64_t prefix;
   {
     const int64_t x = total <= 0x7FFFFFFF ? (uint32_t)start / (uint32_t)units : start / units;  // before * units <= start < (before + mine) * units
-    if (before <= x && x < before + mine) {
-      int t = r0;
-      int64_t p = before;
-      for (;; t++) {
-        const int n = iris_paged_row_places(&cache, a.seq, a.pos, t);
-        if (x < p + n) break;
-        p += n;
+    const bool here = before <= x && x < before + mine;
+    if (few) {
+      const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;  // run is 1: lane t holds row t
+      at.t = from;
+      prefix = __shfl_sync(0xffffffffu, before, from);
+    } else {
+      if (here) {
+        int t = r0;
+        int64_t p = before;
+        for (;; t++) {
+          const int n = iris_paged_row_places(&cache, a.seq, a.pos, t);
+          if (x < p + n) break;
+          p += n;
+        }
+        found_row = t;
+        found_prefix = p;
       }
-      found_row = t;
-      found_prefix = p;
+      __syncthreads();
+      at.t = found_row;
+      prefix = found_prefix;
     }
   }
-  __syncthreads();
-  iris_paged_at_t at;
-  at.t = found_row;
-  const bool any = iris_paged_start(&at, start - found_prefix * units, min(share, total - start), units, &cache, a.seq, a.pos);
+  const bool any = iris_paged_start(&at, start - prefix * units, min(share, total - start), units, &cache, a.seq, a.pos);
   if (tid == 0) joins[blockIdx.x] = make_int4(at.t, at.u, any ? iris_paged_join(&at, share) : 0, 0);
   if (!any) return;
 
@@ -486,9 +499,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 // many units, most of them in two pieces: a block per share border, which works
 // where its border is the first inside a unit, for all heads that fit, and
 // reads the first pieces before it knows how many there are; few units in many
-// pieces (FEW): a block per unit and head, which looks for the unit's first
-// border (one row, 16 heads on one of 128 and 131072 keys, 295 pieces: 63 us in
-// the first way).
+// pieces (FEW): a block per unit and head, which works out the unit's borders from
+// the rows' lengths while the attention kernel runs (one row, 16 heads on one of
+// 128 and 131072 keys, 295 pieces: 63 us in the first way, 22 in the second).
 constexpr int JOIN_THREADS = 512;
 
 template <int HD, int MH, bool FEW>
@@ -498,27 +511,33 @@ paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int pe
   constexpr int COLS = HD / 4;
   __shared__ float4 acc[JOIN_THREADS];
   __shared__ float2 ml[JOIN_THREADS / COLS];
-  __shared__ int border, pieces;
   const int units = iris_paged_units(&a.cache, a.heads), group = a.heads / a.cache.kv_heads;
   const int width = per_block * COLS;  // threads of a part
   const int parts = JOIN_THREADS / width, part = threadIdx.x / width, i = threadIdx.x - part * width;
   const int h = blockIdx.y * per_block + i / COLS, col = i % COLS;
-  iris::grid_dep_wait();
-  iris::grid_dep_launch();
   const bool works = part < parts && h < min(group, MH);
   const int4* joins = reinterpret_cast<const int4*>(a.ws);
   int c = blockIdx.x + 1, row = 0, unit = 0, n = 0;
   if constexpr (FEW) {
+    // the rows are the attention kernel's inputs: nothing that still runs writes them
     row = blockIdx.x / units, unit = blockIdx.x - row * units;
-    if (threadIdx.x == 0) border = 0;
-    __syncthreads();
-    for (int b = threadIdx.x; b < ctas; b += JOIN_THREADS) {
-      const int4 j = joins[b];
-      if (j.z && j.x == row && j.y == unit) border = b, pieces = j.z + 1;
+    int64_t begin = 0, total = 0;
+    int places = 0;
+    for (int t = 0; t < a.rows; t++) {
+      const int n_t = iris_paged_row_places(&a.cache, a.seq, a.pos, t);
+      if (t < row) begin += n_t;
+      if (t == row) places = n_t;
+      total += n_t;
     }
-    __syncthreads();
-    if (!border) return;
-    c = border, n = pieces;
+    begin = begin * units + (int64_t)unit * places;
+    if (places) n = iris_paged_cut(begin, places - IRIS_PAGED_EXTRA, iris_paged_share(total * units, ctas), &c);
+    iris::grid_dep_wait();
+    iris::grid_dep_launch();
+    if (!n) return;
+    n++;
+  } else {
+    iris::grid_dep_wait();
+    iris::grid_dep_launch();
   }
   const float* slots = a.ws + paged_slots_at(ctas);
   auto place = [&](int p) { return slots + (size_t)(p == 0 ? 2 * c - 1 : min(2 * (c + p - 1), 2 * ctas - 1)) * Sh::kSlot; };

@@ -153,4 +153,12 @@ IRIS_HD int iris_paged_join(const iris_paged_at_t *at, int64_t share) {
     return (int)((at->n - at->i + share - 1) / share);
 }
 
+/* The same from the unit: its first tile is place `begin` of the line, n tiles.
+ * Returns the number of later shares that hold pieces of it, *border the first. */
+IRIS_HD int iris_paged_cut(int64_t begin, int n, int64_t share, int *border) {
+    const int64_t c = begin / share + 1, over = begin + n - c * share;
+    *border = (int)c;
+    return over > 0 ? (int)((over + share - 1) / share) : 0;
+}
+
 #endif

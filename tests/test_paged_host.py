@@ -88,6 +88,17 @@ static int shares(std::mt19937 &rng, int rows, int heads, int kv_heads, int long
         for (int slot : p.second) CHECK(slot >= 0 && slot < 2 * ctas);
     }
     CHECK(pieces.size() == wanted.size());
+    int64_t begin = 0;
+    for (int t = 0; t < rows; t++)
+        for (int u = 0; n[t] && u < units; u++, begin += n[t]) {
+            int border = 0;
+            const int later = iris_paged_cut(begin, n[t] - IRIS_PAGED_EXTRA, share, &border);
+            CHECK((later > 0) == (wanted.count({t, u}) > 0));
+            if (!later) continue;
+            std::set<int> slots = {2 * border - 1};
+            for (int p = 0; p < later; p++) slots.insert(2 * (border + p));
+            CHECK((wanted[{t, u}] == slots));
+        }
     for (int t = 0; t < rows; t++)
         for (int u = 0; n[t] && u < units; u++) CHECK(whole.count({t, u}) + pieces.count({t, u}) == 1);
     return 0;
