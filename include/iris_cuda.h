@@ -741,7 +741,8 @@ int iris_gpu_rope_init_freqs(iris_gpu_rope_t *rope, int layout, int rot_dim, con
  * sequence seq[t].  Q and K: RMSNorm per head with q_norm / k_norm [head_dim]
  * (each may be NULL: none), then the rotation (rope NULL: none); f32 inside,
  * rounded once to bf16.  Q goes to q_out[t] [heads, head_dim] (bf16, rows
- * ldq_out apart; may be q itself), K and V to their slots.  heads may be 0
+ * ldq_out apart; may be q itself, in bf16 with its row stride), K and V to
+ * their slots.  heads may be 0
  * (q, q_out NULL).  A token with seq[t] outside [0, num_seqs) or pos[t] < 0 is
  * padding: nothing of it is written.  One past the table's end or with a page
  * number outside the pool gets its q_out and no slot.  Two tokens of one call

@@ -437,8 +437,9 @@ typedef struct {
     float eps;
     const int32_t *seq, *pos;
     int tokens, heads;
+    iris_paged_div_t div;     /* set by iris_launch_rope_append */
 } IrisRopeAppend;
-cudaError_t iris_launch_rope_append(const IrisRopeAppend *a, int f32, int num_sms, cudaStream_t stream);
+cudaError_t iris_launch_rope_append(IrisRopeAppend *a, int f32, int num_sms, cudaStream_t stream);
 typedef struct {
     iris_gpu_kv_cache_t cache;
     void *out;

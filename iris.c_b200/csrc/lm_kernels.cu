@@ -21,99 +21,117 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float x[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const float2 a = unpack2(u.x), b = unpack2(u.y), c = unpack2(u.z), d = unpack2(u.w);
-  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
-}
-
-__device__ __forceinline__ void load8(const float* p, float x[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-
 // ------------------------------------------------------------------ rotary positions into the cache
-// One block per token and slice of its heads.  The angles of a token are the
-// same for all its heads, so the block evaluates them once: pair i turns by
-// pos * turns[i] (64-bit, wrapping at a whole turn), whose top 32 bits as a
-// signed fraction of a half turn go to sincospi.  Then HD / 8 lanes take a
-// head, 8 columns each: norm by a shuffle reduction over them, the half
-// layout's partner columns by one shuffle (rot_dim / 2 is a multiple of 8).
+// Bound by the bytes of Q, K and V, in once and out once.  One block per token
+// and slice of its heads; HD / 8 lanes take a head, two runs of 4 columns each:
+// the two sides of the same 4 pairs in the half layout, neighbouring runs in the
+// interleaved one and behind rot_dim, so that a lane turns its pairs alone and
+// has the same angles for every head.  The angles are evaluated once for the
+// block: pair i turns by pos * turns[i] (64-bit, wrapping at a whole turn), whose
+// top 32 bits as a signed fraction of a half turn go to sincospi.  A lane reads
+// the first ROPE_HEADS of its heads before anything else, so that the chain
+// position -> page -> slot and the angles come at no time of their own.
+// Measured on 8191 tokens of 32 + 8 + 8 heads of 128, f32 (302 MB, 46.5 us at
+// the measured copy rate): 49.5 us with blocks of 64, 52.8 with 128, 57.3 with
+// 256 (the instructions per block and per head are half of the time's issue
+// slots); one warp per token and slice 57.0; eight columns in a row to a lane,
+// partners by shuffle and angles from shared memory for every head 82.
+constexpr int ROPE_HEADS = 4, ROPE_THREADS = 64;
+
+__device__ __forceinline__ float4 values4(uint4 u) {
+  return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+}
+__device__ __forceinline__ float4 values4(uint2 u) {
+  const float2 a = unpack2(u.x), b = unpack2(u.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+template <typename In> struct Raw4 { using T = uint4; };
+template <> struct Raw4<__nv_bfloat16> { using T = uint2; };
+
+// (a, b) of four pairs turned: the pairs' first and second values
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+  const float u = a * c - b * s;
+  b = a * s + b * c;
+  a = u;
+}
+
 template <typename In, int HD>
-__global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ IrisRopeAppend a) {
-  constexpr int LPH = HD / 8, GROUPS = 256 / LPH;
+__global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_constant__ IrisRopeAppend a) {
+  constexpr int LPH = HD / 8, GROUPS = ROPE_THREADS / LPH;
+  using Raw = typename Raw4<In>::T;
   __shared__ __align__(16) float cs[128], sn[128];
   const int t = blockIdx.x;
+  const int nh = a.heads, nkv = a.cache.kv_heads, total = nh + 2 * nkv;
+  const int rd = a.rope.rot_dim, lane = threadIdx.x % LPH;
+  const bool turned = lane < rd / 8, halves = a.rope.layout == IRIS_ROPE_HALF && turned;
+  const int ca = halves ? lane * 4 : lane * 8, cb = halves ? rd / 2 + lane * 4 : lane * 8 + 4;
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  const In* q = (const In*)a.q + (int64_t)t * a.ldq;
+  const In* k = (const In*)a.k + (int64_t)t * a.ldk - nh * HD;
+  const In* v = (const In*)a.v + (int64_t)t * a.ldv - (nh + nkv) * HD;
+  auto row = [&](int h) { return (h < nh ? q : h < nh + nkv ? k : v) + h * HD; };
+  const int first = blockIdx.y * GROUPS + threadIdx.x / LPH, step = gridDim.y * GROUPS;
   const int seq = a.seq[t], pos = a.pos[t];
+  Raw ra[ROPE_HEADS], rb[ROPE_HEADS];
+#pragma unroll
+  for (int i = 0; i < ROPE_HEADS; i++) {
+    ra[i] = rb[i] = Raw();
+    if (first + i * step < total) {
+      const In* x = row(first + i * step);
+      ra[i] = *reinterpret_cast<const Raw*>(x + ca);
+      rb[i] = *reinterpret_cast<const Raw*>(x + cb);
+    }
+  }
   if (seq < 0 || seq >= a.cache.num_seqs || pos < 0) return;
-  const int rd = a.rope.rot_dim;
-  for (int i = threadIdx.x; i < rd / 2; i += 256) {
+  const int block = iris_paged_block(a.div, pos), page = iris_paged_page(&a.cache, seq, block);
+  for (int i = threadIdx.x; i < rd / 2; i += ROPE_THREADS) {
     const uint64_t turn = (uint64_t)pos * a.rope.turns[i];
     float s, c;
     sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
     cs[i] = c * a.rope.amplitude;
     sn[i] = s * a.rope.amplitude;
   }
-  __syncthreads();
-  const int nh = a.heads, nkv = a.cache.kv_heads, total = nh + 2 * nkv;
-  const int lane = threadIdx.x % LPH, c0 = lane * 8;
-  const int block = pos / a.cache.page_size, page = iris_paged_page(&a.cache, seq, block);
   const int64_t slot = page < 0 ? -1 : iris_paged_offset(&a.cache, page, pos - block * a.cache.page_size);
-  for (int h0 = blockIdx.y * GROUPS; h0 < total; h0 += gridDim.y * GROUPS) {
-    const int h = h0 + threadIdx.x / LPH;
-    const bool live = h < total, is_q = h < nh, is_k = !is_q && h < nh + nkv;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const In* src = is_q ? (const In*)a.q + (int64_t)t * a.ldq + h * HD
-                           : is_k ? (const In*)a.k + (int64_t)t * a.ldk + (h - nh) * HD
-                                  : (const In*)a.v + (int64_t)t * a.ldv + (h - nh - nkv) * HD;
-      load8(src + c0, x);
-    }
-    float ss = 0.f;
+  __nv_bfloat16* qo = (__nv_bfloat16*)a.q_out + (int64_t)t * a.ldq_out;
+  __nv_bfloat16* ko = (__nv_bfloat16*)a.cache.k + slot;
+  __nv_bfloat16* vo = (__nv_bfloat16*)a.cache.v + slot;
+  __syncthreads();
+  float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (turned) c4 = *reinterpret_cast<const float4*>(cs + lane * 4), s4 = *reinterpret_cast<const float4*>(sn + lane * 4);
+  auto one = [&](int h, float4 x, float4 y) {
+    const bool is_q = h < nh, is_v = h >= nh + nkv;
+    if (!is_v) {
+      const float* w = is_q ? a.q_norm : a.k_norm;
+      if (w) {
+        float ss = ((x.x * x.x + x.y * x.y) + (x.z * x.z + x.w * x.w)) + ((y.x * y.x + y.y * y.y) + (y.z * y.z + y.w * y.w));
+        // the lanes of a head are together in one warp and take the same way
+        const uint32_t lanes = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1) << (threadIdx.x % 32 / LPH * LPH);
 #pragma unroll
-    for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-#pragma unroll
-    for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float* w = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-    if (live && w) {
-      const float r = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
-      float wv[8];
-      load8(w + c0, wv);
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = x[i] * r * wv[i];
-    }
-    if (rd) {
-      const bool turned = c0 < rd && (is_q || is_k);
-      if (a.rope.layout == IRIS_ROPE_INTERLEAVED) {
-        if (turned) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float c = cs[c0 / 2 + i], s = sn[c0 / 2 + i], u = x[2 * i], v = x[2 * i + 1];
-            x[2 * i] = u * c - v * s;
-            x[2 * i + 1] = u * s + v * c;
-          }
-        }
-      } else {
-        const bool upper = c0 >= rd / 2;
-        const int from = c0 >= rd ? lane : upper ? lane - rd / 16 : lane + rd / 16;
-        const int i0 = upper ? c0 - rd / 2 : c0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float y = __shfl_sync(0xffffffffu, x[i], from, LPH);
-          if (turned) x[i] = upper ? y * sn[i0 + i] + x[i] * cs[i0 + i] : x[i] * cs[i0 + i] - y * sn[i0 + i];
-        }
+        for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
+        const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
+        const float4 wa = *reinterpret_cast<const float4*>(w + ca), wb = *reinterpret_cast<const float4*>(w + cb);
+        x.x *= r * wa.x, x.y *= r * wa.y, x.z *= r * wa.z, x.w *= r * wa.w;
+        y.x *= r * wb.x, y.y *= r * wb.y, y.z *= r * wb.z, y.w *= r * wb.w;
+      }
+      if (halves) {
+        turn(x.x, y.x, c4.x, s4.x), turn(x.y, y.y, c4.y, s4.y), turn(x.z, y.z, c4.z, s4.z), turn(x.w, y.w, c4.w, s4.w);
+      } else if (turned) {
+        turn(x.x, x.y, c4.x, s4.x), turn(x.z, x.w, c4.y, s4.y), turn(y.x, y.y, c4.z, s4.z), turn(y.z, y.w, c4.w, s4.w);
       }
     }
-    if (!live || (!is_q && slot < 0)) continue;
-    __nv_bfloat16* dst;
-    if (is_q)
-      dst = (__nv_bfloat16*)a.q_out + (int64_t)t * a.ldq_out + h * HD;
-    else if (is_k)
-      dst = (__nv_bfloat16*)a.cache.k + slot + (int64_t)(h - nh) * a.cache.head_stride;
-    else
-      dst = (__nv_bfloat16*)a.cache.v + slot + (int64_t)(h - nh - nkv) * a.cache.head_stride;
-    *reinterpret_cast<uint4*>(dst + c0) =
-        make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    if (!is_q && slot < 0) return;
+    __nv_bfloat16* to = is_q ? qo + h * HD : is_v ? vo + (int64_t)(h - nh - nkv) * a.cache.head_stride
+                                                  : ko + (int64_t)(h - nh) * a.cache.head_stride;
+    *reinterpret_cast<uint2*>(to + ca) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
+    *reinterpret_cast<uint2*>(to + cb) = make_uint2(pack2(y.x, y.y), pack2(y.z, y.w));
+  };
+#pragma unroll
+  for (int i = 0; i < ROPE_HEADS; i++)
+    if (first + i * step < total) one(first + i * step, values4(ra[i]), values4(rb[i]));
+  for (int h = first + ROPE_HEADS * step; h < total; h += step) {
+    const In* x = row(h);
+    one(h, values4(*reinterpret_cast<const Raw*>(x + ca)), values4(*reinterpret_cast<const Raw*>(x + cb)));
   }
 }
 
@@ -1051,15 +1069,14 @@ __global__ void __launch_bounds__(THREADS) logprobs_finish_kernel(const __grid_c
 }  // namespace
 
 // ------------------------------------------------------------------ launches
-extern "C" cudaError_t iris_launch_rope_append(const IrisRopeAppend* a, int f32, int num_sms, cudaStream_t stream) {
-  const int groups = 256 / (a->cache.head_dim / 8);
-  const int slices = (a->heads + 2 * a->cache.kv_heads + groups - 1) / groups;
-  // few tokens: a block per slice of heads, so that they run side by side
-  const dim3 grid(a->tokens, a->tokens * slices <= 4 * num_sms ? slices : 1);
-  auto go = [&](auto kernel) {
-    kernel<<<grid, 256, 0, stream>>>(*a);
-    return cudaGetLastError();
-  };
+extern "C" cudaError_t iris_launch_rope_append(IrisRopeAppend* a, int f32, int num_sms, cudaStream_t stream) {
+  a->div = iris_paged_div(a->cache.page_size);
+  const int groups = ROPE_THREADS / (a->cache.head_dim / 8);
+  const int slices = (a->heads + 2 * a->cache.kv_heads + groups - 1) / groups;  // with a head per group of lanes
+  // few tokens: a block per slice, so that they run side by side; else slices of at most ROPE_HEADS heads per group
+  const bool few = (int64_t)a->tokens * slices * ROPE_THREADS <= 1024 * num_sms;
+  const dim3 grid(a->tokens, few ? slices : (slices + ROPE_HEADS - 1) / ROPE_HEADS);
+  auto go = [&](auto kernel) { return iris::launch_overlapped(kernel, grid, dim3(ROPE_THREADS), 0, stream, *a); };
   if (f32) {
     if (a->cache.head_dim == 64) return go(rope_append_kernel<float, 64>);
     if (a->cache.head_dim == 128) return go(rope_append_kernel<float, 128>);

@@ -146,6 +146,8 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
     if (misaligned(k, 16) || misaligned(v, 16) || (heads && (misaligned(q, 16) || misaligned(q_out, 16))) ||
         misaligned(q_norm, 16) || misaligned(k_norm, 16) || misaligned(seq, 4) || misaligned(pos, 4))
         return LM_FAIL("%s: misaligned pointer (16 bytes; seq and pos 4)", what);
+    if (heads && q_out == q && (f32 || ldq != ldq_out))
+        return LM_FAIL("%s: q_out on q needs bf16 and one row stride", what);
     if (!tokens) return 0;
     const void *ptrs[] = {cache->k, cache->v, cache->table, q_out, q, k, v, q_norm, k_norm, seq, pos};
     lm_dev_t d;

@@ -809,28 +809,36 @@ def _ok(rc: int) -> None:
         raise IrisCudaError(last_error())
 
 
+_DTYPES: dict = {}  # dtype object -> its name (a step of one token is a few microseconds: no string work per call)
+
+
 def _dtype(t) -> str:
-    return str(t.dtype).rpartition(".")[2]
+    d = t.dtype
+    name = _DTYPES.get(d)
+    if name is None:
+        name = _DTYPES[d] = str(d).rpartition(".")[2]
+    return name
 
 
-def _need(what: str, t, dtype: str, shape, optional: bool = False):
+def _need(what: str, t, dtype: str, shape: tuple):
     """Address of t after a check of its type, shape and contiguous last axis (None: 0)."""
-    if t is None and optional:
+    if t is None:
         return None
-    if _dtype(t) != dtype or tuple(t.shape) != tuple(shape) or (shape and t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise IrisCudaError(f"{what}: needs {dtype} {tuple(shape)}, contiguous in the last axis; "
+    if _dtype(t) != dtype or t.shape != shape or (shape[-1] > 1 and t.stride()[-1] != 1):
+        raise IrisCudaError(f"{what}: needs {dtype} {shape}, contiguous in the last axis; "
                             f"got {_dtype(t)} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _heads_rows(what: str, t, dtype: str, rows: int, heads: int, head_dim: int):
     """(address, row stride) of [rows, heads, head_dim] or [rows, heads * head_dim]."""
-    shape = tuple(t.shape)
-    if _dtype(t) != dtype or shape not in ((rows, heads, head_dim), (rows, heads * head_dim)) or \
-            t.stride(-1) != 1 or (len(shape) == 3 and heads > 1 and t.stride(1) != head_dim):
+    shape, stride = t.shape, t.stride()
+    if _dtype(t) != dtype or stride[-1] != 1 or not (
+            shape == (rows, heads * head_dim) if len(shape) == 2 else
+            shape == (rows, heads, head_dim) and (heads == 1 or stride[1] == head_dim)):
         raise IrisCudaError(f"{what}: needs {dtype} [{rows}, {heads}, {head_dim}] with contiguous rows; "
-                            f"got {_dtype(t)} {shape}")
-    return t.data_ptr(), t.stride(0) if rows > 1 else heads * head_dim
+                            f"got {_dtype(t)} {tuple(shape)}")
+    return t.data_ptr(), stride[0] if rows > 1 else heads * head_dim
 
 
 def rope_append(cache: KvCache, rope: Rope | None, q_out, q, k, v, seq, pos, *, heads: int, q_norm=None, k_norm=None,
@@ -848,8 +856,8 @@ def rope_append(cache: KvCache, rope: Rope | None, q_out, q, k, v, seq, pos, *, 
         qp, ldq = _heads_rows("q", q, ty, n, heads, d)
         op, ldo = _heads_rows("q_out", q_out, "bfloat16", n, heads, d)
     _ok(lib().iris_gpu_rope_append(cache, rope, op, ldo, qp, kp, vp, ldq, ldk, ldv, ty == "float32",
-                                   _need("q_norm", q_norm, "float32", (d,), True),
-                                   _need("k_norm", k_norm, "float32", (d,), True), eps,
+                                   _need("q_norm", q_norm, "float32", (d,)),
+                                   _need("k_norm", k_norm, "float32", (d,)), eps,
                                    _need("seq", seq, "int32", (n,)), _need("pos", pos, "int32", (n,)), n, heads, stream))
 
 
@@ -866,7 +874,7 @@ def attention_paged(cache: KvCache, out, q, seq, pos, *, scale: float, workspace
     heads = q.shape[1] if len(q.shape) == 3 else q.shape[1] // d
     qp, ldq = _heads_rows("q", q, "bfloat16", n, heads, d)
     op, ldo = _heads_rows("out", out, "bfloat16", n, heads, d)
-    _ok(lib().iris_gpu_attention_paged(cache, op, qp, ldo, ldq, _need("seq", seq, "int32", (n,), True),
+    _ok(lib().iris_gpu_attention_paged(cache, op, qp, ldo, ldq, _need("seq", seq, "int32", (n,)),
                                        _need("pos", pos, "int32", (n,)), n, heads, scale, workspace.data_ptr(),
                                        workspace.numel() * workspace.element_size(), stream))
 
@@ -885,13 +893,12 @@ def token_logprobs(logits, targets, logprob, entropy, top_ids, top_logprobs, *, 
     if ty not in ("float32", "bfloat16") or logits.stride(1) != 1:
         raise IrisCudaError(f"token_logprobs: logits {ty}, stride {logits.stride(1)} between a row's values")
     k = top_ids.shape[1] if top_ids is not None else top_logprobs.shape[1] if top_logprobs is not None else 0
-    if (top_ids is not None and k > 1 and rows > 1 and top_ids.stride(0) != k) or \
-            (top_logprobs is not None and k > 1 and rows > 1 and top_logprobs.stride(0) != k):
+    if k and rows > 1 and any(t is not None and t.stride(0) != k for t in (top_ids, top_logprobs)):
         raise IrisCudaError("token_logprobs: the alternatives' rows lie one after the other")
     _ok(lib().iris_gpu_token_logprobs(logits.data_ptr(), ty == "float32", logits.stride(0) if rows > 1 else vocab, rows,
-                                      vocab, _need("targets", targets, "int32", (rows,), True),
-                                      _need("logprob", logprob, "float32", (rows,), True),
-                                      _need("entropy", entropy, "float32", (rows,), True), k,
-                                      _need("top_ids", top_ids, "int32", (rows, k), True),
-                                      _need("top_logprobs", top_logprobs, "float32", (rows, k), True),
+                                      vocab, _need("targets", targets, "int32", (rows,)),
+                                      _need("logprob", logprob, "float32", (rows,)),
+                                      _need("entropy", entropy, "float32", (rows,)), k,
+                                      _need("top_ids", top_ids, "int32", (rows, k)),
+                                      _need("top_logprobs", top_logprobs, "float32", (rows, k)),
                                       workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))

@@ -93,7 +93,7 @@ BAD_CACHES = [dict(k=None), dict(v=None), dict(table=None), dict(num_pages=0), d
 
 
 def append(c, **kw):
-    d = dict(rope=Rope.of(128, 1e4), q_out=A, ldq_out=512, q=A, k=A, v=A, ldq=512, ldk=256, ldv=256, f32=0, q_norm=A,
+    d = dict(rope=Rope.of(128, 1e4), q_out=4 * A, ldq_out=512, q=A, k=A, v=A, ldq=512, ldk=256, ldv=256, f32=0, q_norm=A,
              k_norm=A, eps=1e-6, seq=A, pos=A, tokens=5, heads=4)
     d.update(kw)
     return iris_cuda.lib().iris_gpu_rope_append(c, *d.values(), None)
@@ -134,7 +134,7 @@ def test_null_cache_is_refused():
     dict(q=None), dict(q_out=None), dict(ldq=511), dict(ldq=504), dict(ldq_out=516), dict(ldk=248), dict(ldv=255), dict(eps=-1.0),
     dict(eps=math.nan), dict(q=A + 2), dict(k=A + 8), dict(v=A + 4), dict(q_out=A + 8), dict(q_norm=A + 4),
     dict(k_norm=A + 8), dict(seq=A + 1), dict(pos=A + 2), dict(rope=Rope.of(256, 1e4)), dict(rope=Rope(layout=7, rot_dim=64)),
-    dict(rope=Rope(layout=0, rot_dim=24))])
+    dict(rope=Rope(layout=0, rot_dim=24)), dict(q_out=2 * A, q=2 * A, f32=1), dict(q_out=2 * A, q=2 * A, ldq_out=520)])
 def test_rope_append_refusals(bad):
     refused(append(cache(), **bad), "rope_append")
 
@@ -240,7 +240,8 @@ def test_binding_refuses_other_tensors():
     f = Fake("float32", 5)
     for bad in (dict(logits=Fake("float16", 5, 100)), dict(logits=Fake("float32", 5, 100, stride=[1, 5])),
                 dict(targets=Fake("int64", 5)), dict(entropy=Fake("float32", 4)), dict(top_ids=Fake("int64", 5, 3)),
-                dict(top_logprobs=Fake("float32", 5, 2)), dict(top_ids=Fake("int32", 5, 3, stride=[6, 1]))):
+                dict(top_logprobs=Fake("float32", 5, 2)), dict(top_ids=Fake("int32", 5, 3, stride=[6, 1])),
+                dict(top_ids=Fake("int32", 5, 1, stride=[4, 1]), top_logprobs=None)):
         d = {**dict(logits=Fake("float32", 5, 100), targets=i, logprob=f, entropy=f, top_ids=Fake("int32", 5, 3),
                     top_logprobs=Fake("float32", 5, 3)), **bad}
         with pytest.raises(E):
