@@ -414,6 +414,36 @@ uint64_t iris_cuda_qwen3_graph_kernels(const iris_cuda_qwen3_t *m);
  * status. */
 int iris_cuda_qwen3_profile(iris_cuda_qwen3_t *m, iris_cuda_kernel_time_t *out, int max_entries);
 
+/* The same model as a language model (no counterpart in the reference, whose
+ * text model only encodes): it can be asked how likely a text is, and goes on
+ * with one a token at a time (rewriting a prompt, for instance), on the
+ * operators of layer 4.  load_lm / random_lm hold every decoder layer, the
+ * final norm and the head (lm_head.weight, or the embeddings where the model
+ * has none) besides what iris_cuda_qwen3_load holds; the result serves as an
+ * encoder too. */
+iris_cuda_qwen3_t *iris_cuda_qwen3_load_lm(const char *model_dir);
+iris_cuda_qwen3_t *iris_cuda_qwen3_random_lm(const iris_cuda_qwen3_config_t *cfg, uint64_t seed);
+/* A session: the paged key-value cache of num_seqs sequences of up to max_len
+ * tokens, and buffers for steps of up to max_tokens.  Free it before its model. */
+typedef struct iris_cuda_qwen3_lm iris_cuda_qwen3_lm_t;
+iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_seqs, int max_len, int max_tokens);
+void iris_cuda_qwen3_lm_free(iris_cuda_qwen3_lm_t *lm);
+size_t iris_cuda_qwen3_lm_cache_bytes(const iris_cuda_qwen3_lm_t *lm);
+/* Feed tokens (host arrays): ids[t] becomes position pos[t] of sequence seq[t],
+ * for any mix of sequences, prompts whole and answers token by token.  In one
+ * call a sequence's positions go up by 1; its first may be at most the
+ * sequence's length (0 at first), and a smaller one cuts the sequence off
+ * there.  Per token, each output optional (NULL): the log probability of
+ * targets[t] (outside the vocabulary: 0) as the next token, the entropy of the
+ * next token's distribution, and its top_k <= 32 likeliest values, likeliest
+ * first.  Returns 0 or an error; one of the arguments leaves the sequences as
+ * they were. */
+int iris_cuda_qwen3_lm_step(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos,
+                            const int *targets, int tokens, int top_k, float *logprob, float *entropy, int *top_ids,
+                            float *top_logprobs);
+/* Tokens a sequence holds, or a negative status. */
+int iris_cuda_qwen3_lm_length(const iris_cuda_qwen3_lm_t *lm, int seq);
+
 /* ------------------------------------------------------------------ 2d. autoencoder decoder
  * The step after the denoising loop: latent -> RGB image on the GPU.  The
  * decoder of AutoencoderKLFlux2 (32 latent channels, batch-norm latent

@@ -13,51 +13,14 @@
  * the one after layer num_layers - 2 ([S, H]).  Only the layers up to the last
  * extracted one run.  One forward per sequence length is a CUDA graph.
  */
-#include "iris_internal.h"
+#include "qwen3_internal.h"
 
 #include <math.h>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
 
-#define Q3_EPS 1e-6f        /* QWEN3_RMS_NORM_EPS */
-#define Q3_MAX_SEQ 512      /* QWEN3_MAX_SEQ_LEN: the reference pads every prompt to it */
 static const int k_flux_layers[3] = {8, 17, 26};  /* QWEN3_OUTPUT_LAYER_1..3 */
-
-typedef struct {
-    uint16_t *w_qkv;   /* [(nh + 2 nkv) * 128, H] */
-    uint16_t *w_o;     /* [H, nh * 128] */
-    uint16_t *w_gu;    /* [2F, H], gate/up rows interleaved in blocks of 128 */
-    uint16_t *w_down;  /* [H, F] */
-    float *ln1, *ln2, *qn, *kn;
-    CUtensorMap tm_qkv, tm_o, tm_gu, tm_down;
-} q3_layer_t;
-
-typedef struct {
-    int valid, S;
-    int *ids;
-    uint8_t *mask;
-    float *x, *qkv, *out, *cosb, *sinb;
-    float *ws;          /* split-K workspace of the H-wide projections (few output tiles at 512 rows) */
-    size_t ws_bytes;
-    uint16_t *xn, *q, *k, *v, *attn, *mlp;
-    CUtensorMap tm_xn, tm_attn, tm_mlp;
-    cudaGraph_t graph;
-    cudaGraphExec_t gexec;
-    int graph_ok, graph_mode;
-    uint64_t graph_kernels;
-} q3_plan_t;
-
-struct iris_cuda_qwen3 {
-    iris_cuda_qwen3_config_t cfg;
-    int mode;              /* 0 Flux, 1 Z-Image extraction */
-    int nlayers;           /* layers held on the device */
-    uint16_t *embed;       /* [vocab, H] */
-    q3_layer_t *layers;
-    float *ones;           /* [H] gate of the residual GEMM epilogues */
-    q3_plan_t plan;
-    size_t weight_bytes;
-};
 
 static int q3_qkv_n(const iris_cuda_qwen3_config_t *c) { return (c->heads + 2 * c->kv_heads) * c->head_dim; }
 
@@ -160,6 +123,39 @@ static int q3_load_layers(iris_cuda_qwen3_t *m, q3_src_t *src) {
     return rc;
 }
 
+/* The language model's end: the final norm, and the head (lm_head.weight, or
+ * the embeddings where the file has none) with its rows filled up with zeros
+ * to the GEMM's tile. */
+static int q3_load_head(iris_cuda_qwen3_t *m, q3_src_t *src) {
+    const iris_cuda_qwen3_config_t *c = &m->cfg;
+    const size_t H = (size_t)c->hidden;
+    const int own = src->file && st_find(&src->file->st, "lm_head.weight") != NULL;
+    m->head_rows = (c->vocab + 127) / 128 * 128;
+    m->norm = (float *)q3_dalloc(m, H * 4);
+    uint16_t *tmp = (uint16_t *)iris_dmalloc(H * 2);
+    int rc = (!m->norm || !tmp) ? iris_fail(IRIS_CUDA_ERR_OOM, "language model head") : 0;
+    if (!rc) rc = q3_get_vec(src, "model.norm.weight", c->hidden, m->norm, tmp);
+    iris_dfree(tmp);
+    if (!rc && !own && m->head_rows == c->vocab) {
+        m->head = m->embed;
+    } else if (!rc) {
+        m->head = (uint16_t *)q3_dalloc(m, (size_t)m->head_rows * H * 2);
+        m->head_own = 1;
+        if (!m->head) rc = iris_fail(IRIS_CUDA_ERR_OOM, "language model head");
+        const size_t held = (size_t)c->vocab * H * 2;
+        if (!rc)
+            rc = iris_cuda_check(cudaMemsetAsync((char *)m->head + held, 0, (size_t)(m->head_rows - c->vocab) * H * 2, g_rt.stream),
+                                 "head rows");
+        if (!rc && own) rc = q3_get_bf16(src, "lm_head.weight", (size_t)c->vocab * H, m->head, 0.f, 0.f);
+        if (!rc && !own)
+            rc = iris_cuda_check(cudaMemcpyAsync(m->head, m->embed, held, cudaMemcpyDeviceToDevice, g_rt.stream), "head");
+    }
+    if (!rc && iris_make_tmap_bf16(&m->tm_head, m->head, (uint64_t)m->head_rows, (uint64_t)H, (uint64_t)H,
+                                   m->head_rows % 256 ? 128 : 256))
+        rc = iris_fail(IRIS_CUDA_ERR_CUDA, "head tensor map");
+    return rc;
+}
+
 static void q3_plan_free(q3_plan_t *P);
 
 void iris_cuda_qwen3_free(iris_cuda_qwen3_t *m) {
@@ -174,6 +170,8 @@ void iris_cuda_qwen3_free(iris_cuda_qwen3_t *m) {
     }
     free(m->layers);
     iris_dfree(m->ones);
+    iris_dfree(m->norm);
+    if (m->head_own) iris_dfree(m->head);
     free(m);
 }
 
@@ -188,14 +186,14 @@ static int q3_check_config(const iris_cuda_qwen3_config_t *c) {
     return 0;
 }
 
-static iris_cuda_qwen3_t *q3_create(const iris_cuda_qwen3_config_t *cfg, q3_src_t *src) {
+static iris_cuda_qwen3_t *q3_create(const iris_cuda_qwen3_config_t *cfg, q3_src_t *src, int lm) {
     if (q3_check_config(cfg)) return NULL;
     iris_cuda_qwen3_t *m = (iris_cuda_qwen3_t *)calloc(1, sizeof(*m));
     if (!m) { iris_fail(IRIS_CUDA_ERR_OOM, "text encoder"); return NULL; }
     m->cfg = *cfg;
     /* every layer up to the later of the two extraction points */
     m->nlayers = cfg->layers - 1 > k_flux_layers[2] + 1 ? cfg->layers - 1 : k_flux_layers[2] + 1;
-    if (m->nlayers > cfg->layers) m->nlayers = cfg->layers;
+    if (lm || m->nlayers > cfg->layers) m->nlayers = cfg->layers;
     m->layers = (q3_layer_t *)calloc((size_t)m->nlayers, sizeof(q3_layer_t));
     float *ones = (float *)malloc((size_t)cfg->hidden * 4);
     m->ones = (float *)iris_dmalloc((size_t)cfg->hidden * 4);
@@ -206,12 +204,13 @@ static iris_cuda_qwen3_t *q3_create(const iris_cuda_qwen3_config_t *cfg, q3_src_
     }
     free(ones);
     if (!rc) rc = q3_load_layers(m, src);
+    if (!rc && lm) rc = q3_load_head(m, src);
     if (!rc) rc = iris_cuda_check(cudaStreamSynchronize(g_rt.stream), "text encoder upload");
     if (rc) { iris_cuda_qwen3_free(m); return NULL; }
     return m;
 }
 
-iris_cuda_qwen3_t *iris_cuda_qwen3_load(const char *model_dir) {
+static iris_cuda_qwen3_t *q3_load(const char *model_dir, int lm) {
     if (!model_dir) { iris_fail(IRIS_CUDA_ERR_ARG, "null model directory"); return NULL; }
     if (iris_rt_ensure()) return NULL;
     /* config.json keys and defaults as parse_qwen3_config / qwen3_set_defaults (iris_qwen3.c:1378-1447) */
@@ -241,19 +240,29 @@ iris_cuda_qwen3_t *iris_cuda_qwen3_load(const char *model_dir) {
         return NULL;
     }
     q3_src_t src = {&ws, 0};
-    iris_cuda_qwen3_t *m = q3_create(&c, &src);
+    iris_cuda_qwen3_t *m = q3_create(&c, &src, lm);
     iris_wsrc_free(&ws);  /* waits for the last uploads */
     st_close(&ws.st);
     return m;
 }
 
-iris_cuda_qwen3_t *iris_cuda_qwen3_random(const iris_cuda_qwen3_config_t *cfg, uint64_t seed) {
+iris_cuda_qwen3_t *iris_cuda_qwen3_load(const char *model_dir) { return q3_load(model_dir, 0); }
+iris_cuda_qwen3_t *iris_cuda_qwen3_load_lm(const char *model_dir) { return q3_load(model_dir, 1); }
+
+static iris_cuda_qwen3_t *q3_random(const iris_cuda_qwen3_config_t *cfg, uint64_t seed, int lm) {
     if (!cfg) { iris_fail(IRIS_CUDA_ERR_ARG, "null config"); return NULL; }
     if (iris_rt_ensure()) return NULL;
     q3_src_t src = {NULL, seed};
-    iris_cuda_qwen3_t *m = q3_create(cfg, &src);
+    iris_cuda_qwen3_t *m = q3_create(cfg, &src, lm);
     if (m && iris_cuda_synchronize()) { iris_cuda_qwen3_free(m); return NULL; }
     return m;
+}
+
+iris_cuda_qwen3_t *iris_cuda_qwen3_random(const iris_cuda_qwen3_config_t *cfg, uint64_t seed) {
+    return q3_random(cfg, seed, 0);
+}
+iris_cuda_qwen3_t *iris_cuda_qwen3_random_lm(const iris_cuda_qwen3_config_t *cfg, uint64_t seed) {
+    return q3_random(cfg, seed, 1);
 }
 
 int iris_cuda_qwen3_get_config(const iris_cuda_qwen3_t *m, iris_cuda_qwen3_config_t *out) {
@@ -337,17 +346,7 @@ static int q3_plan_ensure(iris_cuda_qwen3_t *m, int S) {
 }
 
 /* ------------------------------------------------------------------ enqueue */
-typedef struct {
-    int rc;
-    uint64_t kernels;
-    /* profiling (iris_cuda_qwen3_profile): an event after every launch */
-    iris_cuda_kernel_time_t *prof;
-    cudaEvent_t *ev;
-    int nprof, maxprof;
-    double flops;  /* algorithmic FLOPs of the next accounted launch */
-} q3_enq_t;
-
-static void q3_done(q3_enq_t *E, cudaError_t e, const char *what, int n) {
+void iris_q3_done(q3_enq_t *E, cudaError_t e, const char *what, int n) {
     if (E->rc) return;
     if (e != cudaSuccess) { E->rc = iris_cuda_check(e, what); return; }
     E->kernels += (uint64_t)n;
@@ -362,9 +361,9 @@ static void q3_done(q3_enq_t *E, cudaError_t e, const char *what, int n) {
     E->flops = 0.0;
 }
 
-static void q3_gemm(q3_enq_t *E, const char *name, const CUtensorMap *ta, const CUtensorMap *tb, int M, int N,
-                    int K, int mode, void *out, int ldo, const float *gate, void *mlp_out, int ld_mlp, float *ws,
-                    size_t ws_bytes) {
+void iris_q3_gemm(q3_enq_t *E, const char *name, const CUtensorMap *ta, const CUtensorMap *tb, int M, int N, int K,
+                  int mode, void *out, int ldo, const float *gate, void *mlp_out, int ld_mlp, float *ws,
+                  size_t ws_bytes) {
     if (E->rc) return;
     IrisGemmParams p;
     memset(&p, 0, sizeof(p));
@@ -388,7 +387,7 @@ static void q3_gemm(q3_enq_t *E, const char *name, const CUtensorMap *ta, const 
     int n = 1;
     cudaError_t e = iris_launch_gemm_ex(&p, g_rt.num_sms, g_rt.stream, &n);
     E->flops = 2.0 * M * N * K;
-    q3_done(E, e, name, n);
+    iris_q3_done(E, e, name, n);
 }
 
 static int q3_enqueue(iris_cuda_qwen3_t *m, q3_enq_t *E) {
@@ -397,26 +396,26 @@ static int q3_enqueue(iris_cuda_qwen3_t *m, q3_enq_t *E) {
     const int S = P->S, H = c->hidden, F = c->intermediate, qd = c->heads * 128, kvd = c->kv_heads * 128;
     const int nq = q3_qkv_n(c), last = last_layer(m), td = iris_cuda_qwen3_text_dim(m);
     cudaStream_t st = g_rt.stream;
-    q3_done(E, iris_launch_embed_rows(P->ids, S, m->embed, c->vocab, H, P->x, st), "embed", 1);
+    iris_q3_done(E, iris_launch_embed_rows(P->ids, S, m->embed, c->vocab, H, P->x, st), "embed", 1);
     int slot = 0;
     for (int i = 0; i <= last && !E->rc; i++) {
         const q3_layer_t *L = &m->layers[i];
-        q3_done(E, iris_launch_rmsnorm(P->x, H, L->ln1, NULL, P->xn, H, S, H, Q3_EPS, NULL, st), "rmsnorm", 1);
-        q3_gemm(E, "qkv", &P->tm_xn, &L->tm_qkv, S, nq, H, IRIS_EPI_F32, P->qkv, nq, NULL, NULL, 0, NULL, 0);
-        q3_done(E, iris_launch_qk_norm_rope_half(P->qkv, nq, S, c->heads, c->kv_heads, L->qn, L->kn, P->cosb, P->sinb,
+        iris_q3_done(E, iris_launch_rmsnorm(P->x, H, L->ln1, NULL, P->xn, H, S, H, Q3_EPS, NULL, st), "rmsnorm", 1);
+        iris_q3_gemm(E, "qkv", &P->tm_xn, &L->tm_qkv, S, nq, H, IRIS_EPI_F32, P->qkv, nq, NULL, NULL, 0, NULL, 0);
+        iris_q3_done(E, iris_launch_qk_norm_rope_half(P->qkv, nq, S, c->heads, c->kv_heads, L->qn, L->kn, P->cosb, P->sinb,
                                                  Q3_EPS, P->q, P->k, P->v, st),
                 "qk norm rope", 1);
         E->flops = 2.0 * S * S * qd;  /* causal: half of 4 S^2 d per head */
-        q3_done(E, iris_launch_attention_gqa(P->q, qd, P->k, P->v, kvd, P->attn, qd, S, S, c->heads,
+        iris_q3_done(E, iris_launch_attention_gqa(P->q, qd, P->k, P->v, kvd, P->attn, qd, S, S, c->heads,
                                              c->heads / c->kv_heads, 1, 1.0f / sqrtf(128.0f), P->mask, st),
                 "attention", 1);
-        q3_gemm(E, "o_proj", &P->tm_attn, &L->tm_o, S, H, qd, IRIS_EPI_RESID_GATE, P->x, H, m->ones, NULL, 0, P->ws, P->ws_bytes);
-        q3_done(E, iris_launch_rmsnorm(P->x, H, L->ln2, NULL, P->xn, H, S, H, Q3_EPS, NULL, st), "rmsnorm", 1);
-        q3_gemm(E, "gate_up", &P->tm_xn, &L->tm_gu, S, 2 * F, H, IRIS_EPI_SWIGLU, NULL, 0, NULL, P->mlp, F, NULL, 0);
-        q3_gemm(E, "down", &P->tm_mlp, &L->tm_down, S, H, F, IRIS_EPI_RESID_GATE, P->x, H, m->ones, NULL, 0, P->ws, P->ws_bytes);
+        iris_q3_gemm(E, "o_proj", &P->tm_attn, &L->tm_o, S, H, qd, IRIS_EPI_RESID_GATE, P->x, H, m->ones, NULL, 0, P->ws, P->ws_bytes);
+        iris_q3_done(E, iris_launch_rmsnorm(P->x, H, L->ln2, NULL, P->xn, H, S, H, Q3_EPS, NULL, st), "rmsnorm", 1);
+        iris_q3_gemm(E, "gate_up", &P->tm_xn, &L->tm_gu, S, 2 * F, H, IRIS_EPI_SWIGLU, NULL, 0, NULL, P->mlp, F, NULL, 0);
+        iris_q3_gemm(E, "down", &P->tm_mlp, &L->tm_down, S, H, F, IRIS_EPI_RESID_GATE, P->x, H, m->ones, NULL, 0, P->ws, P->ws_bytes);
         const int extract = m->mode ? (i == last) : (i == k_flux_layers[0] || i == k_flux_layers[1] || i == k_flux_layers[2]);
         if (extract && !E->rc) {
-            q3_done(E, cudaMemcpy2DAsync(P->out + (size_t)slot * H, (size_t)td * 4, P->x, (size_t)H * 4,
+            iris_q3_done(E, cudaMemcpy2DAsync(P->out + (size_t)slot * H, (size_t)td * 4, P->x, (size_t)H * 4,
                                          (size_t)H * 4, (size_t)S, cudaMemcpyDeviceToDevice, st),
                     "extract", 0);
             slot++;

@@ -232,6 +232,14 @@ SIGNATURES = {
     "iris_cuda_qwen3_forward": (C.c_void_p, [C.c_void_p, C.POINTER(C.c_int), C.POINTER(C.c_int), C.c_int]),
     "iris_cuda_qwen3_forward_dev": (C.c_int, [C.c_void_p, C.POINTER(C.c_int), C.POINTER(C.c_int), C.c_int,
                                               C.c_void_p]),
+    "iris_cuda_qwen3_load_lm": (C.c_void_p, [C.c_char_p]),
+    "iris_cuda_qwen3_random_lm": (C.c_void_p, [C.POINTER(Qwen3Config), C.c_uint64]),
+    "iris_cuda_qwen3_lm_create": (C.c_void_p, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "iris_cuda_qwen3_lm_free": (None, [C.c_void_p]),
+    "iris_cuda_qwen3_lm_cache_bytes": (C.c_size_t, [C.c_void_p]),
+    "iris_cuda_qwen3_lm_step": (C.c_int, [C.c_void_p] + [C.POINTER(C.c_int)] * 4 + [C.c_int, C.c_int, _fp, _fp,
+                                                                                  C.POINTER(C.c_int), _fp]),
+    "iris_cuda_qwen3_lm_length": (C.c_int, [C.c_void_p, C.c_int]),
     "iris_cuda_qwen3_graph_kernels": (C.c_uint64, [C.c_void_p]),
     "iris_cuda_qwen3_profile": (C.c_int, [C.c_void_p, C.POINTER(KernelTime), C.c_int]),
     "iris_cuda_vae_profile": (C.c_int, [C.c_void_p, C.POINTER(KernelTime), C.c_int]),
@@ -763,6 +771,15 @@ class Qwen3:
     def random(cls, cfg: Qwen3Config, seed: int) -> "Qwen3":
         return cls(lib().iris_cuda_qwen3_random(C.byref(cfg), seed))
 
+    @classmethod
+    def load_lm(cls, model_dir: str) -> "Qwen3":
+        """With every layer, the final norm and the head: usable by Qwen3Lm."""
+        return cls(lib().iris_cuda_qwen3_load_lm(model_dir.encode()))
+
+    @classmethod
+    def random_lm(cls, cfg: Qwen3Config, seed: int) -> "Qwen3":
+        return cls(lib().iris_cuda_qwen3_random_lm(C.byref(cfg), seed))
+
     def close(self):
         if self.h:
             lib().iris_cuda_qwen3_free(self.h)
@@ -797,6 +814,53 @@ class Qwen3:
         p = lib().iris_cuda_qwen3_forward(self.h, ids.ctypes.data_as(ip),
                                           None if m is None else m.ctypes.data_as(ip), len(ids))
         return _take_floats(p, len(ids) * self.text_dim(), (len(ids), self.text_dim()))
+
+
+class Qwen3Lm:
+    """The text model as a language model (libiris_cuda): a session with a paged
+    key-value cache.  The model comes from Qwen3.load_lm / random_lm."""
+
+    def __init__(self, model: Qwen3, num_seqs: int = 1, max_len: int = 2048, max_tokens: int = 512):
+        self.h = lib().iris_cuda_qwen3_lm_create(model.h, num_seqs, max_len, max_tokens)
+        if not self.h:
+            raise IrisCudaError(last_error() or "language model session failed")
+        self.model = model  # kept alive
+
+    def close(self):
+        if self.h:
+            lib().iris_cuda_qwen3_lm_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def cache_bytes(self) -> int:
+        return lib().iris_cuda_qwen3_lm_cache_bytes(self.h)
+
+    def length(self, seq: int) -> int:
+        n = lib().iris_cuda_qwen3_lm_length(self.h, seq)
+        if n < 0:
+            raise IrisCudaError(last_error())
+        return n
+
+    def step(self, ids, seq, pos, targets=None, top_k: int = 0) -> dict:
+        """Feed tokens; per token: logprob (with targets), entropy, top_ids, top_logprobs."""
+        ip = C.POINTER(C.c_int)
+        arrs = [None if a is None else np.ascontiguousarray(a, np.int32) for a in (ids, seq, pos, targets)]
+        n = len(arrs[0])
+        if any(a is not None and a.shape != (n,) for a in arrs):
+            raise IrisCudaError("step: ids, seq, pos and targets are lists of one length")
+        out = dict(logprob=np.zeros(n, np.float32), entropy=np.zeros(n, np.float32),
+                   top_ids=np.zeros((n, top_k), np.int32), top_logprobs=np.zeros((n, top_k), np.float32))
+        rc = lib().iris_cuda_qwen3_lm_step(
+            self.h, *[None if a is None else a.ctypes.data_as(ip) for a in arrs], n, top_k, _f(out["logprob"]),
+            _f(out["entropy"]), out["top_ids"].ctypes.data_as(ip), _f(out["top_logprobs"]))
+        if rc:
+            raise IrisCudaError(last_error())
+        return out
 
 
 # ---------------------------------------------------------------- language-model operators
