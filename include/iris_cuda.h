@@ -787,7 +787,7 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
  * head_dim], rows ldq elements apart) sees the keys at positions 0 .. pos[t]
  * of sequence seq[t] (seq NULL: row t is sequence t) and reads key-value head
  * h / (heads / kv_heads):  out = softmax(scale * q K^T) V, bf16, rows ldo
- * apart.  So the newest tokens of many sequences are one call, and a run of
+ * apart, not over q or the pools.  So the newest tokens of many sequences are one call, and a run of
  * tokens of one sequence is causal.  A row that sees nothing (pos[t] < 0)
  * gives zeros; a row with seq[t] outside [0, num_seqs) is left as it was.
  * Positions past the table's end and pages outside the pool are not seen.

@@ -1166,10 +1166,11 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   LpPlan plan;
   plan.nblk = lp_blocks(a->vocab);
   constexpr int K = LpShape<In>::kBlocks;
-  // a warp begins and ends with some 100 instructions, as many as 10 values of each lane: it takes up to 8 rounds
-  // of loads, as long as every SM is left three times the 32 warps that it holds
-  const int64_t rounds = (plan.nblk + K - 1) / K * (int64_t)a->rows / ((int64_t)num_sms * 32 * 3);
-  plan.rounds = rounds < 1 ? 1 : rounds > 8 ? 8 : (int)rounds;
+  // a warp begins and ends with some 100 instructions, as many as 10 values of each lane, and in a second round of loads
+  // an SM's warps are out of step: two rounds, as long as every SM is left three times the 32 warps that it holds
+  // (512 f32 rows of 151936: 56.2 us with 1, 55.6 with 2, 56.9 with 3, 62.6 with 8; 2047 bf16 rows of 50021: 56.2,
+  // 54.1, 53.7, 56.8; 64 bf16 rows of 151936, little over one load of the device: 12.8, 15.1)
+  plan.rounds = (plan.nblk + K - 1) / K * (int64_t)a->rows >= (int64_t)num_sms * 32 * 3 * 2 ? 2 : 1;
   plan.warps = (plan.nblk + plan.rounds * K - 1) / (plan.rounds * K);
   plan.sums = (float4*)a->ws;
   plan.maxima = (uint32_t*)(plan.sums + (size_t)a->rows * plan.warps);

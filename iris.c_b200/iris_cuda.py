@@ -118,12 +118,13 @@ class KvCache(C.Structure):
         int32 [sequences, blocks].  The tensors are kept alive."""
         if _dtype(k) != "bfloat16" or _dtype(v) != "bfloat16" or _dtype(table) != "int32":
             raise IrisCudaError("KvCache: pools are bfloat16, the page table int32")
-        if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()):
+        if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or \
+                any(n > 1 and a != b for n, a, b in zip(k.shape, k.stride(), v.stride())):
             raise IrisCudaError("KvCache: pools [pages, slots, heads, columns] laid out alike")
         if k.stride(3) != 1 or len(table.shape) != 2 or table.stride(1) != 1:
             raise IrisCudaError("KvCache: columns and table rows are contiguous")
-        c = cls(k.data_ptr(), v.data_ptr(), table.data_ptr(), k.shape[0], k.shape[1], k.shape[2], k.shape[3],
-                table.shape[0], table.shape[1], table.stride(0), k.stride(0), k.stride(1), k.stride(2))
+        stride = [s if n > 1 else 0 for n, s in zip(k.shape, k.stride())]  # of an axis of one: never used
+        c = cls(k.data_ptr(), v.data_ptr(), table.data_ptr(), *k.shape, *table.shape, table.stride(0), *stride[:3])
         c.tensors = (k, v, table)
         return c
 

@@ -267,6 +267,22 @@ def test_attention_paged_rows_of_sequences(ops):
     assert (wide[:, 768:] == 9).all()
 
 
+def test_attention_paged_few_rows_cut_into_many_pieces(ops):
+    """One long sequence among rows that see nothing, see one key or are padding, in every order."""
+    kp, vp, table, ks, vs = paged([9000, 1, 40], 16, 1, 128, False, 17)
+    q = torch.randn(6, 12, 128, device="cuda", generator=gen(10)).bfloat16()
+    at = {0: (0, 8999), 1: (-1, 50), 2: (1, 0), 3: (2, -4), 4: (2, 39), 5: (7, 3)}
+    for order in ((0, 1, 2, 3, 4, 5), (5, 1, 3, 2, 4, 0), (3, 0, 5, 1, 4, 2)):
+        seq, pos = [at[r][0] for r in order], [at[r][1] for r in order]
+        out = attend(ops, kp, vp, table, q, i32(pos), i32(seq))
+        for i, (s, p) in enumerate(zip(seq, pos)):
+            if not 0 <= s < 3:
+                assert (out[i] == 9).all()
+                continue
+            want, tol = attention64(q[i], ks[s][:max(0, p + 1)], vs[s][:max(0, p + 1)], 1 / math.sqrt(128))
+            assert ((out[i].double().cpu() - want).abs() <= tol).all(), (order, i)
+
+
 def test_attention_paged_positions_and_pages_out_of_range(ops):
     """Positions past the table see the table's keys; pages outside the pool are not seen."""
     page, d = 16, 128

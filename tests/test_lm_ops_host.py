@@ -202,6 +202,9 @@ def test_binding_reads_layouts():
     c = fake_cache()
     assert (c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.num_seqs, c.max_blocks) == (8, 16, 2, 128, 3, 4)
     assert (c.table_stride, c.page_stride, c.token_stride, c.head_stride) == (4, 4096, 256, 128)
+    one = dict(k=Fake("bfloat16", 8, 16, 1, 64, stride=[1024, 64, 3, 1]), v=Fake("bfloat16", 8, 16, 1, 64, stride=[1024, 64, 5, 1]))
+    assert fake_cache(**one).head_stride == 0  # the stride of an axis of one says nothing
+    assert append(fake_cache(**one), rope=None, ldq=256, ldq_out=256, ldk=64, ldv=64, tokens=0) == 0
     by_head = [4096, 128, 2048, 1]
     c = fake_cache(k=Fake("bfloat16", 8, 16, 2, 128, stride=by_head), v=Fake("bfloat16", 8, 16, 2, 128, stride=by_head))
     assert (c.page_stride, c.token_stride, c.head_stride) == (4096, 128, 2048)
