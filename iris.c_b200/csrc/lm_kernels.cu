@@ -211,7 +211,10 @@ struct PagedShape {
 // {row, unit, later pieces, -} of every share
 __host__ __device__ __forceinline__ size_t paged_slots_at(int ctas) { return (size_t)ctas * 4; }
 
-template <int HD, int MH>
+// CLUSTER: few rows and short tables.  A cluster of blocks takes one unit, an
+// equal part of its tiles each, and joins the parts in distributed shared
+// memory: one launch, and no round through the workspace.
+template <int HD, int MH, bool CLUSTER>
 __global__ void __launch_bounds__(PagedShape<HD, MH>::kThreads, PagedShape<HD, MH>::kCtas)
 paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   using Sh = PagedShape<HD, MH>;
@@ -234,72 +237,94 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   iris::grid_dep_wait();
   iris::grid_dep_launch();
 
-  // this share's first place: prefix sums over the rows, a run of rows per thread (up to 32 rows: in each warp by itself)
-  const bool few = a.rows <= 32;
-  const int run = (a.rows + T - 1) / T, r0 = min(a.rows, (few ? lane : tid) * run), r1 = min(a.rows, r0 + run);
-  int64_t mine = 0;
-  for (int t = r0; t < r1; t++) mine += iris_paged_row_places(&cache, a.seq, a.pos, t);
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  int64_t before = incl - mine, total = 0;
-  if (few) {
-    total = __shfl_sync(0xffffffffu, incl, 31);
-  } else {
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    for (int w = 0; w < W; w++) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-    }
-  }
-  total *= units;
-  // (divisions in 32 bits where they do: 64-bit ones take a tenth of a microsecond each)
-  const int64_t share = total <= 0x7FFFFFFF ? iris_paged_share32((uint32_t)total, gridDim.x) : iris_paged_share(total, gridDim.x);
-  const int64_t start = blockIdx.x * share;
-  int4* joins = reinterpret_cast<int4*>(a.ws);
-  // rows that see nothing give zeros
-  for (int t = blockIdx.x; t < a.rows; t += gridDim.x)
-    if (iris_paged_seq(&cache, a.seq, t) >= 0 && a.pos[t] < 0) {
-      uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)t * a.ldo);
-      for (int c = tid; c < a.heads * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
-    }
-  if (start >= total) {
-    if (tid == 0) joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-    return;
-  }
   iris_paged_at_t at;
-  int64_t prefix;
-  {
-    const int64_t x = total <= 0x7FFFFFFF ? (uint32_t)start / (uint32_t)units : start / units;  // before * units <= start < (before + mine) * units
-    const bool here = before <= x && x < before + mine;
-    if (few) {
-      const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;  // run is 1: lane t holds row t
-      at.t = from;
-      prefix = __shfl_sync(0xffffffffu, before, from);
-    } else {
-      if (here) {
-        int t = r0;
-        int64_t p = before;
-        for (;; t++) {
-          const int n = iris_paged_row_places(&cache, a.seq, a.pos, t);
-          if (x < p + n) break;
-          p += n;
-        }
-        found_row = t;
-        found_prefix = p;
+  const uint32_t parts = CLUSTER ? iris::cluster_nctarank() : 1, part = CLUSTER ? iris::cluster_ctarank() : 0;
+  bool any = true;
+  if constexpr (CLUSTER) {
+    const int unit = blockIdx.x / parts;
+    at.t = unit / units;
+    at.u = unit - at.t * units;
+    iris_paged_row(&at, &cache, a.seq, a.pos);
+    if (at.n == 0) {  // nothing to see, for the whole cluster
+      if (at.s >= 0 && part == 0) {
+        const int r = at.u % (units / cache.kv_heads), h0 = at.u / (units / cache.kv_heads) * group + r * MH;
+        uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)h0 * HD);
+        for (int c = tid; c < min(MH, group - r * MH) * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
       }
-      __syncthreads();
-      at.t = found_row;
-      prefix = found_prefix;
+      return;
     }
+    at.i = (int)((int64_t)at.n * part / parts);
+    at.left = (int)((int64_t)at.n * (part + 1) / parts) - at.i;
+    any = at.left > 0;
+  } else {
+    // this share's first place: prefix sums over the rows, a run of rows per thread (up to 32 rows: in each warp by itself)
+    const bool few = a.rows <= 32;
+    const int run = (a.rows + T - 1) / T, r0 = min(a.rows, (few ? lane : tid) * run), r1 = min(a.rows, r0 + run);
+    int64_t mine = 0;
+    for (int t = r0; t < r1; t++) mine += iris_paged_row_places(&cache, a.seq, a.pos, t);
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    int64_t before = incl - mine, total = 0;
+    if (few) {
+      total = __shfl_sync(0xffffffffu, incl, 31);
+    } else {
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      for (int w = 0; w < W; w++) {
+        if (w < warp) before += scan[w];
+        total += scan[w];
+      }
+    }
+    total *= units;
+    // (divisions in 32 bits where they do: 64-bit ones take a tenth of a microsecond each)
+    const int64_t share =
+        total <= 0x7FFFFFFF ? iris_paged_share32((uint32_t)total, gridDim.x) : iris_paged_share(total, gridDim.x);
+    const int64_t start = blockIdx.x * share;
+    int4* joins = reinterpret_cast<int4*>(a.ws);
+    // rows that see nothing give zeros
+    for (int t = blockIdx.x; t < a.rows; t += gridDim.x)
+      if (iris_paged_seq(&cache, a.seq, t) >= 0 && a.pos[t] < 0) {
+        uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)t * a.ldo);
+        for (int c = tid; c < a.heads * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    if (start >= total) {
+      if (tid == 0) joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    int64_t prefix;
+    {
+      // the row whose before * units <= start < (before + mine) * units
+      const int64_t x = total <= 0x7FFFFFFF ? (uint32_t)start / (uint32_t)units : start / units;
+      const bool here = before <= x && x < before + mine;
+      if (few) {
+        const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;  // run is 1: lane t holds row t
+        at.t = from;
+        prefix = __shfl_sync(0xffffffffu, before, from);
+      } else {
+        if (here) {
+          int t = r0;
+          int64_t p = before;
+          for (;; t++) {
+            const int n = iris_paged_row_places(&cache, a.seq, a.pos, t);
+            if (x < p + n) break;
+            p += n;
+          }
+          found_row = t;
+          found_prefix = p;
+        }
+        __syncthreads();
+        at.t = found_row;
+        prefix = found_prefix;
+      }
+    }
+    any = iris_paged_start(&at, start - prefix * units, min(share, total - start), units, &cache, a.seq, a.pos);
+    if (tid == 0) joins[blockIdx.x] = make_int4(at.t, at.u, any ? iris_paged_join(&at, share) : 0, 0);
+    if (!any) return;
   }
-  const bool any = iris_paged_start(&at, start - prefix * units, min(share, total - start), units, &cache, a.seq, a.pos);
-  if (tid == 0) joins[blockIdx.x] = make_int4(at.t, at.u, any ? iris_paged_join(&at, share) : 0, 0);
-  if (!any) return;
 
   const int rtiles = units / cache.kv_heads;
   const uint32_t ring = iris::smem_u32(smem) + kg * Sh::kRing;
@@ -307,7 +332,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 
   // ---- loads, up to D - 1 stages ahead of the arithmetic
   iris_paged_at_t ld = at;
-  bool loads = true;
+  bool loads = any;
   int page, slot;                  // of this lane's key (lanes 16-31 as lanes 0-15) of the next tile to load
   int64_t head = 0;                // its head's offset
   auto find = [&]() {
@@ -317,7 +342,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     if (ld.i == 0) head = (int64_t)(ld.u / rtiles) * cache.head_stride;
   };
   head = (int64_t)(ld.u / rtiles) * cache.head_stride;
-  find();
+  if (loads) find();
   auto issue = [&](int stage) {
     if (loads) {
       const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
@@ -375,7 +400,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   clear();
   bool begun_here = at.i == 0;
   int stage = 0;
-  for (bool more = true; more;) {
+  for (bool more = any; more;) {
     more = iris_paged_more(&at);
     issue(stage == 0 ? D - 1 : stage - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
@@ -470,8 +495,10 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
           *reinterpret_cast<float2*>(to) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
         }
       }
-      const bool whole = ends && begun_here;
-      float* slot = a.ws + paged_slots_at(gridDim.x) + (size_t)(2 * blockIdx.x + (begun_here ? 1 : 0)) * Sh::kSlot;
+      const bool whole = !CLUSTER && ends && begun_here;
+      // a cluster's part stays in shared memory, where its last tile lay
+      float* slot = CLUSTER ? reinterpret_cast<float*>(smem)
+                            : a.ws + paged_slots_at(gridDim.x) + (size_t)(2 * blockIdx.x + (begun_here ? 1 : 0)) * Sh::kSlot;
       __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)head0 * HD;
       const int heads = heads_here;
       if (more) {  // the next unit's queries come while this one is joined
@@ -508,6 +535,34 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       at.i++;
       at.left--;
     }
+  }
+  if constexpr (CLUSTER) {
+    float* slot = reinterpret_cast<float*>(smem);
+    if (!any)
+      for (int h = tid; h < heads_here; h += T) slot[2 * h] = -INFINITY, slot[2 * h + 1] = 0.f;
+    __syncwarp();
+    iris::cluster_sync();
+    __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)head0 * HD;
+    for (int e = tid + part * T; e < heads_here * (HD / 4); e += T * parts) {
+      const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
+      float mm = -INFINITY, sum = 0.f;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t p = 0; p < parts; p++) {
+        const float* from = iris::cluster_map(slot, p);
+        const float2 ml = *reinterpret_cast<const float2*>(from + 2 * h);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key, and nothing in its columns
+        const float4 v = *reinterpret_cast<const float4*>(from + 2 * MH + h * HD + col);
+        const float mn = fmaxf(mm, ml.x), base = mn == -INFINITY ? 0.f : mn;
+        const float f = exp2_approx(mm - base), s = exp2_approx(ml.x - base);
+        mm = mn;
+        sum = f * sum + s * ml.y;
+        y.x = f * y.x + s * v.x, y.y = f * y.y + s * v.y, y.z = f * y.z + s * v.z, y.w = f * y.w + s * v.w;
+      }
+      const float r = sum == 0.f ? 0.f : 1.0f / sum;
+      *reinterpret_cast<uint2*>(out + h * HD + col) = make_uint2(pack2(y.x * r, y.y * r), pack2(y.z * r, y.w * r));
+    }
+    __syncwarp();
+    iris::cluster_sync();  // the others have read this block's part
   }
 }
 
@@ -619,6 +674,7 @@ paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int pe
 // LP_BLOCK = sqrt(vocab / k), 87 for 151936 and k = 20; 256 is one load of the warp
 constexpr int LP_BLOCK = 256;
 constexpr int LP_LOADS = 8;    // 16-byte loads of a lane in flight
+constexpr int LP_CLUSTER = 8, LP_CLUSTER_BLOCKS = 8192;  // blocks on a row where there are few, most blocks of values then
 
 template <typename In>
 struct LpShape {
@@ -783,29 +839,22 @@ __device__ __forceinline__ int row_offset(const In* x) {
   return (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(In));
 }
 
-template <typename In>
-__global__ void __launch_bounds__(256, 4) logprobs_stream_kernel(const __grid_constant__ IrisLogprobs a,
-                                                              const __grid_constant__ LpPlan plan) {
+// Part w of a row, by one warp; its sums and its blocks' maxima go where out says.
+template <typename In, typename Out>
+__device__ __forceinline__ void logprobs_part(const IrisLogprobs& a, const LpPlan& plan, int row, int w, Out out) {
   using Sh = LpShape<In>;
   const int lane = threadIdx.x % 32;
-  const uint32_t wid = blockIdx.x * 8 + threadIdx.x / 32;
-  iris::grid_dep_wait();
-  iris::grid_dep_launch();
-  const int64_t row = wid / (uint32_t)plan.warps;
-  if (row >= a.rows) return;
-  const int w = (int)(wid - (uint32_t)row * plan.warps);
-  const In* x = (const In*)a.logits + row * a.ld;
+  const In* x = (const In*)a.logits + (int64_t)row * a.ld;
   const int off = row_offset(x);
   float m = -INFINITY;                        // the warp's
   uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};    // the lane's, two in each register pair
   constexpr int STEP = LP_LOADS * 32 * Sh::kVec;  // values of a round
   int b = w * plan.rounds * Sh::kBlocks + lane;   // the block whose maximum this lane writes
   int e0 = w * plan.rounds * STEP - off;
-  uint32_t* maxima = plan.maxima + row * plan.nblk;
   const bool keeps = a.top_k && lane < Sh::kBlocks;
   for (int r = 0; r < plan.rounds; r++, b += Sh::kBlocks, e0 += STEP) {
     if (e0 >= a.vocab) {  // blocks are counted for the row that begins furthest from a 16-byte boundary
-      if (keeps && b < plan.nblk) maxima[b] = 0u;
+      if (keeps && b < plan.nblk) out.maximum(row, b, 0u);
       continue;
     }
     uint4 u[LP_LOADS];
@@ -827,7 +876,7 @@ __global__ void __launch_bounds__(256, 4) logprobs_stream_kernel(const __grid_co
       if (lane == i) best = cm;
       now = fmaxf(now, cm);
     }
-    if (keeps && b < plan.nblk) maxima[b] = e0 + lane * LP_BLOCK < a.vocab ? rank_bits(best) : 0u;
+    if (keeps && b < plan.nblk) out.maximum(row, b, e0 + lane * LP_BLOCK < a.vocab ? rank_bits(best) : 0u);
     if (now > m) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
@@ -872,7 +921,26 @@ __global__ void __launch_bounds__(256, 4) logprobs_stream_kernel(const __grid_co
   }
   const float2 u1 = halves(add2(s1[0], s1[1])), u2 = halves(add2(s2[0], s2[1]));
   const float t1 = warp_add(u1.x + u1.y), t2 = warp_add(u2.x + u2.y);
-  if (lane == 0) plan.sums[row * plan.warps + w] = make_float4(m, t1, t2, 0.f);
+  if (lane == 0) out.sum(make_float4(m, t1, t2, 0.f));
+}
+
+struct ToWorkspace {
+  const LpPlan& plan;
+  // parts of all rows in one line: a warp's own number is its place
+  __device__ void sum(float4 v) const { plan.sums[blockIdx.x * 8 + threadIdx.x / 32] = v; }
+  __device__ void maximum(int64_t row, int b, uint32_t r) const { plan.maxima[row * plan.nblk + b] = r; }
+};
+
+template <typename In>
+__global__ void __launch_bounds__(256, 4) logprobs_stream_kernel(const __grid_constant__ IrisLogprobs a,
+                                                                 const __grid_constant__ LpPlan plan) {
+  const uint32_t wid = blockIdx.x * 8 + threadIdx.x / 32;
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  const uint32_t row = wid / (uint32_t)plan.warps;
+  if (row >= (uint32_t)a.rows) return;
+  const int w = (int)(wid - row * plan.warps);
+  logprobs_part<In>(a, plan, (int)row, w, ToWorkspace{plan});
 }
 
 // The k largest of the places that items(f) hands to f (each thread its own
@@ -965,20 +1033,18 @@ __device__ int select_top(TopK<THREADS>& s, int k, uint64_t from, Items items) {
   return min(n, k);
 }
 
-// One block per row: the warps' sums joined, the outputs, the alternatives.
-// Bound by latency (a chain of three reads and some forty barriers).
+// The parts' sums of a row joined, the outputs, the alternatives, by THREADS
+// threads of a block (the others have left it).  Bound by latency: a chain of
+// three reads and some twenty barriers.
 template <typename In, int THREADS>
-__global__ void __launch_bounds__(THREADS) logprobs_finish_kernel(const __grid_constant__ IrisLogprobs a,
-                                                                     const __grid_constant__ LpPlan plan) {
+__device__ __forceinline__ void logprobs_row(const IrisLogprobs& a, const LpPlan& plan, int64_t row, const float4* sums,
+                                             const uint32_t* maxima) {
   using Sh = LpShape<In>;
   constexpr int WARPS = THREADS / 32, HELD = 5;
   __shared__ TopK<THREADS> top;
   __shared__ uint64_t blocks[32];
   __shared__ float red[3][WARPS];
-  const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  iris::grid_dep_wait();
-  iris::grid_dep_launch();
   const In* x = (const In*)a.logits + row * a.ld;
   float given = 0.f;
   bool has = false;
@@ -991,12 +1057,11 @@ __global__ void __launch_bounds__(THREADS) logprobs_finish_kernel(const __grid_c
     }
   }
   uint32_t held[HELD];  // the first maxima, read with the sums
-  const uint32_t* maxima = plan.maxima + row * plan.nblk;
 #pragma unroll
   for (int i = 0; i < HELD; i++) held[i] = a.top_k && tid + i * THREADS < plan.nblk ? maxima[tid + i * THREADS] : 0u;
   float m = -INFINITY, s1 = 0.f, s2 = 0.f;
   for (int w = tid; w < plan.warps; w += THREADS) {
-    float4 v = plan.sums[row * plan.warps + w];
+    float4 v = sums[w];
     const float mn = fmaxf(m, v.x);
     raise(m, s1, s2, mn);
     raise(v.x, v.y, v.z, mn);
@@ -1066,6 +1131,42 @@ __global__ void __launch_bounds__(THREADS) logprobs_finish_kernel(const __grid_c
   }
 }
 
+template <typename In, int THREADS>
+__global__ void __launch_bounds__(THREADS) logprobs_finish_kernel(const __grid_constant__ IrisLogprobs a,
+                                                                  const __grid_constant__ LpPlan plan) {
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  const int64_t row = blockIdx.x;
+  logprobs_row<In, THREADS>(a, plan, row, plan.sums + row * plan.warps, plan.maxima + row * plan.nblk);
+}
+
+// Few rows: both in one launch, a cluster per row, whose barrier stands between;
+// the parts leave their sums and maxima in the first block's shared memory.
+struct ToFirstBlock {
+  float4* sums;
+  uint32_t* maxima;
+  int w;
+  __device__ void sum(float4 v) const { *iris::cluster_map(sums + w, 0) = v; }
+  __device__ void maximum(int64_t, int b, uint32_t r) const { *iris::cluster_map(maxima + b, 0) = r; }
+};
+
+template <typename In>
+__global__ void __launch_bounds__(512, 2) logprobs_cluster_kernel(const __grid_constant__ IrisLogprobs a,
+                                                                  const __grid_constant__ LpPlan plan) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int row = blockIdx.x / LP_CLUSTER, rank = blockIdx.x % LP_CLUSTER;
+  const int w = rank * (blockDim.x / 32) + threadIdx.x / 32;
+  float4* sums = reinterpret_cast<float4*>(smem);
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(sums + plan.warps);
+  iris::cluster_sync();  // the first block is there
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  if (w < plan.warps) logprobs_part<In>(a, plan, row, w, ToFirstBlock{sums, maxima, w});
+  __syncwarp();
+  iris::cluster_sync();
+  if (rank == 0 && threadIdx.x < 128) logprobs_row<In, 128>(a, plan, row, sums, maxima);
+}
+
 }  // namespace
 
 // ------------------------------------------------------------------ launches
@@ -1096,6 +1197,8 @@ static int paged_ctas(const iris_gpu_kv_cache_t* c, int heads, int64_t rows, int
   return (int)(most >= all || most * room >= all ? all : most * room);
 }
 
+constexpr int CLUSTER_TILES = 4;
+
 template <int HD, int MH>
 struct PagedLaunch {
   using Sh = PagedShape<HD, MH>;
@@ -1104,20 +1207,35 @@ struct PagedLaunch {
     return (paged_slots_at(ctas) + (size_t)2 * ctas * Sh::kSlot) * sizeof(float);
   }
   static cudaError_t init() {
-    return cudaFuncSetAttribute(paged_attention_kernel<HD, MH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<HD, MH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               Sh::kSmem);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(paged_attention_kernel<HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
   }
   static cudaError_t launch(const IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
+    // few rows: clusters of up to 8 blocks a unit, all on the device at once, where the tables have room for no more than
+    // CLUSTER_TILES tiles a block.  On the device, two kernels -> one, 32 heads on 8 of 128: a row of 512 keys 5.9 us both,
+    // 8 rows of 512 9.2 -> 7.2, a row of 2048 (4 tiles a block) 8.0 -> 8.4, of 4096 (8 tiles) 9.4 -> 11.6; the caller is
+    // spared a launch, 3 us
+    const int64_t units = (int64_t)a->rows * iris_paged_units(&a->cache, a->heads);
+    const int room = iris_paged_tiles(iris_paged_len(&a->cache, 0x7FFFFFFF));
+    unsigned parts = 8;
+    while (parts > 1 && units * parts > (int64_t)num_sms * Sh::kCtas) parts /= 2;
+    if (parts > 1 && room <= CLUSTER_TILES * (int)parts) {
+      *launches = 1;
+      return iris::launch_cluster_overlapped(paged_attention_kernel<HD, MH, true>, dim3((unsigned)units * parts),
+                                             dim3(Sh::kThreads), Sh::kSmem, parts, stream, *a);
+    }
     const int ctas = paged_ctas<HD, MH>(&a->cache, a->heads, a->rows, num_sms);
-    cudaError_t e = iris::launch_overlapped(paged_attention_kernel<HD, MH>, dim3(ctas), dim3(Sh::kThreads), Sh::kSmem,
+    cudaError_t e = iris::launch_overlapped(paged_attention_kernel<HD, MH, false>, dim3(ctas), dim3(Sh::kThreads), Sh::kSmem,
                                             stream, *a);
     *launches = 1;
     if (e != cudaSuccess || ctas == 1) return e;
     const int group = a->heads / a->cache.kv_heads;
     *launches = 2;
     const int h = group < MH ? group : MH, fit = JOIN_THREADS / (HD / 4);
-    const int64_t all = (int64_t)a->rows * iris_paged_units(&a->cache, a->heads);
-    if (all * 8 <= ctas)
-      return iris::launch_overlapped(paged_join_kernel<HD, MH, true>, dim3((unsigned)all, h), dim3(JOIN_THREADS), 0, stream, *a,
+    if (units * 8 <= ctas)
+      return iris::launch_overlapped(paged_join_kernel<HD, MH, true>, dim3((unsigned)units, h), dim3(JOIN_THREADS), 0, stream, *a,
                                      ctas, 1);
     const int per_block = h < fit ? h : fit;
     return iris::launch_overlapped(paged_join_kernel<HD, MH, false>, dim3(ctas - 1, (h + per_block - 1) / per_block),
@@ -1162,20 +1280,33 @@ extern "C" size_t iris_logprobs_ws_bytes(int rows, int vocab) {
 }
 
 template <typename In>
-static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStream_t stream) {
+static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStream_t stream, int* launches) {
   LpPlan plan;
   plan.nblk = lp_blocks(a->vocab);
   constexpr int K = LpShape<In>::kBlocks;
+  const int all = (plan.nblk + K - 1) / K;  // rounds of loads in a row
+  plan.sums = (float4*)a->ws;
+  // few rows: a cluster of blocks of 16 warps on each, all of them on the device at once.  One launch instead of two:
+  // 3 us less of the caller's time, about as long on the device (one row of 151936, 20 alternatives: 9.1 us for 8.7)
+  const int64_t blocks = (int64_t)a->rows * LP_CLUSTER;
+  if (blocks <= 2 * num_sms && plan.nblk <= LP_CLUSTER_BLOCKS) {
+    plan.rounds = (all + 16 * LP_CLUSTER - 1) / (16 * LP_CLUSTER);
+    plan.warps = (all + plan.rounds - 1) / plan.rounds;
+    *launches = 1;
+    return iris::launch_cluster_overlapped(logprobs_cluster_kernel<In>, dim3((unsigned)blocks), dim3(512),
+                                           plan.warps * sizeof(float4) + plan.nblk * sizeof(uint32_t), LP_CLUSTER, stream, *a,
+                                           plan);
+  }
   // a warp begins and ends with some 100 instructions, as many as 10 values of each lane, and in a second round of loads
   // an SM's warps are out of step: two rounds, as long as every SM is left three times the 32 warps that it holds
   // (512 f32 rows of 151936: 56.2 us with 1, 55.6 with 2, 56.9 with 3, 62.6 with 8; 2047 bf16 rows of 50021: 56.2,
-  // 54.1, 53.7, 56.8; 64 bf16 rows of 151936, little over one load of the device: 12.8, 15.1)
-  plan.rounds = (plan.nblk + K - 1) / K * (int64_t)a->rows >= (int64_t)num_sms * 32 * 3 * 2 ? 2 : 1;
-  plan.warps = (plan.nblk + plan.rounds * K - 1) / (plan.rounds * K);
-  plan.sums = (float4*)a->ws;
+  // 54.1, 53.7, 56.8)
+  plan.rounds = all * (int64_t)a->rows >= (int64_t)num_sms * 32 * 3 * 2 ? 2 : 1;
+  plan.warps = (all + plan.rounds - 1) / plan.rounds;
   plan.maxima = (uint32_t*)(plan.sums + (size_t)a->rows * plan.warps);
   const int64_t ctas = ((int64_t)a->rows * plan.warps + 7) / 8;
   if (ctas * 8 > 0xFFFFFFFFll) return cudaErrorInvalidConfiguration;  // more logits than any device holds
+  *launches = 2;
   cudaError_t e = iris::launch_overlapped(logprobs_stream_kernel<In>, dim3((unsigned)ctas), dim3(256), 0, stream, *a, plan);
   if (e != cudaSuccess) return e;
   // 128 threads a row: 64 are 4 % faster at 2047 rows of 50021 and 8 alternatives, and at one row of 151936 and 20
@@ -1185,6 +1316,6 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
 
 extern "C" cudaError_t iris_launch_logprobs(const IrisLogprobs* a, int f32, int num_sms, cudaStream_t stream,
                                             int* launches) {
-  *launches = 2;
-  return f32 ? launch_logprobs<float>(a, num_sms, stream) : launch_logprobs<__nv_bfloat16>(a, num_sms, stream);
+  return f32 ? launch_logprobs<float>(a, num_sms, stream, launches)
+             : launch_logprobs<__nv_bfloat16>(a, num_sms, stream, launches);
 }
