@@ -812,6 +812,15 @@ __device__ __forceinline__ void vec_pairs(uint4 u, uint64_t x[8 / sizeof(In)]) {
   }
 }
 
+// One of them.
+template <typename In>
+__device__ __forceinline__ float vec_value(uint4 u, int q) {
+  constexpr int PER = 4 / sizeof(In);  // of a word
+  const uint32_t a = q & PER ? u.y : u.x, b = q & PER ? u.w : u.z, w = q & 2 * PER ? b : a;
+  if constexpr (sizeof(In) == 4) return __uint_as_float(w);
+  else return __uint_as_float(q & 1 ? w & 0xFFFF0000u : w << 16);
+}
+
 // The largest of the values, NaN if one is.
 template <typename In>
 __device__ __forceinline__ float vec_max(uint4 u) {
@@ -943,9 +952,9 @@ __global__ void __launch_bounds__(256, 4) logprobs_stream_kernel(const __grid_co
   logprobs_part<In>(a, plan, (int)row, w, ToWorkspace{plan});
 }
 
-// The k largest of the places that items(f) hands to f (each thread its own
-// share of them, the same on every call; all different, none 0), largest first,
-// into best; returns how many there are.  `from`: where it is known that k
+// The k largest of the places that items(least, f) hands to f (each thread its
+// own share of them, the same on every call; all different, none 0; it may leave
+// out values under least()), largest first, into best; returns how many there are.  `from`: where it is known that k
 // places reach it, else 0.  Without one, every thread's largest place is ranked
 // against 32 of them, and the least of the 32 that k of them reach is such a
 // value.  The few places that reach it are put in order by counting.  Only
@@ -966,7 +975,7 @@ __device__ int select_top(TopK<THREADS>& s, int k, uint64_t from, Items items) {
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   if (!from) {
     uint64_t own = 0;
-    items([&](uint64_t p) { own = p > own ? p : own; });
+    items([&]() { return own ? rank_value((uint32_t)(own >> 32)) : -INFINITY; }, [&](uint64_t p) { own = p > own ? p : own; });
     s.own[tid] = own;
     __syncthreads();
     uint64_t o[W], pick = 1;  // 1: fewer than k threads have a place
@@ -993,7 +1002,8 @@ __device__ int select_top(TopK<THREADS>& s, int k, uint64_t from, Items items) {
   while (true) {
     if (tid == 0) s.n = 0;
     __syncthreads();
-    items([&](uint64_t p) {
+    const float least = from > 1 ? rank_value((uint32_t)(from >> 32)) : -INFINITY;
+    items([&]() { return least; }, [&](uint64_t p) {
       if (p >= from) {
         const int at = atomicAdd(&s.n, 1);
         if (at < LP_LIST) s.list[at] = p;
@@ -1007,7 +1017,7 @@ __device__ int select_top(TopK<THREADS>& s, int k, uint64_t from, Items items) {
       if (tid == 0) s.sum = 0;
       __syncthreads();
       unsigned c = 0;
-      items([&](uint64_t p) { c += p >= mid; });
+      items([&]() { return least; }, [&](uint64_t p) { c += p >= mid; });
       c = __reduce_add_sync(0xffffffffu, c);
       if (tid % 32 == 0) atomicAdd(&s.sum, c);
       __syncthreads();
@@ -1087,7 +1097,7 @@ __device__ __forceinline__ void logprobs_row(const IrisLogprobs& a, const LpPlan
     if (a.entropy) a.entropy[row] = s1 == 0.f ? 0.f : log_s1 - s2 / s1;
   }
   if (!a.top_k) return;
-  const int nb = select_top(top, a.top_k, 0, [&](auto f) {
+  const int nb = select_top(top, a.top_k, 0, [&](auto, auto f) {
 #pragma unroll
     for (int i = 0; i < HELD; i++)
       if (held[i]) f(place(held[i], tid + i * THREADS));
@@ -1100,9 +1110,8 @@ __device__ __forceinline__ void logprobs_row(const IrisLogprobs& a, const LpPlan
   __syncthreads();
   // k blocks: each holds a value no less than the k-th maximum
   const uint64_t from = nb == a.top_k ? blocks[nb - 1] >> 32 << 32 : 0;
-  const float least = from ? rank_value((uint32_t)(from >> 32)) : -INFINITY;  // NaN: everything may reach it
   const int off = row_offset(x);
-  select_top(top, a.top_k, from, [&](auto f) {
+  select_top(top, a.top_k, from, [&](auto least, auto f) {
     constexpr int VPB = LP_BLOCK / Sh::kVec, FLY = 5;
     for (int j0 = tid; j0 < nb * VPB; j0 += FLY * THREADS) {
       uint4 u[FLY];
@@ -1115,12 +1124,17 @@ __device__ __forceinline__ void logprobs_row(const IrisLogprobs& a, const LpPlan
       }
 #pragma unroll
       for (int i = 0; i < FLY; i++) {
-        if (vec_max<In>(u[i]) < least) continue;
+        // which values are not under least (a NaN is under nothing): few, so that they are taken one by one
+        const float lo = least();
         float v[Sh::kVec];
         vec_values<In>(u[i], v);
+        uint32_t reach = 0;
 #pragma unroll
-        for (int q = 0; q < Sh::kVec; q++)
-          if (!(v[q] < least) && e[i] + q >= 0 && e[i] + q < a.vocab) f(place(rank_bits(v[q]), (uint32_t)(e[i] + q)));
+        for (int q = 0; q < Sh::kVec; q++) reach |= v[q] < lo ? 0u : 1u << q;
+        for (; reach; reach &= reach - 1) {
+          const int q = __ffs(reach) - 1, id = e[i] + q;
+          if ((uint32_t)id < (uint32_t)a.vocab) f(place(rank_bits(vec_value<In>(u[i], q)), (uint32_t)id));
+        }
       }
     }
   });
@@ -1287,7 +1301,7 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   const int all = (plan.nblk + K - 1) / K;  // rounds of loads in a row
   plan.sums = (float4*)a->ws;
   // few rows: a cluster of blocks of 16 warps on each, all of them on the device at once.  One launch instead of two:
-  // 3 us less of the caller's time, about as long on the device (one row of 151936, 20 alternatives: 9.1 us for 8.7)
+  // 3 us less of the caller's time, about as long on the device (one row of 151936, 20 alternatives: 8.0 us in either)
   const int64_t blocks = (int64_t)a->rows * LP_CLUSTER;
   if (blocks <= 2 * num_sms && plan.nblk <= LP_CLUSTER_BLOCKS) {
     plan.rounds = (all + 16 * LP_CLUSTER - 1) / (16 * LP_CLUSTER);
