@@ -238,13 +238,16 @@ ATT = [  # lengths, heads, kv heads, d, page, head major
 def test_attention_paged(ops, lens, nh, nkv, d, page, hm):
     kp, vp, table, ks, vs = paged(lens, page, nkv, d, hm, len(lens) + d)
     q = (2 * torch.randn(len(lens), nh, d, device="cuda", generator=gen(3))).bfloat16()
-    out = attend(ops, kp, vp, table, q, i32(lens) - 1)
-    again = attend(ops, kp, vp, table, q, i32(lens) - 1)
-    assert torch.equal(out, again)
-    for i in range(len(lens)):
-        want, tol = attention64(q[i], ks[i], vs[i], 1 / math.sqrt(d))
-        err = (out[i].double().cpu() - want).abs()
-        assert (err <= tol).all(), (i, float((err - tol).max()))
+    # tables with room for much longer sequences are worked on in another way
+    roomy = torch.full((len(lens), table.shape[1] + 40000 // page), -1, device="cuda", dtype=torch.int32)
+    roomy[:, :table.shape[1]] = table
+    want = [attention64(q[i], ks[i], vs[i], 1 / math.sqrt(d)) for i in range(len(lens))]
+    for tab in (table, roomy):
+        out = attend(ops, kp, vp, tab, q, i32(lens) - 1)
+        assert torch.equal(out, attend(ops, kp, vp, tab, q, i32(lens) - 1))
+        for i, (w, tol) in enumerate(want):
+            err = (out[i].double().cpu() - w).abs()
+            assert (err <= tol).all(), (i, float((err - tol).max()))
 
 
 def test_attention_paged_rows_of_sequences(ops):
@@ -436,9 +439,12 @@ def test_token_logprobs_hard_rows(ops, f32, vocab):
     t = torch.full((len(rows),), vocab // 3, device="cuda", dtype=torch.int32)
     t[9] = 6
     check_answers(x, t, 20, answers(ops, x, t, 20))
+    x, t = x.repeat(5, 1), t.repeat(5)  # many rows go another way
+    check_answers(x, t, 32, answers(ops, x, t, 32))
 
 
-def test_token_logprobs_rows_without_an_answer(ops):
+@pytest.mark.parametrize("many", [1, 10])
+def test_token_logprobs_rows_without_an_answer(ops, many):
     """-inf everywhere, NaN, +inf: the documented values, and neighbours that do not notice."""
     vocab, k = 5000, 6
     x = torch.randn(6, vocab, device="cuda", generator=gen(2))
@@ -449,16 +455,19 @@ def test_token_logprobs_rows_without_an_answer(ops):
     x[3] = math.nan
     x[4, 9], x[4, 8], x[4, 3000] = math.nan, math.inf, math.inf
     for ty in (torch.float32, torch.bfloat16):
-        y = x.to(ty)
+        y = x.to(ty).repeat(many, 1)
         t = i32([3, 3, 3, 3, 3, 3])
-        lp, en, ids, tl = answers(ops, y, t, k)
+        got = answers(ops, y, t.repeat(many), k)
+        for part in range(1, many):  # (bits: a NaN is not itself)
+            assert all(torch.equal(g[:6].view(torch.int32), g[6 * part:6 * part + 6].view(torch.int32)) for g in got)
+        lp, en, ids, tl = (g[:6] for g in got)
         assert lp[0] == -math.inf and en[0] == 0 and (tl[0] == -math.inf).all()
         assert ids[0].tolist() == list(range(k))
         assert torch.isnan(lp[1:5]).all() and torch.isnan(en[1:5]).all() and torch.isnan(tl[1:5]).all()
         assert ids[1, :2].tolist() == [77, 4000] and ids[2, 0] == 123 and ids[3].tolist() == list(range(k))
         assert ids[4, :3].tolist() == [9, 8, 3000]
         check_answers(plain[None].to(ty), t[5:], k, (lp[5:], en[5:], ids[5:], tl[5:]))
-        lp, en, ids, tl = answers(ops, y, i32([-1] * 6), k)
+        lp, en, ids, tl = answers(ops, y, i32([-1] * 6 * many), k)
         assert (lp == 0).all()
 
 
