@@ -193,9 +193,10 @@ template <int HD, int MH>
 struct PagedShape {
   static constexpr int kPair = HD / 128 ? HD / 128 : 1;          // warps on the same 16 keys, 128 columns of o each
   static constexpr int kThreads = 128 * kPair;
-  // CTAs on an SM and stages of a ring, as measured on 256 rows of 0 to 2048 keys at head_dim 64 (14 heads on 2): 4 x 2
-  // 38 us, 3 x 4 40 us, 2 x 6 46 us (the arithmetic of 16 short keys is latency, and wants warps); at 128 and 256 a ring
-  // of three stages fills shared memory, with MH = 16 two
+  // CTAs on an SM and stages of a ring.  At head_dim 64 (256 rows of 0 to 2048 keys, 14 heads on 2) 4 x 2 took 0.84 and
+  // 3 x 4 0.88 of the time of 2 x 6, 5 x 2 1.03 and 6 x 2 1.4 of that of 4 x 2: the arithmetic of 16 short keys is
+  // latency and wants warps, until registers spill.  At 128 and 256 a ring of three stages fills shared memory, with MH =
+  // 16 two.
   static constexpr int kCtas = HD == 64 ? 4 : HD == 128 ? 2 : 1;
   static constexpr int kStages = HD == 64 || MH == 16 ? 2 : 3;
   static constexpr int kStageBytes = 16 * HD * 2;                // 16 rows of K or of V
@@ -669,8 +670,9 @@ paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int pe
 // e^(m - m').  For the alternatives the pass leaves the largest value of every
 // block: the k largest values of a row lie in the k blocks with the largest
 // maxima (each of k blocks ahead of another one holds a value ahead of all of
-// the other's), so the second kernel reads those k blocks again and nothing else.
-// LP_BLOCK values a block: the second kernel reads vocab / LP_BLOCK maxima and k LP_BLOCK values, alike at
+// the other's), so what follows reads those k blocks again and nothing else.
+
+// LP_BLOCK values a block: vocab / LP_BLOCK maxima and k LP_BLOCK values are read again, alike at
 // LP_BLOCK = sqrt(vocab / k), 87 for 151936 and k = 20; 256 is one load of the warp
 constexpr int LP_BLOCK = 256;
 constexpr int LP_LOADS = 8;    // 16-byte loads of a lane in flight

@@ -20,8 +20,8 @@ struct iris_cuda_qwen3_lm {
     iris_cuda_qwen3_t *m;
     int num_seqs, max_len, max_tokens, blocks;
     /* host: tokens each sequence holds, the same in the step being checked, and which step last named it */
-    int *len, *next, *named;
-    int step;
+    int *len, *next;
+    uint64_t *named, step;
     /* device */
     int32_t *table;         /* [num_seqs, blocks], shared by all layers */
     uint16_t *pools;        /* [layers][k, v][pages, LM_PAGE, kv_heads, 128] */
@@ -101,7 +101,7 @@ iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_se
     lm_cache(lm, 0, &cache);
     lm->len = (int *)calloc((size_t)num_seqs, sizeof(int));
     lm->next = (int *)calloc((size_t)num_seqs, sizeof(int));
-    lm->named = (int *)calloc((size_t)num_seqs, sizeof(int));
+    lm->named = (uint64_t *)calloc((size_t)num_seqs, sizeof(uint64_t));
     lm->h_in = (int32_t *)malloc(4 * T * 4);
     if (!lm->len || !lm->next || !lm->named || !lm->h_in) rc = iris_fail(IRIS_CUDA_ERR_OOM, "language model session");
 #define ALLOC(dst, bytes) \
