@@ -706,10 +706,10 @@ unsigned long iris_gpu_op_failures(void);
  * Manner of iris_gpu_adaln_norm_bf16_noalloc: raw device pointers the caller
  * owns and a cudaStream_t (void *, 0 = default stream); work is queued
  * without synchronising, nothing is allocated, so the calls may be captured
- * into a graph.  Pointers must be device memory of the library's device
- * (iris_cuda_init).  Arguments are checked before anything is queued:
- * IRIS_CUDA_ERR_ARG with the reason in iris_cuda_last_error(), counted by
- * iris_gpu_op_failures().  Values in device memory (positions, sequence and
+ * into a graph (iris_cuda_init before the first capture).  Pointers must be
+ * device memory of the library's device.  Arguments are checked before
+ * anything is queued: IRIS_CUDA_ERR_ARG with the reason in
+ * iris_cuda_last_error(), counted by iris_gpu_op_failures().  Values in device memory (positions, sequence and
  * page numbers, targets) can not be checked then; the kernels bound them and
  * never read or write outside the tensors they are given.  A workspace is
  * scratch of one call: calls that may overlap on the GPU (two streams, two
@@ -791,8 +791,11 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
  * tokens of one sequence is causal.  A row that sees nothing (pos[t] < 0)
  * gives zeros; a row with seq[t] outside [0, num_seqs) is left as it was.
  * Positions past the table's end and pages outside the pool are not seen.
- * The same call gives the same bits every time; among other rows a row's sum
- * may be split elsewhere and differ in its last bits before rounding.
+ * Rows of one sequence that stand next to each other read the cache together
+ * where there are four times as many rows as sequences or more: list the
+ * tokens of a prompt one behind the other.  The same call gives the same bits
+ * every time; among other rows a row's sum may be split elsewhere and differ in
+ * its last bits before rounding.
  * Workspace: iris_gpu_attention_paged_workspace bytes, 16-byte aligned. */
 size_t iris_gpu_attention_paged_workspace(const iris_gpu_kv_cache_t *cache, int heads);
 int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const void *q, int64_t ldo, int64_t ldq,

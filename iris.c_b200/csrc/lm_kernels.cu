@@ -2,6 +2,8 @@
 // cache, attention over the cache, and token log probabilities with entropy
 // and the best alternatives.  Sums, softmax statistics and rotations are f32;
 // bf16 appears where the tensors have it, rounded once on the way out.
+#include <type_traits>
+
 #include "iris_kernels.h"
 #include "paged.h"
 #include "ptx.cuh"
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
 //   s = q k^T      mma m16n8k16, rows = up to 8 query heads of the head's group
 //   p = 2^(s c - m), c = scale log2(e);  l = l 2^(m_old - m) + sum p
 //   o = o 2^(m_old - m) + p v
-// p counts with 16 bits, bf16(p) + bf16(p - bf16(p)) (with 8 the result would be
+// p counts with 16 bits, its first 8 and bf16(the rest) (with 8 the result would be
 // off by sqrt(2) of its own rounding).  Up to 8 heads fill half of the product's
 // rows and the second parts the other half, at no extra instruction; the halves
 // of o are added at the end.  For 9 to 16 heads on a key-value head the second
@@ -183,6 +185,19 @@ __device__ __forceinline__ void mma_bf16(float d[4], uint32_t a0, uint32_t a1, u
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// of two bf16, all bits of each one that is an infinity or NaN
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
+  return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+}
+
+// Two weights as a first part of 8 bits, cut off, and a second one of the next 8, rounded.  The last bit of a weight is
+// set, so that neither part of one above 0 is 0 or less: times an infinite value, both are the infinity.
+__device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  const uint32_t b0 = __float_as_uint(p0) | 1u, b1 = __float_as_uint(p1) | 1u;
+  hi = __byte_perm(b0, b1, 0x7632);
+  lo = pack2(__uint_as_float(b0) - __uint_as_float(b0 & 0xFFFF0000u), __uint_as_float(b1) - __uint_as_float(b1 & 0xFFFF0000u));
+}
+
 // 16 bytes, or zeros where `bytes` is 0 (nothing is read then)
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -209,8 +224,86 @@ struct PagedShape {
 };
 
 // Offset of the first slot in the workspace (floats), after the joins
-// {row, unit, later pieces, -} of every share
+// of every share
 __host__ __device__ __forceinline__ size_t paged_slots_at(int ctas) { return (size_t)ctas * 4; }
+
+// A CTA's first place of the line, and its entry of the joins {row, unit, later pieces, rows of the run}; rows that see
+// nothing get their zeros.  `places`: of one unit of a row.  False where there is no tile in its share.
+template <int T, typename Places>
+__device__ __forceinline__ bool paged_begin(const IrisPagedAttention& a, int units, iris_paged_at_t* at, Places places) {
+  constexpr int W = T / 32;
+  __shared__ int64_t scan[W];
+  __shared__ int64_t found_prefix;
+  __shared__ int found_row;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  // this share's first place: prefix sums over the rows, a run of rows per thread (up to 32 rows: in each warp by itself)
+  const bool few = a.rows <= 32;
+  const int run = (a.rows + T - 1) / T, r0 = min(a.rows, (few ? lane : tid) * run), r1 = min(a.rows, r0 + run);
+  int64_t mine = 0;
+  for (int t = r0; t < r1; t++) mine += places(t);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  int64_t before = incl - mine, total = 0;
+  if (few) {
+    total = __shfl_sync(0xffffffffu, incl, 31);
+  } else {
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    for (int w = 0; w < W; w++) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+  }
+  total *= units;
+  // (divisions in 32 bits where they do: 64-bit ones take a tenth of a microsecond each)
+  const int64_t share =
+      total <= 0x7FFFFFFF ? iris_paged_share32((uint32_t)total, gridDim.x) : iris_paged_share(total, gridDim.x);
+  const int64_t start = blockIdx.x * share;
+  int4* joins = reinterpret_cast<int4*>(a.ws);
+  // rows that see nothing give zeros
+  for (int t = blockIdx.x; t < a.rows; t += gridDim.x)
+    if (iris_paged_seq(&a.cache, a.seq, t) >= 0 && a.pos[t] < 0) {
+      uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)t * a.ldo);
+      for (int c = tid; c < a.heads * (a.cache.head_dim / 8); c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  if (start >= total) {
+    if (tid == 0) joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return false;
+  }
+  int64_t prefix;
+  {
+    // the row whose before * units <= start < (before + mine) * units
+    const int64_t x = total <= 0x7FFFFFFF ? (uint32_t)start / (uint32_t)units : start / units;
+    const bool here = before <= x && x < before + mine;
+    if (few) {
+      const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;  // run is 1: lane t holds row t
+      at->t = from;
+      prefix = __shfl_sync(0xffffffffu, before, from);
+    } else {
+      if (here) {
+        int t = r0;
+        int64_t p = before;
+        for (;; t++) {
+          const int n = places(t);
+          if (x < p + n) break;
+          p += n;
+        }
+        found_row = t;
+        found_prefix = p;
+      }
+      __syncthreads();
+      at->t = found_row;
+      prefix = found_prefix;
+    }
+  }
+  const bool any = iris_paged_start(at, start - prefix * units, min(share, total - start), units, &a.cache, a.seq, a.pos);
+  if (tid == 0) joins[blockIdx.x] = make_int4(at->t, at->u, any ? iris_paged_join(at, share) : 0, at->count);
+  return any;
+}
 
 // CLUSTER: few rows and short tables.  A cluster of blocks takes one unit, an
 // equal part of its tiles each, and joins the parts in distributed shared
@@ -220,12 +313,9 @@ __global__ void __launch_bounds__(PagedShape<HD, MH>::kThreads, PagedShape<HD, M
 paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   using Sh = PagedShape<HD, MH>;
   constexpr int D = Sh::kStages, CH = HD / 8;  // CH: 16-byte chunks of a row
-  constexpr int PAIR = Sh::kPair, T = Sh::kThreads, W = T / 32, OC = HD / PAIR;  // OC: columns of o a warp holds
+  constexpr int PAIR = Sh::kPair, T = Sh::kThreads, OC = HD / PAIR;  // OC: columns of o a warp holds
   constexpr bool WIDE = MH == 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t scan[W];
-  __shared__ int64_t found_prefix;
-  __shared__ int found_row;
   __shared__ uint32_t seen[4][D];  // of each 16 keys of a tile and stage: which exist
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, i4 = lane % 4;
   const int kg = warp / PAIR, half = warp % PAIR;  // which 16 keys of a tile, which columns of o
@@ -239,6 +329,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   iris::grid_dep_launch();
 
   iris_paged_at_t at;
+  at.rows = at.span = at.count = 0;
   const uint32_t parts = CLUSTER ? iris::cluster_nctarank() : 1, part = CLUSTER ? iris::cluster_ctarank() : 0;
   bool any = true;
   if constexpr (CLUSTER) {
@@ -258,72 +349,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     at.left = (int)((int64_t)at.n * (part + 1) / parts) - at.i;
     any = at.left > 0;
   } else {
-    // this share's first place: prefix sums over the rows, a run of rows per thread (up to 32 rows: in each warp by itself)
-    const bool few = a.rows <= 32;
-    const int run = (a.rows + T - 1) / T, r0 = min(a.rows, (few ? lane : tid) * run), r1 = min(a.rows, r0 + run);
-    int64_t mine = 0;
-    for (int t = r0; t < r1; t++) mine += iris_paged_row_places(&cache, a.seq, a.pos, t);
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    int64_t before = incl - mine, total = 0;
-    if (few) {
-      total = __shfl_sync(0xffffffffu, incl, 31);
-    } else {
-      if (lane == 31) scan[warp] = incl;
-      __syncthreads();
-      for (int w = 0; w < W; w++) {
-        if (w < warp) before += scan[w];
-        total += scan[w];
-      }
-    }
-    total *= units;
-    // (divisions in 32 bits where they do: 64-bit ones take a tenth of a microsecond each)
-    const int64_t share =
-        total <= 0x7FFFFFFF ? iris_paged_share32((uint32_t)total, gridDim.x) : iris_paged_share(total, gridDim.x);
-    const int64_t start = blockIdx.x * share;
-    int4* joins = reinterpret_cast<int4*>(a.ws);
-    // rows that see nothing give zeros
-    for (int t = blockIdx.x; t < a.rows; t += gridDim.x)
-      if (iris_paged_seq(&cache, a.seq, t) >= 0 && a.pos[t] < 0) {
-        uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)t * a.ldo);
-        for (int c = tid; c < a.heads * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
-      }
-    if (start >= total) {
-      if (tid == 0) joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-      return;
-    }
-    int64_t prefix;
-    {
-      // the row whose before * units <= start < (before + mine) * units
-      const int64_t x = total <= 0x7FFFFFFF ? (uint32_t)start / (uint32_t)units : start / units;
-      const bool here = before <= x && x < before + mine;
-      if (few) {
-        const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;  // run is 1: lane t holds row t
-        at.t = from;
-        prefix = __shfl_sync(0xffffffffu, before, from);
-      } else {
-        if (here) {
-          int t = r0;
-          int64_t p = before;
-          for (;; t++) {
-            const int n = iris_paged_row_places(&cache, a.seq, a.pos, t);
-            if (x < p + n) break;
-            p += n;
-          }
-          found_row = t;
-          found_prefix = p;
-        }
-        __syncthreads();
-        at.t = found_row;
-        prefix = found_prefix;
-      }
-    }
-    any = iris_paged_start(&at, start - prefix * units, min(share, total - start), units, &cache, a.seq, a.pos);
-    if (tid == 0) joins[blockIdx.x] = make_int4(at.t, at.u, any ? iris_paged_join(&at, share) : 0, 0);
+    any = paged_begin<T>(a, units, &at, [&](int t) { return iris_paged_row_places(&cache, a.seq, a.pos, t); });
     if (!any) return;
   }
 
@@ -445,9 +471,8 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         const float p0 = exp2_approx(x0 - base), p1 = exp2_approx(x1 - base), p2 = exp2_approx(x2 - base),
                     p3 = exp2_approx(x3 - base);
         l[h] = l[h] * f[h] + ((p0 + p1) + (p2 + p3));
-        hi[h][0] = pack2(p0, p1), hi[h][1] = pack2(p2, p3);
-        const float2 u0 = unpack2(hi[h][0]), u1 = unpack2(hi[h][1]);
-        lo[h][0] = pack2(p0 - u0.x, p1 - u0.y), lo[h][1] = pack2(p2 - u1.x, p3 - u1.y);
+        split2(p0, p1, hi[h][0], lo[h][0]);
+        split2(p2, p3, hi[h][1], lo[h][1]);
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -567,6 +592,340 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   }
 }
 
+// Several rows of a sequence, as the tokens of a prompt: a unit is a run of up
+// to 64 / heads (head_dim 256: 128 / heads) consecutive rows of one sequence
+// (paged.h), one key-value head and up to 16 of the query heads on it, so that
+// the cache is read once for all of them.  Each warp holds 16 (row, head) pairs and
+// goes over all keys of a tile, which the block loads together, two tiles ahead;
+// what none of its pairs sees it leaves out.  A unit of up to 16 pairs would leave
+// all warps but one idle: there four warps take 16 keys of a tile each for all
+// pairs, and their sums are joined in shared memory.  Bound by the products, 6 flops
+// a score and column, two of them for the second part of p, and by a warp's softmax
+// between them: registers allow two warps a scheduler, the tensor pipe of mma.sync
+// is active 55 % of the time (a prompt of 8192, 32 heads on 8 of 128: 209 TFLOP/s
+// counting 4 flops).  Three CTAs on an SM with half the scores in registers spilled
+// (240 us for 194 with a prompt of 2048).
+template <int HD>
+struct RunShape {
+  static constexpr int kPairs = HD == 256 ? 128 : 64;             // (row, head) pairs of a unit
+  static constexpr int kWarps = kPairs / 16, kThreads = 32 * kWarps;
+  // CTAs on an SM: what registers allow (a warp holds queries, scores and o of 16 pairs; at head_dim 64 four spill)
+  static constexpr int kCtas = HD == 64 ? 3 : HD == 128 ? 2 : 1;
+  static constexpr int kStages = 3;  // (two: a prompt of 2048, 32 heads on 8 of 128, 244 us for 227)
+  // keys whose scores a warp holds at a time; a prompt of 2048, 8 heads on 2 of 256, with four warps: 16 330 us, 32 248,
+  // with eight 157
+  static constexpr int kKeys = HD == 256 ? 32 : 64;
+  static constexpr int kPart = IRIS_PAGED_TILE * HD * 2;          // bytes of K or of V of a tile
+  static constexpr int kSlot = kPairs * (HD + 2);                 // floats of a piece, as in PagedShape
+  static constexpr int kSmem = kStages * 2 * kPart;
+};
+
+// query heads of a unit of runs
+__device__ __forceinline__ int run_heads(int group) { return group < 16 ? group : 16; }
+
+template <int HD>
+__global__ void __launch_bounds__(RunShape<HD>::kThreads, RunShape<HD>::kCtas)
+paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
+  using Sh = RunShape<HD>;
+  constexpr int D = Sh::kStages, CH = HD / 8, T = Sh::kThreads, NB = HD / 8;
+  constexpr int MINE = IRIS_PAGED_TILE / Sh::kWarps;  // keys of a tile that a warp loads, 16 or 8
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint16_t seen[D][4];  // of each 16 keys of a stage's tile: which exist
+  __shared__ float2 red_ml[64];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, i4 = lane % 4;
+  const iris_gpu_kv_cache_t& cache = a.cache;
+  const int units = iris_paged_units(&cache, a.heads), group = a.heads / cache.kv_heads, rtiles = units / cache.kv_heads;
+  const int hu = run_heads(group), span = Sh::kPairs / hu;
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  iris_paged_at_t at;
+  at.rows = a.rows, at.span = span, at.count = 0;
+  if (!paged_begin<T>(a, units, &at, [&](int t) {
+        return iris_paged_run_places(&cache, a.seq, a.pos, a.rows, span, t);
+      }))
+    return;
+
+  // ---- loads, up to D - 1 stages ahead of the arithmetic: each warp its keys of a tile
+  iris_paged_at_t ld = at;
+  bool loads = true;
+  int page, slot;  // of this lane's key (the lanes past a warp's keys as its first) of the next tile to load
+  int64_t head;    // its head's offset
+  auto find = [&]() {
+    const int p = ld.i * IRIS_PAGED_TILE + warp * MINE + lane % MINE, b = iris_paged_block(a.div, p);
+    slot = p - b * cache.page_size;
+    page = p < ld.len ? iris_paged_page(&cache, ld.s, b) : -1;
+    head = (int64_t)(ld.u / rtiles) * cache.head_stride;
+  };
+  find();
+  const uint32_t ring = iris::smem_u32(smem);
+  auto issue = [&](int stage) {
+    if (loads) {
+      const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & ((1u << MINE) - 1);
+      const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
+      if (lane == 0) {
+        if constexpr (MINE == 16) seen[stage][warp] = (uint16_t)have;
+        else reinterpret_cast<uint8_t*>(seen[stage])[warp] = (uint8_t)have;
+      }
+      const uint32_t kd = ring + stage * 2 * Sh::kPart + warp * MINE * HD * 2, vd = kd + Sh::kPart;
+      constexpr int RPI = 32 / CH;  // rows one instruction of the warp covers
+#pragma unroll
+      for (int j = 0; j < MINE / RPI; j++) {
+        const int r = j * RPI + lane / CH, ch = lane % CH;
+        const int64_t o = __shfl_sync(0xffffffffu, off, r) + ch * 8;
+        const int bytes = (have >> r) & 1 ? 16 : 0;
+        const uint32_t d = r * (HD * 2) + ((ch ^ (r & 7)) << 4);
+        cp_async16(kd + d, (const __nv_bfloat16*)cache.k + o, bytes);
+        cp_async16(vd + d, (const __nv_bfloat16*)cache.v + o, bytes);
+      }
+      loads = iris_paged_more(&ld);
+      if (loads) {
+        iris_paged_next(&ld, units, &cache, a.seq, a.pos);
+        find();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int s = 0; s < D - 1; s++) issue(s);
+
+  // ---- arithmetic.  This lane's pairs: e = warp 16 + g and e + 8; pair e is row e / hu, head e % hu of the unit.
+  // (`narrow`: a unit of up to 16 pairs, e = g and e + 8 in each of four warps)
+  const float c = a.scale * 1.4426950408889634f;
+  uint32_t qf[HD / 16][4];
+  float o[NB][4], m[2], l[2];
+  int row[2], col0[2], len[2];  // the pair's row of the call, its head's first column, its keys (0: no such pair)
+  int most = 0, least = 0;      // of the warp's pairs
+  bool narrow = false;
+  auto begin_unit = [&]() {
+    narrow = at.count * hu <= 16;
+    const int kvh = at.u / rtiles, r = at.u - kvh * rtiles;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int e = (narrow && warp < 4 ? 0 : warp * 16) + g + 8 * h, in = e / hu, hh = e - in * hu;
+      const bool live = in < at.count && hh < group - r * 16;
+      row[h] = at.t + in;
+      col0[h] = (kvh * group + r * 16 + hh) * HD;
+      len[h] = live ? iris_paged_len(&cache, a.pos[at.t + in]) : 0;
+      const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)row[h] * a.ldq + col0[h] + 2 * i4;
+#pragma unroll
+      for (int j = 0; j < HD / 16; j++) {
+        qf[j][h] = live ? *reinterpret_cast<const uint32_t*>(q + j * 16) : 0u;
+        qf[j][2 + h] = live ? *reinterpret_cast<const uint32_t*>(q + j * 16 + 8) : 0u;
+      }
+      if (!live) row[h] = -1;
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+    }
+    // (a pair that does not exist gives nothing, whatever its sums)
+    most = (int)__reduce_max_sync(0xffffffffu, (unsigned)max(len[0], len[1]));
+    least = (int)__reduce_min_sync(0xffffffffu, (unsigned)min(row[0] < 0 ? 0x7FFFFFFF : len[0], row[1] < 0 ? 0x7FFFFFFF : len[1]));
+#pragma unroll
+    for (int j = 0; j < NB; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  };
+  begin_unit();
+  bool begun_here = at.i == 0;
+  int stage = 0;
+  for (bool more = true; more;) {
+    more = iris_paged_more(&at);
+    asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+    __syncthreads();  // this tile has come, and the one before it is done with
+    issue(stage == 0 ? D - 1 : stage - 1);
+    const uint32_t kd = ring + stage * 2 * Sh::kPart, vd = kd + Sh::kPart;
+    const int first = at.i * IRIS_PAGED_TILE;
+    // this warp's pairs and keys k0 .. of the tile; `plain`: all pairs see them all
+    auto step = [&](auto keys, auto plain, int k0) {
+      constexpr int KEYS = decltype(keys)::value;
+      constexpr bool PLAIN = decltype(plain)::value;
+      const int live = most - first - k0, clear = least - first - k0;  // keys from k0 on that a pair sees, that all see
+      // scores of a row and 8 keys: keys 2 i4, 2 i4 + 1 of row g, then of row g + 8
+      float s[KEYS / 8][4];
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      // matrices (keys 0-7, columns 0-7), (keys 0-7, 8-15), (keys 8-15, 0-7), (keys 8-15, 8-15) of each 16 columns
+      const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+#pragma unroll
+      for (int j = 0; j < HD / 16; j++)
+#pragma unroll
+        for (int n = 0; n < KEYS / 16; n++) {
+          if (!PLAIN && n * 16 >= live) continue;
+          uint32_t b[4];
+          ldsm4(b, kd + (k0 + n * 16 + kr) * (HD * 2) + (((2 * j + kc) ^ (kr & 7)) << 4));
+          mma_bf16(s[2 * n], qf[j][0], qf[j][1], qf[j][2], qf[j][3], b[0], b[1]);
+          mma_bf16(s[2 * n + 1], qf[j][0], qf[j][1], qf[j][2], qf[j][3], b[2], b[3]);
+        }
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < KEYS / 16; n++) {
+        const uint32_t have = seen[stage][k0 / 16 + n];
+        const bool all = PLAIN || ((n + 1) * 16 <= clear && have == 0xFFFFu);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int h = e / 2 % 2, key = e / 4 * 8 + 2 * i4 + e % 2;
+          float& x = s[2 * n + e / 4][e % 4];
+          x *= c;
+          if (!all && (n * 16 + key >= len[h] - first - k0 || !(have >> key & 1))) x = -INFINITY;
+          mx[h] = fmaxf(mx[h], x);
+        }
+      }
+      float f[2], base[2];
+      bool moved = false;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float mn = mx[h];
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
+        mn = fmaxf(mn, m[h]);
+        base[h] = mn == -INFINITY ? 0.f : mn;  // scores of -inf weigh nothing
+        f[h] = exp2_approx(m[h] - base[h]);
+        moved |= mn != m[h];
+        m[h] = mn;
+        l[h] *= f[h];
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int j = 0; j < NB; j++) o[j][0] *= f[0], o[j][1] *= f[0], o[j][2] *= f[1], o[j][3] *= f[1];
+      }
+      // transposed: (keys 0-7, columns 0-7), (keys 8-15, 0-7), (keys 0-7, 8-15), (keys 8-15, 8-15)
+      const int vr = lane & 15, vc = lane >> 4;
+      auto add_values = [&](auto finite) {
+#pragma unroll
+        for (int n = 0; n < KEYS / 16; n++) {
+          if (!PLAIN && n * 16 >= live) continue;
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {  // rows g, g + 8, g, g + 8; keys 0-7, 0-7, 8-15, 8-15
+            const int h = k & 1, b = 2 * n + k / 2;
+            const float p0 = exp2_approx(s[b][2 * h] - base[h]), p1 = exp2_approx(s[b][2 * h + 1] - base[h]);
+            l[h] += p0 + p1;
+            split2(p0, p1, hi[k], lo[k]);
+          }
+#pragma unroll
+          for (int j = 0; j < HD / 16; j++) {
+            uint32_t b[4];
+            ldsm4t(b, vd + (k0 + n * 16 + vr) * (HD * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
+            if constexpr (!decltype(finite)::value) {
+#pragma unroll
+              for (int k = 0; k < 4; k++) b[k] &= ~not_finite2(b[k]);
+            }
+            mma_bf16(o[2 * j], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
+            mma_bf16(o[2 * j + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
+            mma_bf16(o[2 * j], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
+            mma_bf16(o[2 * j + 1], lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
+          }
+        }
+      };
+      // A value that one of the rows must not see may be an infinity or NaN, which a weight of zero does not take out of
+      // the product: where there are any, they go in by themselves, to the rows that see them.
+      bool odd = false;
+      if (!PLAIN && clear < KEYS) {
+        for (int e = max(0, clear) * CH + lane; e < min(KEYS, (live + 15) & ~15) * CH; e += 32) {
+          const uint4 v = *reinterpret_cast<const uint4*>(smem + (vd - ring) + (k0 * CH + e) * 16);
+          odd |= (not_finite2(v.x) | not_finite2(v.y) | not_finite2(v.z) | not_finite2(v.w)) != 0;
+        }
+        odd = __any_sync(0xffffffffu, odd);
+      }
+      if (!odd) {
+        add_values(std::true_type());
+      } else {
+        add_values(std::false_type());
+        for (int key = k0; key < k0 + min(KEYS, live); key++)
+#pragma unroll
+          for (int j = 0; j < NB; j++) {
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(smem + (vd - ring) + key * (HD * 2) +
+                                                                  ((j ^ (key & 7)) << 4) + i4 * 4);
+            const uint32_t bad = not_finite2(v);
+            if (!bad) continue;
+            const float2 x = unpack2(v & bad);  // the finite one as 0
+            if (key < len[0] - first) o[j][0] += x.x, o[j][1] += x.y;
+            if (key < len[1] - first) o[j][2] += x.x, o[j][3] += x.y;
+          }
+      }
+    };
+    if (first < most) {
+      const uint2 all = *reinterpret_cast<const uint2*>(seen[stage]);
+      const bool plain = first <= least - IRIS_PAGED_TILE && (all.x & all.y) == 0xFFFFFFFFu;
+      constexpr std::integral_constant<int, 16> few{};
+      constexpr std::integral_constant<int, Sh::kKeys> many{};
+      if (narrow) {
+        if (plain) step(few, std::true_type(), warp * 16);
+        else step(few, std::false_type(), warp * 16);
+      } else if (plain) {
+#pragma unroll
+        for (int k0 = 0; k0 < IRIS_PAGED_TILE; k0 += Sh::kKeys) step(many, std::true_type(), k0);
+      } else {
+#pragma unroll
+        for (int k0 = 0; k0 < IRIS_PAGED_TILE; k0 += Sh::kKeys)
+          if (first + k0 < most) step(many, std::false_type(), k0);
+      }
+    }
+    float* red = reinterpret_cast<float*>(smem + stage * 2 * Sh::kPart);
+    stage = stage == D - 1 ? 0 : stage + 1;
+    const bool ends = at.i == at.n - 1;
+    if (ends || !more) {  // this unit, or the piece of it that is here
+      float* slot = a.ws + paged_slots_at(gridDim.x) + (size_t)(2 * blockIdx.x + (begun_here ? 1 : 0)) * Sh::kSlot;
+      if (narrow) __syncthreads();  // all are done with the tile, whose place the sums take
+      const bool whole = ends && begun_here;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (row[h] < 0) continue;
+        const int e = warp * 16 + g + 8 * h;
+        if (whole && !narrow) {
+          const float r = l[h] == 0.f ? 0.f : 1.0f / l[h];
+          __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)row[h] * a.ldo + col0[h] + 2 * i4;
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+            *reinterpret_cast<uint32_t*>(out + j * 8) = pack2(o[j][2 * h] * r, o[j][2 * h + 1] * r);
+        } else {
+          float* to = (narrow ? red : slot + 2 * Sh::kPairs) + e * HD;
+          const int turn = narrow ? (g & 3) << 3 : 0;  // the eight pairs of a store's half warp fall into different banks
+          if (i4 == 0) (narrow ? red_ml : reinterpret_cast<float2*>(slot))[e] = make_float2(m[h], l[h]);
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+            *reinterpret_cast<float2*>(to + ((j * 8 + 2 * i4) ^ turn)) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+        }
+      }
+      if (narrow) {
+        const int kvh = at.u / rtiles, r = at.u - kvh * rtiles, hs = min(hu, group - r * 16);
+        __syncthreads();
+        for (int x = threadIdx.x; x < at.count * hu * (HD / 4); x += T) {
+          const int e = x / (HD / 4), col = (x % (HD / 4)) * 4, in = e / hu, hh = e - in * hu;
+          if (hh >= hs) continue;
+          float mm = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; w++) mm = fmaxf(mm, red_ml[w * 16 + e].x);
+          const float to_base = mm == -INFINITY ? 0.f : mm;
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const float f = exp2_approx(red_ml[w * 16 + e].x - to_base);
+            sum += f * red_ml[w * 16 + e].y;
+            const float4 v = *reinterpret_cast<const float4*>(red + (w * 16 + e) * HD + (col ^ (e & 3) << 3));
+            y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+          }
+          if (whole) {
+            const float f = sum == 0.f ? 0.f : 1.0f / sum;
+            *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + (int64_t)(at.t + in) * a.ldo +
+                                      (int64_t)(kvh * group + r * 16 + hh) * HD + col) =
+                make_uint2(pack2(y.x * f, y.y * f), pack2(y.z * f, y.w * f));
+          } else {
+            if (col == 0) slot[2 * e] = mm, slot[2 * e + 1] = sum;
+            *reinterpret_cast<float4*>(slot + 2 * Sh::kPairs + e * HD + col) = y;
+          }
+        }
+      }
+      if (more) {
+        iris_paged_next(&at, units, &cache, a.seq, a.pos);
+        begin_unit();
+        begun_here = true;
+      }
+    } else {
+      at.i++;
+      at.left--;
+    }
+  }
+}
+
 // Adds up the pieces of cut units.  A thread takes four columns of a head; where
 // those are fewer than the threads, the block has parts that take every
 // parts-th piece each and are added at the end.  Two ways to find the pieces:
@@ -658,6 +1017,52 @@ paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int pe
   const int head = kvh * group + r * MH + h;
   *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + (int64_t)row * a.ldo + (int64_t)head * HD + col * 4) =
       make_uint2(pack2(y.x * f, y.y * f), pack2(y.z * f, y.w * f));
+}
+
+// The same for pieces of runs: two blocks per share border.
+constexpr int RUN_JOIN_THREADS = 256;
+
+template <int HD>
+__global__ void __launch_bounds__(RUN_JOIN_THREADS)
+paged_runs_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas) {
+  constexpr int COLS = HD / 4, SLOT = RunShape<HD>::kSlot;
+  const int units = iris_paged_units(&a.cache, a.heads), group = a.heads / a.cache.kv_heads, rtiles = units / a.cache.kv_heads;
+  const int c = blockIdx.x + 1, hu = run_heads(group);
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  const int4 j = reinterpret_cast<const int4*>(a.ws)[c];
+  if (j.z == 0) return;
+  const int n = j.z + 1, kvh = j.y / rtiles, r = j.y - kvh * rtiles;
+  const float* slots = a.ws + paged_slots_at(ctas);
+  for (int x = blockIdx.y * RUN_JOIN_THREADS + threadIdx.x; x < j.w * hu * COLS; x += gridDim.y * RUN_JOIN_THREADS) {
+    const int e = x / COLS, col = x % COLS * 4, in = e / hu, hh = e - in * hu;
+    if (hh >= group - r * 16) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < n; p += 4) {
+      float2 s[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int q = min(p + k, n - 1);
+        const float* slot = slots + (size_t)(q == 0 ? 2 * c - 1 : 2 * (c + q - 1)) * SLOT;
+        s[k] = *reinterpret_cast<const float2*>(slot + 2 * e);
+        v[k] = *reinterpret_cast<const float4*>(slot + 2 * RunShape<HD>::kPairs + e * HD + col);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if (p + k >= n) continue;
+        const float mn = fmaxf(m, s[k].x), base = mn == -INFINITY ? 0.f : mn;
+        const float f = exp2_approx(m - base), g = exp2_approx(s[k].x - base);
+        m = mn;
+        l = f * l + g * s[k].y;
+        y.x = f * y.x + g * v[k].x, y.y = f * y.y + g * v[k].y, y.z = f * y.z + g * v[k].z, y.w = f * y.w + g * v[k].w;
+      }
+    }
+    const float f = l == 0.f ? 0.f : 1.0f / l;
+    *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + (int64_t)(j.x + in) * a.ldo + (int64_t)(kvh * group + r * 16 + hh) * HD + col) =
+        make_uint2(pack2(y.x * f, y.y * f), pack2(y.z * f, y.w * f));
+  }
 }
 
 // ------------------------------------------------------------------ log probabilities
@@ -1205,12 +1610,10 @@ extern "C" cudaError_t iris_launch_rope_append(IrisRopeAppend* a, int f32, int n
 }
 
 // CTAs of an attention launch: as many as the device holds at once, no more than the tables have room for tiles
-template <int HD, int MH>
-static int paged_ctas(const iris_gpu_kv_cache_t* c, int heads, int64_t rows, int num_sms) {
-  const int64_t all = (int64_t)num_sms * PagedShape<HD, MH>::kCtas;
+static int paged_ctas(const iris_gpu_kv_cache_t* c, int heads, int64_t rows, int all) {
   const int64_t room = iris_paged_tiles(iris_paged_len(c, 0x7FFFFFFF)) + IRIS_PAGED_EXTRA;
   const int64_t most = rows * iris_paged_units(c, heads);
-  return (int)(most >= all || most * room >= all ? all : most * room);
+  return most >= all || most * room >= all ? all : (int)(most * room);
 }
 
 constexpr int CLUSTER_TILES = 4;
@@ -1218,12 +1621,17 @@ constexpr int CLUSTER_TILES = 4;
 template <int HD, int MH>
 struct PagedLaunch {
   using Sh = PagedShape<HD, MH>;
+  using Runs = RunShape<HD>;
   static size_t ws_bytes(int num_sms) {
-    const int ctas = num_sms * Sh::kCtas;
-    return (paged_slots_at(ctas) + (size_t)2 * ctas * Sh::kSlot) * sizeof(float);
+    const int ctas = num_sms * Sh::kCtas, runs = num_sms * Runs::kCtas;
+    const size_t one = paged_slots_at(ctas) + (size_t)2 * ctas * Sh::kSlot;
+    const size_t several = paged_slots_at(runs) + (size_t)2 * runs * Runs::kSlot;
+    return (one > several ? one : several) * sizeof(float);
   }
   static cudaError_t init() {
-    const cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<HD, MH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(paged_runs_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Runs::kSmem);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(paged_attention_kernel<HD, MH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                Sh::kSmem);
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute(paged_attention_kernel<HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
@@ -1242,7 +1650,20 @@ struct PagedLaunch {
       return iris::launch_cluster_overlapped(paged_attention_kernel<HD, MH, true>, dim3((unsigned)units * parts),
                                              dim3(Sh::kThreads), Sh::kSmem, parts, stream, *a);
     }
-    const int ctas = paged_ctas<HD, MH>(&a->cache, a->heads, a->rows, num_sms);
+    // four times as many rows as sequences: runs of rows.  On the device, 32 heads on 8 of 128, rows by themselves -> runs:
+    // a prompt of 64 9.3 -> 10.3 us, 128 15.4 -> 15.6, 512 84 -> 31, 2048 943 -> 194, 8192 13.9 -> 2.6 ms; 64 tokens behind
+    // 32704 867 -> 188; 4 behind 4092 in 8 sequences 69 -> 38, 2 there 41 -> 36, but 2 behind 1022 in 64, 8 heads on 2 of
+    // 256, 49 -> 55, and 64 single tokens at 1023 beside a prompt of 128 (3 rows a sequence) 55 -> 93, of 512 119 -> 111.
+    // (The host knows no more of the rows; 2048 rows of 4 sequences in random order, no runs in them: 306 -> 550.)
+    if (a->seq && a->rows >= 4 * (int64_t)a->cache.num_seqs) {
+      const int ctas = paged_ctas(&a->cache, a->heads, a->rows, num_sms * Runs::kCtas);
+      const cudaError_t e = iris::launch_overlapped(paged_runs_kernel<HD>, dim3(ctas), dim3(Runs::kThreads), Runs::kSmem, stream, *a);
+      *launches = 1;
+      if (e != cudaSuccess || ctas == 1) return e;
+      *launches = 2;
+      return iris::launch_overlapped(paged_runs_join_kernel<HD>, dim3(ctas - 1, 2), dim3(RUN_JOIN_THREADS), 0, stream, *a, ctas);
+    }
+    const int ctas = paged_ctas(&a->cache, a->heads, a->rows, num_sms * Sh::kCtas);
     cudaError_t e = iris::launch_overlapped(paged_attention_kernel<HD, MH, false>, dim3(ctas), dim3(Sh::kThreads), Sh::kSmem,
                                             stream, *a);
     *launches = 1;
@@ -1303,7 +1724,7 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   const int all = (plan.nblk + K - 1) / K;  // rounds of loads in a row
   plan.sums = (float4*)a->ws;
   // few rows: a cluster of blocks of 16 warps on each, all of them on the device at once.  One launch instead of two:
-  // 3 us less of the caller's time, about as long on the device (one row of 151936, 20 alternatives: 8.0 us in either)
+  // 3 us less of the caller's time, about as long on the device
   const int64_t blocks = (int64_t)a->rows * LP_CLUSTER;
   if (blocks <= 2 * num_sms && plan.nblk <= LP_CLUSTER_BLOCKS) {
     plan.rounds = (all + 16 * LP_CLUSTER - 1) / (16 * LP_CLUSTER);

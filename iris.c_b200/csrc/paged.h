@@ -9,7 +9,9 @@
  * all rows stand in one line (row by row, unit by unit, tile by tile) that is
  * cut into equal shares, one per CTA, whatever the rows' lengths.  To begin and
  * finish a unit takes a CTA about as long as a tile, so that every unit has one
- * empty place in the line behind its tiles (IRIS_PAGED_EXTRA).  A unit cut
+ * empty place in the line behind its tiles (IRIS_PAGED_EXTRA).  Where a call
+ * has several rows of a sequence, a unit can be a run of them instead of one
+ * (iris_paged_run); the first stands in the line for all.  A unit cut
  * by a share's border is summed in pieces: a CTA leaves at most two, slot 2 c
  * for a piece whose unit began in an earlier share, slot 2 c + 1 for one that
  * begins here and goes on.
@@ -62,6 +64,31 @@ IRIS_HD int iris_paged_row_places(const iris_gpu_kv_cache_t *c, const int32_t *s
     return n ? n + IRIS_PAGED_EXTRA : 0;
 }
 
+/* A run: consecutive rows of one sequence, none past a multiple of `span` rows.
+ * The number of rows in the run that begins at row t and the most keys that one
+ * of them sees; 0 where row t is not the first of its run, or padding. */
+IRIS_HD int iris_paged_run(const iris_gpu_kv_cache_t *c, const int32_t *seq, const int32_t *pos, int rows, int span, int t,
+                           int *len) {
+    const int in = t % span, s = seq[t], end = rows - t < span - in ? rows : t - in + span;
+    int n = 0, most = -1, more = 1;
+    *len = 0;
+    if (s < 0 || s >= c->num_seqs || (in && seq[t - 1] == s)) return 0;
+    for (int r = t; r < end; r++) {  /* no way out, so that the loads need not wait for one another */
+        const int p = pos[r];
+        more &= seq[r] == s;
+        n += more;
+        most = more && p > most ? p : most;
+    }
+    *len = iris_paged_len(c, most);
+    return n;
+}
+IRIS_HD int iris_paged_run_places(const iris_gpu_kv_cache_t *c, const int32_t *seq, const int32_t *pos, int rows, int span,
+                                  int t) {
+    int len;
+    iris_paged_run(c, seq, pos, rows, span, t, &len);
+    return len ? iris_paged_tiles(len) + IRIS_PAGED_EXTRA : 0;
+}
+
 /* p / page_size for 0 <= p < 2^31 as p * mul >> shift: shift = 31 + ceil(log2 page_size), mul = ceil(2^shift /
  * page_size) <= 2^32 - 1, and p (mul page_size - 2^shift) < 2^31 page_size <= 2^shift keeps the floor */
 typedef struct { uint32_t mul; int shift; } iris_paged_div_t;
@@ -98,11 +125,14 @@ typedef struct {
     int n;        /* tiles of each of its units   */
     int u;        /* unit                         */
     int i;        /* tile of the unit             */
+    int rows;     /* rows of the call, span: of which a unit may hold so many (0: one row a unit, `rows` and `count` unused) */
+    int span, count; /* count: rows of this run   */
 } iris_paged_at_t;
 
 IRIS_HD void iris_paged_row(iris_paged_at_t *a, const iris_gpu_kv_cache_t *c, const int32_t *seq, const int32_t *pos) {
     a->s = iris_paged_seq(c, seq, a->t);
-    a->len = a->s < 0 ? 0 : iris_paged_len(c, pos[a->t]);
+    if (a->span) a->count = iris_paged_run(c, seq, pos, a->rows, a->span, a->t, &a->len);
+    else a->len = a->s < 0 ? 0 : iris_paged_len(c, pos[a->t]);
     a->n = iris_paged_tiles(a->len);
 }
 
@@ -116,7 +146,7 @@ IRIS_HD void iris_paged_unit(iris_paged_at_t *a, int units, const iris_gpu_kv_ca
     if (++a->u < units) return;
     a->u = 0;
     do {
-        a->t++;
+        a->t += a->span && a->count > 1 ? a->count : 1;
         iris_paged_row(a, c, seq, pos);
     } while (a->n == 0);
 }
