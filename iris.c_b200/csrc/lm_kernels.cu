@@ -305,7 +305,7 @@ __device__ __forceinline__ bool paged_begin(const IrisPagedAttention& a, int uni
   return any;
 }
 
-// CLUSTER: few rows and short tables.  A cluster of blocks takes one unit, an
+// CLUSTER: few rows and short tables.  A cluster of blocks, or one, takes one unit, an
 // equal part of its tiles each, and joins the parts in distributed shared
 // memory: one launch, and no round through the workspace.
 template <int HD, int MH, bool CLUSTER>
@@ -1585,7 +1585,7 @@ __global__ void __launch_bounds__(512, 2) logprobs_cluster_kernel(const __grid_c
   if (w < plan.warps) logprobs_part<In>(a, plan, row, w, ToFirstBlock{sums, maxima, w});
   __syncwarp();
   iris::cluster_sync();
-  if (rank == 0 && threadIdx.x < 128) logprobs_row<In, 128>(a, plan, row, sums, maxima);
+  if (rank == 0 && threadIdx.x < 256) logprobs_row<In, 256>(a, plan, row, sums, maxima);
 }
 
 }  // namespace
@@ -1637,15 +1637,20 @@ struct PagedLaunch {
     return cudaFuncSetAttribute(paged_attention_kernel<HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
   }
   static cudaError_t launch(const IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
-    // few rows: clusters of up to 8 blocks a unit, all on the device at once, where the tables have room for no more than
-    // CLUSTER_TILES tiles a block.  On the device, two kernels -> one, 32 heads on 8 of 128: a row of 512 keys 5.9 us both,
-    // 8 rows of 512 9.2 -> 7.2, a row of 2048 (4 tiles a block) 8.0 -> 8.4, of 4096 (8 tiles) 9.4 -> 11.6; the caller is
-    // spared a launch, 3 us
+    // few rows: a block, or a cluster of up to 8, on each unit, all on the device at once (clusters of 4 and 8 do not fill
+    // every SM: 72 of 4, 288 blocks of 296, took 11.7 us with 512 keys, 72 of 2 7.5), where the tables have room for no
+    // more than CLUSTER_TILES tiles a block, or where the blocks are more than half of what the device holds, up to twice
+    // that: equal shares of all tiles gain the less the fewer CTAs would be idle without.  On the device, two kernels ->
+    // one, 32 heads on 8 of 128: a row of 512 keys 5.9 us both, 8 rows of 512 9.2 -> 7.2, a row of 2048 (4 tiles a block)
+    // 8.0 -> 8.4, of 4096 (8 tiles) 9.4 -> 11.6, 37 rows of 200 10.3 -> 8.3, of 512 (8 tiles, every slot taken) 15.6 ->
+    // 12.9, of 1 to 512 13.0 -> 12.0, 6 rows of 1200 (5 tiles) 11.2 -> 10.0; the caller is spared a launch, 3 us
     const int64_t units = (int64_t)a->rows * iris_paged_units(&a->cache, a->heads);
     const int room = iris_paged_tiles(iris_paged_len(&a->cache, 0x7FFFFFFF));
     unsigned parts = 8;
-    while (parts > 1 && units * parts > (int64_t)num_sms * Sh::kCtas) parts /= 2;
-    if (parts > 1 && room <= CLUSTER_TILES * (int)parts) {
+    const int64_t slots = (int64_t)num_sms * Sh::kCtas;
+    while (parts > 1 && units * parts > (parts > 2 ? slots * 7 / 8 : slots)) parts /= 2;
+    const int64_t tiles = 2 * CLUSTER_TILES * units * parts / slots + 1;  // 2 CLUSTER_TILES with every slot taken
+    if (units * parts <= slots && room <= (tiles < CLUSTER_TILES ? CLUSTER_TILES : tiles) * parts) {
       *launches = 1;
       return iris::launch_cluster_overlapped(paged_attention_kernel<HD, MH, true>, dim3((unsigned)units * parts),
                                              dim3(Sh::kThreads), Sh::kSmem, parts, stream, *a);
@@ -1723,10 +1728,11 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   constexpr int K = LpShape<In>::kBlocks;
   const int all = (plan.nblk + K - 1) / K;  // rounds of loads in a row
   plan.sums = (float4*)a->ws;
-  // few rows: a cluster of blocks of 16 warps on each, all of them on the device at once.  One launch instead of two:
-  // 3 us less of the caller's time, about as long on the device
+  // few rows: a cluster of blocks of 16 warps on each, all of them on the device at once (clusters of 8 do not fill every
+  // SM: 32 of 37).  One launch instead of two: 2.5 us less of the caller's time.  On the device, bf16 rows of 151936 with
+  // 20 alternatives, one launch and two: 1 row 7.9 and 7.6 us, 16 9.0 and 8.5, 32 10.4 and 9.3, 36 12.3 and 9.4
   const int64_t blocks = (int64_t)a->rows * LP_CLUSTER;
-  if (blocks <= 2 * num_sms && plan.nblk <= LP_CLUSTER_BLOCKS) {
+  if (blocks <= 2 * num_sms * 7 / 8 && plan.nblk <= LP_CLUSTER_BLOCKS) {
     plan.rounds = (all + 16 * LP_CLUSTER - 1) / (16 * LP_CLUSTER);
     plan.warps = (all + plan.rounds - 1) / plan.rounds;
     *launches = 1;
@@ -1746,8 +1752,12 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   *launches = 2;
   cudaError_t e = iris::launch_overlapped(logprobs_stream_kernel<In>, dim3((unsigned)ctas), dim3(256), 0, stream, *a, plan);
   if (e != cudaSuccess) return e;
-  // 128 threads a row: 64 are 4 % faster at 2047 rows of 50021 and 8 alternatives, and at one row of 151936 and 20
-  // take 12.7 us for 8.6
+  // Rows that are all on the device at once (4 blocks an SM) take 256 threads each.  128 -> 256: one row of 151936 and 20
+  // alternatives (in the cluster) 8.2 -> 7.9 us, 192 f32 rows of 65537 with 8 14.9 -> 13.0, with 32 21.1 -> 15.3, 512 f32
+  // rows of 151936 with 5 54.5 -> 53.5; with 512 one row takes 8.6 and 100 f32 rows of 151936 with 8 14.8 for 13.6.  More
+  // rows, 128: 2047 bf16 rows of 50021 with 24 59.2 for 67.6 us
+  if (a->rows <= 4 * num_sms)
+    return iris::launch_overlapped(logprobs_finish_kernel<In, 256>, dim3(a->rows), dim3(256), 0, stream, *a, plan);
   return iris::launch_overlapped(logprobs_finish_kernel<In, 128>, dim3(a->rows), dim3(128), 0, stream, *a, plan);
 }
 
