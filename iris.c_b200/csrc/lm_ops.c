@@ -84,7 +84,7 @@ static int rope_layout_check(const iris_gpu_rope_t *r, int layout, int rot_dim, 
 int iris_gpu_rope_init_freqs(iris_gpu_rope_t *rope, int layout, int rot_dim, const double *freqs, double amplitude) {
     if (rope_layout_check(rope, layout, rot_dim, "rope_init")) return IRIS_CUDA_ERR_ARG;
     if (!freqs) return LM_FAIL("rope_init: null frequencies");
-    if (!isfinite(amplitude) || amplitude <= 0.0) return LM_FAIL("rope_init: amplitude %g", amplitude);
+    if (!isfinite((float)amplitude) || !((float)amplitude > 0.0f)) return LM_FAIL("rope_init: amplitude %g", amplitude);
     for (int i = 0; i < rot_dim / 2; i++)
         if (!isfinite(freqs[i]) || freqs[i] < 0.0) return LM_FAIL("rope_init: frequency %d is %g", i, freqs[i]);
     memset(rope, 0, sizeof(*rope));

@@ -249,3 +249,9 @@ def test_binding_refuses_other_tensors():
                     top_logprobs=Fake("float32", 5, 3)), **bad}
         with pytest.raises(E):
             iris_cuda.token_logprobs(*d.values(), workspace=Fake("uint8", 1 << 20))
+
+
+@pytest.mark.parametrize("amplitude", (1e300, 1e-60, 0.0, -1.0, float("nan"), float("inf")))
+def test_rope_amplitude_outside_f32(amplitude):
+    with pytest.raises(iris_cuda.IrisCudaError, match="amplitude"):
+        Rope.of(64, 1e4, amplitude=amplitude)

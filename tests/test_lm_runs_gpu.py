@@ -112,6 +112,20 @@ def test_attention_paged_runs_pages_out_of_range(ops):
     assert (out[7:] == 0).all()
 
 
+@pytest.mark.parametrize("rows,nh,nkv,d,longest", [(30, 32, 8, 128, 256), (37, 8, 8, 128, 500), (70, 8, 4, 64, 130), (12, 16, 8, 256, 300), (9, 32, 8, 128, 512)])
+def test_attention_paged_a_block_a_unit(ops, rows, nh, nkv, d, longest):
+    """As many units as the device holds blocks or half of them, short tables: sequences of no key to all, padding."""
+    lens = [(i * 37) % (longest + 1) for i in range(rows - 2)] + [longest, 1]
+    kp, vp, table, ks, vs = paged(lens, 16, nkv, d, False, 32)
+    pos = [n - 1 for n in lens]
+    seq = list(range(rows))
+    seq[3], seq[5] = -1, rows
+    q = torch.randn(rows, nh, d, device="cuda", generator=gen(33)).bfloat16()
+    out = attend(ops, kp, vp, table, q, i32(pos), i32(seq))
+    check(out, q, seq, pos, ks, vs)
+    assert torch.equal(out, attend(ops, kp, vp, table, q, i32(pos), i32(seq)))
+
+
 def test_attention_paged_runs_captured(ops):
     """A captured call sees the positions, sequences and pages of its replay."""
     kp, vp, table, ks, vs = paged([400, 200], 16, 2, 128, False, 30)
