@@ -1362,10 +1362,11 @@ __global__ void __launch_bounds__(256, 4) logprobs_stream_kernel(const __grid_co
 // The k largest of the places that items(least, f) hands to f (each thread its
 // own share of them, the same on every call; all different, none 0; it may leave
 // out values under least()), largest first, into best; returns how many there are.  `from`: where it is known that k
-// places reach it, else 0.  Without one, every thread's largest place is ranked
-// against 32 of them, and the least of the 32 that k of them reach is such a
-// value.  The few places that reach it are put in order by counting.  Only
-// where more than LP_LIST do, many of the largest in one thread's share, is a
+// places reach it, else 0.  Without one, or where many reach it (the
+// least maximum of a few blocks is not far up), every thread's largest place is
+// ranked against 32 of them, and the least of the 32 that k of them reach is such a
+// value.  The few places that reach it are put in order by counting.  Only where
+// more than LP_LIST do even then, many of the largest in one thread's share, is a
 // closer value searched by halving.
 constexpr int LP_LIST = 512;
 template <int THREADS>
@@ -1380,33 +1381,34 @@ template <int THREADS, typename Items>
 __device__ int select_top(TopK<THREADS>& s, int k, uint64_t from, Items items) {
   constexpr int W = THREADS / 32;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  if (!from) {
-    uint64_t own = 0;
-    items([&]() { return own ? rank_value((uint32_t)(own >> 32)) : -INFINITY; }, [&](uint64_t p) { own = p > own ? p : own; });
-    s.own[tid] = own;
-    __syncthreads();
-    uint64_t o[W], pick = 1;  // 1: fewer than k threads have a place
-    int reach = THREADS + 1;
+  for (int step = from ? 0 : 1;; step++) {  // 0: what is known, 1: with the ranking, then: closer
+    if (step == 1) {
+      uint64_t own = 0;
+      items([&]() { return own ? rank_value((uint32_t)(own >> 32)) : -INFINITY; }, [&](uint64_t p) { own = p > own ? p : own; });
+      s.own[tid] = own;
+      __syncthreads();
+      uint64_t o[W], pick = 1;  // 1: fewer than k threads have a place
+      int reach = THREADS + 1;
 #pragma unroll
-    for (int i = 0; i < W; i++) o[i] = s.own[i * 32 + lane];
+      for (int i = 0; i < W; i++) o[i] = s.own[i * 32 + lane];
 #pragma unroll
-    for (int j = 0; j < 32 / W; j++) {
-      const uint64_t c = s.own[(warp * (32 / W) + j) * W];
-      int n = 0;
+      for (int j = 0; j < 32 / W; j++) {
+        const uint64_t c = s.own[(warp * (32 / W) + j) * W];
+        int n = 0;
 #pragma unroll
-      for (int i = 0; i < W; i++) n += o[i] >= c;
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (c && n >= k && n < reach) pick = c, reach = n;
+        for (int i = 0; i < W; i++) n += o[i] >= c;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (c && n >= k && n < reach) pick = c, reach = n;
+      }
+      if (lane == 0) s.pick[warp] = pick, s.reach[warp] = reach;
+      __syncthreads();
+      uint64_t ranked = s.pick[0];
+      reach = s.reach[0];
+#pragma unroll
+      for (int i = 1; i < W; i++)
+        if (s.reach[i] < reach) ranked = s.pick[i], reach = s.reach[i];
+      from = ranked > from ? ranked : from;
     }
-    if (lane == 0) s.pick[warp] = pick, s.reach[warp] = reach;
-    __syncthreads();
-    from = s.pick[0];
-    reach = s.reach[0];
-#pragma unroll
-    for (int i = 1; i < W; i++)
-      if (s.reach[i] < reach) from = s.pick[i], reach = s.reach[i];
-  }
-  while (true) {
     if (tid == 0) s.n = 0;
     __syncthreads();
     const float least = from > 1 ? rank_value((uint32_t)(from >> 32)) : -INFINITY;
@@ -1417,7 +1419,8 @@ __device__ int select_top(TopK<THREADS>& s, int k, uint64_t from, Items items) {
       }
     });
     __syncthreads();
-    if (s.n <= LP_LIST) break;
+    if (s.n <= (step == 0 ? LP_LIST / 2 : LP_LIST)) break;  // (putting n in order takes n^2 steps)
+    if (step == 0) continue;
     uint64_t hi = 0xFF800002ull << 32;  // over all places
     while (true) {
       const uint64_t mid = from + (hi - from) / 2;
@@ -1754,11 +1757,14 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   if (e != cudaSuccess) return e;
   // Rows that are all on the device at once (4 blocks an SM) take 256 threads each.  128 -> 256: one row of 151936 and 20
   // alternatives (in the cluster) 8.2 -> 7.9 us, 192 f32 rows of 65537 with 8 14.9 -> 13.0, with 32 21.1 -> 15.3, 512 f32
-  // rows of 151936 with 5 54.5 -> 53.5; with 512 one row takes 8.6 and 100 f32 rows of 151936 with 8 14.8 for 13.6.  More
-  // rows, 128: 2047 bf16 rows of 50021 with 24 59.2 for 67.6 us
+  // rows of 151936 with 5 54.5 -> 53.5; with 512 one row takes 8.6 and 100 f32 rows of 151936 with 8 14.8 for 13.6
   if (a->rows <= 4 * num_sms)
     return iris::launch_overlapped(logprobs_finish_kernel<In, 256>, dim3(a->rows), dim3(256), 0, stream, *a, plan);
-  return iris::launch_overlapped(logprobs_finish_kernel<In, 128>, dim3(a->rows), dim3(128), 0, stream, *a, plan);
+  // (9 blocks of 128 an SM) 128 -> 64: 2047 bf16 rows of 50021 with 8 53.3 -> 51.1, with 32 61.3 -> 63.4, 4000 of 32000
+  // with 8 70.9 -> 64.2, 1300 of 32000 with 8 26.0 for 27.8
+  if (a->rows <= 9 * num_sms)
+    return iris::launch_overlapped(logprobs_finish_kernel<In, 128>, dim3(a->rows), dim3(128), 0, stream, *a, plan);
+  return iris::launch_overlapped(logprobs_finish_kernel<In, 64>, dim3(a->rows), dim3(64), 0, stream, *a, plan);
 }
 
 extern "C" cudaError_t iris_launch_logprobs(const IrisLogprobs* a, int f32, int num_sms, cudaStream_t stream,
