@@ -1,0 +1,28 @@
+"""Sessions of the text model with room for many tokens: prompts long enough for
+runs of rows, a few tokens behind one, single tokens over a long table, against
+the numpy oracle's decoder layers with the tolerance of test_qwen3_lm_gpu."""
+import numpy as np
+import pytest
+
+from gpu_util import rel_l2
+from test_qwen3_lm_gpu import TOL, logprobs_ref, model, rows, texts  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def test_long_prompts_and_continuations(iris, model):  # noqa: F811
+    m, _, w = model
+    ids = texts([231, 41], 7)
+    ref = [logprobs_ref(w, t[:-1]) for t in ids]
+    lm = iris.Qwen3Lm(m, num_seqs=2, max_len=8192, max_tokens=256)
+    got, want, at = [], [], [0, 0]
+    # 190 + 20 rows, 12 and 8 rows, single tokens of both, one alone
+    for new in ((190, 20), (12, 8), (1, 1), (1, 1), (1, 0), (25, 10)):
+        parts = [(s, at[s], ids[s][at[s]:at[s] + n]) for s, n in enumerate(new) if n]
+        tg = np.concatenate([ids[s][at[s] + 1:at[s] + n + 1] for s, n in enumerate(new) if n])
+        got += list(lm.step(*rows(parts), targets=tg)["logprob"])
+        want += [ref[s][at[s] + j, ids[s][at[s] + j + 1]] for s, n in enumerate(new) for j in range(n)]
+        at = [a + n for a, n in zip(at, new)]
+    assert [lm.length(s) for s in (0, 1)] == at == [230, 40]
+    assert rel_l2(got, want) < TOL
+    lm.close()
