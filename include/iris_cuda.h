@@ -791,6 +791,11 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
  * tokens of one sequence is causal.  A row that sees nothing (pos[t] < 0)
  * gives zeros; a row with seq[t] outside [0, num_seqs) is left as it was.
  * Positions past the table's end and pages outside the pool are not seen.
+ * Keys and values that are not finite show in the rows that see them and in no
+ * other: a score of -inf weighs nothing (nothing but such scores: zeros), one of
+ * +inf or NaN makes the row's head NaN.  A value of +-inf or NaN makes its column
+ * of the row infinite or NaN, whatever it weighs; all infinite values of one sign
+ * give that infinity where each weighs 2^-100 of the largest weight or more.
  * Rows of one sequence that stand next to each other read the cache together
  * where there are four times as many rows as sequences or more: list the
  * tokens of a prompt one behind the other.  The same call gives the same bits

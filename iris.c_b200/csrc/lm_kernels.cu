@@ -191,7 +191,8 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
 }
 
 // Two weights as a first part of 8 bits, cut off, and a second one of the next 8, rounded.  The last bit of a weight is
-// set, so that neither part of one above 0 is 0 or less: times an infinite value, both are the infinity.
+// set, so that neither part of one of 2^-100 or more is 0 or less: times an infinite value, both are the infinity.  (The
+// second part of a lighter one may round to 0, and 0 times it is NaN.)
 __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
   const uint32_t b0 = __float_as_uint(p0) | 1u, b1 = __float_as_uint(p1) | 1u;
   hi = __byte_perm(b0, b1, 0x7632);
@@ -565,7 +566,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   if constexpr (CLUSTER) {
     float* slot = reinterpret_cast<float*>(smem);
     if (!any)
-      for (int h = tid; h < heads_here; h += T) slot[2 * h] = -INFINITY, slot[2 * h + 1] = 0.f;
+      for (int h = tid; h < heads_here; h += T) slot[2 * h] = -INFINITY, slot[2 * h + 1] = -1.f;  // no key; a sum is never under 0
     __syncwarp();
     iris::cluster_sync();
     __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)head0 * HD;
@@ -576,7 +577,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       for (uint32_t p = 0; p < parts; p++) {
         const float* from = iris::cluster_map(slot, p);
         const float2 ml = *reinterpret_cast<const float2*>(from + 2 * h);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key, and nothing in its columns
+        if (ml.y < 0.f) continue;  // no key: its columns were not written
         const float4 v = *reinterpret_cast<const float4*>(from + 2 * MH + h * HD + col);
         const float mn = fmaxf(mm, ml.x), base = mn == -INFINITY ? 0.f : mn;
         const float f = exp2_approx(mm - base), s = exp2_approx(ml.x - base);

@@ -108,3 +108,84 @@ def test_streams_at_once(ops):
         alone = torch.zeros_like(q)
         o.attention_paged(cache, alone, q, seq, pos, scale=128 ** -0.5, workspace=ws, stream=stream())
         assert torch.equal(out, alone)
+
+
+WAYS = [  # way, rows' positions, query heads on one key-value head, kernels
+    ("few", [511, 140, 69], 4, 1), ("few", [511, 320, 140], 12, 1), ("line", [511, 320, 250, 132, 100, 69], 4, 2),
+    ("line", [511, 140, 69], 12, 2), ("runs", [511, 132, 250, 69], 4, 2), ("runs", [511, 505, 400, 140, 69, 320, 132, 250], 12, 2),
+    ("runs", [511, 460, 500, 448], 4, 2), ("runs", [511, 460, 455, 450, 449, 448, 500, 501], 12, 2),
+]
+
+
+@pytest.mark.parametrize("d", (64, 128, 256))
+@pytest.mark.parametrize("way,pos,nh,kernels", WAYS)
+def test_values_that_are_not_finite(ops, way, pos, nh, kernels, d):
+    """A value that is an infinity or NaN, under an ordinary weight, one of 2^-40 to 2^-90 of the largest, one that is 0 in f32, and a score of
+    -inf: its column of the rows that see it is not finite, and is the infinity where the weight is 2^-100 or more; every
+    other column is as without it (keys whose weight is 0 add nothing there, so that they are left out of the 64-bit form)."""
+    seqs = len(pos) if way == "line" else 1   # with as many sequences as rows no runs
+    lens = [512] + [1] * (seqs - 1)
+    kp, vp, table, ks, vs = paged(lens, 16, 1, d, False, 47)
+    if way != "few":
+        table = with_room(table, 16)
+    cell = lambda x, p: x[int(table[0, p // 16]), p % 16, 0]  # noqa: E731
+    odd = {3: (70, math.inf), 6: (130, -math.inf), 8: (135, -math.inf), 9: (200, math.inf), 11: (300, math.nan)}
+    q = torch.randn(len(pos), nh, d, device="cuda", generator=gen(48)).bfloat16()
+    q[:, :, 0] = 8.0  # column 0 makes keys lighter: scores in powers of 2 of 8 * -50 / sqrt(d) log2(e) = -72, -51, -36
+    keep = torch.ones(512, dtype=torch.bool)
+    for p in range(512):
+        if p in (130, 135) or 192 <= p < 256:
+            cell(kp, p)[0] = {130: -4000.0, 135: -50.0}.get(p, -math.inf)  # -4000: weight 0; 192 ..: four units' whole tile
+            keep[p] = p == 135
+        else:
+            cell(kp, p)[0] = 0.0
+        ks[0][p, 0] = cell(kp, p)
+    for col, (p, x) in odd.items():
+        cell(vp, p)[col] = x
+    seq = [0] * len(pos)
+    out = torch.full_like(q, 9.0)
+    cache = ops.KvCache.of(kp, vp, table)
+    ws = torch.full((ops.attention_paged_workspace(cache, nh),), 255, device="cuda", dtype=torch.uint8)
+    Counted(ops, kernels).attention_paged(cache, out, q, i32(seq), i32(pos), scale=1 / math.sqrt(d), workspace=ws, stream=stream())
+    torch.cuda.synchronize()
+    for i, n in enumerate(pos):
+        got = out[i].double().cpu()
+        sel = keep[:n + 1]
+        want, tol = attention64(q[i], ks[0].cpu()[:n + 1][sel], vs[0].cpu()[:n + 1][sel], 1 / math.sqrt(d))
+        seen = [c for c, (p, _) in odd.items() if p <= n]
+        rest = [c for c in range(d) if c not in seen]
+        assert ((got - want).abs() <= tol)[:, rest].all(), (i, n)
+        assert not torch.isfinite(got[:, seen]).any(), (i, n, got[0, seen])
+        for c in (3, 8):
+            assert odd[c][0] > n or (got[:, c] == odd[c][1]).all(), (i, n, c)
+        assert 11 not in seen or torch.isnan(got[:, 11]).all()
+
+
+@pytest.mark.parametrize("way,pos,nh,kernels", WAYS)
+def test_scores_that_are_not_finite(ops, way, pos, nh, kernels):
+    """Scores of -inf alone: zeros.  One of +inf or NaN: the head is NaN in the rows that see the key."""
+    d = 128
+    for value, at in ((-math.inf, 0), (math.inf, 100), (math.nan, 100)):
+        seqs = len(pos) if way == "line" else 1
+        kp, vp, table, ks, vs = paged([512] + [1] * (seqs - 1), 16, 1, d, False, 49)
+        if way != "few":
+            table = with_room(table, 16)
+        q = torch.randn(len(pos), nh, d, device="cuda", generator=gen(50)).bfloat16()
+        q[:, :, 0] = 1.0
+        for p in range(512) if at == 0 else (at,):
+            kp[int(table[0, p // 16]), p % 16, 0, 0] = value
+        cache = ops.KvCache.of(kp, vp, table)
+        ws = torch.full((ops.attention_paged_workspace(cache, nh),), 255, device="cuda", dtype=torch.uint8)
+        out = torch.full_like(q, 9.0)
+        Counted(ops, kernels).attention_paged(cache, out, q, i32([0] * len(pos)), i32(pos), scale=1 / math.sqrt(d), workspace=ws,
+                                              stream=stream())
+        torch.cuda.synchronize()
+        for i, n in enumerate(pos):
+            got = out[i].double().cpu()
+            if at == 0:
+                assert (got == 0).all(), (i, n)
+            elif n >= at:
+                assert torch.isnan(got).all(), (i, n)
+            else:
+                want, tol = attention64(q[i], ks[0][:n + 1], vs[0][:n + 1], 1 / math.sqrt(d))
+                assert ((got - want).abs() <= tol).all(), (i, n)
