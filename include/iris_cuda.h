@@ -420,7 +420,9 @@ int iris_cuda_qwen3_profile(iris_cuda_qwen3_t *m, iris_cuda_kernel_time_t *out, 
  * operators of layer 4.  load_lm / random_lm hold every decoder layer, the
  * final norm and the head (lm_head.weight, or the embeddings where the model
  * has none) besides what iris_cuda_qwen3_load holds; the result serves as an
- * encoder too. */
+ * encoder too.  load_lm refuses a config.json that scales the rotary positions,
+ * attends within a window, gives the projections biases or has an rms_norm_eps
+ * other than 1e-6. */
 iris_cuda_qwen3_t *iris_cuda_qwen3_load_lm(const char *model_dir);
 iris_cuda_qwen3_t *iris_cuda_qwen3_random_lm(const iris_cuda_qwen3_config_t *cfg, uint64_t seed);
 /* A session: the paged key-value cache of num_seqs sequences of up to max_len

@@ -210,9 +210,37 @@ static iris_cuda_qwen3_t *q3_create(const iris_cuda_qwen3_config_t *cfg, q3_src_
     return m;
 }
 
+/* The value of a key of config.json, NULL where it has none. */
+static const char *q3_json_value(const char *json, const char *key) {
+    char pat[64];
+    snprintf(pat, sizeof(pat), "\"%s\"", key);
+    const char *p = strstr(json, pat);
+    if (!p) return NULL;
+    p += strlen(pat);
+    p += strspn(p, " \t\r\n");
+    return *p == ':' ? p + 1 + strspn(p + 1, " \t\r\n") : NULL;
+}
+
+/* A language model's answers are wrong where its config asks for what the layers do not do; the encoder reads prompts as
+ * the reference does, which looks at none of these. */
+static int q3_lm_config(const char *json) {
+    const char *scaling = q3_json_value(json, "rope_scaling"), *type = q3_json_value(json, "rope_type");
+    const char *window = q3_json_value(json, "use_sliding_window"), *bias = q3_json_value(json, "attention_bias");
+    const int plain = type && !strncmp(type, "\"default\"", 9);
+    double eps;
+    if ((scaling && *scaling == '{' && !plain) || (type && !plain))
+        return iris_fail(IRIS_CUDA_ERR_ARG, "language model: config.json scales rotary positions (rope_scaling / rope_type), which the layers do not");
+    if (!json_get_number(json, "rms_norm_eps", &eps) && (float)eps != Q3_EPS)
+        return iris_fail(IRIS_CUDA_ERR_ARG, "language model: rms_norm_eps %g (%g)", eps, (double)Q3_EPS);
+    if (window && !strncmp(window, "true", 4))
+        return iris_fail(IRIS_CUDA_ERR_ARG, "language model: config.json limits attention to a window (use_sliding_window)");
+    if (bias && !strncmp(bias, "true", 4))
+        return iris_fail(IRIS_CUDA_ERR_ARG, "language model: projections with a bias (attention_bias)");
+    return 0;
+}
+
 static iris_cuda_qwen3_t *q3_load(const char *model_dir, int lm) {
     if (!model_dir) { iris_fail(IRIS_CUDA_ERR_ARG, "null model directory"); return NULL; }
-    if (iris_rt_ensure()) return NULL;
     /* config.json keys and defaults as parse_qwen3_config / qwen3_set_defaults (iris_qwen3.c:1378-1447) */
     iris_cuda_qwen3_config_t c = {2560, 9728, 32, 8, 128, 151936, 36, 1000000.0f};
     char path[4200];
@@ -232,7 +260,9 @@ static iris_cuda_qwen3_t *q3_load(const char *model_dir, int lm) {
         if (!json_get_number(buf, "vocab_size", &d) && d > 0) c.vocab = (int)d;
         if (!json_get_number(buf, "num_hidden_layers", &d) && d > 0) c.layers = (int)d;
         if (!json_get_number(buf, "rope_theta", &d) && d > 0) c.rope_theta = (float)d;
+        if (lm && q3_lm_config(buf)) return NULL;
     }
+    if (iris_rt_ensure()) return NULL;
     iris_wsrc_t ws;
     memset(&ws, 0, sizeof(ws));
     if (st_open_dir(&ws.st, model_dir)) {
