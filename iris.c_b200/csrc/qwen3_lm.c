@@ -5,7 +5,8 @@
  * operators of lm_kernels.cu: the QKV projection's rows go through
  * iris_launch_rope_append into the layer's pages, and every row attends over
  * its sequence's pages.  Then the final norm, the head's GEMM, and the log
- * probabilities.  A step of one token count and top_k is a CUDA graph.
+ * probabilities.  A step whose token count and top_k come again is a CUDA graph
+ * (lm_run).
  */
 #include "qwen3_internal.h"
 
@@ -15,6 +16,16 @@
 
 #define LM_PAGE 16          /* tokens of a page */
 #define LM_MAX_TOKENS 8192  /* of a step: the logits are f32 [tokens, vocab] */
+#define LM_SIZES 16         /* of steps, remembered */
+
+/* a size of step: its graph, once captured */
+typedef struct {
+    int tokens, top_k;      /* tokens 0: none */
+    uint64_t used;          /* the step that last had it */
+    cudaGraph_t graph;
+    cudaGraphExec_t gexec;  /* NULL before its second step */
+    uint64_t kernels;
+} lm_size_t;
 
 struct iris_cuda_qwen3_lm {
     iris_cuda_qwen3_t *m;
@@ -35,19 +46,21 @@ struct iris_cuda_qwen3_lm {
     int32_t *out_ids;       /* [max_tokens, 32] */
     CUtensorMap tm_xn, tm_attn, tm_mlp;
     iris_gpu_rope_t rope;
-    cudaGraph_t graph;
-    cudaGraphExec_t gexec;
-    int graph_tokens, graph_top_k;  /* of the captured step; tokens 0: none */
-    uint64_t graph_kernels;
+    lm_size_t sizes[LM_SIZES];
 };
+
+static void lm_size_free(lm_size_t *z) {
+    if (z->gexec) {
+        cudaGraphExecDestroy(z->gexec);
+        cudaGraphDestroy(z->graph);
+    }
+    memset(z, 0, sizeof(*z));
+}
 
 void iris_cuda_qwen3_lm_free(iris_cuda_qwen3_lm_t *lm) {
     if (!lm) return;
     if (g_rt.initialized) cudaStreamSynchronize(g_rt.stream);
-    if (lm->graph_tokens) {
-        cudaGraphExecDestroy(lm->gexec);
-        cudaGraphDestroy(lm->graph);
-    }
+    for (int i = 0; i < LM_SIZES; i++) lm_size_free(&lm->sizes[i]);
     void *b[] = {lm->table, lm->pools, lm->in, lm->x, lm->qkv, lm->logits, lm->ws, lm->xn, lm->q, lm->attn, lm->mlp,
                  lm->attn_ws, lm->lp_ws, lm->out, lm->out_ids};
     for (size_t i = 0; i < sizeof(b) / sizeof(b[0]); i++) iris_dfree(b[i]);
@@ -209,21 +222,31 @@ static int lm_enqueue(iris_cuda_qwen3_lm_t *lm, int T, int top_k, q3_enq_t *E) {
     return E->rc;
 }
 
+/* A size's first step is queued kernel by kernel and its second captured: a graph spares 0.25 ms of 3.9 (Qwen3-4B, 8
+ * tokens), making one costs 1.2.  The LM_SIZES sizes used last are kept, so that prompts and single tokens may alternate. */
 static int lm_run(iris_cuda_qwen3_lm_t *lm, int T, int top_k) {
     if (iris_fault("launch")) return iris_fail(IRIS_CUDA_ERR_INJECTED, "injected launch failure");
     q3_enq_t E;
     memset(&E, 0, sizeof(E));
-    if (getenv("IRIS_CUDA_NO_GRAPH")) {
+    lm_size_t *z = lm->sizes;  /* this size, or the one not used for longest */
+    for (int i = 0; i < LM_SIZES; i++) {
+        if (lm->sizes[i].tokens == T && lm->sizes[i].top_k == top_k) { z = &lm->sizes[i]; break; }
+        if (lm->sizes[i].used < z->used) z = &lm->sizes[i];
+    }
+    const int known = z->tokens == T && z->top_k == top_k;
+    if (!known || getenv("IRIS_CUDA_NO_GRAPH")) {
+        if (!known) {
+            lm_size_free(z);
+            z->tokens = T;
+            z->top_k = top_k;
+        }
+        z->used = lm->step;
         const int rc = lm_enqueue(lm, T, top_k, &E);
         iris_count_launch(E.kernels);
         return rc;
     }
-    if (lm->graph_tokens && (lm->graph_tokens != T || lm->graph_top_k != top_k)) {
-        cudaGraphExecDestroy(lm->gexec);
-        cudaGraphDestroy(lm->graph);
-        lm->graph_tokens = 0;
-    }
-    if (!lm->graph_tokens) {
+    z->used = lm->step;
+    if (!z->gexec) {
         cudaError_t e = cudaStreamBeginCapture(g_rt.stream, cudaStreamCaptureModeThreadLocal);
         if (e != cudaSuccess) return iris_cuda_check(e, "begin capture");
         const int rc = lm_enqueue(lm, T, top_k, &E);
@@ -231,15 +254,13 @@ static int lm_run(iris_cuda_qwen3_lm_t *lm, int T, int top_k) {
         e = cudaStreamEndCapture(g_rt.stream, &g);
         if (rc) { if (g) cudaGraphDestroy(g); return rc; }
         if (e != cudaSuccess) return iris_cuda_check(e, "end capture");
-        e = cudaGraphInstantiate(&lm->gexec, g, 0);
-        if (e != cudaSuccess) { cudaGraphDestroy(g); return iris_cuda_check(e, "graph instantiate"); }
-        lm->graph = g;
-        lm->graph_tokens = T;
-        lm->graph_top_k = top_k;
-        lm->graph_kernels = E.kernels;
+        e = cudaGraphInstantiate(&z->gexec, g, 0);
+        if (e != cudaSuccess) { z->gexec = NULL; cudaGraphDestroy(g); return iris_cuda_check(e, "graph instantiate"); }
+        z->graph = g;
+        z->kernels = E.kernels;
     }
-    iris_count_launch(lm->graph_kernels);
-    return iris_cuda_check(cudaGraphLaunch(lm->gexec, g_rt.stream), "graph launch");
+    iris_count_launch(z->kernels);
+    return iris_cuda_check(cudaGraphLaunch(z->gexec, g_rt.stream), "graph launch");
 }
 
 /* the step's sequences and positions against what the sequences hold; lm->next gets the lengths after it */
