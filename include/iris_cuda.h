@@ -713,7 +713,8 @@ unsigned long iris_gpu_op_failures(void);
  * anything is queued: IRIS_CUDA_ERR_ARG with the reason in
  * iris_cuda_last_error(), counted by iris_gpu_op_failures().  Values in device memory (positions, sequence and
  * page numbers, targets) can not be checked then; the kernels bound them and
- * never read or write outside the tensors they are given.  A workspace is
+ * never read or write outside the tensors they are given.  A batch of no rows
+ * is no error and needs no tensors (they may be NULL).  A workspace is
  * scratch of one call: calls that may overlap on the GPU (two streams, two
  * graphs) need one each; its contents need not be set or kept. */
 

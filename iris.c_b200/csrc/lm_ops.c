@@ -131,7 +131,8 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
     const char *what = "rope_append";
     if (cache_check(cache, what)) return IRIS_CUDA_ERR_ARG;
     if (tokens < 0 || heads < 0 || heads > 65535) return LM_FAIL("%s: %d tokens, %d heads", what, tokens, heads);
-    if (!k || !v || !seq || !pos || (heads && (!q || !q_out))) return LM_FAIL("%s: null pointer", what);
+    /* a batch of no rows may have no tensors */
+    if (tokens && (!k || !v || !seq || !pos || (heads && (!q || !q_out)))) return LM_FAIL("%s: null pointer", what);
     if (rope) {
         if (rope_layout_check(rope, rope->layout, rope->rot_dim, what)) return IRIS_CUDA_ERR_ARG;
         if (rope->rot_dim > cache->head_dim)
@@ -146,7 +147,7 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
     if (misaligned(k, 16) || misaligned(v, 16) || (heads && (misaligned(q, 16) || misaligned(q_out, 16))) ||
         misaligned(q_norm, 16) || misaligned(k_norm, 16) || misaligned(seq, 4) || misaligned(pos, 4))
         return LM_FAIL("%s: misaligned pointer (16 bytes; seq and pos 4)", what);
-    if (heads && q_out == q && (f32 || ldq != ldq_out))
+    if (tokens && heads && q_out == q && (f32 || ldq != ldq_out))
         return LM_FAIL("%s: q_out on q needs bf16 and one row stride", what);
     if (!tokens) return 0;
     const void *ptrs[] = {cache->k, cache->v, cache->table, q_out, q, k, v, q_norm, k_norm, seq, pos};
@@ -196,7 +197,7 @@ int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const 
     if (cache_check(cache, what) || heads_check(cache, heads, what)) return IRIS_CUDA_ERR_ARG;
     if (rows < 0 || (!seq && rows > cache->num_seqs))
         return LM_FAIL("%s: %d rows for %d sequences", what, rows, cache->num_seqs);
-    if (!out || !q || !pos || !workspace) return LM_FAIL("%s: null pointer", what);
+    if (rows && (!out || !q || !pos || !workspace)) return LM_FAIL("%s: null pointer", what);
     const int64_t width = (int64_t)heads * cache->head_dim;
     if (ldo % 8 || ldq % 8 || ldo < width || ldq < width)
         return LM_FAIL("%s: row strides %lld to %lld (at least %lld, multiples of 8)", what, (long long)ldq,
@@ -239,13 +240,13 @@ int iris_gpu_token_logprobs(const void *logits, int f32, int64_t ld, int rows, i
     if (logprobs_shape(rows, vocab, what)) return IRIS_CUDA_ERR_ARG;
     if (ld < vocab) return LM_FAIL("%s: row stride %lld under %d logits", what, (long long)ld, vocab);
     if (top_k < 0 || top_k > 32 || top_k > vocab) return LM_FAIL("%s: top_k %d (0 to min(32, vocab))", what, top_k);
-    if (!logits || !workspace || (logprob && !targets)) return LM_FAIL("%s: null pointer", what);
-    if (top_k && !top_ids && !top_logprobs) return LM_FAIL("%s: top_k %d without an output", what, top_k);
+    if (rows && (!logits || !workspace || (logprob && !targets))) return LM_FAIL("%s: null pointer", what);
+    if (rows && top_k && !top_ids && !top_logprobs) return LM_FAIL("%s: top_k %d without an output", what, top_k);
     if (misaligned(logits, f32 ? 4 : 2) || misaligned(targets, 4) || misaligned(logprob, 4) || misaligned(entropy, 4) ||
         misaligned(top_ids, 4) || misaligned(top_logprobs, 4) || misaligned(workspace, 16))
         return LM_FAIL("%s: misaligned pointer", what);
     const size_t need = iris_logprobs_ws_bytes(rows, vocab);
-    if (workspace_bytes < need) return LM_FAIL("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+    if (rows && workspace_bytes < need) return LM_FAIL("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
     if (!rows || (!logprob && !entropy && !top_k)) return 0;
     const void *ptrs[] = {logits, targets, logprob, entropy, top_ids, top_logprobs, workspace};
     lm_dev_t d;
