@@ -1752,7 +1752,6 @@ static cudaError_t launch_logprobs(const IrisLogprobs* a, int num_sms, cudaStrea
   plan.warps = (all + plan.rounds - 1) / plan.rounds;
   plan.maxima = (uint32_t*)(plan.sums + (size_t)a->rows * plan.warps);
   const int64_t ctas = ((int64_t)a->rows * plan.warps + 7) / 8;
-  if (ctas * 8 > 0xFFFFFFFFll) return cudaErrorInvalidConfiguration;  // more logits than any device holds
   *launches = 2;
   cudaError_t e = iris::launch_overlapped(logprobs_stream_kernel<In>, dim3((unsigned)ctas), dim3(256), 0, stream, *a, plan);
   if (e != cudaSuccess) return e;

@@ -223,8 +223,9 @@ int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const 
 
 /* ------------------------------------------------------------------ log probabilities */
 static int logprobs_shape(int rows, int vocab, const char *what) {
-    /* ids are int32; the two limits keep the workspace's piece counts within 32 bits */
-    if (rows < 0 || vocab < 1 || vocab > (1 << 30)) return LM_FAIL("%s: %d rows of %d logits", what, rows, vocab);
+    /* ids are int32; 2^40 logits, more than any device holds, are under 2^32 parts (of 1024 values or a row's rest) */
+    if (rows < 0 || vocab < 1 || vocab > (1 << 30) || (int64_t)rows * vocab > (int64_t)1 << 40)
+        return LM_FAIL("%s: %d rows of %d logits", what, rows, vocab);
     return 0;
 }
 

@@ -1,7 +1,7 @@
 """Calls of the language-model operators that need no GPU: batches of no rows,
 shapes that no device holds."""
 import iris_cuda
-from test_lm_ops_host import Fake, append, attend, cache, fake_cache, logprobs
+from test_lm_ops_host import Fake, append, attend, cache, fake_cache, logprobs, refused
 
 
 def none(dtype, *shape):
@@ -23,3 +23,14 @@ def test_batches_of_no_rows():
     assert logprobs(rows=0, logits=None, targets=None, top_ids=None, top_logprobs=None, ws=None, ws_bytes=0) == 0
     # what is wrong whatever the rows is still refused
     assert append(cache(), tokens=0, ldk=255) and attend(cache(), rows=0, heads=3) and logprobs(rows=0, top_k=33)
+
+
+def test_more_logits_than_any_device_holds():
+    """Refused as an argument, in the call and by its workspace's size."""
+    L = iris_cuda.lib()
+    for rows, vocab in ((2 ** 31 - 1, 2 ** 30), (2 ** 31 - 1, 513), (1025, 2 ** 30)):
+        assert L.iris_gpu_token_logprobs_workspace(rows, vocab) == 0
+        refused(logprobs(rows=rows, vocab=vocab, ld=vocab, ws_bytes=2 ** 63), "rows of")
+    for rows, vocab in ((2 ** 31 - 1, 1), (2 ** 31 - 1, 512), (1024, 2 ** 30), (8192, 151936)):
+        # at least the largest values of blocks of 256, four bytes each
+        assert L.iris_gpu_token_logprobs_workspace(rows, vocab) >= rows * -(-vocab // 256) * 4
