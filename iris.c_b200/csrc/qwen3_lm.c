@@ -92,7 +92,7 @@ static void lm_cache(const iris_cuda_qwen3_lm_t *lm, int layer, iris_gpu_kv_cach
 iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_seqs, int max_len, int max_tokens) {
     if (!m || !m->head) { iris_fail(IRIS_CUDA_ERR_ARG, "language model session: needs a model of load_lm / random_lm"); return NULL; }
     if (num_seqs < 1 || max_len < 1 || max_tokens < 1 || max_tokens > LM_MAX_TOKENS ||
-        (int64_t)num_seqs * ((max_len + LM_PAGE - 1) / LM_PAGE) > (1 << 30)) {
+        (int64_t)num_seqs * (((int64_t)max_len + LM_PAGE - 1) / LM_PAGE) > (1 << 30)) {
         iris_fail(IRIS_CUDA_ERR_ARG, "language model session: %d sequences of %d tokens, steps of %d (1..%d)", num_seqs,
                   max_len, max_tokens, LM_MAX_TOKENS);
         return NULL;
@@ -104,7 +104,7 @@ iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_se
     lm->num_seqs = num_seqs;
     lm->max_len = max_len;
     lm->max_tokens = max_tokens;
-    lm->blocks = (max_len + LM_PAGE - 1) / LM_PAGE;
+    lm->blocks = (int)(((int64_t)max_len + LM_PAGE - 1) / LM_PAGE);
     const size_t T = (size_t)max_tokens, H = (size_t)c->hidden, F = (size_t)c->intermediate;
     const size_t qd = (size_t)c->heads * 128, nq = (size_t)(c->heads + 2 * c->kv_heads) * 128;
     const size_t pages = (size_t)num_seqs * lm->blocks;

@@ -26,3 +26,11 @@ def test_long_prompts_and_continuations(iris, model):  # noqa: F811
     assert [lm.length(s) for s in (0, 1)] == at == [230, 40]
     assert rel_l2(got, want) < TOL
     lm.close()
+
+
+def test_sessions_of_the_longest_length(iris, model):  # noqa: F811
+    """Lengths up to the end of int are counted in pages without wrapping: refused by their number of pages."""
+    m, _, _ = model
+    for n in (2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16):
+        with pytest.raises(iris.IrisCudaError, match=f"9 sequences of {n}"):
+            iris.Qwen3Lm(m, num_seqs=9, max_len=n, max_tokens=8)
