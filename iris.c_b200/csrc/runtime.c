@@ -26,6 +26,7 @@ int iris_fail(int code, const char *fmt, ...) {
 
 int iris_cuda_check(cudaError_t e, const char *what) {
     if (e == cudaSuccess) return 0;
+    cudaGetLastError();  /* reported here: not by the next launch that asks for the last error too */
     return iris_fail(IRIS_CUDA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
@@ -169,6 +170,7 @@ void *iris_dmalloc(size_t bytes) {
     if (bytes == 0) bytes = 16;
     cudaError_t e = cudaMalloc(&p, bytes);
     if (e != cudaSuccess) {
+        cudaGetLastError();
         iris_fail(IRIS_CUDA_ERR_OOM, "cudaMalloc(%zu): %s", bytes, cudaGetErrorString(e));
         return NULL;
     }

@@ -34,3 +34,13 @@ def test_sessions_of_the_longest_length(iris, model):  # noqa: F811
     for n in (2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16):
         with pytest.raises(iris.IrisCudaError, match=f"9 sequences of {n}"):
             iris.Qwen3Lm(m, num_seqs=9, max_len=n, max_tokens=8)
+
+
+def test_after_a_session_that_does_not_fit(iris, model):  # noqa: F811
+    """A session whose cache no device holds is refused, and the next calls do not report its error."""
+    m, _, _ = model
+    lm = iris.Qwen3Lm(m, num_seqs=1, max_len=64, max_tokens=8)
+    with pytest.raises(iris.IrisCudaError, match="language model session"):
+        iris.Qwen3Lm(m, num_seqs=1, max_len=2 ** 24, max_tokens=8)  # 28 layers, 2 heads: 481 GB
+    assert np.isfinite(lm.step([1, 2, 3], [0] * 3, [0, 1, 2])["entropy"]).all()
+    lm.close()
