@@ -426,7 +426,8 @@ int iris_cuda_qwen3_profile(iris_cuda_qwen3_t *m, iris_cuda_kernel_time_t *out, 
 iris_cuda_qwen3_t *iris_cuda_qwen3_load_lm(const char *model_dir);
 iris_cuda_qwen3_t *iris_cuda_qwen3_random_lm(const iris_cuda_qwen3_config_t *cfg, uint64_t seed);
 /* A session: the paged key-value cache of num_seqs sequences of up to max_len
- * tokens, and buffers for steps of up to max_tokens.  Free it before its model. */
+ * tokens, and buffers for steps of up to max_tokens.  A model that is freed before
+ * its sessions stays until the last of them is. */
 typedef struct iris_cuda_qwen3_lm iris_cuda_qwen3_lm_t;
 iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_seqs, int max_len, int max_tokens);
 void iris_cuda_qwen3_lm_free(iris_cuda_qwen3_lm_t *lm);

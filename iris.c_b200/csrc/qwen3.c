@@ -160,6 +160,8 @@ static void q3_plan_free(q3_plan_t *P);
 
 void iris_cuda_qwen3_free(iris_cuda_qwen3_t *m) {
     if (!m) return;
+    m->freed = 1;
+    if (m->sessions) return;  /* the last session's end comes here again */
     if (g_rt.initialized) cudaStreamSynchronize(g_rt.stream);
     q3_plan_free(&m->plan);
     iris_dfree(m->embed);

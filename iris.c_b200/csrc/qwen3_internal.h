@@ -49,6 +49,8 @@ struct iris_cuda_qwen3 {
     CUtensorMap tm_head;
     q3_plan_t plan;
     size_t weight_bytes;
+    int sessions;          /* that use it; iris_cuda_qwen3_free waits for the last */
+    int freed;
 };
 
 typedef struct {

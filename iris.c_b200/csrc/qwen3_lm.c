@@ -68,7 +68,9 @@ void iris_cuda_qwen3_lm_free(iris_cuda_qwen3_lm_t *lm) {
     free(lm->len);
     free(lm->next);
     free(lm->named);
+    iris_cuda_qwen3_t *m = lm->m;
     free(lm);
+    if (--m->sessions == 0 && m->freed) iris_cuda_qwen3_free(m);
 }
 
 static void lm_cache(const iris_cuda_qwen3_lm_t *lm, int layer, iris_gpu_kv_cache_t *c) {
@@ -101,6 +103,7 @@ iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_se
     if (!lm) { iris_fail(IRIS_CUDA_ERR_OOM, "language model session"); return NULL; }
     const iris_cuda_qwen3_config_t *c = &m->cfg;
     lm->m = m;
+    m->sessions++;
     lm->num_seqs = num_seqs;
     lm->max_len = max_len;
     lm->max_tokens = max_tokens;

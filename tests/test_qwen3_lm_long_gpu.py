@@ -44,3 +44,25 @@ def test_after_a_session_that_does_not_fit(iris, model):  # noqa: F811
         iris.Qwen3Lm(m, num_seqs=1, max_len=2 ** 24, max_tokens=8)  # 28 layers, 2 heads: 481 GB
     assert np.isfinite(lm.step([1, 2, 3], [0] * 3, [0, 1, 2])["entropy"]).all()
     lm.close()
+
+
+def test_a_model_freed_before_its_sessions(iris):
+    """Its weights stay until the last session is freed (the steps would read freed memory)."""
+    cfg = iris.Qwen3Config(256, 512, 4, 2, 128, 1000, 2, 1e6)
+    want = None
+    for close_first in (False, True):
+        m = iris.Qwen3.random_lm(cfg, 3)
+        a, b = (iris.Qwen3Lm(m, num_seqs=1, max_len=64, max_tokens=8) for _ in range(2))
+        a.step([1, 2], [0, 0], [0, 1])
+        if close_first:
+            m.close()
+            a.close()
+        ids, got = list(range(8)), []
+        for j in range(3):  # queued, captured, replayed
+            got.append(b.step(ids, [0] * 8, range(8 * j, 8 * j + 8), targets=ids, top_k=2))
+        b.close(), a.close(), m.close()
+        if want is None:
+            want = got
+        for x, y in zip(want, got):
+            for key in x:
+                np.testing.assert_array_equal(x[key], y[key])
