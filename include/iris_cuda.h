@@ -794,7 +794,8 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
  * apart, not over q or the pools.  So the newest tokens of many sequences are one call, and a run of
  * tokens of one sequence is causal.  A row that sees nothing (pos[t] < 0)
  * gives zeros; a row with seq[t] outside [0, num_seqs) is left as it was.
- * Positions past the table's end and pages outside the pool are not seen.
+ * Positions past the table's end, pages outside the pool and the position
+ * 2^31 - 1 itself are not seen.
  * Keys and values that are not finite show in the rows that see them and in no
  * other: a score of -inf weighs nothing (nothing but such scores: zeros), one of
  * +inf or NaN makes the row's head NaN.  A value of +-inf or NaN makes its column

@@ -35,10 +35,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
 // that the chain position -> page -> slot and the angles come at no time of
 // their own.
 // Measured on 8191 tokens of 32 + 8 + 8 heads of 128, f32 (302 MB, 46.5 us at
-// the measured copy rate): 49.5 us with blocks of 64, 52.8 with 128, 57.3 with
-// 256 (the instructions per block and per head are half of the time's issue
-// slots); one warp per token and slice 57.0; eight columns in a row to a lane,
-// partners by shuffle and angles from shared memory for every head 82.
+// the measured copy rate): 51 us.  Blocks of 64 threads: with 128 it took 1.07
+// of that, with 256 1.16 (the instructions per block and per head are half of
+// the time's issue slots).
 constexpr int ROPE_HEADS = 4, ROPE_THREADS = 64;
 
 __device__ __forceinline__ float4 values4(uint4 u) {
@@ -145,8 +144,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
 //   s = q k^T      mma m16n8k16, rows = up to 8 query heads of the head's group
 //   p = 2^(s c - m), c = scale log2(e);  l = l 2^(m_old - m) + sum p
 //   o = o 2^(m_old - m) + p v
-// p counts with 16 bits, its first 8 and bf16(the rest) (with 8 the result would be
-// off by sqrt(2) of its own rounding).  Up to 8 heads fill half of the product's
+// p counts with 16 bits in the product, its first 8 and bf16(the rest) (with 8 the
+// result would be off by sqrt(2) of its own rounding; with 16 one value in 500 is
+// rounded the other way than the 64-bit result, with f32 weights one in 2000), and
+// with all of f32 in l.  Up to 8 heads fill half of the product's
 // rows and the second parts the other half, at no extra instruction; the halves
 // of o are added at the end.  For 9 to 16 heads on a key-value head the second
 // part is a second product.  At head_dim 256 two warps share 16 keys and hold
@@ -600,18 +601,18 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 // pairs, and their sums are joined in shared memory.  Bound by the products, 6 flops
 // a score and column, two of them for the second part of p, and by a warp's softmax
 // between them: registers allow two warps a scheduler, the tensor pipe of mma.sync
-// is active 55 % of the time (a prompt of 8192, 32 heads on 8 of 128: 209 TFLOP/s
-// counting 4 flops).  Three CTAs on an SM with half the scores in registers spilled
-// (240 us for 194 with a prompt of 2048).
+// is active 55 % of the time (a prompt of 8192, 32 heads on 8 of 128: 2636 us, 209
+// TFLOP/s counting 4 flops, an eighth of the measured peak).
 template <int HD>
 struct RunShape {
   static constexpr int kPairs = HD == 256 ? 128 : 64;             // (row, head) pairs of a unit
   static constexpr int kWarps = kPairs / 16, kThreads = 32 * kWarps;
-  // CTAs on an SM: what registers allow (a warp holds queries, scores and o of 16 pairs; at head_dim 64 four spill)
+  // CTAs on an SM: what registers allow (a warp holds queries, scores and o of 16 pairs).  At 128 none spills; at 64 three
+  // CTAs spill 34 bytes a thread, at 256 one of eight warps 454
   static constexpr int kCtas = HD == 64 ? 3 : HD == 128 ? 2 : 1;
-  static constexpr int kStages = 3;  // (two: a prompt of 2048, 32 heads on 8 of 128, 244 us for 227)
+  static constexpr int kStages = 3;  // (two took 1.07 of the time with a prompt of 2048, 32 heads on 8 of 128)
   // keys whose scores a warp holds at a time; a prompt of 2048, 8 heads on 2 of 256, with four warps: 16 330 us, 32 248,
-  // with eight 157
+  // with eight warps 162
   static constexpr int kKeys = HD == 256 ? 32 : 64;
   static constexpr int kPart = IRIS_PAGED_TILE * HD * 2;          // bytes of K or of V of a tile
   static constexpr int kSlot = kPairs * (HD + 2);                 // floats of a piece, as in PagedShape
@@ -932,7 +933,7 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
 // reads the first pieces before it knows how many there are; few units in many
 // pieces (FEW): a block per unit and head, which works out the unit's borders from
 // the rows' lengths while the attention kernel runs (one row, 16 heads on one of
-// 128 and 131072 keys, 295 pieces: 63 us in the first way, 22 in the second).
+// 128 and 131072 keys, 295 pieces: 24 us, in the first way some 40 more).
 constexpr int JOIN_THREADS = 512;
 
 template <int HD, int MH, bool FEW>
@@ -1657,10 +1658,12 @@ struct PagedLaunch {
                                              dim3(Sh::kThreads), Sh::kSmem, parts, stream, *a);
     }
     // four times as many rows as sequences: runs of rows.  On the device, 32 heads on 8 of 128, rows by themselves -> runs:
-    // a prompt of 64 9.3 -> 10.3 us, 128 15.4 -> 15.6, 512 84 -> 31, 2048 943 -> 194, 8192 13.9 -> 2.6 ms; 64 tokens behind
-    // 32704 867 -> 188; 4 behind 4092 in 8 sequences 69 -> 38, 2 there 41 -> 36, but 2 behind 1022 in 64, 8 heads on 2 of
-    // 256, 49 -> 55, and 64 single tokens at 1023 beside a prompt of 128 (3 rows a sequence) 55 -> 93, of 512 119 -> 111.
-    // (The host knows no more of the rows; 2048 rows of 4 sequences in random order, no runs in them: 306 -> 550.)
+    // a prompt of 128 15.3 -> 15.8 us, 512 83 -> 31, 2048 934 -> 196, 8192 13.7 -> 2.6 ms; 64 tokens behind 32704 855 ->
+    // 188; 4 behind 4092 in 8 sequences 77 -> 38, 4 behind 1020 in 64 164 -> 65.  Below, 2 behind 4094 in 8 45 -> 36, 2
+    // behind 1022 in 64 94 -> 62, but 8 heads on 2 of 256 51 -> 56 and 64 single tokens at 1023 beside a prompt of 128 56 ->
+    // 93.  The host sees counts only, so that the rule also loses: 64 single tokens beside a prompt of 256 67 -> 98, of 384
+    // 89 -> 103 (of 448 101 -> 103, of 512 116 -> 113, of 1024 295 -> 156); 2048 rows of 4 sequences in random order, no
+    // runs in them, 303 -> 553.
     if (a->seq && a->rows >= 4 * (int64_t)a->cache.num_seqs) {
       const int ctas = paged_ctas(&a->cache, a->heads, a->rows, num_sms * Runs::kCtas);
       const cudaError_t e = iris::launch_overlapped(paged_runs_kernel<HD>, dim3(ctas), dim3(Runs::kThreads), Runs::kSmem, stream, *a);
