@@ -812,6 +812,45 @@ int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const 
                              const int32_t *seq, const int32_t *pos, int rows, int heads, float scale,
                              void *workspace, size_t workspace_bytes, void *stream);
 
+/* The same cache in 8 bits: e4m3 values, each standing for itself times 2^(e -
+ * 127) with one exponent byte e, IRIS_EXP8_MIN to IRIS_EXP8_MAX, for each block
+ * of `block` tokens of a page and each head, in k and in v.  A power of two costs
+ * e4m3 no precision, and a block whose scale grows loses only what falls below the
+ * least e4m3 value. */
+#define IRIS_EXP8_MIN 67      /* 2^-60 */
+#define IRIS_EXP8_MAX 187     /* 2^60  */
+typedef struct {
+    iris_gpu_kv_cache_t pages; /* k, v: e4m3 page pools; strides multiples of 16         */
+    uint8_t *k_exp, *v_exp;   /* exponents [num_pages][page_size / block][kv_heads]      */
+    int block;                /* tokens that share a scale: a divisor of page_size, at most 128 */
+    int64_t exp_page_stride;  /* bytes between the exponents of pages, blocks and heads  */
+    int64_t exp_block_stride;
+    int64_t exp_head_stride;
+} iris_gpu_kv_cache8_t;
+
+/* iris_gpu_rope_append into an 8-bit cache: K and V in f32 are rounded once, to
+ * e4m3 at the block's scale.  That is the least power of two that brings all of
+ * the call's values for the block and head within 448; where the block's first
+ * slot is not among the call's tokens, no less than what it was, and where it
+ * grows, the block's other slots are rounded to it.  Where the first slot is among
+ * them, what the block held counts as dead: its other slots keep their bytes.  So
+ * feed a sequence in order of its positions, in any number of calls; within a call
+ * tokens stand in any order.  Values that are not finite are held as NaN; magnitudes past 448 * 2^60 as
+ * that.  Of two tokens with one slot the later row stays. */
+int iris_gpu_rope_append8(const iris_gpu_kv_cache8_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
+                          const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int f32,
+                          const float *q_norm, const float *k_norm, float eps, const int32_t *seq, const int32_t *pos,
+                          int tokens, int heads, void *stream);
+
+/* iris_gpu_attention_paged over an 8-bit cache.  Keys and values are the numbers
+ * that they stand for, and NaN shows as there (a value of NaN makes its column NaN).
+ * The softmax weight of a key times its value's scale counts with 11 bits, and as 0
+ * under 2^-25 of the row's largest. */
+size_t iris_gpu_attention_paged8_workspace(const iris_gpu_kv_cache8_t *cache, int heads);
+int iris_gpu_attention_paged8(const iris_gpu_kv_cache8_t *cache, void *out, const void *q, int64_t ldo, int64_t ldq,
+                              const int32_t *seq, const int32_t *pos, int rows, int heads, float scale,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
 /* The answer side of a logits matrix [rows, vocab] (bf16, or f32 when f32 !=
  * 0; rows ld elements apart, any alignment of the elements), in one pass over
  * it.  Per row, each output optional (NULL):
@@ -827,6 +866,58 @@ size_t iris_gpu_token_logprobs_workspace(int rows, int vocab);
 int iris_gpu_token_logprobs(const void *logits, int f32, int64_t ld, int rows, int vocab, const int32_t *targets,
                             float *logprob, float *entropy, int top_k, int32_t *top_ids, float *top_logprobs,
                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* The next token of each row of a logits matrix (as above), drawn with random
+ * numbers of the caller's.  The tokens stand in line, largest logit first, equal
+ * ones by id; one of logit x weighs w = exp((x - largest) / temperature).  A first
+ * part of the line is kept: tokens with w >= min_p (over 1: as 1), of these the
+ * first top_k, of these as many as it takes for their weights to reach top_p of the
+ * sum.  The token drawn is the first at which the sum of weights passes uniform *
+ * the sum of what is kept.  Per row, in device memory, each but uniform optional:
+ *   temperature   NULL: 1.  0 or less: the first of the line
+ *   top_k         NULL, 0 or less, vocab or more: all
+ *   top_p         NULL, 1 or more, NaN: all.  0 or less: the first of the line
+ *   min_p         NULL, 0 or less, NaN: all (of the logits above -inf)
+ *   uniform       f64, [0, 1); outside, and NaN: the nearest inside, NaN 0
+ * Out:
+ *   ids           the token; -1 where a row has nothing but -inf, or a NaN or +inf
+ *                 among its logits, or a temperature of NaN
+ *   logprobs      (optional) log of its weight's share of what is kept; with -1 -inf
+ *   kept          (optional) tokens kept; with -1 0
+ * Weights and sums are 64-bit.  The same call gives the same bits every time. */
+int iris_gpu_sample_tokens(const void *logits, int f32, int64_t ld, int rows, int vocab, const float *temperature,
+                           const int32_t *top_k, const float *top_p, const float *min_p, const double *uniform,
+                           int32_t *ids, float *logprobs, int32_t *kept, void *stream);
+
+/* Weights of 4 bits [n, k]: column j of a row is (q - zero) * scale of its group
+ * of `group` columns, q from half j % 2 of byte j / 2 (the low half first). */
+typedef struct {
+    void *q;                  /* [n] rows of k / 2 bytes                                 */
+    void *scale;              /* [n] rows of k / group, bf16, or f32 when scale_f32 != 0 */
+    const uint8_t *zero;      /* the same shape, 0 to 127; NULL: 8                       */
+    int n, k;                 /* k a multiple of group                                   */
+    int group;                /* 32, 64 or a multiple of 128                             */
+    int scale_f32;
+    int64_t q_stride;         /* bytes between rows, a multiple of 16; q 16-byte aligned */
+    int64_t scale_stride;     /* elements between rows of scale, and of zero             */
+    int64_t zero_stride;
+} iris_gpu_weights4_t;
+
+/* Rounds weights w [n, k] (bf16, or f32 when f32 != 0; rows ldw elements apart, a
+ * multiple of 8, 16-byte aligned) into out's q and scale (out's zero has to be
+ * NULL): a group's scale is its largest magnitude / 7, rounded to the scale's type,
+ * and q = round(w / scale) + 8, ties to even, 0 to 15.  A group with an infinity or
+ * NaN gets the scale NaN. */
+int iris_gpu_quantize4(const iris_gpu_weights4_t *out, const void *w, int f32, int64_t ldw, void *stream);
+
+/* out[r] = W x[r] (+ add[r]) for few rows: x bf16 [rows, k] (rows ldx elements
+ * apart, a multiple of 8, 16-byte aligned), out and add [rows, n] bf16, or f32 when
+ * f32 != 0 (add may be out, with its row stride, or NULL; out otherwise not over
+ * what is read).  Weights and x are multiplied as they are, sums are f32, out is
+ * rounded once.  Every 32 rows read the weights once: for prompts a dense product
+ * is the better choice. */
+int iris_gpu_linear4(const iris_gpu_weights4_t *w, const void *x, int64_t ldx, int rows, void *out, int64_t ldo,
+                     const void *add, int64_t ldadd, int f32, void *stream);
 
 #ifdef __cplusplus
 }

@@ -427,6 +427,13 @@ cudaError_t iris_launch_add_bf16(void *out, const void *a, const void *b, long n
 /* ------------------------------------------------------------------ language-model operators (lm_kernels.cu)
  * Arguments as the public entry points of the same names, already checked. */
 #include "paged.h"
+/* the scales of an 8-bit cache: exponent bytes of the blocks of `block` tokens; its pools' places are bytes */
+typedef struct {
+    uint8_t *k, *v;
+    int64_t page_stride, block_stride, head_stride;
+    int block;
+    iris_paged_div_t div;     /* by block; set by the launches */
+} iris_kv_exp_t;
 typedef struct {
     iris_gpu_kv_cache_t cache;
     iris_gpu_rope_t rope;     /* rot_dim 0: no rotation */
@@ -438,6 +445,7 @@ typedef struct {
     const int32_t *seq, *pos;
     int tokens, heads;
     iris_paged_div_t div;     /* set by iris_launch_rope_append */
+    iris_kv_exp_t exp;        /* of an 8-bit cache */
 } IrisRopeAppend;
 cudaError_t iris_launch_rope_append(IrisRopeAppend *a, int f32, int num_sms, cudaStream_t stream);
 typedef struct {
@@ -450,6 +458,7 @@ typedef struct {
     float scale;
     float *ws;
     iris_paged_div_t div;     /* set by iris_launch_paged_attention */
+    iris_kv_exp_t exp;        /* of an 8-bit cache */
 } IrisPagedAttention;
 /* one-time kernel attribute setup, called at library init */
 cudaError_t iris_lm_init(void);
@@ -465,8 +474,48 @@ typedef struct {
     int32_t *top_ids;
     void *ws;
 } IrisLogprobs;
+/* the same over an 8-bit cache (a->exp) */
+cudaError_t iris_launch_rope_append8(IrisRopeAppend *a, int f32, int num_sms, cudaStream_t stream);
+size_t iris_paged_attention8_ws_bytes(const iris_gpu_kv_cache_t *cache, int heads, int num_sms);
+cudaError_t iris_launch_paged_attention8(IrisPagedAttention *a, int num_sms, cudaStream_t stream, int *launches);
 size_t iris_logprobs_ws_bytes(int rows, int vocab);
 cudaError_t iris_launch_logprobs(const IrisLogprobs *a, int f32, int num_sms, cudaStream_t stream, int *launches);
+
+/* sampling_kernels.cu */
+typedef struct {
+    const void *logits;
+    int64_t ld;
+    int rows, vocab;
+    const float *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    const double *uniform;
+    int32_t *ids, *kept;
+    float *logprobs;
+    int parts, held_bytes;    /* set by iris_launch_sample */
+} IrisSample;
+cudaError_t iris_sample_init(void);
+cudaError_t iris_launch_sample(IrisSample *a, int f32, cudaStream_t stream);
+
+/* linear4_kernels.cu */
+typedef struct {
+    const uint8_t *q, *zero;
+    const void *scale, *x, *add;
+    void *out;
+    int64_t ldq, lds, ldz, ldx, ldadd, ldo;
+    int n, k, group, rows, scale_f32, f32;
+    int parts;                /* set by iris_launch_linear4, as div: by the chunks of a group */
+    iris_paged_div_t div;
+} IrisLinear4;
+cudaError_t iris_linear4_init(void);
+cudaError_t iris_launch_linear4(IrisLinear4 *a, int num_sms, cudaStream_t stream);
+typedef struct {
+    uint8_t *q;
+    void *scale;
+    const void *w;
+    int64_t ldq, lds, ldw;
+    int n, k, group, scale_f32;
+} IrisQuantize4;
+cudaError_t iris_launch_quantize4(const IrisQuantize4 *a, int f32, int num_sms, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -5,23 +5,16 @@
 #include <type_traits>
 
 #include "iris_kernels.h"
+#include "lm_device.cuh"
 #include "paged.h"
 #include "ptx.cuh"
 
 #include <cuda_bf16.h>
+#include <cuda_fp8.h>
 #include <math.h>
 #include <stdint.h>
 
 namespace {
-
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-
-__device__ __forceinline__ float2 unpack2(uint32_t u) {
-  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
-}
 
 // ------------------------------------------------------------------ rotary positions into the cache
 // Bound by the bytes of Q, K and V, in once and out once.  One block per token
@@ -57,6 +50,38 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
   a = u;
 }
 
+// A lane's 8 columns of a head (ca .. ca + 3 and cb .. cb + 3) through the norm with weights w (NULL: none) and the rotation
+// by c4, s4: of pairs across x and y where `halves`, else, where `turned`, of neighbours.  The head's lanes are together in a
+// warp and take the same way.
+template <int HD>
+__device__ __forceinline__ void norm_turn(float4& x, float4& y, const float* w, float eps, int ca, int cb, bool halves,
+                                          bool turned, float4 c4, float4 s4) {
+  constexpr int LPH = HD / 8;
+  if (w) {
+    float ss = ((x.x * x.x + x.y * x.y) + (x.z * x.z + x.w * x.w)) + ((y.x * y.x + y.y * y.y) + (y.z * y.z + y.w * y.w));
+    const uint32_t lanes = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1) << (threadIdx.x % 32 / LPH * LPH);
+#pragma unroll
+    for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
+    const float r = rsqrtf(ss * (1.0f / HD) + eps);
+    const float4 wa = *reinterpret_cast<const float4*>(w + ca), wb = *reinterpret_cast<const float4*>(w + cb);
+    x.x *= r * wa.x, x.y *= r * wa.y, x.z *= r * wa.z, x.w *= r * wa.w;
+    y.x *= r * wb.x, y.y *= r * wb.y, y.z *= r * wb.z, y.w *= r * wb.w;
+  }
+  if (halves) {
+    turn(x.x, y.x, c4.x, s4.x), turn(x.y, y.y, c4.y, s4.y), turn(x.z, y.z, c4.z, s4.z), turn(x.w, y.w, c4.w, s4.w);
+  } else if (turned) {
+    turn(x.x, x.y, c4.x, s4.x), turn(x.z, x.w, c4.y, s4.y), turn(y.x, y.y, c4.z, s4.z), turn(y.z, y.w, c4.w, s4.w);
+  }
+}
+
+// cos and sin of pair i at a position
+__device__ __forceinline__ void angle(const iris_gpu_rope_t& rope, int pos, int i, float& c, float& s) {
+  const uint64_t turn = (uint64_t)pos * rope.turns[i];
+  sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
+  c *= rope.amplitude;
+  s *= rope.amplitude;
+}
+
 template <typename In, int HD>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_constant__ IrisRopeAppend a) {
   constexpr int LPH = HD / 8, GROUPS = ROPE_THREADS / LPH;
@@ -87,13 +112,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
   }
   if (seq < 0 || seq >= a.cache.num_seqs || pos < 0) return;
   const int block = iris_paged_block(a.div, pos), page = iris_paged_page(&a.cache, seq, block);
-  for (int i = threadIdx.x; i < rd / 2; i += ROPE_THREADS) {
-    const uint64_t turn = (uint64_t)pos * a.rope.turns[i];
-    float s, c;
-    sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
-    cs[i] = c * a.rope.amplitude;
-    sn[i] = s * a.rope.amplitude;
-  }
+  for (int i = threadIdx.x; i < rd / 2; i += ROPE_THREADS) angle(a.rope, pos, i, cs[i], sn[i]);
   const int64_t slot = page < 0 ? -1 : iris_paged_offset(&a.cache, page, pos - block * a.cache.page_size);
   __nv_bfloat16* qo = (__nv_bfloat16*)a.q_out + (int64_t)t * a.ldq_out;
   __nv_bfloat16* ko = (__nv_bfloat16*)a.cache.k + slot;
@@ -103,25 +122,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
   if (turned) c4 = *reinterpret_cast<const float4*>(cs + lane * 4), s4 = *reinterpret_cast<const float4*>(sn + lane * 4);
   auto one = [&](int h, float4 x, float4 y) {
     const bool is_q = h < nh, is_v = h >= nh + nkv;
-    if (!is_v) {
-      const float* w = is_q ? a.q_norm : a.k_norm;
-      if (w) {
-        float ss = ((x.x * x.x + x.y * x.y) + (x.z * x.z + x.w * x.w)) + ((y.x * y.x + y.y * y.y) + (y.z * y.z + y.w * y.w));
-        // the lanes of a head are together in one warp and take the same way
-        const uint32_t lanes = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1) << (threadIdx.x % 32 / LPH * LPH);
-#pragma unroll
-        for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
-        const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
-        const float4 wa = *reinterpret_cast<const float4*>(w + ca), wb = *reinterpret_cast<const float4*>(w + cb);
-        x.x *= r * wa.x, x.y *= r * wa.y, x.z *= r * wa.z, x.w *= r * wa.w;
-        y.x *= r * wb.x, y.y *= r * wb.y, y.z *= r * wb.z, y.w *= r * wb.w;
-      }
-      if (halves) {
-        turn(x.x, y.x, c4.x, s4.x), turn(x.y, y.y, c4.y, s4.y), turn(x.z, y.z, c4.z, s4.z), turn(x.w, y.w, c4.w, s4.w);
-      } else if (turned) {
-        turn(x.x, x.y, c4.x, s4.x), turn(x.z, x.w, c4.y, s4.y), turn(y.x, y.y, c4.z, s4.z), turn(y.z, y.w, c4.w, s4.w);
-      }
-    }
+    if (!is_v) norm_turn<HD>(x, y, is_q ? a.q_norm : a.k_norm, a.eps, ca, cb, halves, turned, c4, s4);
     if (!is_q && slot < 0) return;
     __nv_bfloat16* to = is_q ? qo + h * HD : is_v ? vo + (int64_t)(h - nh - nkv) * a.cache.head_stride
                                                   : ko + (int64_t)(h - nh) * a.cache.head_stride;
@@ -131,6 +132,161 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
 #pragma unroll
   for (int i = 0; i < ROPE_HEADS; i++)
     if (first + i * step < total) one(first + i * step, values4(ra[i]), values4(rb[i]));
+}
+
+// ------------------------------------------------------------------ keys and values into an 8-bit cache
+// The queries go the way above.  A scale is shared by a block of tokens, so the
+// tokens of a call that belong to one block of the cache (its mates) are taken
+// together, by the thread block of the first of them: it looks for the others among
+// all tokens of the call, in whatever order they stand (a token whose mate is the row
+// before leaves at once, so that a prompt's rows are searched once a block of the
+// cache).  Lanes hold columns as above; a warp has two (head, K or V), and goes over
+// the mates twice, for the largest magnitude and, behind the scale, for the values,
+// which the second time come from L1.
+constexpr int APPEND8_THREADS = 256, APPEND8_ITEMS = 2, APPEND8_SLOTS = 16;  // slots whose angles are held at a time
+
+// four values at a scale as e4m3, what is not finite as NaN
+__device__ __forceinline__ uint32_t to_e4m3(float4 x, float f) {
+  auto value = [&](float v) { return fabsf(v) <= 3.4028235e38f ? v * f : __uint_as_float(0x7FC00000u); };
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
+      "mov.b32 %0, {a, b};\n\t}"
+      : "=r"(r)
+      : "f"(value(x.x)), "f"(value(x.y)), "f"(value(x.z)), "f"(value(x.w)));
+  return r;
+}
+__device__ __forceinline__ uint32_t scaled_e4m3(uint32_t w, float f) {
+  uint32_t lo, hi;
+  e4m3_to_f16(w, lo, hi);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return to_e4m3(make_float4(a.x, a.y, b.x, b.y), f);
+}
+
+// the larger of the magnitudes' bits, of finite ones
+__device__ __forceinline__ uint32_t most_bits(uint32_t top, float4 x) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+    top = b < 0x7F800000u && b > top ? b : top;
+  }
+  return top;
+}
+
+// exponent of the least scale that brings a magnitude within 448 = 1.75 * 2^8
+__device__ __forceinline__ int exponent8(uint32_t bits) {
+  const int e = (int)(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u);
+  return min(max(e, IRIS_EXP8_MIN), IRIS_EXP8_MAX);
+}
+
+template <typename In, int HD>
+__global__ void __launch_bounds__(APPEND8_THREADS) rope_append8_kernel(const __grid_constant__ IrisRopeAppend a) {
+  constexpr int LPH = HD / 8, UNITS = 32 / LPH;  // lanes of a (token, head), of which a warp takes UNITS
+  using Raw = typename Raw4<In>::T;
+  __shared__ __align__(16) float cs[APPEND8_SLOTS][HD / 2], sn[APPEND8_SLOTS][HD / 2];
+  __shared__ int rows[128];  // of the call, by the block's slots
+  __shared__ int first;
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid % LPH, unit = tid % 32 / LPH;
+  const int nkv = a.cache.kv_heads, rd = a.rope.rot_dim, size = a.exp.block;
+  const bool turned = lane < rd / 8, halves = a.rope.layout == IRIS_ROPE_HALF && turned;
+  const int ca = halves ? lane * 4 : lane * 8, cb = halves ? rd / 2 + lane * 4 : lane * 8 + 4;
+  iris::grid_dep_wait();
+  iris::grid_dep_launch();
+  const int seq = a.seq[t], pos = a.pos[t];
+  const int seq_before = t ? a.seq[t - 1] : -1, pos_before = t ? a.pos[t - 1] : -1;
+  if (seq < 0 || seq >= a.cache.num_seqs || pos < 0) return;
+  const int part = iris_paged_block(a.exp.div, pos), begin = part * size;  // the block of the sequence, its first position
+  if (seq_before == seq && pos_before >= 0 && iris_paged_block(a.exp.div, pos_before) == part) return;
+  const int block = iris_paged_block(a.div, pos), page = iris_paged_page(&a.cache, seq, block);
+  if (page < 0) return;
+  for (int i = tid; i < size; i += APPEND8_THREADS) rows[i] = -1;
+  if (tid == 0) first = t;
+  __syncthreads();
+  for (int u0 = tid; u0 < a.tokens; u0 += 4 * APPEND8_THREADS) {
+    int s[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) s[j] = u0 + j * APPEND8_THREADS < a.tokens ? a.seq[u0 + j * APPEND8_THREADS] : -1;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (s[j] != seq) continue;
+      const int u = u0 + j * APPEND8_THREADS, at = a.pos[u] - begin;
+      if (a.pos[u] < 0 || at < 0 || at >= size) continue;
+      atomicMax(&rows[at], u);
+      atomicMin(&first, u);
+    }
+  }
+  __syncthreads();
+  if (first != t) return;
+
+  const int first_slot = begin - block * a.cache.page_size;  // of the page
+  const bool fresh = rows[0] >= 0;
+  const int item0 = (blockIdx.y * (APPEND8_THREADS / 32) + tid / 32) * APPEND8_ITEMS;
+  const int chunks = (size + APPEND8_SLOTS - 1) / APPEND8_SLOTS;
+  uint32_t top[APPEND8_ITEMS] = {};
+  int exp[APPEND8_ITEMS], old[APPEND8_ITEMS];
+  for (int pass = 0; pass < 2; pass++) {
+    for (int c = 0; c < chunks; c++) {
+      const int slot0 = c * APPEND8_SLOTS, slots = min(APPEND8_SLOTS, size - slot0);
+      if (pass == 0 || chunks > 1) {
+        __syncthreads();
+        for (int i = tid; i < slots * (rd / 2); i += APPEND8_THREADS) {
+          const int s = i / (rd / 2), p = i - s * (rd / 2);
+          if (rows[slot0 + s] >= 0) angle(a.rope, begin + slot0 + s, p, cs[s][p], sn[s][p]);
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int k = 0; k < APPEND8_ITEMS; k++) {
+        const int item = item0 + k, head = item < nkv ? item : item - nkv;
+        if (item >= 2 * nkv) continue;
+        const bool is_v = item >= nkv;
+        const In* from = (const In*)(is_v ? a.v : a.k) + head * HD;
+        const int64_t ld = is_v ? a.ldv : a.ldk;
+        uint8_t* to = (uint8_t*)(is_v ? a.cache.v : a.cache.k) + iris_paged_offset(&a.cache, page, first_slot) +
+                      head * a.cache.head_stride;
+        for (int s = unit; s < slots; s += UNITS) {
+          const int row = rows[slot0 + s];
+          uint8_t* at = to + (slot0 + s) * a.cache.token_stride;
+          if (row >= 0) {
+            const In* r = from + row * ld;
+            float4 x = values4(*reinterpret_cast<const Raw*>(r + ca)), y = values4(*reinterpret_cast<const Raw*>(r + cb));
+            if (!is_v) {
+              float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (turned) {
+                c4 = *reinterpret_cast<const float4*>(&cs[s][lane * 4]);
+                s4 = *reinterpret_cast<const float4*>(&sn[s][lane * 4]);
+              }
+              norm_turn<HD>(x, y, a.k_norm, a.eps, ca, cb, halves, turned, c4, s4);
+            }
+            if (pass == 0) {
+              top[k] = most_bits(most_bits(top[k], x), y);
+            } else {
+              const float f = scale8(254 - exp[k]);
+              *reinterpret_cast<uint32_t*>(at + ca) = to_e4m3(x, f);
+              *reinterpret_cast<uint32_t*>(at + cb) = to_e4m3(y, f);
+            }
+          } else if (pass == 1 && !fresh && exp[k] > old[k]) {  // what was there, to the larger scale
+            uint2* w = reinterpret_cast<uint2*>(at + lane * 8);
+            const float f = scale8(127 + old[k] - exp[k]);
+            *w = make_uint2(scaled_e4m3(w->x, f), scaled_e4m3(w->y, f));
+          }
+        }
+      }
+    }
+    if (pass) break;
+#pragma unroll
+    for (int k = 0; k < APPEND8_ITEMS; k++) {
+      const int item = item0 + k;
+      if (item >= 2 * nkv) continue;
+      uint8_t* at = (item < nkv ? a.exp.k + item * a.exp.head_stride : a.exp.v + (item - nkv) * a.exp.head_stride) +
+                    page * a.exp.page_stride + iris_paged_block(a.exp.div, first_slot) * a.exp.block_stride;
+      exp[k] = exponent8(__reduce_max_sync(0xffffffffu, top[k]));
+      old[k] = exp8(*at);
+      if (!fresh) exp[k] = max(exp[k], old[k]);
+      __syncwarp();
+      if (tid % 32 == 0) *at = (uint8_t)exp[k];
+    }
+  }
 }
 
 // ------------------------------------------------------------------ attention over the cache
@@ -155,34 +311,6 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
 // At a unit's end the four warps' sums are joined in shared memory and written,
 // or, where a share's border cuts the unit, left for the join kernel.
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-
-__device__ __forceinline__ void ldsm4t(uint32_t r[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-
-__device__ __forceinline__ void mma_bf16(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // of two bf16, all bits of each one that is an infinity or NaN
 __device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
   return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
@@ -197,13 +325,74 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_
   lo = pack2(__uint_as_float(b0) - __uint_as_float(b0 & 0xFFFF0000u), __uint_as_float(b1) - __uint_as_float(b1 & 0xFFFF0000u));
 }
 
-// 16 bytes, or zeros where `bytes` is 0 (nothing is read then)
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// A cache's elements: bf16, or e4m3 with exponents (an 8-bit cache).
+//
+// Over 8 bits the products are of f16, which holds every e4m3 value; the queries of
+// a head are scaled by a power of two to fill f16's range (what is under 2^-29 of the
+// largest loses bits).  A key's scale multiplies its score.  The value's scale 2^ve
+// joins the weight instead: with t = s c + ve the running maximum is that of t, p =
+// 2^(t - m) is at most 1 and rounded to f16, 11 bits, and l adds up p 2^-ve in f32.
+// So one product of p and the values as they lie does where bf16 takes two.
+typedef __nv_fp8_storage_t e4m3;
+template <typename E> constexpr bool kEight = sizeof(E) == 1;
+
+// bytes of a row of K or V lie in 16-byte chunks; chunk ch of row r is at place swz(ch, r), so that ldmatrix meets no bank
+// conflict
+template <int BYTES>
+__device__ __forceinline__ int swz(int ch, int r) { return BYTES == 64 ? ch ^ (r >> 1 & 3) : ch ^ (r & 7); }
+
+// The scales of 16 (a block's: 64) keys of a stage.
+template <int N>
+struct Scales8 {
+  float k[N];       // 2^(ke - 127)
+  float v[N];       // ve - 127
+  float v_inv[N];   // 2^(127 - ve)
+};
+template <int N>
+__device__ __forceinline__ void put_scales(Scales8<N>& to, int i, int ke, int ve) {
+  to.k[i] = scale8(ke), to.v[i] = (float)(ve - 127), to.v_inv[i] = scale8(254 - ve);
+}
+// exponents of a key's place, both in one number
+__device__ __forceinline__ uint32_t read_exps(const iris_kv_exp_t& x, int page, int slot, int64_t head) {
+  const int64_t at = page * x.page_stride + iris_paged_block(x.div, slot) * x.block_stride + head;
+  return (uint32_t)__ldg(x.k + at) | (uint32_t)__ldg(x.v + at) << 8;
 }
 
+// A head's queries as f16 for the products over 8 bits: columns 16 j + 4 i4 .. + 3 of each 16 into words `lo` and `hi` of
+// qf[j], scaled by a power of two that brings the largest finite one to 2^14 or more.  Returns what undoes it.  (All lanes
+// take part; the four of a head have it together.)
+template <int HD, int N>
+__device__ __forceinline__ float queries8(const __nv_bfloat16* q, bool live, int i4, uint32_t (&qf)[HD / 16][N], int lo, int hi) {
+  uint2 u[HD / 16];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < HD / 16; j++) {
+    u[j] = live ? *reinterpret_cast<const uint2*>(q + 16 * j + 4 * i4) : make_uint2(0u, 0u);
+    const uint32_t w[4] = {u[j].x << 16, u[j].x, u[j].y << 16, u[j].y};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t b = w[i] & 0x7FFF0000u;
+      top = b < 0x7F800000u && b > top ? b : top;
+    }
+  }
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int up = min(268 - (int)(top >> 23), 253);
+  const float f = scale8(up);
+#pragma unroll
+  for (int j = 0; j < HD / 16; j++) {
+    const float2 a = unpack2(u[j].x), b = unpack2(u[j].y);
+    qf[j][lo] = pack2h(a.x * f, a.y * f);
+    qf[j][hi] = pack2h(b.x * f, b.y * f);
+  }
+  return scale8(254 - up);
+}
+
+// of four e4m3, all bits of each one that is NaN
+__device__ __forceinline__ uint32_t nan4(uint32_t x) { return __vcmpeq4(x & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+
 // HD: head_dim.  MH: query heads of a unit (8 or 16).
-template <int HD, int MH>
+template <typename E, int HD, int MH>
 struct PagedShape {
   static constexpr int kPair = HD / 128 ? HD / 128 : 1;          // warps on the same 16 keys, 128 columns of o each
   static constexpr int kThreads = 128 * kPair;
@@ -211,9 +400,10 @@ struct PagedShape {
   // 3 x 4 0.88 of the time of 2 x 6, 5 x 2 1.03 and 6 x 2 1.4 of that of 4 x 2: the arithmetic of 16 short keys is
   // latency and wants warps, until registers spill.  At 128 and 256 a ring of three stages fills shared memory, with MH =
   // 16 two.
-  static constexpr int kCtas = HD == 64 ? 4 : HD == 128 ? 2 : 1;
-  static constexpr int kStages = HD == 64 || MH == 16 ? 2 : 3;
-  static constexpr int kStageBytes = 16 * HD * 2;                // 16 rows of K or of V
+  static constexpr int kRow = HD * (int)sizeof(E);               // bytes of a row
+  static constexpr int kCtas = HD == 64 ? 4 : HD == 128 ? (kEight<E> ? 3 : 2) : 1;
+  static constexpr int kStages = kEight<E> ? 4 : HD == 64 || MH == 16 ? 2 : 3;
+  static constexpr int kStageBytes = 16 * kRow;                  // 16 rows of K or of V
   static constexpr int kRing = kStages * 2 * kStageBytes;        // of 16 keys of a tile
   static constexpr int kSlot = MH * (HD + 2);                    // floats of a piece: m, l, then o
   static constexpr int kSmem = 4 * kRing + 4 * kSlot * 4;
@@ -307,15 +497,17 @@ __device__ __forceinline__ bool paged_begin(const IrisPagedAttention& a, int uni
 // CLUSTER: few rows and short tables.  A cluster of blocks, or one, takes one unit, an
 // equal part of its tiles each, and joins the parts in distributed shared
 // memory: one launch, and no round through the workspace.
-template <int HD, int MH, bool CLUSTER>
-__global__ void __launch_bounds__(PagedShape<HD, MH>::kThreads, PagedShape<HD, MH>::kCtas)
+template <typename E, int HD, int MH, bool CLUSTER>
+__global__ void __launch_bounds__(PagedShape<E, HD, MH>::kThreads, PagedShape<E, HD, MH>::kCtas)
 paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
-  using Sh = PagedShape<HD, MH>;
-  constexpr int D = Sh::kStages, CH = HD / 8;  // CH: 16-byte chunks of a row
+  using Sh = PagedShape<E, HD, MH>;
+  constexpr bool EIGHT = kEight<E>;
+  constexpr int D = Sh::kStages, CH = Sh::kRow / 16;  // CH: 16-byte chunks of a row
   constexpr int PAIR = Sh::kPair, T = Sh::kThreads, OC = HD / PAIR;  // OC: columns of o a warp holds
   constexpr bool WIDE = MH == 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t seen[4][D];  // of each 16 keys of a tile and stage: which exist
+  __shared__ __align__(16) Scales8<EIGHT ? 16 : 1> scales[EIGHT ? 4 : 1][EIGHT ? D : 1];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, i4 = lane % 4;
   const int kg = warp / PAIR, half = warp % PAIR;  // which 16 keys of a tile, which columns of o
   auto sync_keys = [&]() {  // the warps on the same keys
@@ -340,7 +532,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       if (at.s >= 0 && part == 0) {
         const int r = at.u % (units / cache.kv_heads), h0 = at.u / (units / cache.kv_heads) * group + r * MH;
         uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)h0 * HD);
-        for (int c = tid; c < min(MH, group - r * MH) * CH; c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = tid; c < min(MH, group - r * MH) * (HD / 8); c += T) o[c] = make_uint4(0u, 0u, 0u, 0u);
       }
       return;
     }
@@ -361,29 +553,42 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   bool loads = any;
   int page, slot;                  // of this lane's key (lanes 16-31 as lanes 0-15) of the next tile to load
   int64_t head = 0;                // its head's offset
+  int64_t exp_head = 0;            // the same among the exponents
+  uint32_t exps = 0;               // of this lane's key of the tile loaded last, on their way to shared memory
+  int exps_to = -1;                // their stage
   auto find = [&]() {
     const int p = ld.i * IRIS_PAGED_TILE + kg * 16 + (lane & 15), b = iris_paged_block(a.div, p);
     slot = p - b * cache.page_size;
     page = p < ld.len ? iris_paged_page(&cache, ld.s, b) : -1;
-    if (ld.i == 0) head = (int64_t)(ld.u / rtiles) * cache.head_stride;
+    if (ld.i == 0) {
+      head = (int64_t)(ld.u / rtiles) * cache.head_stride;
+      if constexpr (EIGHT) exp_head = (int64_t)(ld.u / rtiles) * a.exp.head_stride;
+    }
   };
   head = (int64_t)(ld.u / rtiles) * cache.head_stride;
+  if constexpr (EIGHT) exp_head = (int64_t)(ld.u / rtiles) * a.exp.head_stride;
   if (loads) find();
   auto issue = [&](int stage) {
+    if constexpr (EIGHT) {
+      // the exponents of the stage before: read a round ago, needed in the next one at the earliest
+      if (exps_to >= 0 && half == 0 && lane < 16) put_scales(scales[kg][exps_to], lane, exp8(exps & 0xFF), exp8(exps >> 8));
+      exps_to = loads ? stage : -1;
+    }
     if (loads) {
       const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
       const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
       if (half == 0 && lane == 0) seen[kg][stage] = have;
+      if constexpr (EIGHT) exps = page >= 0 ? read_exps(a.exp, page, slot, exp_head) : 0x7F7Fu;
       const uint32_t kd = ring + stage * 2 * Sh::kStageBytes, vd = kd + Sh::kStageBytes;
       constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows one instruction of the warp covers
 #pragma unroll
       for (int j = 0; j < 16 / RPI / PAIR; j++) {
         const int r = (j * PAIR + half) * RPI + lane / CH, ch = lane % CH;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r) + ch * 8;
+        const int64_t o = __shfl_sync(0xffffffffu, off, r) + ch * (16 / (int)sizeof(E));
         const int bytes = (have >> r) & 1 ? 16 : 0;
-        const uint32_t d = r * (HD * 2) + ((ch ^ (r & 7)) << 4);
-        cp_async16(kd + d, (const __nv_bfloat16*)cache.k + o, bytes);
-        cp_async16(vd + d, (const __nv_bfloat16*)cache.v + o, bytes);
+        const uint32_t d = r * Sh::kRow + (swz<Sh::kRow>(ch, r) << 4);
+        cp_async16(kd + d, (const E*)cache.k + o, bytes);
+        cp_async16(vd + d, (const E*)cache.v + o, bytes);
       }
       loads = iris_paged_more(&ld);
       if (loads) {
@@ -400,19 +605,24 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   const float c = a.scale * 1.4426950408889634f;
   uint32_t qf[HD / 16][2 * R];
   float o[OC / 8][4], m[R], l[R];
+  float cq[R];  // c times what the queries were divided by
   int heads_here = 0, head0 = 0;
   auto begin_unit = [&]() {
     const int kvh = at.u / rtiles, r = at.u - kvh * rtiles;
     head0 = kvh * group + r * MH;
     heads_here = min(MH, group - r * MH);
-    const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)at.t * a.ldq + (int64_t)(head0 + g) * HD + 2 * i4;
+    const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)at.t * a.ldq + (int64_t)(head0 + g) * HD;
 #pragma unroll
     for (int h = 0; h < R; h++) {
       const bool live = g + 8 * h < heads_here;
+      if constexpr (EIGHT) {
+        cq[h] = c * queries8<HD, 2 * R>(q + h * 8 * HD, live, i4, qf, h, R + h);
+      } else {
 #pragma unroll
-      for (int j = 0; j < HD / 16; j++) {
-        qf[j][h] = live ? *reinterpret_cast<const uint32_t*>(q + h * 8 * HD + j * 16) : 0u;
-        qf[j][R + h] = live ? *reinterpret_cast<const uint32_t*>(q + h * 8 * HD + j * 16 + 8) : 0u;
+        for (int j = 0; j < HD / 16; j++) {
+          qf[j][h] = live ? *reinterpret_cast<const uint32_t*>(q + 2 * i4 + h * 8 * HD + j * 16) : 0u;
+          qf[j][R + h] = live ? *reinterpret_cast<const uint32_t*>(q + 2 * i4 + h * 8 * HD + j * 16 + 8) : 0u;
+        }
       }
       m[h] = -INFINITY;
       l[h] = 0.f;
@@ -438,20 +648,56 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
       // matrices (keys 0-7, columns 0-7), (keys 0-7, 8-15), (keys 8-15, 0-7), (keys 8-15, 8-15) of each 16 columns
       const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+      if constexpr (EIGHT) {
+        // (keys 0-7, columns 0-15), (keys 0-7, 16-31), (keys 8-15, 0-15), (keys 8-15, 16-31) of each 32 columns, four
+        // of them, 4 i4 .. 4 i4 + 3, in a lane's word
 #pragma unroll
-      for (int j = 0; j < HD / 16; j++) {
-        uint32_t b[4];
-        ldsm4(b, kd + kr * (HD * 2) + (((2 * j + kc) ^ (kr & 7)) << 4));
-        const uint32_t a1 = WIDE ? qf[j][1] : 0u, a3 = WIDE ? qf[j][2 * R - 1] : 0u;
-        mma_bf16(s0, qf[j][0], a1, qf[j][R], a3, b[0], b[1]);
-        mma_bf16(s1, qf[j][0], a1, qf[j][R], a3, b[2], b[3]);
+        for (int j = 0; j < HD / 32; j++) {
+          uint32_t b[4];
+          ldsm4(b, kd + kr * Sh::kRow + (swz<Sh::kRow>(2 * j + kc, kr) << 4));
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            const uint32_t* qj = qf[2 * j + n];
+            const uint32_t a1 = WIDE ? qj[1] : 0u, a3 = WIDE ? qj[2 * R - 1] : 0u;
+            uint32_t b0, b1;
+            e4m3_to_f16(b[n], b0, b1);
+            mma_f16(s0, qj[0], a1, qj[R], a3, b0, b1);
+            e4m3_to_f16(b[2 + n], b0, b1);
+            mma_f16(s1, qj[0], a1, qj[R], a3, b0, b1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < HD / 16; j++) {
+          uint32_t b[4];
+          ldsm4(b, kd + kr * (HD * 2) + (((2 * j + kc) ^ (kr & 7)) << 4));
+          const uint32_t a1 = WIDE ? qf[j][1] : 0u, a3 = WIDE ? qf[j][2 * R - 1] : 0u;
+          mma_bf16(s0, qf[j][0], a1, qf[j][R], a3, b[0], b[1]);
+          mma_bf16(s1, qf[j][0], a1, qf[j][R], a3, b[2], b[3]);
+        }
       }
       uint32_t hi[R][2], lo[R][2];
       bool moved = false;
       float f[R];
+      [[maybe_unused]] float2 kx[2], vx[2], vi[2];  // scales of keys 2 i4, 2 i4 + 1, and 8 more
+      if constexpr (EIGHT) {
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          const auto& sc = scales[kg][stage];
+          kx[n] = *reinterpret_cast<const float2*>(sc.k + 8 * n + 2 * i4);
+          vx[n] = *reinterpret_cast<const float2*>(sc.v + 8 * n + 2 * i4);
+          vi[n] = *reinterpret_cast<const float2*>(sc.v_inv + 8 * n + 2 * i4);
+        }
+      }
 #pragma unroll
       for (int h = 0; h < R; h++) {
-        float x0 = s0[2 * h] * c, x1 = s0[2 * h + 1] * c, x2 = s1[2 * h] * c, x3 = s1[2 * h + 1] * c;
+        float x0, x1, x2, x3;
+        if constexpr (EIGHT) {
+          x0 = s0[2 * h] * (cq[h] * kx[0].x) + vx[0].x, x1 = s0[2 * h + 1] * (cq[h] * kx[0].y) + vx[0].y;
+          x2 = s1[2 * h] * (cq[h] * kx[1].x) + vx[1].x, x3 = s1[2 * h + 1] * (cq[h] * kx[1].y) + vx[1].y;
+        } else {
+          x0 = s0[2 * h] * c, x1 = s0[2 * h + 1] * c, x2 = s1[2 * h] * c, x3 = s1[2 * h + 1] * c;
+        }
         if (have != 0xFFFFu) {
           const uint32_t hv = have >> (2 * i4);
           if (!(hv & 1)) x0 = -INFINITY;
@@ -469,9 +715,15 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         m[h] = mn;
         const float p0 = exp2_approx(x0 - base), p1 = exp2_approx(x1 - base), p2 = exp2_approx(x2 - base),
                     p3 = exp2_approx(x3 - base);
-        l[h] = l[h] * f[h] + ((p0 + p1) + (p2 + p3));
-        split2(p0, p1, hi[h][0], lo[h][0]);
-        split2(p2, p3, hi[h][1], lo[h][1]);
+        if constexpr (EIGHT) {
+          l[h] = l[h] * f[h] + ((p0 * vi[0].x + p1 * vi[0].y) + (p2 * vi[1].x + p3 * vi[1].y));
+          hi[h][0] = pack2h(p0, p1);
+          hi[h][1] = pack2h(p2, p3);
+        } else {
+          l[h] = l[h] * f[h] + ((p0 + p1) + (p2 + p3));
+          split2(p0, p1, hi[h][0], lo[h][0]);
+          split2(p2, p3, hi[h][1], lo[h][1]);
+        }
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -481,18 +733,37 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         }
       }
       // transposed: (keys 0-7, columns 0-7), (keys 8-15, 0-7), (keys 0-7, 8-15), (keys 8-15, 8-15)
-      const int vr = lane & 15, vc = (lane >> 4) + half * (OC / 8);
+      const int vr = lane & 15, vc = (lane >> 4) + half * (OC * (int)sizeof(E) / 16);
+      if constexpr (EIGHT) {
+        // a lane's word: columns 2 g and 2 g + 1 of keys 2 i4 and 2 i4 + 1; even and odd columns of a chunk are a
+        // product each, so that c0 and c1 of both are the columns 4 i4 .. 4 i4 + 3
 #pragma unroll
-      for (int j = 0; j < OC / 16; j++) {
-        uint32_t b[4];
-        ldsm4t(b, vd + vr * (HD * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
+        for (int j = 0; j < OC / 32; j++) {
+          uint32_t b[4];
+          ldsm4t(b, vd + vr * Sh::kRow + (swz<Sh::kRow>(2 * j + vc, vr) << 4));
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          if constexpr (WIDE) {
-            mma_bf16(o[2 * j + n], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b[2 * n], b[2 * n + 1]);
-            mma_bf16(o[2 * j + n], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b[2 * n], b[2 * n + 1]);
-          } else {
-            mma_bf16(o[2 * j + n], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b[2 * n], b[2 * n + 1]);
+          for (int n = 0; n < 2; n++) {
+            uint32_t e0, e1, d0, d1;
+            e4m3_to_f16(__byte_perm(b[2 * n], 0u, 0x3120), e0, d0);
+            e4m3_to_f16(__byte_perm(b[2 * n + 1], 0u, 0x3120), e1, d1);
+            const uint32_t a1 = WIDE ? hi[R - 1][0] : 0u, a3 = WIDE ? hi[R - 1][1] : 0u;
+            mma_f16(o[4 * j + 2 * n], hi[0][0], a1, hi[0][1], a3, e0, e1);
+            mma_f16(o[4 * j + 2 * n + 1], hi[0][0], a1, hi[0][1], a3, d0, d1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < OC / 16; j++) {
+          uint32_t b[4];
+          ldsm4t(b, vd + vr * (HD * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            if constexpr (WIDE) {
+              mma_bf16(o[2 * j + n], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b[2 * n], b[2 * n + 1]);
+              mma_bf16(o[2 * j + n], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b[2 * n], b[2 * n + 1]);
+            } else {
+              mma_bf16(o[2 * j + n], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b[2 * n], b[2 * n + 1]);
+            }
           }
         }
       }
@@ -510,8 +781,17 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         if (half == 0 && i4 == 0) mine_f[2 * (g + 8 * h)] = m[h], mine_f[2 * (g + 8 * h) + 1] = l[h];
       }
       float* mine_o = mine_f + 2 * MH + g * HD;
+      if constexpr (EIGHT) {
 #pragma unroll
-      for (int j = 0; j < OC / 8; j++) {
+        for (int j = 0; j < OC / 16; j++) {
+          float* to = mine_o + Sh::col(g, half * OC + j * 16 + 4 * i4);
+          const float *e = o[2 * j], *d = o[2 * j + 1];
+          *reinterpret_cast<float4*>(to) = make_float4(e[0], d[0], e[1], d[1]);
+          if constexpr (WIDE) *reinterpret_cast<float4*>(to + 8 * HD) = make_float4(e[2], d[2], e[3], d[3]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; !EIGHT && j < OC / 8; j++) {
         float* to = mine_o + Sh::col(g, half * OC + j * 8 + 2 * i4);
         if constexpr (WIDE) {
           *reinterpret_cast<float2*>(to) = make_float2(o[j][0], o[j][1]);
@@ -603,7 +883,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 // between them: registers allow two warps a scheduler, the tensor pipe of mma.sync
 // is active 55 % of the time (a prompt of 8192, 32 heads on 8 of 128: 2636 us, 209
 // TFLOP/s counting 4 flops, an eighth of the measured peak).
-template <int HD>
+template <typename E, int HD>
 struct RunShape {
   static constexpr int kPairs = HD == 256 ? 128 : 64;             // (row, head) pairs of a unit
   static constexpr int kWarps = kPairs / 16, kThreads = 32 * kWarps;
@@ -614,23 +894,27 @@ struct RunShape {
   // keys whose scores a warp holds at a time; a prompt of 2048, 8 heads on 2 of 256, with four warps: 16 330 us, 32 248,
   // with eight warps 162
   static constexpr int kKeys = HD == 256 ? 32 : 64;
-  static constexpr int kPart = IRIS_PAGED_TILE * HD * 2;          // bytes of K or of V of a tile
+  static constexpr int kRow = HD * (int)sizeof(E);                // bytes of a row
+  static constexpr int kPart = IRIS_PAGED_TILE * kRow;            // bytes of K or of V of a tile
   static constexpr int kSlot = kPairs * (HD + 2);                 // floats of a piece, as in PagedShape
-  static constexpr int kSmem = kStages * 2 * kPart;
+  // the sums of a narrow unit take the place of the tile used last, which over 8 bits is too small
+  static constexpr int kSmem = kStages * 2 * kPart + (kEight<E> ? 64 * HD * 4 : 0);
 };
 
 // query heads of a unit of runs
 __device__ __forceinline__ int run_heads(int group) { return group < 16 ? group : 16; }
 
-template <int HD>
-__global__ void __launch_bounds__(RunShape<HD>::kThreads, RunShape<HD>::kCtas)
+template <typename E, int HD>
+__global__ void __launch_bounds__(RunShape<E, HD>::kThreads, RunShape<E, HD>::kCtas)
 paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
-  using Sh = RunShape<HD>;
-  constexpr int D = Sh::kStages, CH = HD / 8, T = Sh::kThreads, NB = HD / 8;
+  using Sh = RunShape<E, HD>;
+  constexpr bool EIGHT = kEight<E>;
+  constexpr int D = Sh::kStages, CH = Sh::kRow / 16, T = Sh::kThreads, NB = HD / 8;
   constexpr int MINE = IRIS_PAGED_TILE / Sh::kWarps;  // keys of a tile that a warp loads, 16 or 8
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint16_t seen[D][4];  // of each 16 keys of a stage's tile: which exist
   __shared__ float2 red_ml[64];
+  __shared__ __align__(16) Scales8<EIGHT ? IRIS_PAGED_TILE : 1> scales[EIGHT ? D : 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, i4 = lane % 4;
   const iris_gpu_kv_cache_t& cache = a.cache;
   const int units = iris_paged_units(&cache, a.heads), group = a.heads / cache.kv_heads, rtiles = units / cache.kv_heads;
@@ -649,32 +933,42 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
   bool loads = true;
   int page, slot;  // of this lane's key (the lanes past a warp's keys as its first) of the next tile to load
   int64_t head;    // its head's offset
+  int64_t exp_head = 0;            // the same among the exponents
+  uint32_t exps = 0;               // of this lane's key of the tile loaded last, on their way to shared memory
+  int exps_to = -1;                // their stage
   auto find = [&]() {
     const int p = ld.i * IRIS_PAGED_TILE + warp * MINE + lane % MINE, b = iris_paged_block(a.div, p);
     slot = p - b * cache.page_size;
     page = p < ld.len ? iris_paged_page(&cache, ld.s, b) : -1;
     head = (int64_t)(ld.u / rtiles) * cache.head_stride;
+    if constexpr (EIGHT) exp_head = (int64_t)(ld.u / rtiles) * a.exp.head_stride;
   };
   find();
   const uint32_t ring = iris::smem_u32(smem);
   auto issue = [&](int stage) {
+    if constexpr (EIGHT) {
+      // the exponents of the stage before: read a round ago, needed behind the next barrier at the earliest
+      if (exps_to >= 0 && lane < MINE) put_scales(scales[exps_to], warp * MINE + lane, exp8(exps & 0xFF), exp8(exps >> 8));
+      exps_to = loads ? stage : -1;
+    }
     if (loads) {
+      if constexpr (EIGHT) exps = page >= 0 ? read_exps(a.exp, page, slot, exp_head) : 0x7F7Fu;
       const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & ((1u << MINE) - 1);
       const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
       if (lane == 0) {
         if constexpr (MINE == 16) seen[stage][warp] = (uint16_t)have;
         else reinterpret_cast<uint8_t*>(seen[stage])[warp] = (uint8_t)have;
       }
-      const uint32_t kd = ring + stage * 2 * Sh::kPart + warp * MINE * HD * 2, vd = kd + Sh::kPart;
+      const uint32_t kd = ring + stage * 2 * Sh::kPart + warp * MINE * Sh::kRow, vd = kd + Sh::kPart;
       constexpr int RPI = 32 / CH;  // rows one instruction of the warp covers
 #pragma unroll
       for (int j = 0; j < MINE / RPI; j++) {
         const int r = j * RPI + lane / CH, ch = lane % CH;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r) + ch * 8;
+        const int64_t o = __shfl_sync(0xffffffffu, off, r) + ch * (16 / (int)sizeof(E));
         const int bytes = (have >> r) & 1 ? 16 : 0;
-        const uint32_t d = r * (HD * 2) + ((ch ^ (r & 7)) << 4);
-        cp_async16(kd + d, (const __nv_bfloat16*)cache.k + o, bytes);
-        cp_async16(vd + d, (const __nv_bfloat16*)cache.v + o, bytes);
+        const uint32_t d = r * Sh::kRow + (swz<Sh::kRow>(ch, r) << 4);
+        cp_async16(kd + d, (const E*)cache.k + o, bytes);
+        cp_async16(vd + d, (const E*)cache.v + o, bytes);
       }
       loads = iris_paged_more(&ld);
       if (loads) {
@@ -691,6 +985,7 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
   const float c = a.scale * 1.4426950408889634f;
   uint32_t qf[HD / 16][4];
   float o[NB][4], m[2], l[2];
+  float cq[2];                  // c times what the queries were divided by
   int row[2], col0[2], len[2];  // the pair's row of the call, its head's first column, its keys (0: no such pair)
   int most = 0, least = 0;      // of the warp's pairs
   bool narrow = false;
@@ -704,11 +999,15 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
       row[h] = at.t + in;
       col0[h] = (kvh * group + r * 16 + hh) * HD;
       len[h] = live ? iris_paged_len(&cache, a.pos[at.t + in]) : 0;
-      const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)row[h] * a.ldq + col0[h] + 2 * i4;
+      const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (int64_t)row[h] * a.ldq + col0[h];
+      if constexpr (EIGHT) {
+        cq[h] = c * queries8<HD, 4>(q, live, i4, qf, h, 2 + h);
+      } else {
 #pragma unroll
-      for (int j = 0; j < HD / 16; j++) {
-        qf[j][h] = live ? *reinterpret_cast<const uint32_t*>(q + j * 16) : 0u;
-        qf[j][2 + h] = live ? *reinterpret_cast<const uint32_t*>(q + j * 16 + 8) : 0u;
+        for (int j = 0; j < HD / 16; j++) {
+          qf[j][h] = live ? *reinterpret_cast<const uint32_t*>(q + 2 * i4 + j * 16) : 0u;
+          qf[j][2 + h] = live ? *reinterpret_cast<const uint32_t*>(q + 2 * i4 + j * 16 + 8) : 0u;
+        }
       }
       if (!live) row[h] = -1;
       m[h] = -INFINITY;
@@ -741,8 +1040,27 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
       for (int n = 0; n < KEYS / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
       // matrices (keys 0-7, columns 0-7), (keys 0-7, 8-15), (keys 8-15, 0-7), (keys 8-15, 8-15) of each 16 columns
       const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+      if constexpr (EIGHT) {
 #pragma unroll
-      for (int j = 0; j < HD / 16; j++)
+        for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+          for (int n = 0; n < KEYS / 16; n++) {
+            if (!PLAIN && n * 16 >= live) continue;
+            uint32_t b[4];
+            ldsm4(b, kd + (k0 + n * 16 + kr) * Sh::kRow + (swz<Sh::kRow>(2 * j + kc, kr) << 4));
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const uint32_t* qj = qf[2 * j + i];
+              uint32_t b0, b1;
+              e4m3_to_f16(b[i], b0, b1);
+              mma_f16(s[2 * n], qj[0], qj[1], qj[2], qj[3], b0, b1);
+              e4m3_to_f16(b[2 + i], b0, b1);
+              mma_f16(s[2 * n + 1], qj[0], qj[1], qj[2], qj[3], b0, b1);
+            }
+          }
+      }
+#pragma unroll
+      for (int j = 0; !EIGHT && j < HD / 16; j++)
 #pragma unroll
         for (int n = 0; n < KEYS / 16; n++) {
           if (!PLAIN && n * 16 >= live) continue;
@@ -756,11 +1074,20 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
       for (int n = 0; n < KEYS / 16; n++) {
         const uint32_t have = seen[stage][k0 / 16 + n];
         const bool all = PLAIN || ((n + 1) * 16 <= clear && have == 0xFFFFu);
+        [[maybe_unused]] float2 kx[2], vx[2];  // scales of keys 2 i4, 2 i4 + 1, and 8 more
+        if constexpr (EIGHT) {
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            kx[i] = *reinterpret_cast<const float2*>(scales[stage].k + k0 + n * 16 + 8 * i + 2 * i4);
+            vx[i] = *reinterpret_cast<const float2*>(scales[stage].v + k0 + n * 16 + 8 * i + 2 * i4);
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const int h = e / 2 % 2, key = e / 4 * 8 + 2 * i4 + e % 2;
           float& x = s[2 * n + e / 4][e % 4];
-          x *= c;
+          if constexpr (EIGHT) x = x * (cq[h] * (e % 2 ? kx[e / 4].y : kx[e / 4].x)) + (e % 2 ? vx[e / 4].y : vx[e / 4].x);
+          else x *= c;
           if (!all && (n * 16 + key >= len[h] - first - k0 || !(have >> key & 1))) x = -INFINITY;
           mx[h] = fmaxf(mx[h], x);
         }
@@ -790,15 +1117,42 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
         for (int n = 0; n < KEYS / 16; n++) {
           if (!PLAIN && n * 16 >= live) continue;
           uint32_t hi[4], lo[4];
+          [[maybe_unused]] float2 vi[2];
+          if constexpr (EIGHT) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+              vi[i] = *reinterpret_cast<const float2*>(scales[stage].v_inv + k0 + n * 16 + 8 * i + 2 * i4);
+          }
 #pragma unroll
           for (int k = 0; k < 4; k++) {  // rows g, g + 8, g, g + 8; keys 0-7, 0-7, 8-15, 8-15
             const int h = k & 1, b = 2 * n + k / 2;
             const float p0 = exp2_approx(s[b][2 * h] - base[h]), p1 = exp2_approx(s[b][2 * h + 1] - base[h]);
-            l[h] += p0 + p1;
-            split2(p0, p1, hi[k], lo[k]);
+            if constexpr (EIGHT) {
+              l[h] += p0 * vi[k / 2].x + p1 * vi[k / 2].y;
+              hi[k] = pack2h(p0, p1);
+            } else {
+              l[h] += p0 + p1;
+              split2(p0, p1, hi[k], lo[k]);
+            }
+          }
+          if constexpr (EIGHT) {
+#pragma unroll
+            for (int j = 0; j < HD / 32; j++) {
+              uint32_t b[4];
+              ldsm4t(b, vd + (k0 + n * 16 + vr) * Sh::kRow + (swz<Sh::kRow>(2 * j + vc, vr) << 4));
+#pragma unroll
+              for (int i = 0; i < 2; i++) {
+                if constexpr (!decltype(finite)::value) b[2 * i] &= ~nan4(b[2 * i]), b[2 * i + 1] &= ~nan4(b[2 * i + 1]);
+                uint32_t e0, e1, d0, d1;  // even and odd columns
+                e4m3_to_f16(__byte_perm(b[2 * i], 0u, 0x3120), e0, d0);
+                e4m3_to_f16(__byte_perm(b[2 * i + 1], 0u, 0x3120), e1, d1);
+                mma_f16(o[4 * j + 2 * i], hi[0], hi[1], hi[2], hi[3], e0, e1);
+                mma_f16(o[4 * j + 2 * i + 1], hi[0], hi[1], hi[2], hi[3], d0, d1);
+              }
+            }
           }
 #pragma unroll
-          for (int j = 0; j < HD / 16; j++) {
+          for (int j = 0; !EIGHT && j < HD / 16; j++) {
             uint32_t b[4];
             ldsm4t(b, vd + (k0 + n * 16 + vr) * (HD * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
             if constexpr (!decltype(finite)::value) {
@@ -818,7 +1172,8 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
       if (!PLAIN && clear < KEYS) {
         for (int e = max(0, clear) * CH + lane; e < min(KEYS, (live + 15) & ~15) * CH; e += 32) {
           const uint4 v = *reinterpret_cast<const uint4*>(smem + (vd - ring) + (k0 * CH + e) * 16);
-          odd |= (not_finite2(v.x) | not_finite2(v.y) | not_finite2(v.z) | not_finite2(v.w)) != 0;
+          if constexpr (EIGHT) odd |= (nan4(v.x) | nan4(v.y) | nan4(v.z) | nan4(v.w)) != 0;
+          else odd |= (not_finite2(v.x) | not_finite2(v.y) | not_finite2(v.z) | not_finite2(v.w)) != 0;
         }
         odd = __any_sync(0xffffffffu, odd);
       }
@@ -826,7 +1181,22 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
         add_values(std::true_type());
       } else {
         add_values(std::false_type());
-        for (int key = k0; key < k0 + min(KEYS, live); key++)
+        if constexpr (EIGHT) {
+          for (int key = k0; key < k0 + min(KEYS, live); key++)
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) {
+              const uint32_t bad = nan4(*reinterpret_cast<const uint32_t*>(smem + (vd - ring) + key * Sh::kRow +
+                                                                           (swz<Sh::kRow>(j, key) << 4) + i4 * 4));
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                if (!(bad >> 8 * i & 1)) continue;
+                float* to = o[2 * j + i % 2];
+                if (key < len[0] - first) to[i / 2] = NAN;
+                if (key < len[1] - first) to[2 + i / 2] = NAN;
+              }
+            }
+        }
+        for (int key = k0; !EIGHT && key < k0 + min(KEYS, live); key++)
 #pragma unroll
           for (int j = 0; j < NB; j++) {
             const uint32_t v = *reinterpret_cast<const uint32_t*>(smem + (vd - ring) + key * (HD * 2) +
@@ -856,7 +1226,7 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
           if (first + k0 < most) step(many, std::false_type(), k0);
       }
     }
-    float* red = reinterpret_cast<float*>(smem + stage * 2 * Sh::kPart);
+    float* red = reinterpret_cast<float*>(smem + (EIGHT ? D : stage) * 2 * Sh::kPart);
     stage = stage == D - 1 ? 0 : stage + 1;
     const bool ends = at.i == at.n - 1;
     if (ends || !more) {  // this unit, or the piece of it that is here
@@ -871,17 +1241,33 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
         const int e = warp * 16 + g + 8 * h;
         if (whole && !narrow) {
           const float r = l[h] == 0.f ? 0.f : 1.0f / l[h];
-          __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)row[h] * a.ldo + col0[h] + 2 * i4;
+          __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)row[h] * a.ldo + col0[h];
+          if constexpr (EIGHT) {
 #pragma unroll
-          for (int j = 0; j < NB; j++)
-            *reinterpret_cast<uint32_t*>(out + j * 8) = pack2(o[j][2 * h] * r, o[j][2 * h + 1] * r);
+            for (int j = 0; j < HD / 16; j++) {
+              const float *x = o[2 * j] + 2 * h, *y = o[2 * j + 1] + 2 * h;
+              *reinterpret_cast<uint2*>(out + j * 16 + 4 * i4) = make_uint2(pack2(x[0] * r, y[0] * r), pack2(x[1] * r, y[1] * r));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+              *reinterpret_cast<uint32_t*>(out + 2 * i4 + j * 8) = pack2(o[j][2 * h] * r, o[j][2 * h + 1] * r);
+          }
         } else {
           float* to = (narrow ? red : slot + 2 * Sh::kPairs) + e * HD;
           const int turn = narrow ? (g & 3) << 3 : 0;  // the eight pairs of a store's half warp fall into different banks
           if (i4 == 0) (narrow ? red_ml : reinterpret_cast<float2*>(slot))[e] = make_float2(m[h], l[h]);
+          if constexpr (EIGHT) {
 #pragma unroll
-          for (int j = 0; j < NB; j++)
-            *reinterpret_cast<float2*>(to + ((j * 8 + 2 * i4) ^ turn)) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+            for (int j = 0; j < HD / 16; j++) {
+              const float *x = o[2 * j] + 2 * h, *y = o[2 * j + 1] + 2 * h;
+              *reinterpret_cast<float4*>(to + ((j * 16 + 4 * i4) ^ turn)) = make_float4(x[0], y[0], x[1], y[1]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+              *reinterpret_cast<float2*>(to + ((j * 8 + 2 * i4) ^ turn)) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+          }
         }
       }
       if (narrow) {
@@ -939,7 +1325,7 @@ constexpr int JOIN_THREADS = 512;
 template <int HD, int MH, bool FEW>
 __global__ void __launch_bounds__(JOIN_THREADS)
 paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int per_block) {
-  using Sh = PagedShape<HD, MH>;
+  using Sh = PagedShape<__nv_bfloat16, HD, MH>;  // pieces are f32, alike for both
   constexpr int COLS = HD / 4;
   __shared__ float4 acc[JOIN_THREADS];
   __shared__ float2 ml[JOIN_THREADS / COLS];
@@ -1024,7 +1410,8 @@ constexpr int RUN_JOIN_THREADS = 256;
 template <int HD>
 __global__ void __launch_bounds__(RUN_JOIN_THREADS)
 paged_runs_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas) {
-  constexpr int COLS = HD / 4, SLOT = RunShape<HD>::kSlot;
+  using Sh = RunShape<__nv_bfloat16, HD>;
+  constexpr int COLS = HD / 4, SLOT = Sh::kSlot;
   const int units = iris_paged_units(&a.cache, a.heads), group = a.heads / a.cache.kv_heads, rtiles = units / a.cache.kv_heads;
   const int c = blockIdx.x + 1, hu = run_heads(group);
   iris::grid_dep_wait();
@@ -1046,7 +1433,7 @@ paged_runs_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas) {
         const int q = min(p + k, n - 1);
         const float* slot = slots + (size_t)(q == 0 ? 2 * c - 1 : 2 * (c + q - 1)) * SLOT;
         s[k] = *reinterpret_cast<const float2*>(slot + 2 * e);
-        v[k] = *reinterpret_cast<const float4*>(slot + 2 * RunShape<HD>::kPairs + e * HD + col);
+        v[k] = *reinterpret_cast<const float4*>(slot + 2 * Sh::kPairs + e * HD + col);
       }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
@@ -1088,16 +1475,6 @@ struct LpShape {
   static constexpr int kPer = LP_BLOCK / (32 * kVec);           // loads of a block
   static constexpr int kBlocks = LP_LOADS / kPer;               // blocks in flight
 };
-
-// Order of the alternatives: larger values first, equal ones by id, NaN before
-// all; as one whole number a value, larger first, 0 for none.
-__device__ __forceinline__ uint32_t rank_bits(float x) {
-  if (x != x) return 0xFF800001u;  // one above +inf
-  const uint32_t u = __float_as_uint(x + 0.0f);  // -0 counts as 0
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float rank_value(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r & 0x7FFFFFFFu : ~r); }
-__device__ __forceinline__ uint64_t place(uint32_t rank, uint32_t id) { return (uint64_t)rank << 32 | (uint32_t)~id; }
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
   float y;
@@ -1147,58 +1524,12 @@ __device__ __forceinline__ void raise(float& m, float& s1, float& s2, float mn) 
   }
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
 // over the warp, NaN if one is
 __device__ __forceinline__ float warp_max_nan(float v) {
   float y;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
   return y;
 }
-__device__ __forceinline__ float warp_add(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// The values at [e, e + kVec) of a row of `vocab` <= 2^30 values, 16-byte
-// aligned; -inf where the row has none.  Nothing outside the row is read.
-template <typename In>
-__device__ __forceinline__ uint4 row_vec(const In* x, int e, int vocab) {
-  constexpr int VEC = 16 / sizeof(In);
-  if (e >= 0 && e + VEC <= vocab) return __ldg(reinterpret_cast<const uint4*>(x + e));
-  uint32_t w[4];
-  if (e >= vocab || e + VEC <= 0) {
-    w[0] = sizeof(In) == 4 ? 0xFF800000u : 0xFF80FF80u;
-    return make_uint4(w[0], w[0], w[0], w[0]);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if constexpr (sizeof(In) == 4) {
-      w[i] = e + i >= 0 && e + i < vocab ? __float_as_uint(x[e + i]) : 0xFF800000u;
-    } else {
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
-      const uint32_t lo = e + 2 * i >= 0 && e + 2 * i < vocab ? h[e + 2 * i] : 0xFF80u;
-      const uint32_t hi = e + 2 * i + 1 >= 0 && e + 2 * i + 1 < vocab ? h[e + 2 * i + 1] : 0xFF80u;
-      w[i] = lo | hi << 16;
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <typename In>
-__device__ __forceinline__ void vec_values(uint4 u, float x[16 / sizeof(In)]) {
-  if constexpr (sizeof(In) == 4) {
-    x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
-  } else {
-    const float2 a = unpack2(u.x), b = unpack2(u.y), c = unpack2(u.z), d = unpack2(u.w);
-    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
-  }
-}
-
 // The same in pairs, -inf (and what is below it in f32's terms) as -1e37.
 template <typename In>
 __device__ __forceinline__ void vec_pairs(uint4 u, uint64_t x[8 / sizeof(In)]) {
@@ -1247,12 +1578,6 @@ struct LpPlan {
   float4* sums;     // [rows][warps] m, s1, s2
   uint32_t* maxima; // [rows][nblk] rank of each block's largest value, 0 for a block outside the row
 };
-
-// First value of block 0 before the row's first one: blocks are cut at 16-byte boundaries.
-template <typename In>
-__device__ __forceinline__ int row_offset(const In* x) {
-  return (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(In));
-}
 
 // Part w of a row, by one warp; its sums and its blocks' maxima go where out says.
 template <typename In, typename Out>
@@ -1611,6 +1936,28 @@ extern "C" cudaError_t iris_launch_rope_append(IrisRopeAppend* a, int f32, int n
   return go(rope_append_kernel<__nv_bfloat16, 256>);
 }
 
+extern "C" cudaError_t iris_launch_rope_append8(IrisRopeAppend* a, int f32, int num_sms, cudaStream_t stream) {
+  a->div = iris_paged_div(a->cache.page_size);
+  a->exp.div = iris_paged_div(a->exp.block);
+  if (a->heads) {
+    IrisRopeAppend q = *a;
+    q.cache.kv_heads = 0;
+    const cudaError_t e = iris_launch_rope_append(&q, f32, num_sms, stream);
+    if (e != cudaSuccess) return e;
+  }
+  constexpr int items = APPEND8_THREADS / 32 * APPEND8_ITEMS;
+  const dim3 grid(a->tokens, (2 * a->cache.kv_heads + items - 1) / items);
+  auto go = [&](auto kernel) { return iris::launch_overlapped(kernel, grid, dim3(APPEND8_THREADS), 0, stream, *a); };
+  if (f32) {
+    if (a->cache.head_dim == 64) return go(rope_append8_kernel<float, 64>);
+    if (a->cache.head_dim == 128) return go(rope_append8_kernel<float, 128>);
+    return go(rope_append8_kernel<float, 256>);
+  }
+  if (a->cache.head_dim == 64) return go(rope_append8_kernel<__nv_bfloat16, 64>);
+  if (a->cache.head_dim == 128) return go(rope_append8_kernel<__nv_bfloat16, 128>);
+  return go(rope_append8_kernel<__nv_bfloat16, 256>);
+}
+
 // CTAs of an attention launch: as many as the device holds at once, no more than the tables have room for tiles
 static int paged_ctas(const iris_gpu_kv_cache_t* c, int heads, int64_t rows, int all) {
   const int64_t room = iris_paged_tiles(iris_paged_len(c, 0x7FFFFFFF)) + IRIS_PAGED_EXTRA;
@@ -1620,10 +1967,10 @@ static int paged_ctas(const iris_gpu_kv_cache_t* c, int heads, int64_t rows, int
 
 constexpr int CLUSTER_TILES = 4;
 
-template <int HD, int MH>
+template <typename E, int HD, int MH>
 struct PagedLaunch {
-  using Sh = PagedShape<HD, MH>;
-  using Runs = RunShape<HD>;
+  using Sh = PagedShape<E, HD, MH>;
+  using Runs = RunShape<E, HD>;
   static size_t ws_bytes(int num_sms) {
     const int ctas = num_sms * Sh::kCtas, runs = num_sms * Runs::kCtas;
     const size_t one = paged_slots_at(ctas) + (size_t)2 * ctas * Sh::kSlot;
@@ -1631,12 +1978,12 @@ struct PagedLaunch {
     return (one > several ? one : several) * sizeof(float);
   }
   static cudaError_t init() {
-    cudaError_t e = cudaFuncSetAttribute(paged_runs_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Runs::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(paged_runs_kernel<E, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Runs::kSmem);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(paged_attention_kernel<HD, MH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                Sh::kSmem);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(paged_attention_kernel<HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    return cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
   }
   static cudaError_t launch(const IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
     // few rows: a block, or a cluster of up to 8, on each unit, all on the device at once (clusters of 4 and 8 do not fill
@@ -1654,7 +2001,7 @@ struct PagedLaunch {
     const int64_t tiles = 2 * CLUSTER_TILES * units * parts / slots + 1;  // 2 CLUSTER_TILES with every slot taken
     if (units * parts <= slots && room <= (tiles < CLUSTER_TILES ? CLUSTER_TILES : tiles) * parts) {
       *launches = 1;
-      return iris::launch_cluster_overlapped(paged_attention_kernel<HD, MH, true>, dim3((unsigned)units * parts),
+      return iris::launch_cluster_overlapped(paged_attention_kernel<E, HD, MH, true>, dim3((unsigned)units * parts),
                                              dim3(Sh::kThreads), Sh::kSmem, parts, stream, *a);
     }
     // four times as many rows as sequences: runs of rows.  On the device, 32 heads on 8 of 128, rows by themselves -> runs:
@@ -1666,14 +2013,14 @@ struct PagedLaunch {
     // runs in them, 303 -> 553.
     if (a->seq && a->rows >= 4 * (int64_t)a->cache.num_seqs) {
       const int ctas = paged_ctas(&a->cache, a->heads, a->rows, num_sms * Runs::kCtas);
-      const cudaError_t e = iris::launch_overlapped(paged_runs_kernel<HD>, dim3(ctas), dim3(Runs::kThreads), Runs::kSmem, stream, *a);
+      const cudaError_t e = iris::launch_overlapped(paged_runs_kernel<E, HD>, dim3(ctas), dim3(Runs::kThreads), Runs::kSmem, stream, *a);
       *launches = 1;
       if (e != cudaSuccess || ctas == 1) return e;
       *launches = 2;
       return iris::launch_overlapped(paged_runs_join_kernel<HD>, dim3(ctas - 1, 2), dim3(RUN_JOIN_THREADS), 0, stream, *a, ctas);
     }
     const int ctas = paged_ctas(&a->cache, a->heads, a->rows, num_sms * Sh::kCtas);
-    cudaError_t e = iris::launch_overlapped(paged_attention_kernel<HD, MH, false>, dim3(ctas), dim3(Sh::kThreads), Sh::kSmem,
+    cudaError_t e = iris::launch_overlapped(paged_attention_kernel<E, HD, MH, false>, dim3(ctas), dim3(Sh::kThreads), Sh::kSmem,
                                             stream, *a);
     *launches = 1;
     if (e != cudaSuccess || ctas == 1) return e;
@@ -1690,29 +2037,44 @@ struct PagedLaunch {
 };
 
 // f(PagedLaunch) of the variant for this cache and group of query heads
-template <typename F>
+template <typename E, typename F>
 static auto paged_variant(const iris_gpu_kv_cache_t* c, int heads, F f) {
   const bool wide = iris_paged_heads(heads / c->kv_heads) == 16;
-  if (c->head_dim == 64) return wide ? f(PagedLaunch<64, 16>()) : f(PagedLaunch<64, 8>());
-  if (c->head_dim == 128) return wide ? f(PagedLaunch<128, 16>()) : f(PagedLaunch<128, 8>());
-  return wide ? f(PagedLaunch<256, 16>()) : f(PagedLaunch<256, 8>());
+  if (c->head_dim == 64) return wide ? f(PagedLaunch<E, 64, 16>()) : f(PagedLaunch<E, 64, 8>());
+  if (c->head_dim == 128) return wide ? f(PagedLaunch<E, 128, 16>()) : f(PagedLaunch<E, 128, 8>());
+  return wide ? f(PagedLaunch<E, 256, 16>()) : f(PagedLaunch<E, 256, 8>());
 }
 
 extern "C" size_t iris_paged_attention_ws_bytes(const iris_gpu_kv_cache_t* cache, int heads, int num_sms) {
-  return paged_variant(cache, heads, [&](auto v) { return v.ws_bytes(num_sms); });
+  return paged_variant<__nv_bfloat16>(cache, heads, [&](auto v) { return v.ws_bytes(num_sms); });
 }
 
 extern "C" cudaError_t iris_launch_paged_attention(IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
   a->div = iris_paged_div(a->cache.page_size);
-  return paged_variant(&a->cache, a->heads, [&](auto v) { return v.launch(a, num_sms, stream, launches); });
+  return paged_variant<__nv_bfloat16>(&a->cache, a->heads, [&](auto v) { return v.launch(a, num_sms, stream, launches); });
+}
+
+extern "C" size_t iris_paged_attention8_ws_bytes(const iris_gpu_kv_cache_t* cache, int heads, int num_sms) {
+  return paged_variant<e4m3>(cache, heads, [&](auto v) { return v.ws_bytes(num_sms); });
+}
+
+extern "C" cudaError_t iris_launch_paged_attention8(IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
+  a->div = iris_paged_div(a->cache.page_size);
+  a->exp.div = iris_paged_div(a->exp.block);
+  return paged_variant<e4m3>(&a->cache, a->heads, [&](auto v) { return v.launch(a, num_sms, stream, launches); });
 }
 
 // dynamic shared memory limits, once per device, so that launches may be captured
 extern "C" cudaError_t iris_lm_init(void) {
-  const cudaError_t e[] = {PagedLaunch<64, 8>::init(),  PagedLaunch<64, 16>::init(),  PagedLaunch<128, 8>::init(),
-                           PagedLaunch<128, 16>::init(), PagedLaunch<256, 8>::init(), PagedLaunch<256, 16>::init()};
-  for (cudaError_t x : e)
-    if (x != cudaSuccess) return x;
+  iris_gpu_kv_cache_t c = {};
+  c.kv_heads = 1;
+  for (int head_dim : {64, 128, 256})
+    for (int heads : {8, 16}) {
+      c.head_dim = head_dim;
+      cudaError_t e = paged_variant<__nv_bfloat16>(&c, heads, [](auto v) { return v.init(); });
+      if (e == cudaSuccess) e = paged_variant<e4m3>(&c, heads, [](auto v) { return v.init(); });
+      if (e != cudaSuccess) return e;
+    }
   return cudaSuccess;
 }
 

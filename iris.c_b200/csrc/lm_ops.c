@@ -52,7 +52,8 @@ static int lm_leave(lm_dev_t *d, cudaError_t e, const char *what, int launches) 
 }
 
 /* ------------------------------------------------------------------ paged cache */
-static int cache_check(const iris_gpu_kv_cache_t *c, const char *what) {
+static int cache_check_of(const iris_gpu_kv_cache_t *c, int eight, const char *what) {
+    const int step = eight ? 16 : 8;
     if (!c || !c->k || !c->v || !c->table) return LM_FAIL("%s: null cache, pool or page table", what);
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return LM_FAIL("%s: head_dim %d (64, 128 or 256)", what, c->head_dim);
@@ -62,14 +63,34 @@ static int cache_check(const iris_gpu_kv_cache_t *c, const char *what) {
     if (c->kv_heads > 65535) return LM_FAIL("%s: %d key-value heads (at most 65535)", what, c->kv_heads);
     if (misaligned(c->k, 16) || misaligned(c->v, 16) || misaligned(c->table, 4))
         return LM_FAIL("%s: misaligned pointer (pools need 16-byte, the table 4-byte alignment)", what);
-    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->page_stride % 8 || c->token_stride % 8 ||
-        c->head_stride % 8 || (c->num_pages > 1 && !c->page_stride) || (c->page_size > 1 && !c->token_stride) ||
+    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->page_stride % step ||
+        c->token_stride % step || c->head_stride % step || (c->num_pages > 1 && !c->page_stride) || (c->page_size > 1 && !c->token_stride) ||
         (c->kv_heads > 1 && !c->head_stride))
-        return LM_FAIL("%s: strides %lld / %lld / %lld of pages, slots and heads (positive multiples of 8)", what,
-                       (long long)c->page_stride, (long long)c->token_stride, (long long)c->head_stride);
+        return LM_FAIL("%s: strides %lld / %lld / %lld of pages, slots and heads (positive multiples of %d)", what,
+                       (long long)c->page_stride, (long long)c->token_stride, (long long)c->head_stride, step);
     if (c->table_stride < 0 || (c->num_seqs > 1 && c->table_stride < c->max_blocks))
         return LM_FAIL("%s: table stride %lld under its %d entries", what, (long long)c->table_stride, c->max_blocks);
     return 0;
+}
+
+static int cache_check(const iris_gpu_kv_cache_t *c, const char *what) { return cache_check_of(c, 0, what); }
+
+static int cache8_check(const iris_gpu_kv_cache8_t *c, const char *what) {
+    if (!c || !c->k_exp || !c->v_exp) return LM_FAIL("%s: null cache or exponents", what);
+    if (cache_check_of(&c->pages, 1, what)) return IRIS_CUDA_ERR_ARG;
+    if (c->block < 1 || c->block > 128 || c->pages.page_size % c->block)
+        return LM_FAIL("%s: blocks of %d tokens in pages of %d (a divisor, at most 128)", what, c->block, c->pages.page_size);
+    if (c->exp_page_stride < 0 || c->exp_block_stride < 0 || c->exp_head_stride < 0 ||
+        (c->pages.num_pages > 1 && !c->exp_page_stride) || (c->pages.page_size > c->block && !c->exp_block_stride) ||
+        (c->pages.kv_heads > 1 && !c->exp_head_stride))
+        return LM_FAIL("%s: strides %lld / %lld / %lld of the exponents of pages, blocks and heads (positive)", what,
+                       (long long)c->exp_page_stride, (long long)c->exp_block_stride, (long long)c->exp_head_stride);
+    return 0;
+}
+
+static iris_kv_exp_t exp_of(const iris_gpu_kv_cache8_t *c) {
+    iris_kv_exp_t e = {c->k_exp, c->v_exp, c->exp_page_stride, c->exp_block_stride, c->exp_head_stride, c->block, {0, 0}};
+    return e;
 }
 
 /* ------------------------------------------------------------------ rotary positions */
@@ -124,12 +145,11 @@ int iris_gpu_rope_init(iris_gpu_rope_t *rope, int layout, int rot_dim, double th
     return iris_gpu_rope_init_freqs(rope, layout, rot_dim, f, scaling ? scaling->amplitude : 1.0);
 }
 
-int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
-                         const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int f32,
-                         const float *q_norm, const float *k_norm, float eps, const int32_t *seq, const int32_t *pos,
-                         int tokens, int heads, void *stream) {
-    const char *what = "rope_append";
-    if (cache_check(cache, what)) return IRIS_CUDA_ERR_ARG;
+/* cache8: the 8-bit cache that `cache` is the pages of, or NULL */
+static int append_to(const char *what, const iris_gpu_kv_cache_t *cache, const iris_gpu_kv_cache8_t *cache8,
+                     const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out, const void *q, const void *k, const void *v,
+                     int64_t ldq, int64_t ldk, int64_t ldv, int f32, const float *q_norm, const float *k_norm, float eps,
+                     const int32_t *seq, const int32_t *pos, int tokens, int heads, void *stream) {
     if (tokens < 0 || heads < 0 || heads > 65535) return LM_FAIL("%s: %d tokens, %d heads", what, tokens, heads);
     /* a batch of no rows may have no tensors */
     if (tokens && (!k || !v || !seq || !pos || (heads && (!q || !q_out)))) return LM_FAIL("%s: null pointer", what);
@@ -150,7 +170,8 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
     if (tokens && heads && q_out == q && (f32 || ldq != ldq_out))
         return LM_FAIL("%s: q_out on q needs bf16 and one row stride", what);
     if (!tokens) return 0;
-    const void *ptrs[] = {cache->k, cache->v, cache->table, q_out, q, k, v, q_norm, k_norm, seq, pos};
+    const void *ptrs[] = {cache->k, cache->v, cache->table, q_out, q, k, v, q_norm, k_norm, seq, pos,
+                          cache8 ? cache8->k_exp : NULL, cache8 ? cache8->v_exp : NULL};
     lm_dev_t d;
     int rc = lm_enter(&d, what, ptrs, (int)(sizeof(ptrs) / sizeof(ptrs[0])));
     if (rc) return rc;
@@ -173,7 +194,29 @@ int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t
     a.pos = pos;
     a.tokens = tokens;
     a.heads = heads;
-    return lm_leave(&d, iris_launch_rope_append(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, 1);
+    if (!cache8) return lm_leave(&d, iris_launch_rope_append(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, 1);
+    a.exp = exp_of(cache8);
+    return lm_leave(&d, iris_launch_rope_append8(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, heads ? 2 : 1);
+}
+
+int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
+                         const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int f32,
+                         const float *q_norm, const float *k_norm, float eps, const int32_t *seq, const int32_t *pos,
+                         int tokens, int heads, void *stream) {
+    const char *what = "rope_append";
+    if (cache_check(cache, what)) return IRIS_CUDA_ERR_ARG;
+    return append_to(what, cache, NULL, rope, q_out, ldq_out, q, k, v, ldq, ldk, ldv, f32, q_norm, k_norm, eps, seq, pos,
+                     tokens, heads, stream);
+}
+
+int iris_gpu_rope_append8(const iris_gpu_kv_cache8_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
+                          const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int f32,
+                          const float *q_norm, const float *k_norm, float eps, const int32_t *seq, const int32_t *pos,
+                          int tokens, int heads, void *stream) {
+    const char *what = "rope_append8";
+    if (cache8_check(cache, what)) return IRIS_CUDA_ERR_ARG;
+    return append_to(what, &cache->pages, cache, rope, q_out, ldq_out, q, k, v, ldq, ldk, ldv, f32, q_norm, k_norm, eps, seq,
+                     pos, tokens, heads, stream);
 }
 
 /* ------------------------------------------------------------------ attention over the cache */
@@ -190,11 +233,11 @@ size_t iris_gpu_attention_paged_workspace(const iris_gpu_kv_cache_t *cache, int 
     return iris_paged_attention_ws_bytes(cache, heads, g_rt.num_sms);
 }
 
-int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const void *q, int64_t ldo, int64_t ldq,
-                             const int32_t *seq, const int32_t *pos, int rows, int heads, float scale,
-                             void *workspace, size_t workspace_bytes, void *stream) {
-    const char *what = "attention_paged";
-    if (cache_check(cache, what) || heads_check(cache, heads, what)) return IRIS_CUDA_ERR_ARG;
+/* cache8: the 8-bit cache that `cache` is the pages of, or NULL */
+static int attend_to(const char *what, const iris_gpu_kv_cache_t *cache, const iris_gpu_kv_cache8_t *cache8, void *out,
+                     const void *q, int64_t ldo, int64_t ldq, const int32_t *seq, const int32_t *pos, int rows, int heads,
+                     float scale, void *workspace, size_t workspace_bytes, void *stream) {
+    if (heads_check(cache, heads, what)) return IRIS_CUDA_ERR_ARG;
     if (rows < 0 || (!seq && rows > cache->num_seqs))
         return LM_FAIL("%s: %d rows for %d sequences", what, rows, cache->num_seqs);
     if (rows && (!out || !q || !pos || !workspace)) return LM_FAIL("%s: null pointer", what);
@@ -206,19 +249,52 @@ int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const 
     if (misaligned(out, 16) || misaligned(q, 16) || misaligned(workspace, 16) || misaligned(seq, 4) || misaligned(pos, 4))
         return LM_FAIL("%s: misaligned pointer (16 bytes; seq and pos 4)", what);
     if (!rows) return 0;
-    const void *ptrs[] = {cache->k, cache->v, cache->table, out, q, seq, pos, workspace};
+    const void *ptrs[] = {cache->k, cache->v, cache->table, out, q, seq, pos, workspace,
+                          cache8 ? cache8->k_exp : NULL, cache8 ? cache8->v_exp : NULL};
     lm_dev_t d;
     int rc = lm_enter(&d, what, ptrs, (int)(sizeof(ptrs) / sizeof(ptrs[0])));
     if (rc) return rc;
-    const size_t need = iris_paged_attention_ws_bytes(cache, heads, g_rt.num_sms);
+    const size_t need = cache8 ? iris_paged_attention8_ws_bytes(cache, heads, g_rt.num_sms)
+                               : iris_paged_attention_ws_bytes(cache, heads, g_rt.num_sms);
     if (workspace_bytes < need) {
         lm_leave(&d, cudaSuccess, what, 0);
         return LM_FAIL("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
     }
-    IrisPagedAttention a = {*cache, out, q, ldo, ldq, seq, pos, rows, heads, scale, (float *)workspace, {0, 0}};
+    IrisPagedAttention a = {*cache, out, q, ldo, ldq, seq, pos, rows, heads, scale, (float *)workspace, {0, 0},
+                            {NULL, NULL, 0, 0, 0, 0, {0, 0}}};
     int launches = 0;
-    cudaError_t e = iris_launch_paged_attention(&a, g_rt.num_sms, (cudaStream_t)stream, &launches);
+    cudaError_t e;
+    if (cache8) {
+        a.exp = exp_of(cache8);
+        e = iris_launch_paged_attention8(&a, g_rt.num_sms, (cudaStream_t)stream, &launches);
+    } else {
+        e = iris_launch_paged_attention(&a, g_rt.num_sms, (cudaStream_t)stream, &launches);
+    }
     return lm_leave(&d, e, what, launches);
+}
+
+int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const void *q, int64_t ldo, int64_t ldq,
+                             const int32_t *seq, const int32_t *pos, int rows, int heads, float scale,
+                             void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "attention_paged";
+    if (cache_check(cache, what)) return IRIS_CUDA_ERR_ARG;
+    return attend_to(what, cache, NULL, out, q, ldo, ldq, seq, pos, rows, heads, scale, workspace, workspace_bytes, stream);
+}
+
+size_t iris_gpu_attention_paged8_workspace(const iris_gpu_kv_cache8_t *cache, int heads) {
+    const char *what = "attention_paged8_workspace";
+    if (cache8_check(cache, what) || heads_check(&cache->pages, heads, what)) return 0;
+    if (iris_rt_ensure()) { op_fail(IRIS_CUDA_ERR_NODEV, "%s: no usable device", what); return 0; }
+    return iris_paged_attention8_ws_bytes(&cache->pages, heads, g_rt.num_sms);
+}
+
+int iris_gpu_attention_paged8(const iris_gpu_kv_cache8_t *cache, void *out, const void *q, int64_t ldo, int64_t ldq,
+                              const int32_t *seq, const int32_t *pos, int rows, int heads, float scale,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "attention_paged8";
+    if (cache8_check(cache, what)) return IRIS_CUDA_ERR_ARG;
+    return attend_to(what, &cache->pages, cache, out, q, ldo, ldq, seq, pos, rows, heads, scale, workspace, workspace_bytes,
+                     stream);
 }
 
 /* ------------------------------------------------------------------ log probabilities */
@@ -257,4 +333,78 @@ int iris_gpu_token_logprobs(const void *logits, int f32, int64_t ld, int rows, i
     int launches = 0;
     cudaError_t e = iris_launch_logprobs(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream, &launches);
     return lm_leave(&d, e, what, launches);
+}
+
+/* ------------------------------------------------------------------ sampling */
+int iris_gpu_sample_tokens(const void *logits, int f32, int64_t ld, int rows, int vocab, const float *temperature,
+                           const int32_t *top_k, const float *top_p, const float *min_p, const double *uniform,
+                           int32_t *ids, float *logprobs, int32_t *kept, void *stream) {
+    const char *what = "sample_tokens";
+    /* eight blocks a row; ids are int32 */
+    if (rows < 0 || rows > 1 << 24 || vocab < 1 || vocab > (1 << 30))
+        return LM_FAIL("%s: %d rows of %d logits", what, rows, vocab);
+    if (ld < vocab) return LM_FAIL("%s: row stride %lld under %d logits", what, (long long)ld, vocab);
+    if (rows && (!logits || !uniform || !ids)) return LM_FAIL("%s: null pointer", what);
+    if (misaligned(logits, f32 ? 4 : 2) || misaligned(temperature, 4) || misaligned(top_k, 4) || misaligned(top_p, 4) ||
+        misaligned(min_p, 4) || misaligned(uniform, 8) || misaligned(ids, 4) || misaligned(logprobs, 4) || misaligned(kept, 4))
+        return LM_FAIL("%s: misaligned pointer", what);
+    if (!rows) return 0;
+    const void *ptrs[] = {logits, temperature, top_k, top_p, min_p, uniform, ids, logprobs, kept};
+    lm_dev_t d;
+    int rc = lm_enter(&d, what, ptrs, (int)(sizeof(ptrs) / sizeof(ptrs[0])));
+    if (rc) return rc;
+    IrisSample a = {logits, ld, rows, vocab, temperature, top_p, min_p, top_k, uniform, ids, kept, logprobs, 0, 0};
+    return lm_leave(&d, iris_launch_sample(&a, f32 != 0, (cudaStream_t)stream), what, 1);
+}
+
+/* ------------------------------------------------------------------ weights of 4 bits */
+static int weights4_check(const iris_gpu_weights4_t *w, const char *what) {
+    if (!w || !w->q || !w->scale) return LM_FAIL("%s: null weights or scales", what);
+    if (w->n < 1 || w->k < 1 || (w->group != 32 && w->group != 64 && (w->group < 128 || w->group % 128)) || w->k % w->group)
+        return LM_FAIL("%s: weights [%d, %d] in groups of %d (32, 64 or a multiple of 128, and of it a whole number in a row)",
+                       what, w->n, w->k, w->group);
+    const int groups = w->k / w->group;
+    if (w->n > 1 && (w->q_stride < w->k / 2 || w->q_stride % 16 || w->scale_stride < groups || (w->zero && w->zero_stride < groups)))
+        return LM_FAIL("%s: row strides %lld, %lld, %lld of weights (a multiple of 16), scales and zeros", what,
+                       (long long)w->q_stride, (long long)w->scale_stride, (long long)w->zero_stride);
+    if (misaligned(w->q, 16) || misaligned(w->scale, w->scale_f32 ? 4 : 2)) return LM_FAIL("%s: misaligned weights or scales", what);
+    return 0;
+}
+
+int iris_gpu_quantize4(const iris_gpu_weights4_t *out, const void *w, int f32, int64_t ldw, void *stream) {
+    const char *what = "quantize4";
+    if (weights4_check(out, what)) return IRIS_CUDA_ERR_ARG;
+    if (out->zero) return LM_FAIL("%s: weights with zeros of their own", what);
+    if (!w) return LM_FAIL("%s: null pointer", what);
+    if (out->n > 1 && (ldw < out->k || ldw % 8)) return LM_FAIL("%s: row stride %lld of the weights", what, (long long)ldw);
+    if (misaligned(w, 16)) return LM_FAIL("%s: misaligned weights", what);
+    const void *ptrs[] = {out->q, out->scale, w};
+    lm_dev_t d;
+    int rc = lm_enter(&d, what, ptrs, (int)(sizeof(ptrs) / sizeof(ptrs[0])));
+    if (rc) return rc;
+    IrisQuantize4 a = {(uint8_t *)out->q, out->scale, w, out->q_stride, out->scale_stride, ldw, out->n, out->k, out->group,
+                       out->scale_f32 != 0};
+    return lm_leave(&d, iris_launch_quantize4(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, 1);
+}
+
+int iris_gpu_linear4(const iris_gpu_weights4_t *w, const void *x, int64_t ldx, int rows, void *out, int64_t ldo,
+                     const void *add, int64_t ldadd, int f32, void *stream) {
+    const char *what = "linear4";
+    if (weights4_check(w, what)) return IRIS_CUDA_ERR_ARG;
+    if (rows < 0 || rows > 1 << 19) return LM_FAIL("%s: %d rows (at most %d)", what, rows, 1 << 19);
+    if (rows && (!x || !out)) return LM_FAIL("%s: null pointer", what);
+    if (rows > 1 && (ldx < w->k || ldx % 8 || ldo < w->n || (add && ldadd < w->n)))
+        return LM_FAIL("%s: row strides %lld (a multiple of 8), %lld, %lld", what, (long long)ldx, (long long)ldo,
+                       (long long)ldadd);
+    const size_t size = f32 ? 4 : 2;
+    if (misaligned(x, 16) || misaligned(out, size) || misaligned(add, size)) return LM_FAIL("%s: misaligned pointer", what);
+    if (rows > 1 && add == out && ldadd != ldo) return LM_FAIL("%s: out on add needs one row stride", what);
+    if (!rows) return 0;
+    const void *ptrs[] = {w->q, w->scale, w->zero, x, out, add};
+    lm_dev_t d;
+    int rc = lm_enter(&d, what, ptrs, (int)(sizeof(ptrs) / sizeof(ptrs[0])));
+    if (rc) return rc;
+    IrisLinear4 a = {(const uint8_t *)w->q, w->zero, w->scale, x, add, out, w->q_stride, w->scale_stride, w->zero_stride, ldx,
+                     ldadd, ldo, w->n, w->k, w->group, rows, w->scale_f32 != 0, f32 != 0, 1, {0, 0}};
+    return lm_leave(&d, iris_launch_linear4(&a, g_rt.num_sms, (cudaStream_t)stream), what, 1);
 }

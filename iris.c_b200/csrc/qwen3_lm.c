@@ -201,7 +201,7 @@ static int lm_enqueue(iris_cuda_qwen3_lm_t *lm, int T, int top_k, q3_enq_t *E) {
         r.heads = nh;
         if (!E->rc) iris_q3_done(E, iris_launch_rope_append(&r, 1, g_rt.num_sms, st), "rope append", 1);
         IrisPagedAttention a = {r.cache, lm->attn, lm->q, qd, qd, seq, pos, T, nh, 1.0f / sqrtf(128.0f), (float *)lm->attn_ws,
-                                {0, 0}};
+                                {0, 0}, {NULL, NULL, 0, 0, 0, 0, {0, 0}}};
         if (!E->rc) {
             const cudaError_t e = iris_launch_paged_attention(&a, g_rt.num_sms, st, &n);
             iris_q3_done(E, e, "attention", n);

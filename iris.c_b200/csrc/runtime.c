@@ -102,6 +102,8 @@ int iris_cuda_init(int device) {
     if ((e = iris_gemm_init()) != cudaSuccess) return iris_cuda_check(e, "gemm init");
     if ((e = iris_attention_tc_init()) != cudaSuccess) return iris_cuda_check(e, "attention init");
     if ((e = iris_lm_init()) != cudaSuccess) return iris_cuda_check(e, "language-model operators init");
+    if ((e = iris_sample_init()) != cudaSuccess || (e = iris_linear4_init()) != cudaSuccess)
+        return iris_cuda_check(e, "sampling and 4-bit products init");
     iris_attention_set_status(g_rt.d_status);
     g_rt.initialized = 1;
     return IRIS_CUDA_OK;

@@ -118,14 +118,69 @@ class KvCache(C.Structure):
         int32 [sequences, blocks].  The tensors are kept alive."""
         if _dtype(k) != "bfloat16" or _dtype(v) != "bfloat16" or _dtype(table) != "int32":
             raise IrisCudaError("KvCache: pools are bfloat16, the page table int32")
-        if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or \
-                any(n > 1 and a != b for n, a, b in zip(k.shape, k.stride(), v.stride())):
-            raise IrisCudaError("KvCache: pools [pages, slots, heads, columns] laid out alike")
-        if k.stride(3) != 1 or len(table.shape) != 2 or table.stride(1) != 1:
-            raise IrisCudaError("KvCache: columns and table rows are contiguous")
-        stride = [s if n > 1 else 0 for n, s in zip(k.shape, k.stride())]  # of an axis of one: never used
-        c = cls(k.data_ptr(), v.data_ptr(), table.data_ptr(), *k.shape, *table.shape, table.stride(0), *stride[:3])
+        c = _pages("KvCache", k, v, table)
         c.tensors = (k, v, table)
+        return c
+
+
+def _pages(what: str, k, v, table) -> KvCache:
+    """The pools' and the table's description."""
+    if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or \
+            any(n > 1 and a != b for n, a, b in zip(k.shape, k.stride(), v.stride())):
+        raise IrisCudaError(f"{what}: pools [pages, slots, heads, columns] laid out alike")
+    if k.stride(3) != 1 or len(table.shape) != 2 or table.stride(1) != 1:
+        raise IrisCudaError(f"{what}: columns and table rows are contiguous")
+    stride = [s if n > 1 else 0 for n, s in zip(k.shape, k.stride())]  # of an axis of one: never used
+    return KvCache(k.data_ptr(), v.data_ptr(), table.data_ptr(), *k.shape, *table.shape, table.stride(0), *stride[:3])
+
+
+class KvCache8(C.Structure):
+    """iris_gpu_kv_cache8_t: the same in 8 bits, with an exponent for each block of tokens and head."""
+    _fields_ = [("pages", KvCache), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p), ("block", C.c_int),
+                ("exp_page_stride", C.c_int64), ("exp_block_stride", C.c_int64), ("exp_head_stride", C.c_int64)]
+
+    @classmethod
+    def of(cls, k, v, k_exp, v_exp, table) -> "KvCache8":
+        """k, v: float8_e4m3fn (or uint8) device tensors as KvCache.of takes them; k_exp, v_exp: uint8 [pages, blocks
+        of a page, heads], laid out alike; table: int32 [sequences, blocks].  The tensors are kept alive."""
+        if any(_dtype(t) not in ("float8_e4m3fn", "uint8") for t in (k, v)) or _dtype(table) != "int32" or \
+                _dtype(k_exp) != "uint8" or _dtype(v_exp) != "uint8":
+            raise IrisCudaError("KvCache8: pools are float8_e4m3fn, exponents uint8, the page table int32")
+        c = cls(_pages("KvCache8", k, v, table))
+        pages, slots, heads = k.shape[:3]
+        if len(k_exp.shape) != 3 or tuple(k_exp.shape) != tuple(v_exp.shape) or k_exp.shape[0] != pages or \
+                k_exp.shape[2] != heads or not k_exp.shape[1] or slots % k_exp.shape[1] or \
+                any(n > 1 and a != b for n, a, b in zip(k_exp.shape, k_exp.stride(), v_exp.stride())):
+            raise IrisCudaError("KvCache8: exponents [pages, blocks of a page, heads] laid out alike")
+        c.k_exp, c.v_exp, c.block = k_exp.data_ptr(), v_exp.data_ptr(), slots // k_exp.shape[1]
+        c.exp_page_stride, c.exp_block_stride, c.exp_head_stride = (
+            s if n > 1 else 0 for n, s in zip(k_exp.shape, k_exp.stride()))
+        c.tensors = (k, v, k_exp, v_exp, table)
+        c.head_dim, c.kv_heads = c.pages.head_dim, c.pages.kv_heads
+        return c
+
+
+class Weights4(C.Structure):
+    """iris_gpu_weights4_t: weights of 4 bits with a scale for each group of columns."""
+    _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("zero", C.c_void_p), ("n", C.c_int), ("k", C.c_int),
+                ("group", C.c_int), ("scale_f32", C.c_int), ("q_stride", C.c_int64), ("scale_stride", C.c_int64),
+                ("zero_stride", C.c_int64)]
+
+    @classmethod
+    def of(cls, q, scale, zero=None) -> "Weights4":
+        """q: uint8 [n, k / 2], two columns a byte, the low half first; scale: bfloat16 or float32 [n, groups]; zero:
+        uint8 [n, groups], or None: 8.  The tensors are kept alive."""
+        if _dtype(q) != "uint8" or _dtype(scale) not in ("bfloat16", "float32") or (zero is not None and _dtype(zero) != "uint8"):
+            raise IrisCudaError("Weights4: weights are uint8, scales bfloat16 or float32, zeros uint8")
+        if len(q.shape) != 2 or len(scale.shape) != 2 or scale.shape[0] != q.shape[0] or not scale.shape[1] or \
+                2 * q.shape[1] % scale.shape[1] or (zero is not None and tuple(zero.shape) != tuple(scale.shape)):
+            raise IrisCudaError("Weights4: weights [n, k / 2], scales and zeros [n, groups]")
+        if any(t is not None and t.shape[1] > 1 and t.stride(1) != 1 for t in (q, scale, zero)):
+            raise IrisCudaError("Weights4: rows are contiguous")
+        n, k = q.shape[0], 2 * q.shape[1]
+        c = cls(q.data_ptr(), scale.data_ptr(), None if zero is None else zero.data_ptr(), n, k, k // scale.shape[1],
+                _dtype(scale) == "float32", *(0 if t is None or n == 1 else t.stride(0) for t in (q, scale, zero)))
+        c.tensors = (q, scale, zero)
         return c
 
 
@@ -351,6 +406,17 @@ SIGNATURES = {
     "iris_gpu_token_logprobs": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
                                           C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                           C.c_void_p]),
+    "iris_gpu_rope_append8": (C.c_int, [C.POINTER(KvCache8), C.POINTER(Rope), C.c_void_p, C.c_int64, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
+                                        C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "iris_gpu_attention_paged8_workspace": (C.c_size_t, [C.POINTER(KvCache8), C.c_int]),
+    "iris_gpu_attention_paged8": (C.c_int, [C.POINTER(KvCache8), C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                            C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_void_p,
+                                            C.c_size_t, C.c_void_p]),
+    "iris_gpu_sample_tokens": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int] + [C.c_void_p] * 9),
+    "iris_gpu_quantize4": (C.c_int, [C.POINTER(Weights4), C.c_void_p, C.c_int, C.c_int64, C.c_void_p]),
+    "iris_gpu_linear4": (C.c_int, [C.POINTER(Weights4), C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64,
+                                   C.c_void_p, C.c_int64, C.c_int, C.c_void_p]),
 }
 
 _libc = C.CDLL(None)
@@ -909,6 +975,16 @@ def _heads_rows(what: str, t, dtype: str, rows: int, heads: int, head_dim: int):
 def rope_append(cache: KvCache, rope: Rope | None, q_out, q, k, v, seq, pos, *, heads: int, q_norm=None, k_norm=None,
                 eps: float = 1e-6, stream: int = 0) -> None:
     """iris_gpu_rope_append: rotate the new tokens' Q and K, write K and V to the cache."""
+    _append(lib().iris_gpu_rope_append, cache, rope, q_out, q, k, v, seq, pos, heads, q_norm, k_norm, eps, stream)
+
+
+def rope_append8(cache: KvCache8, rope: Rope | None, q_out, q, k, v, seq, pos, *, heads: int, q_norm=None, k_norm=None,
+                 eps: float = 1e-6, stream: int = 0) -> None:
+    """iris_gpu_rope_append8: the same into an 8-bit cache."""
+    _append(lib().iris_gpu_rope_append8, cache, rope, q_out, q, k, v, seq, pos, heads, q_norm, k_norm, eps, stream)
+
+
+def _append(call, cache, rope, q_out, q, k, v, seq, pos, heads, q_norm, k_norm, eps, stream) -> None:
     n, d, nkv = seq.shape[0], cache.head_dim, cache.kv_heads
     ty = _dtype(k)
     if ty not in ("float32", "bfloat16"):
@@ -920,10 +996,9 @@ def rope_append(cache: KvCache, rope: Rope | None, q_out, q, k, v, seq, pos, *, 
     if heads:
         qp, ldq = _heads_rows("q", q, ty, n, heads, d)
         op, ldo = _heads_rows("q_out", q_out, "bfloat16", n, heads, d)
-    _ok(lib().iris_gpu_rope_append(cache, rope, op, ldo, qp, kp, vp, ldq, ldk, ldv, ty == "float32",
-                                   _need("q_norm", q_norm, "float32", (d,)),
-                                   _need("k_norm", k_norm, "float32", (d,)), eps,
-                                   _need("seq", seq, "int32", (n,)), _need("pos", pos, "int32", (n,)), n, heads, stream))
+    _ok(call(cache, rope, op, ldo, qp, kp, vp, ldq, ldk, ldv, ty == "float32", _need("q_norm", q_norm, "float32", (d,)),
+             _need("k_norm", k_norm, "float32", (d,)), eps, _need("seq", seq, "int32", (n,)),
+             _need("pos", pos, "int32", (n,)), n, heads, stream))
 
 
 def attention_paged_workspace(cache: KvCache, heads: int) -> int:
@@ -935,13 +1010,28 @@ def attention_paged_workspace(cache: KvCache, heads: int) -> int:
 
 def attention_paged(cache: KvCache, out, q, seq, pos, *, scale: float, workspace, stream: int = 0) -> None:
     """iris_gpu_attention_paged: q, out [rows, heads, head_dim]; seq None: row t is sequence t."""
+    _attend(lib().iris_gpu_attention_paged, cache, out, q, seq, pos, scale, workspace, stream)
+
+
+def attention_paged8_workspace(cache: KvCache8, heads: int) -> int:
+    n = lib().iris_gpu_attention_paged8_workspace(cache, heads)
+    if not n:
+        raise IrisCudaError(last_error())
+    return n
+
+
+def attention_paged8(cache: KvCache8, out, q, seq, pos, *, scale: float, workspace, stream: int = 0) -> None:
+    """iris_gpu_attention_paged8: the same over an 8-bit cache."""
+    _attend(lib().iris_gpu_attention_paged8, cache, out, q, seq, pos, scale, workspace, stream)
+
+
+def _attend(call, cache, out, q, seq, pos, scale, workspace, stream) -> None:
     n, d = pos.shape[0], cache.head_dim
     heads = q.shape[1] if len(q.shape) == 3 else q.shape[1] // d
     qp, ldq = _heads_rows("q", q, "bfloat16", n, heads, d)
     op, ldo = _heads_rows("out", out, "bfloat16", n, heads, d)
-    _ok(lib().iris_gpu_attention_paged(cache, op, qp, ldo, ldq, _need("seq", seq, "int32", (n,)),
-                                       _need("pos", pos, "int32", (n,)), n, heads, scale, workspace.data_ptr(),
-                                       workspace.numel() * workspace.element_size(), stream))
+    _ok(call(cache, op, qp, ldo, ldq, _need("seq", seq, "int32", (n,)), _need("pos", pos, "int32", (n,)), n, heads, scale,
+             workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
 
 
 def token_logprobs_workspace(rows: int, vocab: int) -> int:
@@ -967,3 +1057,40 @@ def token_logprobs(logits, targets, logprob, entropy, top_ids, top_logprobs, *, 
                                       _need("top_ids", top_ids, "int32", (rows, k)),
                                       _need("top_logprobs", top_logprobs, "float32", (rows, k)),
                                       workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
+
+
+def sample_tokens(logits, uniform, ids, *, temperature=None, top_k=None, top_p=None, min_p=None, logprobs=None, kept=None,
+                  stream: int = 0) -> None:
+    """iris_gpu_sample_tokens: the next token of each row of logits [rows, vocab] into ids, drawn with uniform (float64);
+    the settings are tensors [rows] or None."""
+    rows, vocab = logits.shape
+    ty = _dtype(logits)
+    if ty not in ("float32", "bfloat16") or logits.stride(1) != 1:
+        raise IrisCudaError(f"sample_tokens: logits {ty}, stride {logits.stride(1)} between a row's values")
+    of = (rows,)
+    _ok(lib().iris_gpu_sample_tokens(logits.data_ptr(), ty == "float32", logits.stride(0) if rows > 1 else vocab, rows,
+                                     vocab, _need("temperature", temperature, "float32", of),
+                                     _need("top_k", top_k, "int32", of), _need("top_p", top_p, "float32", of),
+                                     _need("min_p", min_p, "float32", of), _need("uniform", uniform, "float64", of),
+                                     _need("ids", ids, "int32", of), _need("logprobs", logprobs, "float32", of),
+                                     _need("kept", kept, "int32", of), stream))
+
+
+def quantize4(w: Weights4, weights, stream: int = 0) -> None:
+    """iris_gpu_quantize4: round weights [n, k] (bfloat16 or float32) into w's tensors."""
+    ty = _dtype(weights)
+    if ty not in ("float32", "bfloat16") or tuple(weights.shape) != (w.n, w.k) or weights.stride(1) != 1:
+        raise IrisCudaError(f"quantize4: needs float32 or bfloat16 [{w.n}, {w.k}] with contiguous rows; got {ty} "
+                            f"{tuple(weights.shape)}")
+    _ok(lib().iris_gpu_quantize4(w, weights.data_ptr(), ty == "float32", weights.stride(0), stream))
+
+
+def linear4(out, x, w: Weights4, *, add=None, stream: int = 0) -> None:
+    """iris_gpu_linear4: out [rows, n] = x [rows, k] times the weights (+ add [rows, n])."""
+    rows = x.shape[0]
+    ty = _dtype(out)
+    if ty not in ("float32", "bfloat16"):
+        raise IrisCudaError(f"linear4: out is {ty}")
+    _ok(lib().iris_gpu_linear4(w, _need("x", x, "bfloat16", (rows, w.k)), x.stride(0), rows,
+                               _need("out", out, ty, (rows, w.n)), out.stride(0), _need("add", add, ty, (rows, w.n)),
+                               0 if add is None else add.stride(0), ty == "float32", stream))
