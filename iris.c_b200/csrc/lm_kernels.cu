@@ -401,15 +401,16 @@ struct PagedShape {
   // latency and wants warps, until registers spill.  At 128 and 256 a ring of three stages fills shared memory, with MH =
   // 16 two.
   static constexpr int kRow = HD * (int)sizeof(E);               // bytes of a row
-  static constexpr int kCtas = HD == 64 ? 4 : HD == 128 ? (kEight<E> ? 3 : 2) : 1;
-  static constexpr int kStages = kEight<E> ? 4 : HD == 64 || MH == 16 ? 2 : 3;
+  static constexpr int kCtas = kEight<E> ? (HD == 64 ? (MH == 16 ? 4 : 5) : HD == 128 ? (MH == 16 ? 3 : 4) : MH == 16 ? 1 : 2)
+                                         : HD == 64 ? 4 : HD == 128 ? 2 : 1;
+  static constexpr int kStages = kEight<E> ? (HD == 64 ? 3 : 2) : HD == 64 || MH == 16 ? 2 : 3;
   static constexpr int kStageBytes = 16 * kRow;                  // 16 rows of K or of V
   static constexpr int kRing = kStages * 2 * kStageBytes;        // of 16 keys of a tile
   static constexpr int kSlot = MH * (HD + 2);                    // floats of a piece: m, l, then o
   static constexpr int kSmem = 4 * kRing + 4 * kSlot * 4;
-  // column of o of head h in the sums of 16 keys in shared memory, which are laid out as a piece: the eight heads of a
-  // store's half warp fall into different banks
-  __device__ static int col(int h, int c) { return c ^ (h & 3) << 3; }
+  // column of o of head h in the sums of 16 keys in shared memory, which are laid out as a piece: the heads of a store's
+  // half warp, eight or every other one of them, fall into different banks
+  __device__ static int col(int h, int c) { return c ^ ((kEight<E> ? h >> 1 : h) & 3) << 3; }
 };
 
 // Offset of the first slot in the workspace (floats), after the joins
@@ -603,9 +604,10 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   // ---- arithmetic.  Rows of the products: head g, and head g + 8 where MH is 16.
   constexpr int R = WIDE ? 2 : 1;
   const float c = a.scale * 1.4426950408889634f;
+  constexpr int S = EIGHT ? 2 * R : R;  // heads whose sums a lane has part of: g and g + 8; over 8 bits 2 i4, 2 i4 + 1 and 8 more
   uint32_t qf[HD / 16][2 * R];
-  float o[OC / 8][4], m[R], l[R];
-  float cq[R];  // c times what the queries were divided by
+  float o[EIGHT ? R * OC / 16 : OC / 8][4], m[S], l[S];
+  [[maybe_unused]] float cq[S];  // c times what the queries were divided by
   int heads_here = 0, head0 = 0;
   auto begin_unit = [&]() {
     const int kvh = at.u / rtiles, r = at.u - kvh * rtiles;
@@ -616,7 +618,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     for (int h = 0; h < R; h++) {
       const bool live = g + 8 * h < heads_here;
       if constexpr (EIGHT) {
-        cq[h] = c * queries8<HD, 2 * R>(q + h * 8 * HD, live, i4, qf, h, R + h);
+        const float f = c * queries8<HD, 2 * R>(q + h * 8 * HD, live, i4, qf, 2 * h, 2 * h + 1);
+        cq[2 * h] = __shfl_sync(0xffffffffu, f, 8 * i4);
+        cq[2 * h + 1] = __shfl_sync(0xffffffffu, f, 8 * i4 + 4);
       } else {
 #pragma unroll
         for (int j = 0; j < HD / 16; j++) {
@@ -624,13 +628,13 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
           qf[j][R + h] = live ? *reinterpret_cast<const uint32_t*>(q + 2 * i4 + h * 8 * HD + j * 16 + 8) : 0u;
         }
       }
-      m[h] = -INFINITY;
-      l[h] = 0.f;
     }
+#pragma unroll
+    for (int h = 0; h < S; h++) m[h] = -INFINITY, l[h] = 0.f;
   };
   auto clear = [&]() {
 #pragma unroll
-    for (int j = 0; j < OC / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (auto& x : o) x[0] = x[1] = x[2] = x[3] = 0.f;
   };
   begin_unit();
   clear();
@@ -643,61 +647,25 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     sync_keys();
     const uint32_t kd = ring + stage * 2 * Sh::kStageBytes, vd = kd + Sh::kStageBytes;
     const uint32_t have = seen[kg][stage];
-    if (have) {
+    if (!EIGHT && have) {
       // scores of a row and 16 keys: s0 keys 2 i4, 2 i4 + 1 (of head g, then of head g + 8), s1 the same + 8
       float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
       // matrices (keys 0-7, columns 0-7), (keys 0-7, 8-15), (keys 8-15, 0-7), (keys 8-15, 8-15) of each 16 columns
       const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
-      if constexpr (EIGHT) {
-        // (keys 0-7, columns 0-15), (keys 0-7, 16-31), (keys 8-15, 0-15), (keys 8-15, 16-31) of each 32 columns, four
-        // of them, 4 i4 .. 4 i4 + 3, in a lane's word
 #pragma unroll
-        for (int j = 0; j < HD / 32; j++) {
-          uint32_t b[4];
-          ldsm4(b, kd + kr * Sh::kRow + (swz<Sh::kRow>(2 * j + kc, kr) << 4));
-#pragma unroll
-          for (int n = 0; n < 2; n++) {
-            const uint32_t* qj = qf[2 * j + n];
-            const uint32_t a1 = WIDE ? qj[1] : 0u, a3 = WIDE ? qj[2 * R - 1] : 0u;
-            uint32_t b0, b1;
-            e4m3_to_f16(b[n], b0, b1);
-            mma_f16(s0, qj[0], a1, qj[R], a3, b0, b1);
-            e4m3_to_f16(b[2 + n], b0, b1);
-            mma_f16(s1, qj[0], a1, qj[R], a3, b0, b1);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < HD / 16; j++) {
-          uint32_t b[4];
-          ldsm4(b, kd + kr * (HD * 2) + (((2 * j + kc) ^ (kr & 7)) << 4));
-          const uint32_t a1 = WIDE ? qf[j][1] : 0u, a3 = WIDE ? qf[j][2 * R - 1] : 0u;
-          mma_bf16(s0, qf[j][0], a1, qf[j][R], a3, b[0], b[1]);
-          mma_bf16(s1, qf[j][0], a1, qf[j][R], a3, b[2], b[3]);
-        }
+      for (int j = 0; j < HD / 16; j++) {
+        uint32_t b[4];
+        ldsm4(b, kd + kr * (HD * 2) + (((2 * j + kc) ^ (kr & 7)) << 4));
+        const uint32_t a1 = WIDE ? qf[j][1] : 0u, a3 = WIDE ? qf[j][2 * R - 1] : 0u;
+        mma_bf16(s0, qf[j][0], a1, qf[j][R], a3, b[0], b[1]);
+        mma_bf16(s1, qf[j][0], a1, qf[j][R], a3, b[2], b[3]);
       }
       uint32_t hi[R][2], lo[R][2];
       bool moved = false;
       float f[R];
-      [[maybe_unused]] float2 kx[2], vx[2], vi[2];  // scales of keys 2 i4, 2 i4 + 1, and 8 more
-      if constexpr (EIGHT) {
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const auto& sc = scales[kg][stage];
-          kx[n] = *reinterpret_cast<const float2*>(sc.k + 8 * n + 2 * i4);
-          vx[n] = *reinterpret_cast<const float2*>(sc.v + 8 * n + 2 * i4);
-          vi[n] = *reinterpret_cast<const float2*>(sc.v_inv + 8 * n + 2 * i4);
-        }
-      }
 #pragma unroll
       for (int h = 0; h < R; h++) {
-        float x0, x1, x2, x3;
-        if constexpr (EIGHT) {
-          x0 = s0[2 * h] * (cq[h] * kx[0].x) + vx[0].x, x1 = s0[2 * h + 1] * (cq[h] * kx[0].y) + vx[0].y;
-          x2 = s1[2 * h] * (cq[h] * kx[1].x) + vx[1].x, x3 = s1[2 * h + 1] * (cq[h] * kx[1].y) + vx[1].y;
-        } else {
-          x0 = s0[2 * h] * c, x1 = s0[2 * h + 1] * c, x2 = s1[2 * h] * c, x3 = s1[2 * h + 1] * c;
-        }
+        float x0 = s0[2 * h] * c, x1 = s0[2 * h + 1] * c, x2 = s1[2 * h] * c, x3 = s1[2 * h + 1] * c;
         if (have != 0xFFFFu) {
           const uint32_t hv = have >> (2 * i4);
           if (!(hv & 1)) x0 = -INFINITY;
@@ -715,15 +683,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         m[h] = mn;
         const float p0 = exp2_approx(x0 - base), p1 = exp2_approx(x1 - base), p2 = exp2_approx(x2 - base),
                     p3 = exp2_approx(x3 - base);
-        if constexpr (EIGHT) {
-          l[h] = l[h] * f[h] + ((p0 * vi[0].x + p1 * vi[0].y) + (p2 * vi[1].x + p3 * vi[1].y));
-          hi[h][0] = pack2h(p0, p1);
-          hi[h][1] = pack2h(p2, p3);
-        } else {
-          l[h] = l[h] * f[h] + ((p0 + p1) + (p2 + p3));
-          split2(p0, p1, hi[h][0], lo[h][0]);
-          split2(p2, p3, hi[h][1], lo[h][1]);
-        }
+        l[h] = l[h] * f[h] + ((p0 + p1) + (p2 + p3));
+        split2(p0, p1, hi[h][0], lo[h][0]);
+        split2(p2, p3, hi[h][1], lo[h][1]);
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -733,37 +695,101 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         }
       }
       // transposed: (keys 0-7, columns 0-7), (keys 8-15, 0-7), (keys 0-7, 8-15), (keys 8-15, 8-15)
-      const int vr = lane & 15, vc = (lane >> 4) + half * (OC * (int)sizeof(E) / 16);
-      if constexpr (EIGHT) {
-        // a lane's word: columns 2 g and 2 g + 1 of keys 2 i4 and 2 i4 + 1; even and odd columns of a chunk are a
-        // product each, so that c0 and c1 of both are the columns 4 i4 .. 4 i4 + 3
+      const int vr = lane & 15, vc = (lane >> 4) + half * (OC / 8);
+#pragma unroll
+      for (int j = 0; j < OC / 16; j++) {
+        uint32_t b[4];
+        ldsm4t(b, vd + vr * (HD * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          if constexpr (WIDE) {
+            mma_bf16(o[2 * j + n], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b[2 * n], b[2 * n + 1]);
+            mma_bf16(o[2 * j + n], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b[2 * n], b[2 * n + 1]);
+          } else {
+            mma_bf16(o[2 * j + n], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b[2 * n], b[2 * n + 1]);
+          }
+        }
+      }
+    }
+    if constexpr (EIGHT) {
+      if (have) {
+        // The products the other way round, keys (then columns) as the 16 rows and heads as the 8 columns: no row is idle, and o
+        // of 8 heads takes half the registers.  Scores of keys g (0, 1) and g + 8 (2, 3), heads 2 i4 and 2 i4 + 1, and 8 more.
+        float x[R][4];
+#pragma unroll
+        for (int r = 0; r < R; r++) x[r][0] = x[r][1] = x[r][2] = x[r][3] = 0.f;
+        // (keys 0-7, columns 0-15), (keys 0-7, 16-31), (keys 8-15, 0-15), (keys 8-15, 16-31) of each 32 columns, four of
+        // them, 4 i4 .. 4 i4 + 3, in a lane's word
+        const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++) {
+          uint32_t b[4];
+          ldsm4(b, kd + kr * Sh::kRow + (swz<Sh::kRow>(2 * j + kc, kr) << 4));
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            uint32_t a0, a1, a2, a3;
+            e4m3_to_f16(b[n], a0, a2);
+            e4m3_to_f16(b[2 + n], a1, a3);
+#pragma unroll
+            for (int r = 0; r < R; r++) mma_f16(x[r], a0, a1, a2, a3, qf[2 * j + n][2 * r], qf[2 * j + n][2 * r + 1]);
+          }
+        }
+        const auto& sc = scales[kg][stage];
+        const float kx[2] = {sc.k[g], sc.k[g + 8]}, vx[2] = {sc.v[g], sc.v[g + 8]}, vi[2] = {sc.v_inv[g], sc.v_inv[g + 8]};
+        uint32_t pt[R][2];
+        float f[S];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int e = 2 * r + h;
+            float &y0 = x[r][h], &y1 = x[r][2 + h];
+            y0 = y0 * (cq[e] * kx[0]) + vx[0];
+            y1 = y1 * (cq[e] * kx[1]) + vx[1];
+            if (have != 0xFFFFu) {
+              if (!(have >> g & 1)) y0 = -INFINITY;
+              if (!(have >> g & 0x100)) y1 = -INFINITY;
+            }
+            float mn = fmaxf(y0, y1);
+            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 4));
+            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
+            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
+            mn = fmaxf(mn, m[e]);
+            const float base = mn == -INFINITY ? 0.f : mn;  // scores of -inf weigh nothing
+            f[e] = exp2_approx(m[e] - base);
+            moved |= mn != m[e];
+            m[e] = mn;
+            y0 = exp2_approx(y0 - base);
+            y1 = exp2_approx(y1 - base);
+            l[e] = l[e] * f[e] + (y0 * vi[0] + y1 * vi[1]);
+          }
+          pt[r][0] = transposed(pack2h(x[r][0], x[r][1]));
+          pt[r][1] = transposed(pack2h(x[r][2], x[r][3]));
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int j = 0; j < OC / 16; j++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+              float* y = o[j * R + r];
+              y[0] *= f[2 * r], y[1] *= f[2 * r + 1], y[2] *= f[2 * r], y[3] *= f[2 * r + 1];
+            }
+        }
+        // a lane's word: columns 2 g and 2 g + 1 of keys 2 i4 and 2 i4 + 1 (transposed, as over 16 bits); the rows of the product
+        // are the even columns of a chunk and then the odd ones
+        const int vr = lane & 15, vc = (lane >> 4) + half * (OC / 16);
 #pragma unroll
         for (int j = 0; j < OC / 32; j++) {
           uint32_t b[4];
           ldsm4t(b, vd + vr * Sh::kRow + (swz<Sh::kRow>(2 * j + vc, vr) << 4));
 #pragma unroll
           for (int n = 0; n < 2; n++) {
-            uint32_t e0, e1, d0, d1;
-            e4m3_to_f16(__byte_perm(b[2 * n], 0u, 0x3120), e0, d0);
-            e4m3_to_f16(__byte_perm(b[2 * n + 1], 0u, 0x3120), e1, d1);
-            const uint32_t a1 = WIDE ? hi[R - 1][0] : 0u, a3 = WIDE ? hi[R - 1][1] : 0u;
-            mma_f16(o[4 * j + 2 * n], hi[0][0], a1, hi[0][1], a3, e0, e1);
-            mma_f16(o[4 * j + 2 * n + 1], hi[0][0], a1, hi[0][1], a3, d0, d1);
-          }
-        }
-      } else {
+            uint32_t a0, a1, a2, a3;
+            e4m3_to_f16(__byte_perm(b[2 * n], 0u, 0x3120), a0, a1);
+            e4m3_to_f16(__byte_perm(b[2 * n + 1], 0u, 0x3120), a2, a3);
 #pragma unroll
-        for (int j = 0; j < OC / 16; j++) {
-          uint32_t b[4];
-          ldsm4t(b, vd + vr * (HD * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
-#pragma unroll
-          for (int n = 0; n < 2; n++) {
-            if constexpr (WIDE) {
-              mma_bf16(o[2 * j + n], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b[2 * n], b[2 * n + 1]);
-              mma_bf16(o[2 * j + n], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b[2 * n], b[2 * n + 1]);
-            } else {
-              mma_bf16(o[2 * j + n], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b[2 * n], b[2 * n + 1]);
-            }
+            for (int r = 0; r < R; r++) mma_f16(o[(2 * j + n) * R + r], a0, a1, a2, a3, pt[r][0], pt[r][1]);
           }
         }
       }
@@ -775,19 +801,24 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       // the sums of the tile's four key groups joined: this unit, or the piece of it that is here
       float* mine_f = red + kg * Sh::kSlot;
 #pragma unroll
-      for (int h = 0; h < R; h++) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if (half == 0 && i4 == 0) mine_f[2 * (g + 8 * h)] = m[h], mine_f[2 * (g + 8 * h) + 1] = l[h];
+      for (int h = 0; h < S; h++) {
+        constexpr int step = EIGHT ? 4 : 1;  // between the lanes that have a head's parts
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], step);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2 * step);
+        if constexpr (EIGHT) l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+        const int head = EIGHT ? h / 2 * 8 + 2 * i4 + h % 2 : g + 8 * h;
+        if (half == 0 && (EIGHT ? g : i4) == 0) mine_f[2 * head] = m[h], mine_f[2 * head + 1] = l[h];
       }
       float* mine_o = mine_f + 2 * MH + g * HD;
       if constexpr (EIGHT) {
 #pragma unroll
-        for (int j = 0; j < OC / 16; j++) {
-          float* to = mine_o + Sh::col(g, half * OC + j * 16 + 4 * i4);
-          const float *e = o[2 * j], *d = o[2 * j + 1];
-          *reinterpret_cast<float4*>(to) = make_float4(e[0], d[0], e[1], d[1]);
-          if constexpr (WIDE) *reinterpret_cast<float4*>(to + 8 * HD) = make_float4(e[2], d[2], e[3], d[3]);
+        for (int h = 0; h < S; h++) {
+          const int head = h / 2 * 8 + 2 * i4 + h % 2;
+#pragma unroll
+          for (int j = 0; j < OC / 16; j++) {
+            const float* y = o[j * R + h / 2] + h % 2;
+            *reinterpret_cast<float2*>(mine_f + 2 * MH + head * HD + Sh::col(head, half * OC + j * 16 + 2 * g)) = make_float2(y[0], y[2]);
+          }
         }
       }
 #pragma unroll
