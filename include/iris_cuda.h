@@ -820,7 +820,7 @@ int iris_gpu_attention_paged(const iris_gpu_kv_cache_t *cache, void *out, const 
 #define IRIS_EXP8_MIN 67      /* 2^-60 */
 #define IRIS_EXP8_MAX 187     /* 2^60  */
 typedef struct {
-    iris_gpu_kv_cache_t pages; /* k, v: e4m3 page pools; strides multiples of 16         */
+    iris_gpu_kv_cache_t pages; /* k, v: e4m3 page pools of up to 64 GiB, strides mult. of 16 */
     uint8_t *k_exp, *v_exp;   /* exponents [num_pages][page_size / block][kv_heads]      */
     int block;                /* tokens that share a scale: a divisor of page_size, at most 128 */
     int64_t exp_page_stride;  /* bytes between the exponents of pages, blocks and heads  */

@@ -352,10 +352,17 @@ template <int N>
 __device__ __forceinline__ void put_scales(Scales8<N>& to, int i, int ke, int ve) {
   to.k[i] = scale8(ke), to.v[i] = (float)(ve - 127), to.v_inv[i] = scale8(254 - ve);
 }
-// exponents of a key's place, both in one number
-__device__ __forceinline__ uint32_t read_exps(const iris_kv_exp_t& x, int page, int slot, int64_t head) {
+// Exponents of a key's place (nothing is done with them here, which would wait for them).
+__device__ __forceinline__ void read_exps(const iris_kv_exp_t& x, int page, int slot, int64_t head, int& ke, int& ve) {
   const int64_t at = page * x.page_stride + iris_paged_block(x.div, slot) * x.block_stride + head;
-  return (uint32_t)__ldg(x.k + at) | (uint32_t)__ldg(x.v + at) << 8;
+  ke = __ldg(x.k + at);
+  ve = __ldg(x.v + at);
+}
+
+// Page of block b of sequence s as the table has it, to be held to the pool when it is used, a round later: a comparison
+// here would wait for it.
+__device__ __forceinline__ int table_page(const iris_gpu_kv_cache_t& c, int s, int b) {
+  return b < c.max_blocks ? __ldg(c.table + (int64_t)s * c.table_stride + b) : -1;
 }
 
 // A head's queries as f16 for the products over 8 bits: columns 16 j + 4 i4 .. + 3 of each 16 into words `lo` and `hi` of
@@ -391,23 +398,32 @@ __device__ __forceinline__ float queries8(const __nv_bfloat16* q, bool live, int
 // of four e4m3, all bits of each one that is NaN
 __device__ __forceinline__ uint32_t nan4(uint32_t x) { return __vcmpeq4(x & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
 
-// HD: head_dim.  MH: query heads of a unit (8 or 16).
-template <typename E, int HD, int MH>
+// HD: head_dim.  MH: query heads of a unit (8 or 16).  CLUSTER: few rows (see the kernel).
+template <typename E, int HD, int MH, bool CLUSTER>
 struct PagedShape {
-  static constexpr int kPair = HD / 128 ? HD / 128 : 1;          // warps on the same 16 keys, 128 columns of o each
-  static constexpr int kThreads = 128 * kPair;
+  // Keys of a tile that a warp takes.  Over 8 bits 32 have half the steps' shuffles, page numbers and scales (64 rows of 1 to
+  // 8192 keys, 32 heads on 8 of 128: 357 instructions for 16 keys instead of 500, 100.3 us instead of 102.6); few rows want
+  // more warps (one of 512 keys: 6.6 us with 32, 5.6 with 16).
+  static constexpr int kKeys = kEight<E> && (!CLUSTER || MH == 16) ? 32 : 16;
+  static constexpr int kGroups = IRIS_PAGED_TILE / kKeys;        // of them
+  static constexpr int kPair = HD / 128 ? HD / 128 : 1;          // warps on the same keys, 128 columns of o each
+  static constexpr int kThreads = 32 * kGroups * kPair;
   // CTAs on an SM and stages of a ring.  At head_dim 64 (256 rows of 0 to 2048 keys, 14 heads on 2) 4 x 2 took 0.84 and
   // 3 x 4 0.88 of the time of 2 x 6, 5 x 2 1.03 and 6 x 2 1.4 of that of 4 x 2: the arithmetic of 16 short keys is
   // latency and wants warps, until registers spill.  At 128 and 256 a ring of three stages fills shared memory, with MH =
   // 16 two.
   static constexpr int kRow = HD * (int)sizeof(E);               // bytes of a row
-  static constexpr int kCtas = kEight<E> ? (HD == 64 ? (MH == 16 ? 4 : 5) : HD == 128 ? (MH == 16 ? 3 : 4) : MH == 16 ? 1 : 2)
+  // Over 8 bits (64 rows of 1 to 8192 keys, 32 heads on 8 of 128) 4 CTAs of two warps with 3 stages 100.3 us, 5 x 2 103.7, 6 x 2
+  // 109, 3 x 4 168: loads in flight as much as warps.
+  static constexpr int kCtas = kEight<E> ? (HD == 64 ? (kKeys == 16 ? 5 : MH == 16 ? 6 : 8) : HD == 128 ? 4 : 2)
                                          : HD == 64 ? 4 : HD == 128 ? 2 : 1;
-  static constexpr int kStages = kEight<E> ? (HD == 64 ? 3 : 2) : HD == 64 || MH == 16 ? 2 : 3;
-  static constexpr int kStageBytes = 16 * kRow;                  // 16 rows of K or of V
-  static constexpr int kRing = kStages * 2 * kStageBytes;        // of 16 keys of a tile
+  static constexpr int kStages = kEight<E> ? 3 : HD == 64 || MH == 16 ? 2 : 3;
+  static constexpr int kStageBytes = kKeys * kRow;               // a warp's rows of K or of V
+  static constexpr int kRing = kStages * 2 * kStageBytes;        // of its keys of a tile
   static constexpr int kSlot = MH * (HD + 2);                    // floats of a piece: m, l, then o
-  static constexpr int kSmem = 4 * kRing + 4 * kSlot * 4;
+  // the sums of a unit's end lie behind the rings; over 8 bits in the place of the tile used last, which is as large
+  static constexpr int kSmem = kGroups * (kRing + (kEight<E> ? 0 : kSlot * 4));
+  static_assert(!kEight<E> || 2 * kStageBytes >= MH * HD * 4, "a warp's sums fit");
   // column of o of head h in the sums of 16 keys in shared memory, which are laid out as a piece: the heads of a store's
   // half warp, eight or every other one of them, fall into different banks
   __device__ static int col(int h, int c) { return c ^ ((kEight<E> ? h >> 1 : h) & 3) << 3; }
@@ -499,18 +515,19 @@ __device__ __forceinline__ bool paged_begin(const IrisPagedAttention& a, int uni
 // equal part of its tiles each, and joins the parts in distributed shared
 // memory: one launch, and no round through the workspace.
 template <typename E, int HD, int MH, bool CLUSTER>
-__global__ void __launch_bounds__(PagedShape<E, HD, MH>::kThreads, PagedShape<E, HD, MH>::kCtas)
+__global__ void __launch_bounds__(PagedShape<E, HD, MH, CLUSTER>::kThreads, PagedShape<E, HD, MH, CLUSTER>::kCtas)
 paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
-  using Sh = PagedShape<E, HD, MH>;
+  using Sh = PagedShape<E, HD, MH, CLUSTER>;
   constexpr bool EIGHT = kEight<E>;
   constexpr int D = Sh::kStages, CH = Sh::kRow / 16;  // CH: 16-byte chunks of a row
   constexpr int PAIR = Sh::kPair, T = Sh::kThreads, OC = HD / PAIR;  // OC: columns of o a warp holds
   constexpr bool WIDE = MH == 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t seen[4][D];  // of each 16 keys of a tile and stage: which exist
-  __shared__ __align__(16) Scales8<EIGHT ? 16 : 1> scales[EIGHT ? 4 : 1][EIGHT ? D : 1];
+  constexpr int KEYS = Sh::kKeys, GROUPS = Sh::kGroups;
+  __shared__ uint32_t seen[GROUPS][D];  // of a warp's keys of a tile and stage: which exist
+  __shared__ __align__(16) Scales8<EIGHT ? KEYS : 1> scales[EIGHT ? GROUPS : 1][EIGHT ? D : 1];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, i4 = lane % 4;
-  const int kg = warp / PAIR, half = warp % PAIR;  // which 16 keys of a tile, which columns of o
+  const int kg = warp / PAIR, half = warp % PAIR;  // which keys of a tile, which columns of o
   auto sync_keys = [&]() {  // the warps on the same keys
     if constexpr (PAIR == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * PAIR) : "memory");
@@ -547,20 +564,33 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 
   const int rtiles = units / cache.kv_heads;
   const uint32_t ring = iris::smem_u32(smem) + kg * Sh::kRing;
-  float* red = reinterpret_cast<float*>(smem + 4 * Sh::kRing);
+  // m and l, and o, of the sums of key group w at a unit's end, behind the use of stage `used`
+  __shared__ float2 sums8[EIGHT ? GROUPS : 1][EIGHT ? MH : 1];
+  int used = 0;
+  auto ml_of = [&](int w) {
+    return EIGHT ? sums8[w] : reinterpret_cast<float2*>(smem + GROUPS * Sh::kRing + w * Sh::kSlot * 4);
+  };
+  auto o_of = [&](int w) {
+    return reinterpret_cast<float*>(EIGHT ? smem + w * Sh::kRing + used * 2 * Sh::kStageBytes
+                                          : smem + GROUPS * Sh::kRing + (w * Sh::kSlot + 2 * MH) * 4);
+  };
+  // a cluster's part stays in shared memory, where the first stage's tiles lay (over 8 bits in the sums' order of columns,
+  // since the first group's may lie just there: a thread writes what it alone read)
+  __shared__ float2 part8[EIGHT ? MH : 1];
+  auto part_o = [&](float* slot, int h, int col) { return EIGHT ? slot + h * HD + Sh::col(h, col) : slot + 2 * MH + h * HD + col; };
 
   // ---- loads, up to D - 1 stages ahead of the arithmetic
   iris_paged_at_t ld = at;
   bool loads = any;
-  int page, slot;                  // of this lane's key (lanes 16-31 as lanes 0-15) of the next tile to load
+  int page, slot;                  // of this lane's key (with 16, lanes 16-31 as lanes 0-15) of the next tile to load
   int64_t head = 0;                // its head's offset
   int64_t exp_head = 0;            // the same among the exponents
-  uint32_t exps = 0;               // of this lane's key of the tile loaded last, on their way to shared memory
+  int ke = 127, ve = 127;          // exponents of this lane's key of the tile loaded last, on their way to shared memory
   int exps_to = -1;                // their stage
   auto find = [&]() {
-    const int p = ld.i * IRIS_PAGED_TILE + kg * 16 + (lane & 15), b = iris_paged_block(a.div, p);
+    const int p = ld.i * IRIS_PAGED_TILE + kg * KEYS + lane % KEYS, b = iris_paged_block(a.div, p);
     slot = p - b * cache.page_size;
-    page = p < ld.len ? iris_paged_page(&cache, ld.s, b) : -1;
+    page = p < ld.len ? table_page(cache, ld.s, b) : -1;
     if (ld.i == 0) {
       head = (int64_t)(ld.u / rtiles) * cache.head_stride;
       if constexpr (EIGHT) exp_head = (int64_t)(ld.u / rtiles) * a.exp.head_stride;
@@ -572,18 +602,39 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   auto issue = [&](int stage) {
     if constexpr (EIGHT) {
       // the exponents of the stage before: read a round ago, needed in the next one at the earliest
-      if (exps_to >= 0 && half == 0 && lane < 16) put_scales(scales[kg][exps_to], lane, exp8(exps & 0xFF), exp8(exps >> 8));
+      if (exps_to >= 0 && half == 0 && lane < KEYS) put_scales(scales[kg][exps_to], lane, exp8(ke), exp8(ve));
       exps_to = loads ? stage : -1;
     }
     if (loads) {
-      const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
+      page = (uint32_t)page < (uint32_t)cache.num_pages ? page : -1;
+      const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & (0xffffffffu >> (32 - KEYS));
       const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
       if (half == 0 && lane == 0) seen[kg][stage] = have;
-      if constexpr (EIGHT) exps = page >= 0 ? read_exps(a.exp, page, slot, exp_head) : 0x7F7Fu;
+      if constexpr (EIGHT) {
+        ke = ve = 127;
+        if (page >= 0) read_exps(a.exp, page, slot, exp_head, ke, ve);
+      }
       const uint32_t kd = ring + stage * 2 * Sh::kStageBytes, vd = kd + Sh::kStageBytes;
       constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows one instruction of the warp covers
+      if constexpr (EIGHT) {
+        // places in 32 bits, counted in 16 bytes: half the instructions of 64-bit ones
+        const uint32_t place = (uint32_t)(off >> 4);
+        auto copy = [&](auto all) {
 #pragma unroll
-      for (int j = 0; j < 16 / RPI / PAIR; j++) {
+          for (int j = 0; j < KEYS / RPI / PAIR; j++) {
+            const int r = (j * PAIR + half) * RPI + lane / CH, ch = lane % CH;
+            const size_t o = (size_t)(__shfl_sync(0xffffffffu, place, r) + ch) * 16;
+            const int bytes = decltype(all)::value || (have >> r) & 1 ? 16 : 0;
+            const uint32_t d = r * Sh::kRow + (swz<Sh::kRow>(ch, r) << 4);
+            cp_async16(kd + d, (const E*)cache.k + o, bytes);
+            cp_async16(vd + d, (const E*)cache.v + o, bytes);
+          }
+        };
+        if (have == 0xffffffffu >> (32 - KEYS)) copy(std::true_type());
+        else copy(std::false_type());
+      }
+#pragma unroll
+      for (int j = 0; !EIGHT && j < KEYS / RPI / PAIR; j++) {
         const int r = (j * PAIR + half) * RPI + lane / CH, ch = lane % CH;
         const int64_t o = __shfl_sync(0xffffffffu, off, r) + ch * (16 / (int)sizeof(E));
         const int bytes = (have >> r) & 1 ? 16 : 0;
@@ -714,29 +765,37 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
     if constexpr (EIGHT) {
       if (have) {
         // The products the other way round, keys (then columns) as the 16 rows and heads as the 8 columns: no row is idle, and o
-        // of 8 heads takes half the registers.  Scores of keys g (0, 1) and g + 8 (2, 3), heads 2 i4 and 2 i4 + 1, and 8 more.
-        float x[R][4];
-#pragma unroll
-        for (int r = 0; r < R; r++) x[r][0] = x[r][1] = x[r][2] = x[r][3] = 0.f;
+        // of 8 heads takes half the registers.  Of each 16 keys k: scores of g (0, 1) and g + 8 (2, 3), heads 2 i4 and 2 i4 +
+        // 1, and 8 more.
+        constexpr int KS = KEYS / 16;
+        float x[KS][R][4];
         // (keys 0-7, columns 0-15), (keys 0-7, 16-31), (keys 8-15, 0-15), (keys 8-15, 16-31) of each 32 columns, four of
         // them, 4 i4 .. 4 i4 + 3, in a lane's word
         const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
 #pragma unroll
-        for (int j = 0; j < HD / 32; j++) {
-          uint32_t b[4];
-          ldsm4(b, kd + kr * Sh::kRow + (swz<Sh::kRow>(2 * j + kc, kr) << 4));
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-          for (int n = 0; n < 2; n++) {
-            uint32_t a0, a1, a2, a3;
-            e4m3_to_f16(b[n], a0, a2);
-            e4m3_to_f16(b[2 + n], a1, a3);
+          for (int r = 0; r < R; r++) x[k][r][0] = x[k][r][1] = x[k][r][2] = x[k][r][3] = 0.f;
 #pragma unroll
-            for (int r = 0; r < R; r++) mma_f16(x[r], a0, a1, a2, a3, qf[2 * j + n][2 * r], qf[2 * j + n][2 * r + 1]);
+        for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+          for (int k = 0; k < KS; k++) {  // (a product waits for the one before it on the same 16 keys)
+            uint32_t b[4];
+            ldsm4(b, kd + (k * 16 + kr) * Sh::kRow + (swz<Sh::kRow>(2 * j + kc, kr) << 4));
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+              uint32_t a0, a1, a2, a3;
+              e4m3_to_f16(b[n], a0, a2);
+              e4m3_to_f16(b[2 + n], a1, a3);
+#pragma unroll
+              for (int r = 0; r < R; r++) mma_f16(x[k][r], a0, a1, a2, a3, qf[2 * j + n][2 * r], qf[2 * j + n][2 * r + 1]);
+            }
           }
-        }
         const auto& sc = scales[kg][stage];
-        const float kx[2] = {sc.k[g], sc.k[g + 8]}, vx[2] = {sc.v[g], sc.v[g + 8]}, vi[2] = {sc.v_inv[g], sc.v_inv[g + 8]};
-        uint32_t pt[R][2];
+        float kx[2 * KS], vx[2 * KS], vi[2 * KS];  // of keys 8 i + g
+#pragma unroll
+        for (int i = 0; i < 2 * KS; i++) kx[i] = sc.k[8 * i + g], vx[i] = sc.v[8 * i + g], vi[i] = sc.v_inv[8 * i + g];
+        uint32_t pt[KS][R][2];
         float f[S];
         bool moved = false;
 #pragma unroll
@@ -744,28 +803,35 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             const int e = 2 * r + h;
-            float &y0 = x[r][h], &y1 = x[r][2 + h];
-            y0 = y0 * (cq[e] * kx[0]) + vx[0];
-            y1 = y1 * (cq[e] * kx[1]) + vx[1];
-            if (have != 0xFFFFu) {
-              if (!(have >> g & 1)) y0 = -INFINITY;
-              if (!(have >> g & 0x100)) y1 = -INFINITY;
+            float mn = m[e];
+#pragma unroll
+            for (int i = 0; i < 2 * KS; i++) {
+              float& y = x[i / 2][r][i % 2 * 2 + h];
+              y = y * (cq[e] * kx[i]) + vx[i];
+              if (have != (0xffffffffu >> (32 - KEYS)) && !(have >> g & 1u << 8 * i)) y = -INFINITY;
+              mn = fmaxf(mn, y);
             }
-            float mn = fmaxf(y0, y1);
             mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 4));
             mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
             mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
-            mn = fmaxf(mn, m[e]);
             const float base = mn == -INFINITY ? 0.f : mn;  // scores of -inf weigh nothing
             f[e] = exp2_approx(m[e] - base);
             moved |= mn != m[e];
             m[e] = mn;
-            y0 = exp2_approx(y0 - base);
-            y1 = exp2_approx(y1 - base);
-            l[e] = l[e] * f[e] + (y0 * vi[0] + y1 * vi[1]);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * KS; i++) {
+              float& y = x[i / 2][r][i % 2 * 2 + h];
+              y = exp2_approx(y - base);
+              sum += y * vi[i];
+            }
+            l[e] = l[e] * f[e] + sum;
           }
-          pt[r][0] = transposed(pack2h(x[r][0], x[r][1]));
-          pt[r][1] = transposed(pack2h(x[r][2], x[r][3]));
+#pragma unroll
+          for (int k = 0; k < KS; k++) {
+            pt[k][r][0] = transposed(pack2h(x[k][r][0], x[k][r][1]));
+            pt[k][r][1] = transposed(pack2h(x[k][r][2], x[k][r][3]));
+          }
         }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -780,26 +846,28 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         // are the even columns of a chunk and then the odd ones
         const int vr = lane & 15, vc = (lane >> 4) + half * (OC / 16);
 #pragma unroll
-        for (int j = 0; j < OC / 32; j++) {
-          uint32_t b[4];
-          ldsm4t(b, vd + vr * Sh::kRow + (swz<Sh::kRow>(2 * j + vc, vr) << 4));
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-          for (int n = 0; n < 2; n++) {
-            uint32_t a0, a1, a2, a3;
-            e4m3_to_f16(__byte_perm(b[2 * n], 0u, 0x3120), a0, a1);
-            e4m3_to_f16(__byte_perm(b[2 * n + 1], 0u, 0x3120), a2, a3);
+          for (int j = 0; j < OC / 32; j++) {
+            uint32_t b[4];
+            ldsm4t(b, vd + (k * 16 + vr) * Sh::kRow + (swz<Sh::kRow>(2 * j + vc, vr) << 4));
 #pragma unroll
-            for (int r = 0; r < R; r++) mma_f16(o[(2 * j + n) * R + r], a0, a1, a2, a3, pt[r][0], pt[r][1]);
+            for (int n = 0; n < 2; n++) {
+              uint32_t a0, a1, a2, a3;
+              e4m3_to_f16(__byte_perm(b[2 * n], 0u, 0x3120), a0, a1);
+              e4m3_to_f16(__byte_perm(b[2 * n + 1], 0u, 0x3120), a2, a3);
+#pragma unroll
+              for (int r = 0; r < R; r++) mma_f16(o[(2 * j + n) * R + r], a0, a1, a2, a3, pt[k][r][0], pt[k][r][1]);
+            }
           }
-        }
       }
     }
     sync_keys();  // this stage is filled again by the next iteration's issue
+    used = stage;
     stage = stage == D - 1 ? 0 : stage + 1;
     const bool ends = at.i == at.n - 1;
     if (ends || !more) {
-      // the sums of the tile's four key groups joined: this unit, or the piece of it that is here
-      float* mine_f = red + kg * Sh::kSlot;
+      // the sums of the tile's key groups joined: this unit, or the piece of it that is here
 #pragma unroll
       for (int h = 0; h < S; h++) {
         constexpr int step = EIGHT ? 4 : 1;  // between the lanes that have a head's parts
@@ -807,9 +875,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2 * step);
         if constexpr (EIGHT) l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
         const int head = EIGHT ? h / 2 * 8 + 2 * i4 + h % 2 : g + 8 * h;
-        if (half == 0 && (EIGHT ? g : i4) == 0) mine_f[2 * head] = m[h], mine_f[2 * head + 1] = l[h];
+        if (half == 0 && (EIGHT ? g : i4) == 0) ml_of(kg)[head] = make_float2(m[h], l[h]);
       }
-      float* mine_o = mine_f + 2 * MH + g * HD;
+      float* mine_o = o_of(kg) + g * HD;
       if constexpr (EIGHT) {
 #pragma unroll
         for (int h = 0; h < S; h++) {
@@ -817,7 +885,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 #pragma unroll
           for (int j = 0; j < OC / 16; j++) {
             const float* y = o[j * R + h / 2] + h % 2;
-            *reinterpret_cast<float2*>(mine_f + 2 * MH + head * HD + Sh::col(head, half * OC + j * 16 + 2 * g)) = make_float2(y[0], y[2]);
+            *reinterpret_cast<float2*>(o_of(kg) + head * HD + Sh::col(head, half * OC + j * 16 + 2 * g)) = make_float2(y[0], y[2]);
           }
         }
       }
@@ -832,7 +900,6 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         }
       }
       const bool whole = !CLUSTER && ends && begun_here;
-      // a cluster's part stays in shared memory, where its last tile lay
       float* slot = CLUSTER ? reinterpret_cast<float*>(smem)
                             : a.ws + paged_slots_at(gridDim.x) + (size_t)(2 * blockIdx.x + (begun_here ? 1 : 0)) * Sh::kSlot;
       __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)head0 * HD;
@@ -847,22 +914,24 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         const int h = e / (HD / 4), col = (e % (HD / 4)) * 4;
         float mm = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) mm = fmaxf(mm, red[w * Sh::kSlot + 2 * h]);
+        for (int w = 0; w < GROUPS; w++) mm = fmaxf(mm, ml_of(w)[h].x);
         const float base = mm == -INFINITY ? 0.f : mm;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-          const float s = exp2_approx(red[w * Sh::kSlot + 2 * h] - base);
-          sum += s * red[w * Sh::kSlot + 2 * h + 1];
-          const float4 v = *reinterpret_cast<const float4*>(red + w * Sh::kSlot + 2 * MH + h * HD + Sh::col(h, col));
+        for (int w = 0; w < GROUPS; w++) {
+          const float2 ml = ml_of(w)[h];
+          const float s = exp2_approx(ml.x - base);
+          sum += s * ml.y;
+          const float4 v = *reinterpret_cast<const float4*>(o_of(w) + h * HD + Sh::col(h, col));
           y.x += s * v.x, y.y += s * v.y, y.z += s * v.z, y.w += s * v.w;
         }
         if (whole) {
           const float r = sum == 0.f ? 0.f : 1.0f / sum;
           *reinterpret_cast<uint2*>(out + h * HD + col) = make_uint2(pack2(y.x * r, y.y * r), pack2(y.z * r, y.w * r));
         } else {
-          if (col == 0) slot[2 * h] = mm, slot[2 * h + 1] = sum;
-          *reinterpret_cast<float4*>(slot + 2 * MH + h * HD + col) = y;
+          float2* ml = CLUSTER && EIGHT ? part8 : reinterpret_cast<float2*>(slot);
+          if (col == 0) ml[h] = make_float2(mm, sum);
+          *reinterpret_cast<float4*>(CLUSTER ? part_o(slot, h, col) : slot + 2 * MH + h * HD + col) = y;
         }
       }
       clear();
@@ -874,8 +943,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   }
   if constexpr (CLUSTER) {
     float* slot = reinterpret_cast<float*>(smem);
+    float2* part_ml = EIGHT ? part8 : reinterpret_cast<float2*>(slot);
     if (!any)
-      for (int h = tid; h < heads_here; h += T) slot[2 * h] = -INFINITY, slot[2 * h + 1] = -1.f;  // no key; a sum is never under 0
+      for (int h = tid; h < heads_here; h += T) part_ml[h] = make_float2(-INFINITY, -1.f);  // no key; a sum is never under 0
     __syncwarp();
     iris::cluster_sync();
     __nv_bfloat16* out = (__nv_bfloat16*)a.out + (int64_t)at.t * a.ldo + (int64_t)head0 * HD;
@@ -884,10 +954,9 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
       float mm = -INFINITY, sum = 0.f;
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
       for (uint32_t p = 0; p < parts; p++) {
-        const float* from = iris::cluster_map(slot, p);
-        const float2 ml = *reinterpret_cast<const float2*>(from + 2 * h);
+        const float2 ml = iris::cluster_map(part_ml, p)[h];
         if (ml.y < 0.f) continue;  // no key: its columns were not written
-        const float4 v = *reinterpret_cast<const float4*>(from + 2 * MH + h * HD + col);
+        const float4 v = *reinterpret_cast<const float4*>(part_o(iris::cluster_map(slot, p), h, col));
         const float mn = fmaxf(mm, ml.x), base = mn == -INFINITY ? 0.f : mn;
         const float f = exp2_approx(mm - base), s = exp2_approx(ml.x - base);
         mm = mn;
@@ -965,12 +1034,12 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
   int page, slot;  // of this lane's key (the lanes past a warp's keys as its first) of the next tile to load
   int64_t head;    // its head's offset
   int64_t exp_head = 0;            // the same among the exponents
-  uint32_t exps = 0;               // of this lane's key of the tile loaded last, on their way to shared memory
+  int ke = 127, ve = 127;          // exponents of this lane's key of the tile loaded last, on their way to shared memory
   int exps_to = -1;                // their stage
   auto find = [&]() {
     const int p = ld.i * IRIS_PAGED_TILE + warp * MINE + lane % MINE, b = iris_paged_block(a.div, p);
     slot = p - b * cache.page_size;
-    page = p < ld.len ? iris_paged_page(&cache, ld.s, b) : -1;
+    page = p < ld.len ? table_page(cache, ld.s, b) : -1;
     head = (int64_t)(ld.u / rtiles) * cache.head_stride;
     if constexpr (EIGHT) exp_head = (int64_t)(ld.u / rtiles) * a.exp.head_stride;
   };
@@ -979,11 +1048,15 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
   auto issue = [&](int stage) {
     if constexpr (EIGHT) {
       // the exponents of the stage before: read a round ago, needed behind the next barrier at the earliest
-      if (exps_to >= 0 && lane < MINE) put_scales(scales[exps_to], warp * MINE + lane, exp8(exps & 0xFF), exp8(exps >> 8));
+      if (exps_to >= 0 && lane < MINE) put_scales(scales[exps_to], warp * MINE + lane, exp8(ke), exp8(ve));
       exps_to = loads ? stage : -1;
     }
     if (loads) {
-      if constexpr (EIGHT) exps = page >= 0 ? read_exps(a.exp, page, slot, exp_head) : 0x7F7Fu;
+      page = (uint32_t)page < (uint32_t)cache.num_pages ? page : -1;
+      if constexpr (EIGHT) {
+        ke = ve = 127;
+        if (page >= 0) read_exps(a.exp, page, slot, exp_head, ke, ve);
+      }
       const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & ((1u << MINE) - 1);
       const int64_t off = page >= 0 ? iris_paged_offset(&cache, page, slot) + head : 0;
       if (lane == 0) {
@@ -1356,7 +1429,7 @@ constexpr int JOIN_THREADS = 512;
 template <int HD, int MH, bool FEW>
 __global__ void __launch_bounds__(JOIN_THREADS)
 paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int per_block) {
-  using Sh = PagedShape<__nv_bfloat16, HD, MH>;  // pieces are f32, alike for both
+  using Sh = PagedShape<__nv_bfloat16, HD, MH, false>;  // pieces are f32, alike for both
   constexpr int COLS = HD / 4;
   __shared__ float4 acc[JOIN_THREADS];
   __shared__ float2 ml[JOIN_THREADS / COLS];
@@ -2000,7 +2073,8 @@ constexpr int CLUSTER_TILES = 4;
 
 template <typename E, int HD, int MH>
 struct PagedLaunch {
-  using Sh = PagedShape<E, HD, MH>;
+  using Sh = PagedShape<E, HD, MH, false>;
+  using Few = PagedShape<E, HD, MH, true>;
   using Runs = RunShape<E, HD>;
   static size_t ws_bytes(int num_sms) {
     const int ctas = num_sms * Sh::kCtas, runs = num_sms * Runs::kCtas;
@@ -2014,7 +2088,7 @@ struct PagedLaunch {
     e = cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                Sh::kSmem);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    return cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few::kSmem);
   }
   static cudaError_t launch(const IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
     // few rows: a block, or a cluster of up to 8, on each unit, all on the device at once (clusters of 4 and 8 do not fill
@@ -2027,13 +2101,13 @@ struct PagedLaunch {
     const int64_t units = (int64_t)a->rows * iris_paged_units(&a->cache, a->heads);
     const int room = iris_paged_tiles(iris_paged_len(&a->cache, 0x7FFFFFFF));
     unsigned parts = 8;
-    const int64_t slots = (int64_t)num_sms * Sh::kCtas;
+    const int64_t slots = (int64_t)num_sms * Few::kCtas;
     while (parts > 1 && units * parts > (parts > 2 ? slots * 7 / 8 : slots)) parts /= 2;
     const int64_t tiles = 2 * CLUSTER_TILES * units * parts / slots + 1;  // 2 CLUSTER_TILES with every slot taken
     if (units * parts <= slots && room <= (tiles < CLUSTER_TILES ? CLUSTER_TILES : tiles) * parts) {
       *launches = 1;
       return iris::launch_cluster_overlapped(paged_attention_kernel<E, HD, MH, true>, dim3((unsigned)units * parts),
-                                             dim3(Sh::kThreads), Sh::kSmem, parts, stream, *a);
+                                             dim3(Few::kThreads), Few::kSmem, parts, stream, *a);
     }
     // four times as many rows as sequences: runs of rows.  On the device, 32 heads on 8 of 128, rows by themselves -> runs:
     // a prompt of 128 15.3 -> 15.8 us, 512 83 -> 31, 2048 934 -> 196, 8192 13.7 -> 2.6 ms; 64 tokens behind 32704 855 ->

@@ -80,6 +80,12 @@ static int cache8_check(const iris_gpu_kv_cache8_t *c, const char *what) {
     if (cache_check_of(&c->pages, 1, what)) return IRIS_CUDA_ERR_ARG;
     if (c->block < 1 || c->block > 128 || c->pages.page_size % c->block)
         return LM_FAIL("%s: blocks of %d tokens in pages of %d (a divisor, at most 128)", what, c->block, c->pages.page_size);
+    /* the kernels count places in 16 bytes, in 32 bits */
+    if (((c->pages.num_pages - 1) * c->pages.page_stride >> 36) || ((c->pages.page_size - 1) * c->pages.token_stride >> 36) ||
+        ((c->pages.kv_heads - 1) * c->pages.head_stride >> 36) ||
+        (c->pages.num_pages - 1) * c->pages.page_stride + (c->pages.page_size - 1) * c->pages.token_stride +
+                (c->pages.kv_heads - 1) * c->pages.head_stride + c->pages.head_dim > (int64_t)1 << 36)
+        return LM_FAIL("%s: pools of more than 64 GiB", what);
     if (c->exp_page_stride < 0 || c->exp_block_stride < 0 || c->exp_head_stride < 0 ||
         (c->pages.num_pages > 1 && !c->exp_page_stride) || (c->pages.page_size > c->block && !c->exp_block_stride) ||
         (c->pages.kv_heads > 1 && !c->exp_head_stride))
