@@ -1580,12 +1580,6 @@ struct LpShape {
   static constexpr int kBlocks = LP_LOADS / kPer;               // blocks in flight
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Two f32 in one register pair, for the packed instructions.

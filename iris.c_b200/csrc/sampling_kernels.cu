@@ -21,20 +21,26 @@ namespace {
 // The row is read once, by a cluster of blocks that hold it in shared memory.
 // With top-k of up to SMP_TOP, or where min-p leaves few, the tokens above a bound
 // (which k of the threads' own largest reach) are few: one block puts them in order
-// and has the answer.  Else the sums are needed over the whole row: every
-// thread adds up its values in 16 bins of its own (no atomics, always the same order), the bin in
-// which the number is crossed is cut into 16 again, until SMP_LIST tokens are left
-// to be put in order, or tokens of one value, of which the id decides.
+// and has the answer.  Else a histogram over the distance from m, in parts of
+// SMP_SPAN / SMP_BINS of t, says to 2^-14 (large vocabularies: less closely) how the sum grows along the line
+// (each value adds its weight relative to its bin's, a whole number of 16 bits, so
+// that no order of additions shows); a pass over the row adds up exactly what
+// stands ahead of the bins in which the number is crossed and collects their
+// tokens, some hundreds, which one block puts in order.  Where they are too many
+// (equal logits, high temperatures) the bins are cut further, each time into 16,
+// with exact sums, until few are left, or tokens of one value, of which the id decides.
 // Weights and sums are 64-bit: a token is taken by where a sum of 100000 weights
 // ends, and with 32 bits one row in a hundred would take its neighbour.
-constexpr int SMP_THREADS = 256, SMP_WARPS = SMP_THREADS / 32, SMP_PARTS = 8, SMP_BINS = 16;
-constexpr int SMP_LIST = 512;  // tokens put in order
-constexpr int SMP_TOP = 256;   // largest top-k whose tokens are looked for through a bound
-constexpr float SMP_SPAN = 24.f;  // (m - x) / t that the first bins cover; the last one holds all that is below
+constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32, SMP_PARTS = 8;
+constexpr int SMP_LIST = 1024;  // tokens put in order: two a thread
+constexpr int SMP_TOP = 512;    // largest top-k whose tokens are looked for through a bound
+constexpr int SMP_BINS = 1024;
+constexpr float SMP_SPAN = 24.f;      // (m - x) / t that the bins cover; the last one holds all that is below
+constexpr int SMP_CUT = 16, SMP_CUTTERS = 64;  // bins of a closer look, threads that fill bins of their own
 
-struct SmpSums {  // of the bins, from each block of the cluster
-  double mass[SMP_PARTS][SMP_BINS];
-  uint32_t count[SMP_PARTS][SMP_BINS];
+struct SmpSums {  // of the closer bins, from each block of the cluster
+  double mass[SMP_PARTS][SMP_CUT];
+  uint32_t count[SMP_PARTS][SMP_CUT];
 };
 
 struct SmpFound {
@@ -43,18 +49,27 @@ struct SmpFound {
   uint32_t count;
 };
 
-struct SmpShared {
-  SmpSums first, next[2];      // next: in turn, so that one round's may be read while the next one's come
-  uint32_t one[2][SMP_PARTS];  // a number from each block
-  double scan[SMP_WARPS];
-  uint32_t iscan[SMP_WARPS];
-  SmpFound found;
-  uint32_t n;
+struct SmpExact {  // of a block
+  double all, ahead;      // sums of all tokens, of those ahead of the window
+  uint32_t n_all, n_ahead, n;  // tokens: all, ahead, in the window
 };
 
-// shared memory besides the row: the bins; a list of places and its order in the same bytes
-constexpr int SMP_WORK = SMP_BINS * SMP_THREADS * (8 + 2);
-static_assert(SMP_WORK >= 2 * SMP_LIST * 8 + SMP_THREADS * 4, "the lists fit");
+struct SmpShared {
+  SmpSums next[2];             // in turn, so that one round's may be read while the next one's come
+  SmpExact exact[2][SMP_PARTS];
+  uint32_t one[2][SMP_PARTS];  // a number from each block
+  double scan[SMP_WARPS], scan2[SMP_WARPS];
+  uint32_t iscan[SMP_WARPS];
+  double root[32];             // 2^(i / 32)
+  SmpFound found;
+  uint32_t n, lo, hi;
+};
+
+// shared memory besides the row: two histograms, the sums along the bins, and the list, in whose place the closer bins stand
+constexpr int SMP_HIST = SMP_BINS * 4, SMP_ALONG = SMP_BINS * 8;
+constexpr int SMP_TAIL = SMP_CUT * SMP_CUTTERS * (8 + 4);
+constexpr int SMP_WORK = 2 * SMP_HIST + SMP_ALONG + SMP_TAIL;
+static_assert(SMP_TAIL >= SMP_LIST * 8 && SMP_ALONG >= SMP_LIST * 8, "the lists fit");
 
 struct SmpWindow {  // part of the line: ranks lo .. hi, `count` tokens, with sums over what stands ahead of it
   uint32_t lo, hi;
@@ -73,10 +88,14 @@ struct SmpRow {
   uint8_t* smem;
   const In* x;
   int tid, part, parts, off, v0, nv;
-  float m, floor_;
-  double top, inv_t;
+  float m, floor_, cut_off;  // cut_off: what lies further under m weighs nothing, e^-620
+  double top, inv_t, rate;   // rate: 32 log2(e) / t
   float inv_bin;
+  float unit;                // of the histogram's weights, so that a block's tokens in one bin stay within 32 bits
+  double near_;              // relative error of the histogram's sums, with room to spare: half a unit of rounding, 2^-18 for the
+                             // bins' edges and 2^-19 for what the weight's series leaves out
   uint32_t turn = 0;
+  int hists = 0;
 
   __device__ SmpRow(const IrisSample& a, SmpShared& sh, uint8_t* smem) : a(a), sh(sh), smem(smem) {
     tid = threadIdx.x;
@@ -87,13 +106,17 @@ struct SmpRow {
     const int all = (int)(((int64_t)a.vocab + off + VEC - 1) / VEC), per = (all + parts - 1) / parts;
     v0 = part * per;
     nv = max(0, min(per, all - v0));
+    unit = 65536.f;
+    while (unit * ((float)per * VEC) > 4.2e9f) unit *= 0.5f;
+    near_ = 1.0 / 32768 + 1.0 / unit;
   }
   __device__ uint8_t* work() const { return smem + (HELD ? a.held_bytes : 0); }
-  __device__ double* masses() const { return reinterpret_cast<double*>(work()); }
-  __device__ uint16_t* counts() const { return reinterpret_cast<uint16_t*>(work() + SMP_BINS * SMP_THREADS * 8); }
-  __device__ uint64_t* list() const { return reinterpret_cast<uint64_t*>(work()); }
-  __device__ uint64_t* order() const { return list() + SMP_LIST; }
-  __device__ uint32_t* owns() const { return reinterpret_cast<uint32_t*>(order() + SMP_LIST); }
+  __device__ uint32_t* hist(int i) const { return reinterpret_cast<uint32_t*>(work() + i * SMP_HIST); }
+  __device__ double* along() const { return reinterpret_cast<double*>(work() + 2 * SMP_HIST); }  // sums up to and with a bin
+  __device__ uint64_t* list() const { return reinterpret_cast<uint64_t*>(work() + 2 * SMP_HIST + SMP_ALONG); }
+  __device__ uint64_t* own_list() const { return reinterpret_cast<uint64_t*>(along()); }         // before there are sums
+  __device__ double* cut_mass() const { return reinterpret_cast<double*>(list()); }
+  __device__ uint32_t* cut_count() const { return reinterpret_cast<uint32_t*>(cut_mass() + SMP_CUT * SMP_CUTTERS); }
 
   __device__ void all_sync() const {
     __syncwarp();
@@ -102,7 +125,7 @@ struct SmpRow {
   }
   template <typename T>
   __device__ T* at(T* p, int rank) const { return parts > 1 ? iris::cluster_map(p, (uint32_t)rank) : p; }
-  // this block's number, by thread 0, to all of them; the numbers of the blocks after the barrier
+  // this block's number, the same in all threads, to all of them; the numbers of the blocks after the barrier
   __device__ const uint32_t* tell(uint32_t v) {
     uint32_t* to = sh.one[turn++ & 1];
     if (tid < parts) *at(to + part, tid) = v;
@@ -115,24 +138,60 @@ struct SmpRow {
     if constexpr (HELD) return reinterpret_cast<const uint4*>(smem)[v];
     else return row_vec(x, first_id(v), a.vocab);
   }
+  // f(values, id of the first): a vector; values outside the row are -inf
   template <typename F>
-  __device__ void each(F f) const {
-    for (int v = tid; v < nv; v += SMP_THREADS) {
+  __device__ void vectors(F f, int threads = SMP_THREADS) const {
+    for (int v = tid; v < nv; v += threads) {
       float y[VEC];
       vec_values<In>(vec(v), y);
-#pragma unroll
-      for (int i = 0; i < VEC; i++) f(y[i], first_id(v) + i);
+      f(y, first_id(v));
     }
   }
-  __device__ double weight(float y) const { return exp(((double)y - top) * inv_t); }
+  template <typename F>
+  __device__ void each(F f) const {
+    vectors([&](const float* y, int id) {
+#pragma unroll
+      for (int i = 0; i < VEC; i++) f(y[i], id + i);
+    });
+  }
+
+  // w of y >= floor_, to some 2^-47: 2^(z / 32) with z = 32 log2(e) (y - m) / t as 2^(n >> 5), a root of 2 for n & 31 from
+  // a table, and the series of e^r for the rest, |r| <= ln 2 / 64 (Tang, Table-driven implementation of the exponential
+  // function, 1989).
+  __device__ double weight(float y) const {
+    const double z = ((double)y - top) * rate;
+    const double shifted = z + 0x1.8p52;
+    const int n = __double2loint(shifted);
+    const double r = (z - (shifted - 0x1.8p52)) * (0.69314718055994530942 / 32);
+    double p = fma(r, 1.0 / 120, 1.0 / 24);
+    p = fma(r, p, 1.0 / 6);
+    p = fma(r, p, 0.5);
+    p = fma(r, p, 1.0);
+    p = fma(r, p, 1.0) * sh.root[n & 31];
+    const double w = __hiloint2double(__double2hiint(p) + (n >> 5) * (1 << 20), __double2loint(p));
+    return m - y > cut_off ? 0.0 : w;
+  }
 
   // over the block, the same in all threads
   __device__ uint32_t block_max(uint32_t v) {
     v = __reduce_max_sync(0xffffffffu, v);
     if (tid % 32 == 0) sh.iscan[tid / 32] = v;
     __syncthreads();
-    for (int w = 0; w < SMP_WARPS; w++) v = max(v, sh.iscan[w]);
+    v = __reduce_max_sync(0xffffffffu, sh.iscan[tid % SMP_WARPS]);
     __syncthreads();
+    return v;
+  }
+  __device__ uint32_t block_sum(uint32_t v) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    if (tid % 32 == 0) sh.iscan[tid / 32] = v;
+    __syncthreads();
+    v = __reduce_add_sync(0xffffffffu, tid % 32 < SMP_WARPS ? sh.iscan[tid % SMP_WARPS] : 0u);
+    __syncthreads();
+    return v;
+  }
+  __device__ static double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }
   // sum of what the threads ahead have
@@ -163,25 +222,24 @@ struct SmpRow {
     }
     if (tid % 32 == 31) sh.scan[tid / 32] = incl;
     __syncthreads();
-    double before = incl - v;
+    const double before = incl - v;
     double ahead = 0;
     for (int w = 0; w < tid / 32; w++) ahead += sh.scan[w];
     __syncthreads();
     return ahead + before;
   }
 
-  // ---- the row, its largest value; each thread's own largest stays in `own`
+  // ---- the row, its largest value (NaN if there is one); each thread's own largest stays in `own`
   __device__ uint32_t load(uint32_t& own) {
     float best = -INFINITY;
-    bool nan = false;
-    constexpr int FLY = 8;
+    constexpr int FLY = 5;
     for (int b = tid; b < nv; b += FLY * SMP_THREADS) {
       uint4 u[FLY];
 #pragma unroll
       for (int j = 0; j < FLY; j++) {
         const int v = b + j * SMP_THREADS;
-        u[j] = v < nv ? row_vec(x, first_id(v), a.vocab) : make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
-        if (v >= nv && sizeof(In) == 4) u[j] = make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
+        const uint32_t none = sizeof(In) == 4 ? 0xFF800000u : 0xFF80FF80u;
+        u[j] = v < nv ? row_vec(x, first_id(v), a.vocab) : make_uint4(none, none, none, none);
       }
 #pragma unroll
       for (int j = 0; j < FLY; j++) {
@@ -190,13 +248,10 @@ struct SmpRow {
         float y[VEC];
         vec_values<In>(u[j], y);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-          nan |= y[i] != y[i];
-          best = fmaxf(best, y[i]);
-        }
+        for (int i = 0; i < VEC; i++) best = max_nan(best, y[i]);
       }
     }
-    own = rank_bits(nan ? NAN : best);
+    own = rank_bits(best);
     const uint32_t* all = tell(block_max(own));
     uint32_t r = 0;
     for (int p = 0; p < parts; p++) r = max(r, all[p]);
@@ -211,7 +266,7 @@ struct SmpRow {
       if (y >= from) {
         if (*(volatile uint32_t*)&sh.n > SMP_LIST) return;  // too many already
         const uint32_t n = atomicAdd(&sh.n, 1);
-        if (n < SMP_LIST) order()[n] = place(rank_bits(y), (uint32_t)id);
+        if (n < SMP_LIST) own_list()[n] = place(rank_bits(y), (uint32_t)id);
       }
     });
     __syncthreads();
@@ -221,25 +276,31 @@ struct SmpRow {
     return n;
   }
 
-  // ---- by the first block: list()[0, n) in order; a sum before each pair of tokens of this thread, their weights
-  __device__ void put_in_order(int n, double w[2], double& before) {
+  // ---- by the first block: list()[0, n) in order, largest first (bitonic; what is missing to a power of two as 0)
+  __device__ void put_in_order(int n) {
+    int size = 2;
+    while (size < n) size *= 2;
+    uint64_t* l = list();
     __syncthreads();
-    uint64_t mine[2];
-    int ahead[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 2; j++) mine[j] = tid + j * SMP_THREADS < n ? list()[tid + j * SMP_THREADS] : ~0ull;
-#pragma unroll 4
-    for (int i = 0; i < n; i++) {
-      const uint64_t p = list()[i];
-      ahead[0] += p > mine[0], ahead[1] += p > mine[1];
-    }
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-      if (tid + j * SMP_THREADS < n) order()[ahead[j]] = mine[j];
+    for (int i = n + tid; i < size; i += SMP_THREADS) l[i] = 0;
     __syncthreads();
+    for (int k = 2; k <= size; k *= 2)
+      for (int j = k / 2; j; j /= 2) {
+        // within 64 places a warp has them to itself
+        if (j >= 32) __syncthreads();
+        else __syncwarp();
+        if (2 * tid < size) {
+          const int i = 2 * (tid & ~(j - 1)) + (tid & (j - 1));
+          const uint64_t p = l[i], q = l[i + j];
+          if ((p < q) == ((i & k) == 0)) l[i] = q, l[i + j] = p;
+        }
+      }
+    __syncthreads();
+  }
+  // weights of this thread's two tokens of the list
+  __device__ void weights(int n, double w[2]) const {
 #pragma unroll
-    for (int j = 0; j < 2; j++) w[j] = 2 * tid + j < n ? weight(rank_value((uint32_t)(order()[2 * tid + j] >> 32))) : 0.0;
-    before = scan_mass(w[0] + w[1]);
+    for (int j = 0; j < 2; j++) w[j] = 2 * tid + j < n ? weight(rank_value((uint32_t)(list()[2 * tid + j] >> 32))) : 0.0;
   }
 
   __device__ void answer(int id, double logprob, uint32_t kept) const {
@@ -254,73 +315,261 @@ struct SmpRow {
 
   // ---- all that can be kept is in list(): by the first block
   __device__ void finish(int n, int k, float p, double u) {
-    double w[2], before;
-    if (k) {
-      put_in_order(n, w, before);
-      n = min(n, k);
-      if (2 * tid >= n) w[0] = 0.0;
-      if (2 * tid + 1 >= n) w[1] = 0.0;
-      before = scan_mass(w[0] + w[1]);
-    } else {
-      put_in_order(n, w, before);
-    }
-    const double c0 = before + w[0], c1 = c0 + w[1];
-    __shared__ double sums[SMP_LIST];
+    put_in_order(n);
+    if (k) n = min(n, k);
+    double w[2];
+    weights(n, w);
+    const double before = scan_mass(w[0] + w[1]), c0 = before + w[0], c1 = c0 + w[1];
+    double* sums = along();
     sums[2 * tid] = c0, sums[2 * tid + 1] = c1;
     __syncthreads();
     const double mass = sums[n - 1];
     uint32_t kept = n;
     if (p < 1.f) {
       const double goal = (double)p * mass;
-      uint32_t some;
-      scan_count((2 * tid < n && before < goal) + (2 * tid + 1 < n && c0 < goal), &some);
-      kept = max(some, 1u);
+      kept = max(block_sum((2 * tid < n && before < goal) + (2 * tid + 1 < n && c0 < goal)), 1u);
     }
     const double m_kept = sums[kept - 1], goal = u * m_kept;
-    uint32_t pick, heavy;
-    scan_count((2 * tid < kept && c0 <= goal) + (2 * tid + 1 < kept && c1 <= goal), &pick);
-    scan_count((2 * tid < kept && w[0] > 0.0) + (2 * tid + 1 < kept && w[1] > 0.0), &heavy);
+    uint32_t pick = block_sum((2 * tid < kept && c0 <= goal) + (2 * tid + 1 < kept && c1 <= goal));
+    const uint32_t heavy = block_sum((2 * tid < kept && w[0] > 0.0) + (2 * tid + 1 < kept && w[1] > 0.0));
     pick = min(pick, heavy - 1);  // the first one weighs 1
-    if (tid == 0) answer((int)~(uint32_t)order()[pick], logprob(order()[pick], m_kept), kept);
+    if (tid == 0) answer((int)~(uint32_t)list()[pick], logprob(list()[pick], m_kept), kept);
   }
 
-  // ---- sums over bins of the tokens with ranks lo .. hi, in every block
-  template <typename Bin>
-  __device__ void bins(SmpSums& to, uint32_t lo, uint32_t hi, Bin bin) {
-    double* mass = masses() + tid;
-    uint16_t* count = counts() + tid;
-#pragma unroll
-    for (int b = 0; b < SMP_BINS; b++) mass[b * SMP_THREADS] = 0.0, count[b * SMP_THREADS] = 0;
+  // ---- how the line grows along the bins: along()[b] is the sum (or count) up to and with bin b, to near_
+  __device__ float distance(float y) const { return fminf(m - y, FLT_MAX) * inv_bin; }
+  __device__ static int bin_of(float d) { return min(SMP_BINS - 1, (int)d); }
+  __device__ void measure(bool counts) {
+    uint32_t* h = hist(hists++ & 1);
+    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) h[i] = 0;
+    __syncthreads();
     each([&](float y, int) {
-      if (rank_bits(y) - lo <= hi - lo) {
-        const int b = bin(y) * SMP_THREADS;
-        mass[b] += weight(y);
-        count[b]++;
+      if (y < floor_) return;
+      const float d = distance(y);
+      const int b = bin_of(d);
+      if (counts) {
+        atomicAdd(h + b, 1u);
+      } else if (d < SMP_BINS - 1) {
+        // e^-r for the way r into the bin, r < 24 / 1024: the series' next term is under 2^-18
+        const float r = (d - (float)b) * (SMP_SPAN / SMP_BINS);
+        atomicAdd(h + b, (uint32_t)(unit - unit * (r - 0.5f * r * r) + 0.5f));
       }
     });
-    __syncthreads();
-    // 16 threads a bin
-    const int b = tid / 16, i = tid % 16;
-    double s = 0.0;
-    uint32_t n = 0;
-    for (int j = i; j < SMP_THREADS; j += 16) s += masses()[b * SMP_THREADS + j], n += counts()[b * SMP_THREADS + j];
+    all_sync();
+    double mass[2];
+    uint32_t n[2];
 #pragma unroll
-    for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), n += __shfl_xor_sync(0xffffffffu, n, o);
+    for (int j = 0; j < 2; j++) {
+      const int b = 2 * tid + j;
+      uint64_t s = 0;
+      for (int p = 0; p < parts; p++) s += at(h, p)[b];
+      n[j] = (uint32_t)s;
+      mass[j] = counts ? 0.0 : (double)s / unit * exp(-(double)b * (SMP_SPAN / SMP_BINS));
+    }
+    double before;
+    if (counts) {
+      uint32_t all;
+      before = scan_count(n[0] + n[1], &all);
+      mass[0] = n[0], mass[1] = n[1];
+    } else {
+      before = scan_mass(mass[0] + mass[1]);
+    }
+    along()[2 * tid] = before + mass[0];
+    along()[2 * tid + 1] = before + mass[0] + mass[1];
+    __syncthreads();
+  }
+  // Most that the tokens of the last bin, which was not measured, can weigh.
+  __device__ double tail() const { return (double)a.vocab * exp(-(double)SMP_SPAN * (SMP_BINS - 1) / SMP_BINS); }
+
+  // ---- exact sums and counts of all tokens (all: else only the counts), of those ahead of bin b0, and the tokens of bins b0
+  // .. b1 into the first block's list, as far as there is room
+  __device__ SmpExact exactly(bool all, int b0, int b1, uint32_t& before) {
+    if (tid == 0) sh.n = 0;
+    all_sync();  // the first block's list is free, its count 0
+    double s_all = 0.0, s_ahead = 0.0;
+    uint32_t n_all = 0, n_ahead = 0, n = 0;
+    uint32_t* count = at(&sh.n, 0);
+    uint64_t* to = at(list(), 0);
+    vectors([&](const float* y, int id) {
+      int b[VEC];
+      bool ahead = false, here = false;
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        b[i] = y[i] >= floor_ ? bin_of(distance(y[i])) : SMP_BINS;
+        n_all += b[i] < SMP_BINS;
+        n_ahead += b[i] < b0;
+        ahead |= b[i] < b0;
+        here |= b[i] >= b0 && b[i] <= b1;
+      }
+      if (all || ahead) {
+        double w[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) w[i] = weight(y[i]);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          if (all) s_all += b[i] < SMP_BINS ? w[i] : 0.0;
+          if (b[i] < b0) s_ahead += w[i];
+        }
+      }
+      if (here) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++)
+          if (b[i] >= b0 && b[i] <= b1) {
+            n++;
+            const uint32_t k = atomicAdd(count, 1u);
+            if (k < SMP_LIST) to[k] = place(rank_bits(y[i]), (uint32_t)(id + i));
+          }
+      }
+    });
+    s_all = warp_sum(s_all), s_ahead = warp_sum(s_ahead);
+    if (tid % 32 == 0) sh.scan[tid / 32] = s_all, sh.scan2[tid / 32] = s_ahead;
+    n_all = block_sum(n_all), n_ahead = block_sum(n_ahead), n = block_sum(n);  // (and a barrier)
+    SmpExact* e = sh.exact[turn++ & 1];
+    if (tid < parts) {
+      SmpExact mine = {0.0, 0.0, n_all, n_ahead, n};
+      for (int w = 0; w < SMP_WARPS; w++) mine.all += sh.scan[w], mine.ahead += sh.scan2[w];
+      *at(e + part, tid) = mine;
+    }
+    all_sync();
+    SmpExact r = {0.0, 0.0, 0, 0, 0};
+    before = 0;
+    for (int p = 0; p < parts; p++) {
+      r.all += e[p].all, r.ahead += e[p].ahead;
+      if (p < part) before += e[p].n;
+      r.n_all += e[p].n_all, r.n_ahead += e[p].n_ahead, r.n += e[p].n;
+    }
+    return r;
+  }
+
+  __device__ static bool crosses(SmpKind kind, double mass, uint32_t count, double goal) {
+    return kind == SMP_COUNT ? (double)count >= goal : kind == SMP_REACH ? mass >= goal : mass > goal;
+  }
+
+  // ---- the token at which the count or the sum crosses `goal`; before the sum of all tokens is known, share of it.  all:
+  // gets that sum, and the number of tokens
+  __device__ SmpFound search(SmpKind kind, double goal, double share, double* all, uint32_t* n_all) {
+    double from = goal, to = goal;
+    const double last = along()[SMP_BINS - 1];
+    if (all) from = share * last * (1 - near_), to = share * (last * (1 + near_) + tail());
+    const double e = kind == SMP_COUNT ? 0.0 : near_;
+    if (tid == 0) sh.lo = sh.hi = SMP_BINS - 1;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int b = 2 * tid + j;
+      const double y = along()[b], prev = b ? along()[b - 1] : 0.0;
+      // the first bin with which the number may be crossed, and the first with which it surely is
+      if (b < SMP_BINS - 1 && y * (1 + e) >= from && !(b && prev * (1 + e) >= from)) sh.lo = b;
+      if (b < SMP_BINS - 1 && (kind == SMP_COUNT ? y >= to : y * (1 - e) > to) &&
+          !(b && (kind == SMP_COUNT ? prev >= to : prev * (1 - e) > to)))
+        sh.hi = b;
+    }
+    __syncthreads();
+    const int b0 = (int)sh.lo, b1 = (int)sh.hi;
+    SmpWindow w;
+    const SmpExact r = exactly(all != nullptr, b0, b1, w.before);
+    if (all) *all = r.all, *n_all = r.n_all, goal = share * r.all;
+    w.mass = r.ahead, w.ahead = r.n_ahead, w.count = r.n;
+    if (w.count <= SMP_LIST) return among(kind, goal, w);
+    // the ranks of these bins, which are monotone in the value
+    const uint32_t least = rank_bits(floor_), most = rank_bits(m);
+    uint32_t lo = least, hi = most;
+    while (lo < hi) {  // smallest rank whose bin is b1 or an earlier one
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (bin_of(distance(rank_value(mid))) <= b1) hi = mid;
+      else lo = mid + 1;
+    }
+    w.lo = lo;
+    hi = most;
+    while (lo < hi) {  // largest whose bin is b0 or a later one
+      const uint32_t mid = hi - (hi - lo) / 2;
+      if (bin_of(distance(rank_value(mid))) >= b0) lo = mid;
+      else hi = mid - 1;
+    }
+    w.hi = lo;
+    return closer(kind, goal, w);
+  }
+
+  // ---- the window's tokens are in the first block's list
+  __device__ SmpFound among(SmpKind kind, double goal, const SmpWindow& w) {
+    if (part == 0) {
+      put_in_order((int)w.count);
+      double wt[2];
+      weights((int)w.count, wt);
+      const double before = scan_mass(wt[0] + wt[1]);
+      const double c0 = w.mass + (before + wt[0]), c1 = w.mass + (before + wt[0] + wt[1]);
+      const uint32_t i0 = 2 * tid, i1 = i0 + 1, n = w.count;
+      uint32_t ahead = block_sum((i0 < n && !crosses(kind, c0, w.ahead + i0 + 1, goal)) +
+                                 (i1 < n && !crosses(kind, c1, w.ahead + i1 + 1, goal)));
+      ahead = min(ahead, n - 1);
+      if (ahead / 2 == tid) {
+        const SmpFound f = {list()[ahead], ahead % 2 ? c1 : c0, w.ahead + ahead + 1};
+        for (int p = 0; p < parts; p++) *at(&sh.found, p) = f;
+      }
+    }
+    all_sync();
+    return sh.found;
+  }
+
+  // ---- a window of many tokens: exact sums over 16 bins of its ranks, the one with the crossing becomes the window
+  __device__ SmpFound closer(SmpKind kind, double goal, SmpWindow w) {
+    while (true) {
+      all_sync();  // what was found, or listed, before has been read
+      if (w.count <= SMP_LIST) {
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        uint64_t* to = at(list(), 0);
+        each([&](float y, int id) {
+          const uint32_t r = rank_bits(y);
+          if (r - w.lo <= w.hi - w.lo) to[w.before + atomicAdd(&sh.n, 1)] = place(r, (uint32_t)id);
+        });
+        all_sync();
+        return among(kind, goal, w);
+      }
+      if (w.lo == w.hi) return tied(kind, goal, w);
+      const uint32_t range = w.hi - w.lo, hi = w.hi, shift = max(0, 28 - __clz(range));
+      SmpSums& s = sh.next[turn++ & 1];
+      cut(s, w.lo, w.hi, shift);
+      const int b = choose(s, kind, goal, w);
+      w.hi = hi - ((uint32_t)b << shift);
+      const uint64_t below = ((uint64_t)(b + 1) << shift) - 1;
+      w.lo = below < hi - w.lo ? hi - (uint32_t)below : w.lo;
+    }
+  }
+  __device__ void cut(SmpSums& to, uint32_t lo, uint32_t hi, uint32_t shift) {
+    if (tid < SMP_CUTTERS) {
+      double* mass = cut_mass() + tid;
+      uint32_t* count = cut_count() + tid;
+#pragma unroll
+      for (int b = 0; b < SMP_CUT; b++) mass[b * SMP_CUTTERS] = 0.0, count[b * SMP_CUTTERS] = 0;
+      vectors([&](const float* y, int) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          const uint32_t r = rank_bits(y[i]);
+          if (r - lo > hi - lo) continue;
+          const int b = (int)((hi - r) >> shift) * SMP_CUTTERS;
+          mass[b] += weight(y[i]);
+          count[b]++;
+        }
+      }, SMP_CUTTERS);
+    }
+    __syncthreads();
+    // 32 threads a bin
+    const int b = tid / 32, i = tid % 32;
+    double s = cut_mass()[b * SMP_CUTTERS + i] + cut_mass()[b * SMP_CUTTERS + 32 + i];
+    const uint32_t n = __reduce_add_sync(0xffffffffu, cut_count()[b * SMP_CUTTERS + i] + cut_count()[b * SMP_CUTTERS + 32 + i]);
+    s = warp_sum(s);
     if (i < parts) {
       *at(&to.mass[part][b], i) = s;
       *at(&to.count[part][b], i) = n;
     }
     all_sync();
   }
-
-  __device__ static bool crosses(SmpKind kind, double mass, uint32_t count, double goal) {
-    return kind == SMP_COUNT ? (double)count >= goal : kind == SMP_REACH ? mass >= goal : mass > goal;
-  }
   // the bin of the window in which the number is crossed (rounding: else the last with a token), into w; its number
   __device__ int choose(const SmpSums& s, SmpKind kind, double goal, SmpWindow& w) const {
     int last = 0;
     SmpWindow at = w, hit = w;
-    for (int b = 0; b < SMP_BINS; b++) {
+    for (int b = 0; b < SMP_CUT; b++) {
       double mass = 0.0;
       uint32_t n = 0, before = 0;
       for (int p = 0; p < parts; p++) {
@@ -340,104 +589,41 @@ struct SmpRow {
     w.mass = hit.mass, w.ahead = hit.ahead, w.count = hit.count, w.before = hit.before;
     return last;
   }
-  __device__ int first_bin(float y) const { return min(SMP_BINS - 1, (int)((m - y) * inv_bin)); }
-
-  // ---- the token at which the count or the sum crosses `goal`
-  __device__ SmpFound search(SmpKind kind, double goal) {
-    SmpWindow w;
-    w.mass = 0.0;
-    w.ahead = 0;
-    const int b1 = choose(sh.first, kind, goal, w);
-    {
-      // the ranks of this bin: the bins are monotone in the value
-      const uint32_t least = rank_bits(floor_), most = rank_bits(m);
-      uint32_t lo = least, hi = most;
-      while (lo < hi) {  // smallest rank whose bin is b1 or an earlier one
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (first_bin(rank_value(mid)) <= b1) hi = mid;
-        else lo = mid + 1;
-      }
-      w.lo = lo;
-      hi = most;
-      while (lo < hi) {  // largest whose bin is b1
-        const uint32_t mid = hi - (hi - lo) / 2;
-        if (first_bin(rank_value(mid)) >= b1) lo = mid;
-        else hi = mid - 1;
-      }
-      w.hi = lo;
+  // ---- many tokens of one value: the id decides
+  __device__ SmpFound tied(SmpKind kind, double goal, const SmpWindow& w) {
+    const float y = rank_value(w.lo);
+    const double wt = weight(y);
+    double j;
+    if (kind == SMP_COUNT) {
+      j = goal - w.ahead;
+    } else {
+      j = wt > 0.0 ? floor((goal - w.mass) / wt) : 0.0;
+      j = fmin(fmax(j, 1.0), (double)w.count);
+      for (int i = 0; i < 4 && j > 1.0 && crosses(kind, w.mass + (j - 1.0) * wt, 0, goal); i++) j -= 1.0;
+      for (int i = 0; i < 4 && j < (double)w.count && !crosses(kind, w.mass + j * wt, 0, goal); i++) j += 1.0;
     }
-    for (uint32_t round = 0;; round++) {
-      if (w.count <= SMP_LIST) {
-        __syncthreads();
-        if (tid == 0) sh.n = 0;
-        all_sync();  // the first block is done with its bins
-        uint64_t* to = at(list(), 0);
-        each([&](float y, int id) {
-          const uint32_t r = rank_bits(y);
-          if (r - w.lo <= w.hi - w.lo) to[w.before + atomicAdd(&sh.n, 1)] = place(r, (uint32_t)id);
-        });
-        all_sync();
-        if (part == 0) {
-          double wt[2], before;
-          put_in_order((int)w.count, wt, before);
-          const double c0 = w.mass + (before + wt[0]), c1 = w.mass + (before + wt[0] + wt[1]);
-          const uint32_t i0 = 2 * tid, i1 = i0 + 1, n = w.count;
-          uint32_t ahead;
-          scan_count((i0 < n && !crosses(kind, c0, w.ahead + i0 + 1, goal)) + (i1 < n && !crosses(kind, c1, w.ahead + i1 + 1, goal)),
-                     &ahead);
-          ahead = min(ahead, n - 1);
-          if (ahead / 2 == tid) {
-            const SmpFound f = {order()[ahead], ahead % 2 ? c1 : c0, w.ahead + ahead + 1};
+    const uint32_t nth = (uint32_t)fmin(fmax(j, 1.0), (double)w.count);  // from 1
+    uint32_t seen = w.before;
+    for (int b = 0; b < nv && seen < nth; b += SMP_THREADS) {
+      float v[VEC];
+      const bool has = b + tid < nv;
+      if (has) vec_values<In>(vec(b + tid), v);
+      uint32_t here = 0, total;
+#pragma unroll
+      for (int i = 0; i < VEC; i++) here += has && v[i] == y;
+      uint32_t before = seen + scan_count(here, &total);
+      if (has && before < nth && nth <= before + here) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++)
+          if (v[i] == y && ++before == nth) {
+            const SmpFound f = {place(w.lo, (uint32_t)(first_id(b + tid) + i)), w.mass + nth * wt, w.ahead + nth};
             for (int p = 0; p < parts; p++) *at(&sh.found, p) = f;
           }
-        }
-        all_sync();
-        return sh.found;
       }
-      if (w.lo == w.hi) {  // one value: the id decides
-        all_sync();        // an earlier answer has been read
-        const float y = rank_value(w.lo);
-        const double wt = weight(y);
-        double j;
-        if (kind == SMP_COUNT) {
-          j = goal - w.ahead;
-        } else {
-          j = wt > 0.0 ? floor((goal - w.mass) / wt) : 0.0;
-          j = fmin(fmax(j, 1.0), (double)w.count);
-          for (int i = 0; i < 4 && j > 1.0 && crosses(kind, w.mass + (j - 1.0) * wt, 0, goal); i++) j -= 1.0;
-          for (int i = 0; i < 4 && j < (double)w.count && !crosses(kind, w.mass + j * wt, 0, goal); i++) j += 1.0;
-        }
-        const uint32_t nth = (uint32_t)fmin(fmax(j, 1.0), (double)w.count);  // from 1
-        uint32_t seen = w.before;
-        for (int b = 0; b < nv && seen < nth; b += SMP_THREADS) {
-          float v[VEC];
-          const bool has = b + tid < nv;
-          if (has) vec_values<In>(vec(b + tid), v);
-          uint32_t here = 0, total;
-#pragma unroll
-          for (int i = 0; i < VEC; i++) here += has && v[i] == y;
-          uint32_t before = seen + scan_count(here, &total);
-          if (has && before < nth && nth <= before + here) {
-#pragma unroll
-            for (int i = 0; i < VEC; i++)
-              if (v[i] == y && ++before == nth) {
-                const SmpFound f = {place(w.lo, (uint32_t)(first_id(b + tid) + i)), w.mass + nth * wt, w.ahead + nth};
-                for (int p = 0; p < parts; p++) *at(&sh.found, p) = f;
-              }
-          }
-          seen += total;
-        }
-        all_sync();
-        return sh.found;
-      }
-      const uint32_t range = w.hi - w.lo, hi = w.hi, shift = max(0, 28 - __clz(range));
-      SmpSums& s = sh.next[turn++ & 1];
-      bins(s, w.lo, w.hi, [&](float y) { return (int)((hi - rank_bits(y)) >> shift); });
-      const int b = choose(s, kind, goal, w);
-      w.hi = hi - ((uint32_t)b << shift);
-      const uint64_t below = ((uint64_t)(b + 1) << shift) - 1;
-      w.lo = below < hi - w.lo ? hi - (uint32_t)below : w.lo;
+      seen += total;
     }
+    all_sync();
+    return sh.found;
   }
 
   __device__ void run() {
@@ -448,6 +634,7 @@ struct SmpRow {
     if (k < 0 || k >= a.vocab) k = 0;
     double u = a.uniform[row];
     u = u > 0.0 ? fmin(u, 0x1.fffffffffffffp-1) : 0.0;
+    if (tid < 32) sh.root[tid] = exp2(tid / 32.0);
     uint32_t own;
     const uint32_t most = load(own);
     m = rank_value(most);
@@ -469,19 +656,20 @@ struct SmpRow {
     }
     top = m;
     inv_t = 1.0 / (double)t;
+    rate = inv_t * (32 * 1.44269504088896340736);
+    cut_off = 620.f * t;
     floor_ = -FLT_MAX;
     if (min_p >= 1.f) floor_ = m;
     else if (min_p > 0.f) floor_ = fmaxf(floor_, __double2float_ru(top + (double)t * log((double)min_p)));
     if ((k && k <= SMP_TOP) || min_p > 0.f) {
       float from = floor_;
-      const int each_k = (k + parts - 1) / parts;
       if (k && k <= SMP_TOP) {
-        // a value that each_k of this block's tokens reach, 0 if there are not so many threads with one
-        owns()[tid] = own;
-        __syncthreads();
-        int ahead = 0;
-        for (int i = 0; i < SMP_THREADS; i++) ahead += owns()[i] > own || (owns()[i] == own && i < tid);
-        const uint32_t* all = tell(block_max(ahead >= each_k - 1 ? own : 0u));
+        // a value that this block's share of k tokens reaches, to 20 bits; 0 if there are not so many threads with one
+        const int share = (k + parts - 1) / parts;
+        uint32_t reach = 0;
+        for (int bit = 31; bit >= 12; bit--)
+          if (__syncthreads_count(own >= (reach | 1u << bit)) >= share) reach |= 1u << bit;
+        const uint32_t* all = tell(reach);
         uint32_t least = 0xFFFFFFFFu;
         for (int q = 0; q < parts; q++) least = min(least, all[q]);
         from = fmaxf(from, rank_value(max(least, rank_bits(-FLT_MAX))));
@@ -491,36 +679,40 @@ struct SmpRow {
       if (n <= SMP_LIST) {
         uint32_t before = 0;
         for (int q = 0; q < part; q++) before += all[q];
-        for (uint32_t i = tid; i < all[part]; i += SMP_THREADS) at(list(), 0)[before + i] = order()[i];
+        for (uint32_t i = tid; i < all[part]; i += SMP_THREADS) at(list(), 0)[before + i] = own_list()[i];
         all_sync();
         if (part == 0) finish((int)n, k, p, u);
         return;
       }
     }
-    inv_bin = SMP_BINS / (SMP_SPAN * t);
+    inv_bin = fminf(SMP_BINS / (SMP_SPAN * t), FLT_MAX);
     __syncthreads();
-    bins(sh.first, rank_bits(floor_), most, [&](float y) { return first_bin(y); });
     double mass = 0.0;
     uint32_t kept = 0;
-    for (int b = 0; b < SMP_BINS; b++)
-      for (int q = 0; q < parts; q++) mass += sh.first.mass[q][b], kept += sh.first.count[q][b];
-    uint64_t last = 0;  // the last place that is kept, where that is known
-    if (k && (uint32_t)k < kept) {
-      const SmpFound f = search(SMP_COUNT, (double)k);
-      mass = f.mass, kept = f.count, last = f.place;
+    uint64_t last = 0;      // the last place that is kept, where that is known
+    bool known = false;     // whether mass and kept are
+    if (k) {
+      measure(true);
+      if ((uint32_t)k < (uint32_t)along()[SMP_BINS - 1]) {
+        const SmpFound f = search(SMP_COUNT, (double)k, 0.0, nullptr, nullptr);
+        mass = f.mass, kept = f.count, last = f.place;
+        known = true;
+      }
     }
+    measure(false);
     if (p < 1.f) {
-      const SmpFound f = search(SMP_REACH, (double)p * mass);
+      const SmpFound f = search(SMP_REACH, (double)p * mass, (double)p, known ? nullptr : &mass, &kept);
       if (f.count < kept) mass = f.mass, kept = f.count, last = f.place;
+      known = true;
     }
-    SmpFound f = search(SMP_PASS, u * mass);
+    SmpFound f = search(SMP_PASS, u * mass, u, known ? nullptr : &mass, &kept);
     if (f.count > kept) f.place = last;  // by rounding alone
     if (part == 0 && tid == 0) answer((int)~(uint32_t)f.place, logprob(f.place, mass), kept);
   }
 };
 
 template <typename In, bool HELD>
-__global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const __grid_constant__ IrisSample a) {
+__global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_constant__ IrisSample a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ SmpShared sh;
   if (a.parts > 1) iris::cluster_sync();  // all blocks are there
