@@ -93,6 +93,8 @@ __device__ __forceinline__ uint32_t rank_bits(float x) {
 __device__ __forceinline__ float rank_value(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r & 0x7FFFFFFFu : ~r); }
 __device__ __forceinline__ uint64_t place(uint32_t rank, uint32_t id) { return (uint64_t)rank << 32 | (uint32_t)~id; }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -142,6 +144,19 @@ __device__ __forceinline__ void vec_values(uint4 u, float x[16 / sizeof(In)]) {
   } else {
     const float2 a = unpack2(u.x), b = unpack2(u.y), c = unpack2(u.z), d = unpack2(u.w);
     x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
+  }
+}
+
+// The largest of the values, NaN if one is.
+template <typename In>
+__device__ __forceinline__ float vec_max(uint4 u) {
+  if constexpr (sizeof(In) == 4) {
+    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)),
+                   max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else {
+    auto h = [](uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); };
+    const __nv_bfloat162 v = __hmax2_nan(__hmax2_nan(h(u.x), h(u.y)), __hmax2_nan(h(u.z), h(u.w)));
+    return max_nan(__low2float(v), __high2float(v));
   }
 }
 

@@ -1580,8 +1580,6 @@ struct LpShape {
   static constexpr int kBlocks = LP_LOADS / kPer;               // blocks in flight
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
-
 // Two f32 in one register pair, for the packed instructions.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t v;
@@ -1654,19 +1652,6 @@ __device__ __forceinline__ float vec_value(uint4 u, int q) {
   const uint32_t a = q & PER ? u.y : u.x, b = q & PER ? u.w : u.z, w = q & 2 * PER ? b : a;
   if constexpr (sizeof(In) == 4) return __uint_as_float(w);
   else return __uint_as_float(q & 1 ? w & 0xFFFF0000u : w << 16);
-}
-
-// The largest of the values, NaN if one is.
-template <typename In>
-__device__ __forceinline__ float vec_max(uint4 u) {
-  if constexpr (sizeof(In) == 4) {
-    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)),
-                   max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
-  } else {
-    auto h = [](uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); };
-    const __nv_bfloat162 v = __hmax2_nan(__hmax2_nan(h(u.x), h(u.y)), __hmax2_nan(h(u.z), h(u.w)));
-    return max_nan(__low2float(v), __high2float(v));
-  }
 }
 
 struct LpPlan {

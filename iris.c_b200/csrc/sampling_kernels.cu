@@ -34,9 +34,10 @@ namespace {
 constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32, SMP_PARTS = 8;
 constexpr int SMP_LIST = 1024;  // tokens put in order: two a thread
 constexpr int SMP_TOP = 512;    // largest top-k whose tokens are looked for through a bound
-constexpr int SMP_BINS = 1024;
+constexpr int SMP_BINS = 2048;  // four a thread
 constexpr float SMP_SPAN = 24.f;      // (m - x) / t that the bins cover; the last one holds all that is below
 constexpr int SMP_CUT = 16, SMP_CUTTERS = 64;  // bins of a closer look, threads that fill bins of their own
+static_assert(SMP_BINS == 4 * SMP_THREADS && SMP_LIST == 2 * SMP_THREADS && SMP_CUT == SMP_WARPS, "shares of a thread, and warp");
 
 struct SmpSums {  // of the closer bins, from each block of the cluster
   double mass[SMP_PARTS][SMP_CUT];
@@ -58,18 +59,20 @@ struct SmpShared {
   SmpSums next[2];             // in turn, so that one round's may be read while the next one's come
   SmpExact exact[2][SMP_PARTS];
   uint32_t one[2][SMP_PARTS];  // a number from each block
-  double scan[SMP_WARPS], scan2[SMP_WARPS];
+  SmpExact parts[SMP_WARPS];   // of a block's warps
+  double scan[SMP_WARPS];
+  float fscan[SMP_WARPS];
   uint32_t iscan[SMP_WARPS];
-  double root[32];             // 2^(i / 32)
+  double root[64];             // 2^(i / 64)
   SmpFound found;
   uint32_t n, lo, hi;
 };
 
-// shared memory besides the row: two histograms, the sums along the bins, and the list, in whose place the closer bins stand
-constexpr int SMP_HIST = SMP_BINS * 4, SMP_ALONG = SMP_BINS * 8;
+// shared memory besides the row: the histogram, the sums along the bins, and the list, in whose place the closer bins stand
+constexpr int SMP_HIST = SMP_BINS * 4, SMP_ALONG = SMP_BINS * 4;
 constexpr int SMP_TAIL = SMP_CUT * SMP_CUTTERS * (8 + 4);
-constexpr int SMP_WORK = 2 * SMP_HIST + SMP_ALONG + SMP_TAIL;
-static_assert(SMP_TAIL >= SMP_LIST * 8 && SMP_ALONG >= SMP_LIST * 8, "the lists fit");
+constexpr int SMP_WORK = SMP_HIST + SMP_ALONG + SMP_TAIL;
+static_assert(SMP_TAIL >= SMP_LIST * 8 && SMP_ALONG >= SMP_LIST * 8 && SMP_HIST >= SMP_LIST * 8, "the lists fit");
 
 struct SmpWindow {  // part of the line: ranks lo .. hi, `count` tokens, with sums over what stands ahead of it
   uint32_t lo, hi;
@@ -89,13 +92,12 @@ struct SmpRow {
   const In* x;
   int tid, part, parts, off, v0, nv;
   float m, floor_, cut_off;  // cut_off: what lies further under m weighs nothing, e^-620
-  double top, inv_t, rate;   // rate: 32 log2(e) / t
+  double top, inv_t, rate;   // rate: 64 log2(e) / t
   float inv_bin;
   float unit;                // of the histogram's weights, so that a block's tokens in one bin stay within 32 bits
-  double near_;              // relative error of the histogram's sums, with room to spare: half a unit of rounding, 2^-18 for the
-                             // bins' edges and 2^-19 for what the weight's series leaves out
+  float near_;               // relative error of the sums along the bins, with room to spare: half a unit of rounding, 2^-17 for
+                             // distances and bins' weights in 32 bits, 2^-20 for sums in 32 bits
   uint32_t turn = 0;
-  int hists = 0;
 
   __device__ SmpRow(const IrisSample& a, SmpShared& sh, uint8_t* smem) : a(a), sh(sh), smem(smem) {
     tid = threadIdx.x;
@@ -108,13 +110,14 @@ struct SmpRow {
     nv = max(0, min(per, all - v0));
     unit = 65536.f;
     while (unit * ((float)per * VEC) > 4.2e9f) unit *= 0.5f;
-    near_ = 1.0 / 32768 + 1.0 / unit;
+    near_ = 1.f / 32768 + 1.f / unit;
   }
   __device__ uint8_t* work() const { return smem + (HELD ? a.held_bytes : 0); }
-  __device__ uint32_t* hist(int i) const { return reinterpret_cast<uint32_t*>(work() + i * SMP_HIST); }
-  __device__ double* along() const { return reinterpret_cast<double*>(work() + 2 * SMP_HIST); }  // sums up to and with a bin
-  __device__ uint64_t* list() const { return reinterpret_cast<uint64_t*>(work() + 2 * SMP_HIST + SMP_ALONG); }
-  __device__ uint64_t* own_list() const { return reinterpret_cast<uint64_t*>(along()); }         // before there are sums
+  __device__ uint32_t* hist() const { return reinterpret_cast<uint32_t*>(work()); }
+  __device__ float* along() const { return reinterpret_cast<float*>(work() + SMP_HIST); }  // sums up to and with a bin, or counts
+  __device__ uint64_t* list() const { return reinterpret_cast<uint64_t*>(work() + SMP_HIST + SMP_ALONG); }
+  __device__ uint64_t* own_list() const { return reinterpret_cast<uint64_t*>(along()); }  // before there are sums; again for what is in order
+  __device__ double* line() const { return reinterpret_cast<double*>(hist()); }           // when there is no histogram
   __device__ double* cut_mass() const { return reinterpret_cast<double*>(list()); }
   __device__ uint32_t* cut_count() const { return reinterpret_cast<uint32_t*>(cut_mass() + SMP_CUT * SMP_CUTTERS); }
 
@@ -155,20 +158,20 @@ struct SmpRow {
     });
   }
 
-  // w of y >= floor_, to some 2^-47: 2^(z / 32) with z = 32 log2(e) (y - m) / t as 2^(n >> 5), a root of 2 for n & 31 from
-  // a table, and the series of e^r for the rest, |r| <= ln 2 / 64 (Tang, Table-driven implementation of the exponential
+  // w of y >= floor_, to some 2^-44: 2^(z / 64) with z = 64 log2(e) (y - m) / t as 2^(n >> 6), a root of 2 for n & 63 from
+  // a table, and the series of e^r for the rest, |r| <= ln 2 / 128 (Tang, Table-driven implementation of the exponential
   // function, 1989).
   __device__ double weight(float y) const {
+    constexpr double c = 0.69314718055994530942 / 64;
     const double z = ((double)y - top) * rate;
     const double shifted = z + 0x1.8p52;
     const int n = __double2loint(shifted);
-    const double r = (z - (shifted - 0x1.8p52)) * (0.69314718055994530942 / 32);
-    double p = fma(r, 1.0 / 120, 1.0 / 24);
-    p = fma(r, p, 1.0 / 6);
-    p = fma(r, p, 0.5);
-    p = fma(r, p, 1.0);
-    p = fma(r, p, 1.0) * sh.root[n & 31];
-    const double w = __hiloint2double(__double2hiint(p) + (n >> 5) * (1 << 20), __double2loint(p));
+    const double r = z - (shifted - 0x1.8p52);
+    double p = fma(r, c * c * c * c / 24, c * c * c / 6);
+    p = fma(r, p, c * c / 2);
+    p = fma(r, p, c);
+    p = fma(r, p, 1.0) * sh.root[n & 63];
+    const double w = __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p));
     return m - y > cut_off ? 0.0 : w;
   }
 
@@ -213,6 +216,20 @@ struct SmpRow {
     __syncthreads();
     return before;
   }
+  __device__ float scan_float(float v) {
+    float incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (tid % 32 >= o) incl += y;
+    }
+    if (tid % 32 == 31) sh.fscan[tid / 32] = incl;
+    __syncthreads();
+    float ahead = 0.f;
+    for (int w = 0; w < tid / 32; w++) ahead += sh.fscan[w];
+    __syncthreads();
+    return ahead + (incl - v);
+  }
   __device__ double scan_mass(double v) {
     double incl = v;
 #pragma unroll
@@ -229,10 +246,10 @@ struct SmpRow {
     return ahead + before;
   }
 
-  // ---- the row, its largest value (NaN if there is one); each thread's own largest stays in `own`
+  // ---- the row, its largest value (NaN if there is one); each thread's own largest in `own`, each warp's in sh.iscan
   __device__ uint32_t load(uint32_t& own) {
     float best = -INFINITY;
-    constexpr int FLY = 5;
+    constexpr int FLY = 10;  // 76 KB of a row in one round
     for (int b = tid; b < nv; b += FLY * SMP_THREADS) {
       uint4 u[FLY];
 #pragma unroll
@@ -245,29 +262,53 @@ struct SmpRow {
       for (int j = 0; j < FLY; j++) {
         const int v = b + j * SMP_THREADS;
         if (HELD && v < nv) reinterpret_cast<uint4*>(smem)[v] = u[j];
-        float y[VEC];
-        vec_values<In>(u[j], y);
-#pragma unroll
-        for (int i = 0; i < VEC; i++) best = max_nan(best, y[i]);
+        best = max_nan(best, vec_max<In>(u[j]));
       }
     }
+    if (tid >= SMP_THREADS - 64) sh.root[tid & 63] = exp2((tid & 63) / 64.0);
     own = rank_bits(best);
-    const uint32_t* all = tell(block_max(own));
+    const uint32_t w = __reduce_max_sync(0xffffffffu, own);
+    if (tid % 32 == 0) sh.iscan[tid / 32] = w;
+    __syncthreads();
+    const uint32_t* all = tell(__reduce_max_sync(0xffffffffu, sh.iscan[tid % SMP_WARPS]));
     uint32_t r = 0;
     for (int p = 0; p < parts; p++) r = max(r, all[p]);
     return r;
+  }
+
+  // ---- a value that `share` of this block's tokens reach, 0 if it may have fewer; sh.iscan as load() leaves it
+  __device__ uint32_t reached(int share, uint32_t own) {
+    if (share <= SMP_WARPS / 2) {  // by the warps' largest
+      const uint32_t mine = sh.iscan[tid % SMP_WARPS];
+      int ahead = 0;
+#pragma unroll
+      for (int i = 0; i < SMP_WARPS; i++) {
+        const uint32_t o = __shfl_sync(0xffffffffu, mine, i);
+        ahead += o > mine || (o == mine && i < tid % SMP_WARPS);
+      }
+      return __reduce_max_sync(0xffffffffu, ahead == share - 1 ? mine : 0u);
+    }
+    uint32_t reach = 0;  // by the threads', to 20 bits
+    for (int bit = 31; bit >= 12; bit--)
+      if (__syncthreads_count(own >= (reach | 1u << bit)) >= share) reach |= 1u << bit;
+    return reach;
   }
 
   // ---- the tokens from `from` on, each block's in its own list; how many there are in the whole row (each block's in `all`)
   __device__ uint32_t gather(float from, const uint32_t*& all) {
     if (tid == 0) sh.n = 0;
     __syncthreads();
-    each([&](float y, int id) {
-      if (y >= from) {
-        if (*(volatile uint32_t*)&sh.n > SMP_LIST) return;  // too many already
-        const uint32_t n = atomicAdd(&sh.n, 1);
-        if (n < SMP_LIST) own_list()[n] = place(rank_bits(y), (uint32_t)id);
-      }
+    vectors([&](const float* y, int id) {
+      float most = y[0];
+#pragma unroll
+      for (int i = 1; i < VEC; i++) most = fmaxf(most, y[i]);
+      if (most < from || *(volatile uint32_t*)&sh.n > SMP_LIST) return;  // none, or too many already
+#pragma unroll
+      for (int i = 0; i < VEC; i++)
+        if (y[i] >= from) {
+          const uint32_t n = atomicAdd(&sh.n, 1);
+          if (n < SMP_LIST) own_list()[n] = place(rank_bits(y[i]), (uint32_t)(id + i));
+        }
     });
     __syncthreads();
     all = tell(sh.n);
@@ -276,12 +317,27 @@ struct SmpRow {
     return n;
   }
 
-  // ---- by the first block: list()[0, n) in order, largest first (bitonic; what is missing to a power of two as 0)
+  // ---- by the first block: list()[0, n) in order, largest first.  Few by counting how many are ahead of each, all threads
+  // at it (n^2 steps); more by a bitonic sort, with what is missing to a power of two as 0.
   __device__ void put_in_order(int n) {
-    int size = 2;
-    while (size < n) size *= 2;
     uint64_t* l = list();
     __syncthreads();
+    if (n <= 256) {
+      int per = 2;  // threads to a token
+      while (per < 32 && 2 * per * n <= SMP_THREADS) per *= 2;
+      const int i = tid / per;
+      const uint64_t mine = i < n ? l[i] : 0;
+      int ahead = 0;
+#pragma unroll 4
+      for (int j = tid % per; j < n; j += per) ahead += l[j] > mine;
+      for (int o = per / 2; o; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+      __syncthreads();
+      if (i < n && tid % per == 0) l[ahead] = mine;
+      __syncthreads();
+      return;
+    }
+    int size = 512;
+    while (size < n) size *= 2;
     for (int i = n + tid; i < size; i += SMP_THREADS) l[i] = 0;
     __syncthreads();
     for (int k = 2; k <= size; k *= 2)
@@ -320,7 +376,7 @@ struct SmpRow {
     double w[2];
     weights(n, w);
     const double before = scan_mass(w[0] + w[1]), c0 = before + w[0], c1 = c0 + w[1];
-    double* sums = along();
+    double* sums = line();
     sums[2 * tid] = c0, sums[2 * tid + 1] = c1;
     __syncthreads();
     const double mass = sums[n - 1];
@@ -336,107 +392,122 @@ struct SmpRow {
     if (tid == 0) answer((int)~(uint32_t)list()[pick], logprob(list()[pick], m_kept), kept);
   }
 
-  // ---- how the line grows along the bins: along()[b] is the sum (or count) up to and with bin b, to near_
-  __device__ float distance(float y) const { return fminf(m - y, FLT_MAX) * inv_bin; }
-  __device__ static int bin_of(float d) { return min(SMP_BINS - 1, (int)d); }
-  __device__ void measure(bool counts) {
-    uint32_t* h = hist(hists++ & 1);
+  // ---- how the line grows along the bins: along()[b] is the sum up to and with bin b, to near_ (or the count, a whole number)
+  __device__ float distance(float y) const { return fminf(fminf(m - y, FLT_MAX) * inv_bin, SMP_BINS - 1); }
+  __device__ static float nearest(float d) { return (d + 0x1.8p23f) - 0x1.8p23f; }  // whole number, ties to even
+  __device__ float bin_of(float y) const { return nearest(distance(y)); }           // the bins are around whole numbers
+  template <bool COUNTS>
+  __device__ void measure() {
+    uint32_t* h = hist();
     for (int i = tid; i < SMP_BINS; i += SMP_THREADS) h[i] = 0;
     __syncthreads();
-    each([&](float y, int) {
-      if (y < floor_) return;
-      const float d = distance(y);
-      const int b = bin_of(d);
-      if (counts) {
-        atomicAdd(h + b, 1u);
-      } else if (d < SMP_BINS - 1) {
-        // e^-r for the way r into the bin, r < 24 / 1024: the series' next term is under 2^-18
-        const float r = (d - (float)b) * (SMP_SPAN / SMP_BINS);
-        atomicAdd(h + b, (uint32_t)(unit - unit * (r - 0.5f * r * r) + 0.5f));
+    vectors([&](const float* y, int) {
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        const float d = distance(y[i]), b = nearest(d);
+        const int at = __float_as_int(d + 0x1.8p23f) & (SMP_BINS - 1);
+        if (COUNTS) {
+          if (y[i] >= floor_) atomicAdd(h + at, 1u);
+        } else {
+          // unit e^-r for the way r behind the bin's middle, |r| <= 12 / 2048 (the series' next term is under 2^-24), as a
+          // whole number
+          const float r = (d - b) * (SMP_SPAN / SMP_BINS);
+          const float w = fmaf(unit, r * fmaf(0.5f, r, -1.f), unit + 0x1p23f);
+          if (y[i] >= floor_ && b < SMP_BINS - 1) atomicAdd(h + at, __float_as_uint(w) - 0x4B000000u);
+        }
       }
     });
     all_sync();
-    double mass[2];
-    uint32_t n[2];
+    float mass[4];
+    uint32_t n[4] = {0, 0, 0, 0};
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < parts; p++) {
+      const uint4 u = *reinterpret_cast<const uint4*>(at(h, p) + 4 * tid);
+      if (COUNTS) n[0] += u.x, n[1] += u.y, n[2] += u.z, n[3] += u.w;
+      else s[0] += (float)u.x, s[1] += (float)u.y, s[2] += (float)u.z, s[3] += (float)u.w;
+    }
+    if (COUNTS) {
+      uint32_t all, before = scan_count(n[0] + n[1] + n[2] + n[3], &all);
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int b = 2 * tid + j;
-      uint64_t s = 0;
-      for (int p = 0; p < parts; p++) s += at(h, p)[b];
-      n[j] = (uint32_t)s;
-      mass[j] = counts ? 0.0 : (double)s / unit * exp(-(double)b * (SMP_SPAN / SMP_BINS));
-    }
-    double before;
-    if (counts) {
-      uint32_t all;
-      before = scan_count(n[0] + n[1], &all);
-      mass[0] = n[0], mass[1] = n[1];
+      for (int j = 0; j < 4; j++) before += n[j], mass[j] = __uint_as_float(before);
     } else {
-      before = scan_mass(mass[0] + mass[1]);
+      const float one = exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * 4 * tid) / unit;
+#pragma unroll
+      for (int j = 0; j < 4; j++) s[j] *= one * exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * j);
+      float before = scan_float((s[0] + s[1]) + (s[2] + s[3]));
+#pragma unroll
+      for (int j = 0; j < 4; j++) before += s[j], mass[j] = before;
     }
-    along()[2 * tid] = before + mass[0];
-    along()[2 * tid + 1] = before + mass[0] + mass[1];
+    *reinterpret_cast<float4*>(along() + 4 * tid) = make_float4(mass[0], mass[1], mass[2], mass[3]);
     __syncthreads();
   }
   // Most that the tokens of the last bin, which was not measured, can weigh.
-  __device__ double tail() const { return (double)a.vocab * exp(-(double)SMP_SPAN * (SMP_BINS - 1) / SMP_BINS); }
+  __device__ double tail() const { return (double)a.vocab * exp2_approx(-kLog2e * SMP_SPAN * (SMP_BINS - 2) / SMP_BINS); }
 
   // ---- exact sums and counts of all tokens (all: else only the counts), of those ahead of bin b0, and the tokens of bins b0
   // .. b1 into the first block's list, as far as there is room
-  __device__ SmpExact exactly(bool all, int b0, int b1, uint32_t& before) {
+  __device__ SmpExact exactly(bool all, float b0, float b1, uint32_t& before) {
     if (tid == 0) sh.n = 0;
     all_sync();  // the first block's list is free, its count 0
-    double s_all = 0.0, s_ahead = 0.0;
-    uint32_t n_all = 0, n_ahead = 0, n = 0;
+    SmpExact e = {0.0, 0.0, 0, 0, 0};
     uint32_t* count = at(&sh.n, 0);
     uint64_t* to = at(list(), 0);
     vectors([&](const float* y, int id) {
-      int b[VEC];
-      bool ahead = false, here = false;
+      float b[VEC], first = 2 * SMP_BINS;
 #pragma unroll
       for (int i = 0; i < VEC; i++) {
-        b[i] = y[i] >= floor_ ? bin_of(distance(y[i])) : SMP_BINS;
-        n_all += b[i] < SMP_BINS;
-        n_ahead += b[i] < b0;
-        ahead |= b[i] < b0;
-        here |= b[i] >= b0 && b[i] <= b1;
+        b[i] = y[i] >= floor_ ? bin_of(y[i]) : 2 * SMP_BINS;
+        e.n_all += b[i] < SMP_BINS;
+        first = fminf(first, b[i]);
       }
-      if (all || ahead) {
-        double w[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; i++) w[i] = weight(y[i]);
+      if (all || first < b0) {
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
-          if (all) s_all += b[i] < SMP_BINS ? w[i] : 0.0;
-          if (b[i] < b0) s_ahead += w[i];
+          const double w = weight(y[i]);
+          if (all) e.all += b[i] < SMP_BINS ? w : 0.0;
+          if (b[i] < b0) e.ahead += w, e.n_ahead++;
         }
       }
-      if (here) {
+      if (first <= b1) {
 #pragma unroll
         for (int i = 0; i < VEC; i++)
           if (b[i] >= b0 && b[i] <= b1) {
-            n++;
+            e.n++;
             const uint32_t k = atomicAdd(count, 1u);
             if (k < SMP_LIST) to[k] = place(rank_bits(y[i]), (uint32_t)(id + i));
           }
       }
     });
-    s_all = warp_sum(s_all), s_ahead = warp_sum(s_ahead);
-    if (tid % 32 == 0) sh.scan[tid / 32] = s_all, sh.scan2[tid / 32] = s_ahead;
-    n_all = block_sum(n_all), n_ahead = block_sum(n_ahead), n = block_sum(n);  // (and a barrier)
-    SmpExact* e = sh.exact[turn++ & 1];
-    if (tid < parts) {
-      SmpExact mine = {0.0, 0.0, n_all, n_ahead, n};
-      for (int w = 0; w < SMP_WARPS; w++) mine.all += sh.scan[w], mine.ahead += sh.scan2[w];
-      *at(e + part, tid) = mine;
+    auto over_lanes = [](SmpExact& v, int lanes) {
+      for (int o = lanes / 2; o; o >>= 1) {
+        v.all += __shfl_xor_sync(0xffffffffu, v.all, o);
+        v.ahead += __shfl_xor_sync(0xffffffffu, v.ahead, o);
+      }
+    };
+    over_lanes(e, 32);
+    e.n_all = __reduce_add_sync(0xffffffffu, e.n_all);
+    e.n_ahead = __reduce_add_sync(0xffffffffu, e.n_ahead);
+    e.n = __reduce_add_sync(0xffffffffu, e.n);
+    if (tid % 32 == 0) sh.parts[tid / 32] = e;
+    __syncthreads();
+    SmpExact* told = sh.exact[turn++ & 1];
+    if (tid < 32) {
+      SmpExact v = sh.parts[tid % SMP_WARPS];
+      over_lanes(v, SMP_WARPS);
+      if (tid >= SMP_WARPS) v.n_all = v.n_ahead = v.n = 0;
+      v.n_all = __reduce_add_sync(0xffffffffu, v.n_all);
+      v.n_ahead = __reduce_add_sync(0xffffffffu, v.n_ahead);
+      v.n = __reduce_add_sync(0xffffffffu, v.n);
+      if (tid < parts) *at(told + part, tid) = v;
     }
     all_sync();
     SmpExact r = {0.0, 0.0, 0, 0, 0};
     before = 0;
     for (int p = 0; p < parts; p++) {
-      r.all += e[p].all, r.ahead += e[p].ahead;
-      if (p < part) before += e[p].n;
-      r.n_all += e[p].n_all, r.n_ahead += e[p].n_ahead, r.n += e[p].n;
+      r.all += told[p].all, r.ahead += told[p].ahead;
+      if (p < part) before += told[p].n;
+      r.n_all += told[p].n_all, r.n_ahead += told[p].n_ahead, r.n += told[p].n;
     }
     return r;
   }
@@ -448,24 +519,26 @@ struct SmpRow {
   // ---- the token at which the count or the sum crosses `goal`; before the sum of all tokens is known, share of it.  all:
   // gets that sum, and the number of tokens
   __device__ SmpFound search(SmpKind kind, double goal, double share, double* all, uint32_t* n_all) {
-    double from = goal, to = goal;
-    const double last = along()[SMP_BINS - 1];
-    if (all) from = share * last * (1 - near_), to = share * (last * (1 + near_) + tail());
-    const double e = kind == SMP_COUNT ? 0.0 : near_;
+    // the first bin with which the number may be crossed, and the first with which it surely is
     if (tid == 0) sh.lo = sh.hi = SMP_BINS - 1;
     __syncthreads();
+    const float4 four = *reinterpret_cast<const float4*>(along() + 4 * tid);
+    const float y[5] = {tid ? along()[4 * tid - 1] : 0.f, four.x, four.y, four.z, four.w};
+    double from = goal, to = goal;
+    if (all) {
+      const float last = along()[SMP_BINS - 1];
+      from = share * last * (1.0 - near_), to = share * (last * (1.0 + near_) + tail());
+    }
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int b = 2 * tid + j;
-      const double y = along()[b], prev = b ? along()[b - 1] : 0.0;
-      // the first bin with which the number may be crossed, and the first with which it surely is
-      if (b < SMP_BINS - 1 && y * (1 + e) >= from && !(b && prev * (1 + e) >= from)) sh.lo = b;
-      if (b < SMP_BINS - 1 && (kind == SMP_COUNT ? y >= to : y * (1 - e) > to) &&
-          !(b && (kind == SMP_COUNT ? prev >= to : prev * (1 - e) > to)))
-        sh.hi = b;
+    for (int j = 0; j < 4; j++) {
+      auto may = [&](float v) { return kind == SMP_COUNT ? (double)__float_as_uint(v) >= goal : v * (1.0 + near_) >= from; };
+      auto must = [&](float v) { return kind == SMP_COUNT ? (double)__float_as_uint(v) >= goal : v * (1.0 - near_) > to; };
+      const int b = 4 * tid + j;
+      if (b < SMP_BINS - 1 && may(y[j + 1]) && !(b && may(y[j]))) sh.lo = b;
+      if (b < SMP_BINS - 1 && must(y[j + 1]) && !(b && must(y[j]))) sh.hi = b;
     }
     __syncthreads();
-    const int b0 = (int)sh.lo, b1 = (int)sh.hi;
+    const float b0 = (float)sh.lo, b1 = (float)sh.hi;
     SmpWindow w;
     const SmpExact r = exactly(all != nullptr, b0, b1, w.before);
     if (all) *all = r.all, *n_all = r.n_all, goal = share * r.all;
@@ -476,14 +549,14 @@ struct SmpRow {
     uint32_t lo = least, hi = most;
     while (lo < hi) {  // smallest rank whose bin is b1 or an earlier one
       const uint32_t mid = lo + (hi - lo) / 2;
-      if (bin_of(distance(rank_value(mid))) <= b1) hi = mid;
+      if (bin_of(rank_value(mid)) <= b1) hi = mid;
       else lo = mid + 1;
     }
     w.lo = lo;
     hi = most;
     while (lo < hi) {  // largest whose bin is b0 or a later one
       const uint32_t mid = hi - (hi - lo) / 2;
-      if (bin_of(distance(rank_value(mid))) >= b0) lo = mid;
+      if (bin_of(rank_value(mid)) >= b0) lo = mid;
       else hi = mid - 1;
     }
     w.hi = lo;
@@ -628,15 +701,14 @@ struct SmpRow {
 
   __device__ void run() {
     const int row = blockIdx.x / parts;
-    const float t = a.temperature ? a.temperature[row] : 1.f, p = a.top_p ? a.top_p[row] : 1.f;
+    float t = a.temperature ? a.temperature[row] : 1.f, p = a.top_p ? a.top_p[row] : 1.f;
     const float min_p = a.min_p ? a.min_p[row] : 0.f;
     int k = a.top_k ? a.top_k[row] : 0;
-    if (k < 0 || k >= a.vocab) k = 0;
     double u = a.uniform[row];
-    u = u > 0.0 ? fmin(u, 0x1.fffffffffffffp-1) : 0.0;
-    if (tid < 32) sh.root[tid] = exp2(tid / 32.0);
     uint32_t own;
     const uint32_t most = load(own);
+    if (k < 0 || k >= a.vocab) k = 0;
+    u = u > 0.0 ? fmin(u, 0x1.fffffffffffffp-1) : 0.0;
     m = rank_value(most);
     if (!(fabsf(m) <= FLT_MAX) || t != t) {  // nothing to choose from, or no sense in it
       if (part == 0 && tid == 0) answer(-1, -INFINITY, 0);
@@ -656,7 +728,7 @@ struct SmpRow {
     }
     top = m;
     inv_t = 1.0 / (double)t;
-    rate = inv_t * (32 * 1.44269504088896340736);
+    rate = inv_t * (64 * 1.44269504088896340736);
     cut_off = 620.f * t;
     floor_ = -FLT_MAX;
     if (min_p >= 1.f) floor_ = m;
@@ -664,12 +736,7 @@ struct SmpRow {
     if ((k && k <= SMP_TOP) || min_p > 0.f) {
       float from = floor_;
       if (k && k <= SMP_TOP) {
-        // a value that this block's share of k tokens reaches, to 20 bits; 0 if there are not so many threads with one
-        const int share = (k + parts - 1) / parts;
-        uint32_t reach = 0;
-        for (int bit = 31; bit >= 12; bit--)
-          if (__syncthreads_count(own >= (reach | 1u << bit)) >= share) reach |= 1u << bit;
-        const uint32_t* all = tell(reach);
+        const uint32_t* all = tell(reached((k + parts - 1) / parts, own));
         uint32_t least = 0xFFFFFFFFu;
         for (int q = 0; q < parts; q++) least = min(least, all[q]);
         from = fmaxf(from, rank_value(max(least, rank_bits(-FLT_MAX))));
@@ -692,14 +759,15 @@ struct SmpRow {
     uint64_t last = 0;      // the last place that is kept, where that is known
     bool known = false;     // whether mass and kept are
     if (k) {
-      measure(true);
-      if ((uint32_t)k < (uint32_t)along()[SMP_BINS - 1]) {
+      measure<true>();
+      if ((uint32_t)k < __float_as_uint(along()[SMP_BINS - 1])) {
         const SmpFound f = search(SMP_COUNT, (double)k, 0.0, nullptr, nullptr);
         mass = f.mass, kept = f.count, last = f.place;
         known = true;
       }
+      all_sync();  // the histogram has been read
     }
-    measure(false);
+    measure<false>();
     if (p < 1.f) {
       const SmpFound f = search(SMP_REACH, (double)p * mass, (double)p, known ? nullptr : &mass, &kept);
       if (f.count < kept) mass = f.mass, kept = f.count, last = f.place;
