@@ -494,7 +494,7 @@ typedef struct {
     int parts, held_bytes;    /* set by iris_launch_sample */
 } IrisSample;
 cudaError_t iris_sample_init(void);
-cudaError_t iris_launch_sample(IrisSample *a, int f32, cudaStream_t stream);
+cudaError_t iris_launch_sample(IrisSample *a, int f32, int num_sms, cudaStream_t stream);
 
 /* linear4_kernels.cu */
 typedef struct {

@@ -360,7 +360,7 @@ int iris_gpu_sample_tokens(const void *logits, int f32, int64_t ld, int rows, in
     int rc = lm_enter(&d, what, ptrs, (int)(sizeof(ptrs) / sizeof(ptrs[0])));
     if (rc) return rc;
     IrisSample a = {logits, ld, rows, vocab, temperature, top_p, min_p, top_k, uniform, ids, kept, logprobs, 0, 0};
-    return lm_leave(&d, iris_launch_sample(&a, f32 != 0, (cudaStream_t)stream), what, 1);
+    return lm_leave(&d, iris_launch_sample(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, 1);
 }
 
 /* ------------------------------------------------------------------ weights of 4 bits */

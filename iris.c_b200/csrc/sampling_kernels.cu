@@ -37,7 +37,9 @@ constexpr int SMP_TOP = 512;    // largest top-k whose tokens are looked for thr
 constexpr int SMP_BINS = 2048;  // four a thread
 constexpr float SMP_SPAN = 24.f;      // (m - x) / t that the bins cover; the last one holds all that is below
 constexpr int SMP_CUT = 16, SMP_CUTTERS = 64;  // bins of a closer look, threads that fill bins of their own
-static_assert(SMP_BINS == 4 * SMP_THREADS && SMP_LIST == 2 * SMP_THREADS && SMP_CUT == SMP_WARPS, "shares of a thread, and warp");
+constexpr int SMP_SORT = 1024;  // places of the sort by value
+static_assert(SMP_BINS == 4 * SMP_THREADS && SMP_LIST == 2 * SMP_THREADS && SMP_SORT == 2 * SMP_THREADS && SMP_CUT == SMP_WARPS,
+              "shares of a thread, and warp");
 
 struct SmpSums {  // of the closer bins, from each block of the cluster
   double mass[SMP_PARTS][SMP_CUT];
@@ -50,29 +52,30 @@ struct SmpFound {
   uint32_t count;
 };
 
-struct SmpExact {  // of a block
-  double all, ahead;      // sums of all tokens, of those ahead of the window
-  uint32_t n_all, n_ahead, n;  // tokens: all, ahead, in the window
+struct SmpExact {  // of a block, or a warp of it
+  double all, ahead[2];          // sums of all tokens, of those ahead of either window
+  uint32_t n_all, n_ahead[2], n[2];  // tokens: all, ahead, in the window
 };
 
 struct SmpShared {
   SmpSums next[2];             // in turn, so that one round's may be read while the next one's come
   SmpExact exact[2][SMP_PARTS];
-  uint32_t one[2][SMP_PARTS];  // a number from each block
+  uint2 two[2][SMP_PARTS];     // two numbers from each block
   SmpExact parts[SMP_WARPS];   // of a block's warps
   double scan[SMP_WARPS];
   float fscan[SMP_WARPS];
   uint32_t iscan[SMP_WARPS];
   double root[64];             // 2^(i / 64)
   SmpFound found;
-  uint32_t n, lo, hi;
+  uint32_t n[2], lo, hi;
 };
 
-// shared memory besides the row: the histogram, the sums along the bins, and the list, in whose place the closer bins stand
+// shared memory besides the row: the histogram, the sums along the bins, and two lists, in whose place the closer bins stand
 constexpr int SMP_HIST = SMP_BINS * 4, SMP_ALONG = SMP_BINS * 4;
-constexpr int SMP_TAIL = SMP_CUT * SMP_CUTTERS * (8 + 4);
+constexpr int SMP_TAIL = 2 * SMP_LIST * 8;
 constexpr int SMP_WORK = SMP_HIST + SMP_ALONG + SMP_TAIL;
-static_assert(SMP_TAIL >= SMP_LIST * 8 && SMP_ALONG >= SMP_LIST * 8 && SMP_HIST >= SMP_LIST * 8, "the lists fit");
+static_assert(SMP_TAIL >= SMP_CUT * SMP_CUTTERS * (8 + 4) && SMP_ALONG >= SMP_SORT * 4 && SMP_ALONG >= SMP_LIST * 8 &&
+              SMP_HIST >= SMP_LIST * 8, "the bins and lists fit");
 
 struct SmpWindow {  // part of the line: ranks lo .. hi, `count` tokens, with sums over what stands ahead of it
   uint32_t lo, hi;
@@ -91,7 +94,7 @@ struct SmpRow {
   uint8_t* smem;
   const In* x;
   int tid, part, parts, off, v0, nv;
-  float m, floor_, cut_off;  // cut_off: what lies further under m weighs nothing, e^-620
+  float m, floor_, lowest;   // lowest: what lies under it weighs nothing, e^-600 or less
   double top, inv_t, rate;   // rate: 64 log2(e) / t
   float inv_bin;
   float unit;                // of the histogram's weights, so that a block's tokens in one bin stay within 32 bits
@@ -115,9 +118,12 @@ struct SmpRow {
   __device__ uint8_t* work() const { return smem + (HELD ? a.held_bytes : 0); }
   __device__ uint32_t* hist() const { return reinterpret_cast<uint32_t*>(work()); }
   __device__ float* along() const { return reinterpret_cast<float*>(work() + SMP_HIST); }  // sums up to and with a bin, or counts
-  __device__ uint64_t* list() const { return reinterpret_cast<uint64_t*>(work() + SMP_HIST + SMP_ALONG); }
-  __device__ uint64_t* own_list() const { return reinterpret_cast<uint64_t*>(along()); }  // before there are sums; again for what is in order
-  __device__ double* line() const { return reinterpret_cast<double*>(hist()); }           // when there is no histogram
+  // the tokens that the blocks have found, each in a part of its own of the first one's lists
+  __device__ uint64_t* list(int i = 0) const { return reinterpret_cast<uint64_t*>(work() + SMP_HIST + SMP_ALONG) + i * SMP_LIST; }
+  __device__ int quota() const { return SMP_LIST / parts; }
+  // by the first block, when there is no histogram: the tokens in order; when there are no sums along the bins: sums along them
+  __device__ uint64_t* ordered() const { return reinterpret_cast<uint64_t*>(hist()); }
+  __device__ double* line() const { return reinterpret_cast<double*>(along()); }
   __device__ double* cut_mass() const { return reinterpret_cast<double*>(list()); }
   __device__ uint32_t* cut_count() const { return reinterpret_cast<uint32_t*>(cut_mass() + SMP_CUT * SMP_CUTTERS); }
 
@@ -128,10 +134,10 @@ struct SmpRow {
   }
   template <typename T>
   __device__ T* at(T* p, int rank) const { return parts > 1 ? iris::cluster_map(p, (uint32_t)rank) : p; }
-  // this block's number, the same in all threads, to all of them; the numbers of the blocks after the barrier
-  __device__ const uint32_t* tell(uint32_t v) {
-    uint32_t* to = sh.one[turn++ & 1];
-    if (tid < parts) *at(to + part, tid) = v;
+  // this block's numbers, the same in all threads, to all blocks; those of the blocks after the barrier
+  __device__ const uint2* tell(uint32_t v, uint32_t w = 0) {
+    uint2* to = sh.two[turn++ & 1];
+    if (tid < parts) *at(to + part, tid) = make_uint2(v, w);
     all_sync();
     return to;
   }
@@ -163,16 +169,15 @@ struct SmpRow {
   // function, 1989).
   __device__ double weight(float y) const {
     constexpr double c = 0.69314718055994530942 / 64;
-    const double z = ((double)y - top) * rate;
+    const double z = ((double)fmaxf(y, lowest) - top) * rate;
     const double shifted = z + 0x1.8p52;
-    const int n = __double2loint(shifted);
+    const int n = max(__double2loint(shifted), -64 * 1000);
     const double r = z - (shifted - 0x1.8p52);
     double p = fma(r, c * c * c * c / 24, c * c * c / 6);
     p = fma(r, p, c * c / 2);
     p = fma(r, p, c);
     p = fma(r, p, 1.0) * sh.root[n & 63];
-    const double w = __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p));
-    return m - y > cut_off ? 0.0 : w;
+    return __hiloint2double(__double2hiint(p) + (n >> 6) * (1 << 20), __double2loint(p));
   }
 
   // over the block, the same in all threads
@@ -184,70 +189,52 @@ struct SmpRow {
     __syncthreads();
     return v;
   }
-  __device__ uint32_t block_sum(uint32_t v) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    if (tid % 32 == 0) sh.iscan[tid / 32] = v;
-    __syncthreads();
-    v = __reduce_add_sync(0xffffffffu, tid % 32 < SMP_WARPS ? sh.iscan[tid % SMP_WARPS] : 0u);
-    __syncthreads();
-    return v;
-  }
   __device__ static double warp_sum(double v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }
-  // sum of what the threads ahead have
-  __device__ uint32_t scan_count(uint32_t v, uint32_t* total) {
-    uint32_t incl = v;
+  // sum of what the threads ahead have; *total over the block
+  template <typename T>
+  __device__ T scan(T v, T* of_warps, T* total) {
+    const int lane = tid % 32;
+    T incl = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (tid % 32 >= o) incl += y;
+      const T y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
     }
-    if (tid % 32 == 31) sh.iscan[tid / 32] = incl;
+    if (lane == 31) of_warps[tid / 32] = incl;
     __syncthreads();
-    uint32_t before = incl - v;
-    *total = 0;
-    for (int w = 0; w < SMP_WARPS; w++) {
-      if (w < tid / 32) before += sh.iscan[w];
-      *total += sh.iscan[w];
-    }
-    __syncthreads();
-    return before;
-  }
-  __device__ float scan_float(float v) {
-    float incl = v;
+    T w = of_warps[lane % SMP_WARPS];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (tid % 32 >= o) incl += y;
+    for (int o = 1; o < SMP_WARPS; o <<= 1) {
+      const T y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
     }
-    if (tid % 32 == 31) sh.fscan[tid / 32] = incl;
+    // (lane i of the first 16: the warps up to and with i)
+    const T ahead = __shfl_sync(0xffffffffu, w, (tid / 32 + SMP_WARPS - 1) % SMP_WARPS);
+    *total = __shfl_sync(0xffffffffu, w, SMP_WARPS - 1);
     __syncthreads();
-    float ahead = 0.f;
-    for (int w = 0; w < tid / 32; w++) ahead += sh.fscan[w];
-    __syncthreads();
-    return ahead + (incl - v);
+    return (tid < 32 ? (T)0 : ahead) + (incl - v);
   }
+  __device__ uint32_t scan_count(uint32_t v, uint32_t* total) { return scan(v, sh.iscan, total); }
+  __device__ float scan_float(float v, float* total) { return scan(v, sh.fscan, total); }
   __device__ double scan_mass(double v) {
-    double incl = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (tid % 32 >= o) incl += y;
-    }
-    if (tid % 32 == 31) sh.scan[tid / 32] = incl;
-    __syncthreads();
-    const double before = incl - v;
-    double ahead = 0;
-    for (int w = 0; w < tid / 32; w++) ahead += sh.scan[w];
-    __syncthreads();
-    return ahead + before;
+    double total;
+    return scan(v, sh.scan, &total);
+  }
+  // over the blocks' numbers
+  __device__ uint32_t most_of(const uint32_t* first_of_pairs) const {
+    return __reduce_max_sync(0xffffffffu, tid % 32 < parts ? first_of_pairs[tid % 32 * 2] : 0u);
+  }
+  __device__ uint32_t least_of(const uint32_t* first_of_pairs) const {
+    return __reduce_min_sync(0xffffffffu, tid % 32 < parts ? first_of_pairs[tid % 32 * 2] : 0xffffffffu);
   }
 
-  // ---- the row, its largest value (NaN if there is one); each thread's own largest in `own`, each warp's in sh.iscan
-  __device__ uint32_t load(uint32_t& own) {
+  // ---- the row.  From each block its largest value (NaN if there is one), and with top_k = k of 1 to SMP_TOP a value that its
+  // share of k tokens reaches
+  __device__ const uint2* load(int k) {
     float best = -INFINITY;
     constexpr int FLY = 10;  // 76 KB of a row in one round
     for (int b = tid; b < nv; b += FLY * SMP_THREADS) {
@@ -266,17 +253,15 @@ struct SmpRow {
       }
     }
     if (tid >= SMP_THREADS - 64) sh.root[tid & 63] = exp2((tid & 63) / 64.0);
-    own = rank_bits(best);
+    const uint32_t own = rank_bits(best);
     const uint32_t w = __reduce_max_sync(0xffffffffu, own);
     if (tid % 32 == 0) sh.iscan[tid / 32] = w;
     __syncthreads();
-    const uint32_t* all = tell(__reduce_max_sync(0xffffffffu, sh.iscan[tid % SMP_WARPS]));
-    uint32_t r = 0;
-    for (int p = 0; p < parts; p++) r = max(r, all[p]);
-    return r;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, sh.iscan[tid % SMP_WARPS]);
+    return tell(most, k > 0 && k <= SMP_TOP ? reached((k + parts - 1) / parts, own) : 0u);
   }
 
-  // ---- a value that `share` of this block's tokens reach, 0 if it may have fewer; sh.iscan as load() leaves it
+  // a value that `share` of this block's tokens reach, 0 if it may have fewer; sh.iscan: the warps' largest
   __device__ uint32_t reached(int share, uint32_t own) {
     if (share <= SMP_WARPS / 2) {  // by the warps' largest
       const uint32_t mine = sh.iscan[tid % SMP_WARPS];
@@ -294,69 +279,116 @@ struct SmpRow {
     return reach;
   }
 
-  // ---- the tokens from `from` on, each block's in its own list; how many there are in the whole row (each block's in `all`)
-  __device__ uint32_t gather(float from, const uint32_t*& all) {
-    if (tid == 0) sh.n = 0;
+  // ---- the tokens from `from` on into the first block's list; how many each block has
+  __device__ const uint2* gather(float from) {
+    if (tid == 0) sh.n[0] = 0;
     __syncthreads();
+    uint64_t* to = at(list(), 0) + part * quota();
     vectors([&](const float* y, int id) {
       float most = y[0];
 #pragma unroll
       for (int i = 1; i < VEC; i++) most = fmaxf(most, y[i]);
-      if (most < from || *(volatile uint32_t*)&sh.n > SMP_LIST) return;  // none, or too many already
+      if (most < from || *(volatile uint32_t*)sh.n > quota()) return;  // none, or too many already
 #pragma unroll
       for (int i = 0; i < VEC; i++)
         if (y[i] >= from) {
-          const uint32_t n = atomicAdd(&sh.n, 1);
-          if (n < SMP_LIST) own_list()[n] = place(rank_bits(y[i]), (uint32_t)(id + i));
+          const uint32_t n = atomicAdd(sh.n, 1);
+          if (n < quota()) to[n] = place(rank_bits(y[i]), (uint32_t)(id + i));
         }
     });
     __syncthreads();
-    all = tell(sh.n);
-    uint32_t n = 0;
-    for (int p = 0; p < parts; p++) n += min(all[p], SMP_LIST + 1);
-    return n;
+    return tell(sh.n[0]);
+  }
+  // whether the blocks' tokens have all found room
+  __device__ bool room(const uint2* n) const {
+    return most_of(&n->x) <= quota();
   }
 
-  // ---- by the first block: list()[0, n) in order, largest first.  Few by counting how many are ahead of each, all threads
-  // at it (n^2 steps); more by a bitonic sort, with what is missing to a power of two as 0.
-  __device__ void put_in_order(int n) {
-    uint64_t* l = list();
+  // ---- by the first block: the blocks' tokens, n in all, in order, largest first, into ordered().  (Of many, the sums along
+  // the bins are lost, those of the first block)
+  __device__ void put_in_order(const uint2* from, int n, int which = 0) {
+    uint64_t* l = ordered();
     __syncthreads();
-    if (n <= 256) {
-      int per = 2;  // threads to a token
+    uint64_t mine[2];  // tokens tid and tid + SMP_THREADS of all
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      int i = tid + j * SMP_THREADS, p = 0;
+      mine[j] = 0;
+      if (i >= n) continue;
+      while (i >= (int)from[p].x) i -= (int)from[p++].x;
+      mine[j] = list(which)[p * quota() + i];
+    }
+    if (n <= 128) {
+      // how many are ahead of each: n^2 comparisons, 4 to 32 threads a token
+      if (tid < n) l[tid] = mine[0];
+      __syncthreads();
+      int per = 4;
       while (per < 32 && 2 * per * n <= SMP_THREADS) per *= 2;
       const int i = tid / per;
-      const uint64_t mine = i < n ? l[i] : 0;
+      const uint64_t p = i < n ? l[i] : 0;
       int ahead = 0;
 #pragma unroll 4
-      for (int j = tid % per; j < n; j += per) ahead += l[j] > mine;
+      for (int j = tid % per; j < n; j += per) ahead += l[j] > p;
       for (int o = per / 2; o; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
       __syncthreads();
-      if (i < n && tid % per == 0) l[ahead] = mine;
+      if (i < n && tid % per == 0) l[ahead] = p;
       __syncthreads();
       return;
     }
-    int size = 512;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += SMP_THREADS) l[i] = 0;
+    // by value into SMP_SORT places, then by comparison within a place
+    uint32_t* count = reinterpret_cast<uint32_t*>(along());
+    uint64_t* sorted = list(which);
+    uint32_t top_rank = 0, low_rank = 0;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      count[tid + j * SMP_THREADS] = 0;
+      const uint32_t r = (uint32_t)(mine[j] >> 32);
+      if (r) top_rank = max(top_rank, r), low_rank = max(low_rank, ~r);
+    }
+    top_rank = block_max(top_rank);
+    low_rank = ~block_max(low_rank);
+    const int shift = max(0, 22 - __clz(top_rank - low_rank));
+    auto where = [&](uint64_t p) { return (top_rank - (uint32_t)(p >> 32)) >> shift; };
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (mine[j]) atomicAdd(count + where(mine[j]), 1u);
     __syncthreads();
-    for (int k = 2; k <= size; k *= 2)
-      for (int j = k / 2; j; j /= 2) {
-        // within 64 places a warp has them to itself
-        if (j >= 32) __syncthreads();
-        else __syncwarp();
-        if (2 * tid < size) {
-          const int i = 2 * (tid & ~(j - 1)) + (tid & (j - 1));
-          const uint64_t p = l[i], q = l[i + j];
-          if ((p < q) == ((i & k) == 0)) l[i] = q, l[i + j] = p;
-        }
-      }
+    const uint2 two = reinterpret_cast<uint2*>(count)[tid];
+    uint32_t all, before = scan_count(two.x + two.y, &all);
+    reinterpret_cast<uint2*>(count)[tid] = make_uint2(before, before + two.x);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (mine[j]) sorted[atomicAdd(count + where(mine[j]), 1u)] = mine[j];  // a place's count becomes its end
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      if (!mine[j]) continue;
+      const uint32_t w = where(mine[j]), begin = w ? count[w - 1] : 0, end = count[w];
+      uint32_t ahead = begin;
+      for (uint32_t i = begin; i < end; i++) ahead += sorted[i] > mine[j];
+      l[ahead] = mine[j];
+    }
     __syncthreads();
   }
-  // weights of this thread's two tokens of the list
-  __device__ void weights(int n, double w[2]) const {
-#pragma unroll
-    for (int j = 0; j < 2; j++) w[j] = 2 * tid + j < n ? weight(rank_value((uint32_t)(list()[2 * tid + j] >> 32))) : 0.0;
+  // number of tokens for which f(token's number, sum up to and with it) holds; those of `n` in order, w and c as sums_of() has it
+  template <typename F>
+  __device__ uint32_t number(int n, const double c[2], F f) const {
+    uint32_t r = __syncthreads_count(tid < n && f(tid, c[0]));
+    if (n > SMP_THREADS) r += __syncthreads_count(tid + SMP_THREADS < n && f(tid + SMP_THREADS, c[1]));
+    return r;
+  }
+  // the sums of the weights up to and with tokens tid and tid + SMP_THREADS of n in order
+  __device__ void sums_of(int n, double w[2], double c[2]) {
+    auto one = [&](int i) { return i < n ? weight(rank_value((uint32_t)(ordered()[i] >> 32))) : 0.0; };
+    w[0] = one(tid);
+    double first;
+    c[0] = scan(w[0], sh.scan, &first) + w[0];
+    w[1] = c[1] = 0.0;
+    if (n > SMP_THREADS) {
+        w[1] = one(tid + SMP_THREADS);
+      c[1] = first + (scan_mass(w[1]) + w[1]);
+    }
   }
 
   __device__ void answer(int id, double logprob, uint32_t kept) const {
@@ -369,35 +401,35 @@ struct SmpRow {
     return ((double)rank_value((uint32_t)(p >> 32)) - top) * inv_t - log(mass);
   }
 
-  // ---- all that can be kept is in list(): by the first block
-  __device__ void finish(int n, int k, float p, double u) {
-    put_in_order(n);
+  // ---- all that can be kept is in the list: by the first block
+  __device__ void finish(const uint2* from, int n, int k, float p, double u) {
+    put_in_order(from, n);
     if (k) n = min(n, k);
-    double w[2];
-    weights(n, w);
-    const double before = scan_mass(w[0] + w[1]), c0 = before + w[0], c1 = c0 + w[1];
+    double w[2], c[2];
+    sums_of(n, w, c);
     double* sums = line();
-    sums[2 * tid] = c0, sums[2 * tid + 1] = c1;
+    sums[tid] = c[0], sums[tid + SMP_THREADS] = c[1];
     __syncthreads();
     const double mass = sums[n - 1];
     uint32_t kept = n;
     if (p < 1.f) {
       const double goal = (double)p * mass;
-      kept = max(block_sum((2 * tid < n && before < goal) + (2 * tid + 1 < n && c0 < goal)), 1u);
+      kept = max(number(n, c, [&](int i, double s) { return (i ? sums[i - 1] : 0.0) < goal; }), 1u);
     }
     const double m_kept = sums[kept - 1], goal = u * m_kept;
-    uint32_t pick = block_sum((2 * tid < kept && c0 <= goal) + (2 * tid + 1 < kept && c1 <= goal));
-    const uint32_t heavy = block_sum((2 * tid < kept && w[0] > 0.0) + (2 * tid + 1 < kept && w[1] > 0.0));
-    pick = min(pick, heavy - 1);  // the first one weighs 1
-    if (tid == 0) answer((int)~(uint32_t)list()[pick], logprob(list()[pick], m_kept), kept);
+    uint32_t pick = number((int)kept, c, [&](int, double s) { return s <= goal; });
+    if (pick == kept)  // by rounding: the last with a weight (the first one weighs 1)
+      pick = number((int)kept, c, [&](int i, double) { return w[i >= SMP_THREADS] > 0.0; }) - 1;
+    if (tid == 0) answer((int)~(uint32_t)ordered()[pick], logprob(ordered()[pick], m_kept), kept);
   }
 
   // ---- how the line grows along the bins: along()[b] is the sum up to and with bin b, to near_ (or the count, a whole number)
   __device__ float distance(float y) const { return fminf(fminf(m - y, FLT_MAX) * inv_bin, SMP_BINS - 1); }
   __device__ static float nearest(float d) { return (d + 0x1.8p23f) - 0x1.8p23f; }  // whole number, ties to even
   __device__ float bin_of(float y) const { return nearest(distance(y)); }           // the bins are around whole numbers
+  // y: the sums up to and with this thread's four bins, and the bin before them
   template <bool COUNTS>
-  __device__ void measure() {
+  __device__ void measure(float y[5], float& last) {
     uint32_t* h = hist();
     for (int i = tid; i < SMP_BINS; i += SMP_THREADS) h[i] = 0;
     __syncthreads();
@@ -407,52 +439,57 @@ struct SmpRow {
         const float d = distance(y[i]), b = nearest(d);
         const int at = __float_as_int(d + 0x1.8p23f) & (SMP_BINS - 1);
         if (COUNTS) {
-          if (y[i] >= floor_) atomicAdd(h + at, 1u);
+          atomicAdd(h + at, y[i] >= floor_ ? 1u : 0u);
         } else {
           // unit e^-r for the way r behind the bin's middle, |r| <= 12 / 2048 (the series' next term is under 2^-24), as a
           // whole number
           const float r = (d - b) * (SMP_SPAN / SMP_BINS);
           const float w = fmaf(unit, r * fmaf(0.5f, r, -1.f), unit + 0x1p23f);
-          if (y[i] >= floor_ && b < SMP_BINS - 1) atomicAdd(h + at, __float_as_uint(w) - 0x4B000000u);
+          // (no branches around the additions: they would keep those of a vector apart)
+          atomicAdd(h + at, y[i] >= floor_ && b < SMP_BINS - 1 ? __float_as_uint(w) - 0x4B000000u : 0u);
         }
       }
     });
     all_sync();
-    float mass[4];
     uint32_t n[4] = {0, 0, 0, 0};
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = 0; p < parts; p++) {
+#pragma unroll
+    for (int p = 0; p < SMP_PARTS; p++) {
+      if (p >= parts) break;
       const uint4 u = *reinterpret_cast<const uint4*>(at(h, p) + 4 * tid);
       if (COUNTS) n[0] += u.x, n[1] += u.y, n[2] += u.z, n[3] += u.w;
       else s[0] += (float)u.x, s[1] += (float)u.y, s[2] += (float)u.z, s[3] += (float)u.w;
     }
     if (COUNTS) {
       uint32_t all, before = scan_count(n[0] + n[1] + n[2] + n[3], &all);
+      last = __uint_as_float(all);
+      y[0] = __uint_as_float(before);
 #pragma unroll
-      for (int j = 0; j < 4; j++) before += n[j], mass[j] = __uint_as_float(before);
+      for (int j = 0; j < 4; j++) before += n[j], y[j + 1] = __uint_as_float(before);
     } else {
       const float one = exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * 4 * tid) / unit;
 #pragma unroll
       for (int j = 0; j < 4; j++) s[j] *= one * exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * j);
-      float before = scan_float((s[0] + s[1]) + (s[2] + s[3]));
+      float before = scan_float((s[0] + s[1]) + (s[2] + s[3]), &last);
+      y[0] = before;
 #pragma unroll
-      for (int j = 0; j < 4; j++) before += s[j], mass[j] = before;
+      for (int j = 0; j < 4; j++) before += s[j], y[j + 1] = before;
     }
-    *reinterpret_cast<float4*>(along() + 4 * tid) = make_float4(mass[0], mass[1], mass[2], mass[3]);
-    __syncthreads();
   }
   // Most that the tokens of the last bin, which was not measured, can weigh.
   __device__ double tail() const { return (double)a.vocab * exp2_approx(-kLog2e * SMP_SPAN * (SMP_BINS - 2) / SMP_BINS); }
 
-  // ---- exact sums and counts of all tokens (all: else only the counts), of those ahead of bin b0, and the tokens of bins b0
-  // .. b1 into the first block's list, as far as there is room
-  __device__ SmpExact exactly(bool all, float b0, float b1, uint32_t& before) {
-    if (tid == 0) sh.n = 0;
-    all_sync();  // the first block's list is free, its count 0
-    SmpExact e = {0.0, 0.0, 0, 0, 0};
-    uint32_t* count = at(&sh.n, 0);
-    uint64_t* to = at(list(), 0);
+  // ---- exact sums and counts of all tokens (all: else only the counts) and of those ahead of bin b0[i], and the tokens of bins
+  // b0[i] .. b1[i] into the first block's lists, as far as there is room, for one window or two.  n_of[i]: how many each block
+  // has; before: of the first window, in the blocks ahead of this one
+  template <int WINDOWS>
+  __device__ SmpExact exactly(bool all, const float b0[WINDOWS], const float b1[WINDOWS], uint32_t& before,
+                              uint2 n_of[WINDOWS][SMP_PARTS]) {
+    if (tid < 2) sh.n[tid] = 0;
+    __syncthreads();
+    SmpExact e = {};
+    float behind = b0[0], last = b1[0];
+    if (WINDOWS == 2) behind = fmaxf(behind, b0[WINDOWS - 1]), last = fmaxf(last, b1[WINDOWS - 1]);
     vectors([&](const float* y, int id) {
       float b[VEC], first = 2 * SMP_BINS;
 #pragma unroll
@@ -461,53 +498,74 @@ struct SmpRow {
         e.n_all += b[i] < SMP_BINS;
         first = fminf(first, b[i]);
       }
-      if (all || first < b0) {
+      const bool some = __any_sync(__activemask(), first < behind);
+      if (all || some) {
+        double w[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-          const double w = weight(y[i]);
-          if (all) e.all += b[i] < SMP_BINS ? w : 0.0;
-          if (b[i] < b0) e.ahead += w, e.n_ahead++;
+        for (int i = 0; i < VEC; i++) w[i] = weight(y[i]);
+        if (all) {
+#pragma unroll
+          for (int i = 0; i < VEC; i++) e.all += b[i] < SMP_BINS ? w[i] : 0.0;
+        }
+        if (some) {
+#pragma unroll
+          for (int k = 0; k < WINDOWS; k++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+              e.ahead[k] += b[i] < b0[k] ? w[i] : 0.0;
+              e.n_ahead[k] += b[i] < b0[k];
+            }
         }
       }
-      if (first <= b1) {
+      if (first <= last) {
 #pragma unroll
-        for (int i = 0; i < VEC; i++)
-          if (b[i] >= b0 && b[i] <= b1) {
-            e.n++;
-            const uint32_t k = atomicAdd(count, 1u);
-            if (k < SMP_LIST) to[k] = place(rank_bits(y[i]), (uint32_t)(id + i));
-          }
+        for (int k = 0; k < WINDOWS; k++)
+#pragma unroll
+          for (int i = 0; i < VEC; i++)
+            if (b[i] >= b0[k] && b[i] <= b1[k]) {
+              e.n[k]++;
+              const int n = (int)atomicAdd(sh.n + k, 1u);
+              if (n < quota()) at(list(k), 0)[part * quota() + n] = place(rank_bits(y[i]), (uint32_t)(id + i));
+            }
       }
     });
-    auto over_lanes = [](SmpExact& v, int lanes) {
+    auto sums = [](SmpExact& v, int lanes) {
       for (int o = lanes / 2; o; o >>= 1) {
         v.all += __shfl_xor_sync(0xffffffffu, v.all, o);
-        v.ahead += __shfl_xor_sync(0xffffffffu, v.ahead, o);
+#pragma unroll
+        for (int k = 0; k < WINDOWS; k++) v.ahead[k] += __shfl_xor_sync(0xffffffffu, v.ahead[k], o);
+      }
+      v.n_all = __reduce_add_sync(0xffffffffu, v.n_all);
+#pragma unroll
+      for (int k = 0; k < WINDOWS; k++) {
+        v.n_ahead[k] = __reduce_add_sync(0xffffffffu, v.n_ahead[k]);
+        v.n[k] = __reduce_add_sync(0xffffffffu, v.n[k]);
       }
     };
-    over_lanes(e, 32);
-    e.n_all = __reduce_add_sync(0xffffffffu, e.n_all);
-    e.n_ahead = __reduce_add_sync(0xffffffffu, e.n_ahead);
-    e.n = __reduce_add_sync(0xffffffffu, e.n);
+    sums(e, 32);
     if (tid % 32 == 0) sh.parts[tid / 32] = e;
     __syncthreads();
     SmpExact* told = sh.exact[turn++ & 1];
     if (tid < 32) {
       SmpExact v = sh.parts[tid % SMP_WARPS];
-      over_lanes(v, SMP_WARPS);
-      if (tid >= SMP_WARPS) v.n_all = v.n_ahead = v.n = 0;
-      v.n_all = __reduce_add_sync(0xffffffffu, v.n_all);
-      v.n_ahead = __reduce_add_sync(0xffffffffu, v.n_ahead);
-      v.n = __reduce_add_sync(0xffffffffu, v.n);
+      if (tid >= SMP_WARPS) v = {};
+      sums(v, 32);
       if (tid < parts) *at(told + part, tid) = v;
     }
     all_sync();
-    SmpExact r = {0.0, 0.0, 0, 0, 0};
+    SmpExact r = {};
     before = 0;
-    for (int p = 0; p < parts; p++) {
-      r.all += told[p].all, r.ahead += told[p].ahead;
-      if (p < part) before += told[p].n;
-      r.n_all += told[p].n_all, r.n_ahead += told[p].n_ahead, r.n += told[p].n;
+#pragma unroll
+    for (int p = 0; p < SMP_PARTS; p++) {
+      if (p >= parts) break;
+      const SmpExact v = told[p];
+      r.all += v.all, r.n_all += v.n_all;
+      if (p < part) before += v.n[0];
+#pragma unroll
+      for (int k = 0; k < WINDOWS; k++) {
+        r.ahead[k] += v.ahead[k], r.n_ahead[k] += v.n_ahead[k], r.n[k] += v.n[k];
+        n_of[k][p].x = v.n[k];
+      }
     }
     return r;
   }
@@ -516,34 +574,102 @@ struct SmpRow {
     return kind == SMP_COUNT ? (double)count >= goal : kind == SMP_REACH ? mass >= goal : mass > goal;
   }
 
-  // ---- the token at which the count or the sum crosses `goal`; before the sum of all tokens is known, share of it.  all:
-  // gets that sum, and the number of tokens
-  __device__ SmpFound search(SmpKind kind, double goal, double share, double* all, uint32_t* n_all) {
-    // the first bin with which the number may be crossed, and the first with which it surely is
+  // ---- the first bin with which a sum of `from` may be reached (a count: is), and the first with which one of `to` surely is
+  // passed; y as measure() gives it
+  __device__ void bins(bool counts, double from, double to, const float y[5], float& b0, float& b1) {
     if (tid == 0) sh.lo = sh.hi = SMP_BINS - 1;
     __syncthreads();
-    const float4 four = *reinterpret_cast<const float4*>(along() + 4 * tid);
-    const float y[5] = {tid ? along()[4 * tid - 1] : 0.f, four.x, four.y, four.z, four.w};
-    double from = goal, to = goal;
-    if (all) {
-      const float last = along()[SMP_BINS - 1];
-      from = share * last * (1.0 - near_), to = share * (last * (1.0 + near_) + tail());
+    bool may[5], must[5];
+#pragma unroll
+    for (int j = 0; j < 5; j++) {
+      may[j] = counts ? (double)__float_as_uint(y[j]) >= from : (double)(y[j] * (1.f + near_)) >= from;
+      must[j] = counts ? may[j] : (double)(y[j] * (1.f - near_)) > to;
     }
+    if (tid == 0) may[0] = must[0] = false;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      auto may = [&](float v) { return kind == SMP_COUNT ? (double)__float_as_uint(v) >= goal : v * (1.0 + near_) >= from; };
-      auto must = [&](float v) { return kind == SMP_COUNT ? (double)__float_as_uint(v) >= goal : v * (1.0 - near_) > to; };
       const int b = 4 * tid + j;
-      if (b < SMP_BINS - 1 && may(y[j + 1]) && !(b && may(y[j]))) sh.lo = b;
-      if (b < SMP_BINS - 1 && must(y[j + 1]) && !(b && must(y[j]))) sh.hi = b;
+      if (b < SMP_BINS - 1 && may[j + 1] && !may[j]) sh.lo = b;
+      if (b < SMP_BINS - 1 && must[j + 1] && !must[j]) sh.hi = b;
     }
     __syncthreads();
-    const float b0 = (float)sh.lo, b1 = (float)sh.hi;
+    b0 = (float)sh.lo, b1 = (float)sh.hi;
+    __syncthreads();
+  }
+  // least and most that the sum of all tokens can be, from what was measured
+  __device__ double least_sum(float last) const { return (double)last * (1.0 - near_); }
+  __device__ double most_sum(float last) const { return (double)last * (1.0 + near_) + tail(); }
+
+  // ---- no top-k: top-p, and the token, in one pass.  How much is kept is known well enough from the bins to say where the
+  // token may be.  False where the tokens there find no room; then the sum and number of all are known.
+  __device__ bool at_once(float p, double u, const float y[5], float last, double& all, uint32_t& n_all) {
+    float b0[2], b1[2];
+    double from = least_sum(last), to = most_sum(last);
+    if (p < 1.f) {
+      from *= (double)p, to *= (double)p;
+      bins(false, from, to, y, b0[1], b1[1]);
+      // what is kept ends in these bins
+      if (tid == (int)b1[1] / 4) sh.fscan[0] = y[(int)b1[1] % 4 + 1];
+      __syncthreads();
+      to = b1[1] < SMP_BINS - 1 ? (double)sh.fscan[0] * (1.0 + near_) : most_sum(last);
+      __syncthreads();
+    } else {
+      b0[1] = 3 * SMP_BINS, b1[1] = 2.5f * SMP_BINS;  // no window
+    }
+    bins(false, u * from, u * to, y, b0[0], b1[0]);
+    uint32_t before;
+    uint2 n_of[2][SMP_PARTS];
+    SmpExact r;
+    if (p < 1.f) {
+      r = exactly<2>(true, b0, b1, before, n_of);
+    } else {
+      r = exactly<1>(true, b0, b1, before, n_of);
+    }
+    all = r.all, n_all = r.n_all;
+    bool fits = true;
+#pragma unroll
+    for (int q = 0; q < SMP_PARTS; q++)
+      if (q < parts) fits &= n_of[0][q].x <= quota() && (p >= 1.f || n_of[1][q].x <= quota());
+    if (!fits) return false;
+    if (part) return true;
+    double mass = r.all, wt[2], c[2];
+    uint32_t kept = r.n_all;
+    uint64_t last_place = 0;
+    if (p < 1.f) {
+      const uint32_t n = r.n[1];
+      put_in_order(n_of[1], (int)n, 1);
+      sums_of((int)n, wt, c);
+      const double goal = (double)p * mass;
+      const uint32_t ahead = min(number((int)n, c, [&](int, double s) { return r.ahead[1] + s < goal; }), n - 1);
+      if (ahead % SMP_THREADS == tid) sh.found = {ordered()[ahead], r.ahead[1] + c[ahead / SMP_THREADS], r.n_ahead[1] + ahead + 1};
+      __syncthreads();
+      mass = sh.found.mass, kept = sh.found.count, last_place = sh.found.place;
+    }
+    const uint32_t n = r.n[0];
+    put_in_order(n_of[0], (int)n, 0);
+    sums_of((int)n, wt, c);
+    const double goal = u * mass;
+    const uint32_t ahead = min(number((int)n, c, [&](int, double s) { return r.ahead[0] + s <= goal; }), n - 1);
+    if (tid == 0) {
+      const uint64_t found = r.n_ahead[0] + ahead < kept ? ordered()[ahead] : last_place;  // (else by rounding alone)
+      answer((int)~(uint32_t)found, logprob(found, mass), kept);
+    }
+    return true;
+  }
+
+  // ---- the token at which the count or the sum crosses `goal`.  (kind SMP_PASS, the last one: for the first block alone)
+  __device__ SmpFound search(SmpKind kind, double goal, const float y[5]) {
+    float b0, b1;
+    bins(kind == SMP_COUNT, goal, goal, y, b0, b1);
     SmpWindow w;
-    const SmpExact r = exactly(all != nullptr, b0, b1, w.before);
-    if (all) *all = r.all, *n_all = r.n_all, goal = share * r.all;
-    w.mass = r.ahead, w.ahead = r.n_ahead, w.count = r.n;
-    if (w.count <= SMP_LIST) return among(kind, goal, w);
+    uint2 n_of[1][SMP_PARTS];
+    const SmpExact r = exactly<1>(false, &b0, &b1, w.before, n_of);
+    w.mass = r.ahead[0], w.ahead = r.n_ahead[0], w.count = r.n[0];
+    bool fits = true;
+#pragma unroll
+    for (int q = 0; q < SMP_PARTS; q++)
+      if (q < parts) fits &= n_of[0][q].x <= quota();
+    if (fits) return among(kind, goal, w, n_of[0]);
     // the ranks of these bins, which are monotone in the value
     const uint32_t least = rank_bits(floor_), most = rank_bits(m);
     uint32_t lo = least, hi = most;
@@ -564,23 +690,21 @@ struct SmpRow {
   }
 
   // ---- the window's tokens are in the first block's list
-  __device__ SmpFound among(SmpKind kind, double goal, const SmpWindow& w) {
+  __device__ SmpFound among(SmpKind kind, double goal, const SmpWindow& w, const uint2* from) {
     if (part == 0) {
-      put_in_order((int)w.count);
-      double wt[2];
-      weights((int)w.count, wt);
-      const double before = scan_mass(wt[0] + wt[1]);
-      const double c0 = w.mass + (before + wt[0]), c1 = w.mass + (before + wt[0] + wt[1]);
-      const uint32_t i0 = 2 * tid, i1 = i0 + 1, n = w.count;
-      uint32_t ahead = block_sum((i0 < n && !crosses(kind, c0, w.ahead + i0 + 1, goal)) +
-                                 (i1 < n && !crosses(kind, c1, w.ahead + i1 + 1, goal)));
+      const uint32_t n = w.count;
+      put_in_order(from, (int)n);
+      double wt[2], c[2];
+      sums_of((int)n, wt, c);
+      uint32_t ahead = number((int)n, c, [&](int i, double s) { return !crosses(kind, w.mass + s, w.ahead + i + 1, goal); });
       ahead = min(ahead, n - 1);
-      if (ahead / 2 == tid) {
-        const SmpFound f = {list()[ahead], ahead % 2 ? c1 : c0, w.ahead + ahead + 1};
-        for (int p = 0; p < parts; p++) *at(&sh.found, p) = f;
+      if (ahead % SMP_THREADS == tid) {
+        const SmpFound f = {ordered()[ahead], w.mass + c[ahead / SMP_THREADS], w.ahead + ahead + 1};
+        for (int p = 0; p < (kind == SMP_PASS ? 1 : parts); p++) *at(&sh.found, p) = f;
       }
+      __syncthreads();
     }
-    all_sync();
+    if (kind != SMP_PASS) all_sync();
     return sh.found;
   }
 
@@ -589,15 +713,17 @@ struct SmpRow {
     while (true) {
       all_sync();  // what was found, or listed, before has been read
       if (w.count <= SMP_LIST) {
-        if (tid == 0) sh.n = 0;
+        if (tid == 0) sh.n[0] = 0;
         __syncthreads();
+        // one list, whatever the blocks' shares: the first block's part of it is all
         uint64_t* to = at(list(), 0);
         each([&](float y, int id) {
           const uint32_t r = rank_bits(y);
-          if (r - w.lo <= w.hi - w.lo) to[w.before + atomicAdd(&sh.n, 1)] = place(r, (uint32_t)id);
+          if (r - w.lo <= w.hi - w.lo) to[w.before + atomicAdd(sh.n, 1)] = place(r, (uint32_t)id);
         });
         all_sync();
-        return among(kind, goal, w);
+        const uint2 all_in_first = make_uint2(w.count, 0);
+        return among(kind, goal, w, &all_in_first);
       }
       if (w.lo == w.hi) return tied(kind, goal, w);
       const uint32_t range = w.hi - w.lo, hi = w.hi, shift = max(0, 28 - __clz(range));
@@ -705,8 +831,8 @@ struct SmpRow {
     const float min_p = a.min_p ? a.min_p[row] : 0.f;
     int k = a.top_k ? a.top_k[row] : 0;
     double u = a.uniform[row];
-    uint32_t own;
-    const uint32_t most = load(own);
+    const uint2* told = load(k);
+    const uint32_t most = most_of(&told->x);
     if (k < 0 || k >= a.vocab) k = 0;
     u = u > 0.0 ? fmin(u, 0x1.fffffffffffffp-1) : 0.0;
     m = rank_value(most);
@@ -719,36 +845,33 @@ struct SmpRow {
       each([&](float y, int id) {
         if (y == m) first = max(first, ~(uint32_t)id);
       });
-      const uint32_t* all = tell(block_max(first));
+      told = tell(block_max(first));
       if (part == 0 && tid == 0) {
-        for (int q = 0; q < parts; q++) first = max(first, all[q]);
+        for (int q = 0; q < parts; q++) first = max(first, told[q].x);
         answer((int)~first, 0.0, 1);
       }
       return;
     }
     top = m;
     inv_t = 1.0 / (double)t;
-    rate = inv_t * (64 * 1.44269504088896340736);
-    cut_off = 620.f * t;
+    // A temperature under 2^-10 of m's last bit leaves nothing but m, as that one does, and keeps z within 32 bits.
+    const float below = rank_value(most - 1), t_weight = fmaxf(t, (m - below) * 0x1p-10f);
+    rate = 64 * 1.44269504088896340736 / (double)t_weight;
+    lowest = fminf(m - 600.f * t_weight, below);
     floor_ = -FLT_MAX;
     if (min_p >= 1.f) floor_ = m;
     else if (min_p > 0.f) floor_ = fmaxf(floor_, __double2float_ru(top + (double)t * log((double)min_p)));
     if ((k && k <= SMP_TOP) || min_p > 0.f) {
       float from = floor_;
       if (k && k <= SMP_TOP) {
-        const uint32_t* all = tell(reached((k + parts - 1) / parts, own));
-        uint32_t least = 0xFFFFFFFFu;
-        for (int q = 0; q < parts; q++) least = min(least, all[q]);
+        const uint32_t least = least_of(&told->y);
         from = fmaxf(from, rank_value(max(least, rank_bits(-FLT_MAX))));
       }
-      const uint32_t* all;
-      const uint32_t n = gather(from, all);
-      if (n <= SMP_LIST) {
-        uint32_t before = 0;
-        for (int q = 0; q < part; q++) before += all[q];
-        for (uint32_t i = tid; i < all[part]; i += SMP_THREADS) at(list(), 0)[before + i] = own_list()[i];
-        all_sync();
-        if (part == 0) finish((int)n, k, p, u);
+      told = gather(from);
+      if (room(told)) {
+        int n = 0;
+        for (int q = 0; q < parts; q++) n += (int)told[q].x;
+        if (part == 0) finish(told, n, k, p, u);
         return;
       }
     }
@@ -756,25 +879,26 @@ struct SmpRow {
     __syncthreads();
     double mass = 0.0;
     uint32_t kept = 0;
-    uint64_t last = 0;      // the last place that is kept, where that is known
+    uint64_t end = 0;       // the last place that is kept, where that is known
+    float y[5], last;
     bool known = false;     // whether mass and kept are
     if (k) {
-      measure<true>();
-      if ((uint32_t)k < __float_as_uint(along()[SMP_BINS - 1])) {
-        const SmpFound f = search(SMP_COUNT, (double)k, 0.0, nullptr, nullptr);
-        mass = f.mass, kept = f.count, last = f.place;
+      measure<true>(y, last);
+      if ((uint32_t)k < __float_as_uint(last)) {
+        const SmpFound f = search(SMP_COUNT, (double)k, y);
+        mass = f.mass, kept = f.count, end = f.place;
         known = true;
       }
       all_sync();  // the histogram has been read
     }
-    measure<false>();
+    measure<false>(y, last);
+    if (!known && at_once(p, u, y, last, mass, kept)) return;
     if (p < 1.f) {
-      const SmpFound f = search(SMP_REACH, (double)p * mass, (double)p, known ? nullptr : &mass, &kept);
-      if (f.count < kept) mass = f.mass, kept = f.count, last = f.place;
-      known = true;
+      const SmpFound f = search(SMP_REACH, (double)p * mass, y);
+      if (f.count < kept) mass = f.mass, kept = f.count, end = f.place;
     }
-    SmpFound f = search(SMP_PASS, u * mass, u, known ? nullptr : &mass, &kept);
-    if (f.count > kept) f.place = last;  // by rounding alone
+    SmpFound f = search(SMP_PASS, u * mass, y);
+    if (f.count > kept) f.place = end;  // by rounding alone
     if (part == 0 && tid == 0) answer((int)~(uint32_t)f.place, logprob(f.place, mass), kept);
   }
 };
@@ -791,13 +915,18 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const __grid_con
 }
 
 constexpr int SMP_MOST = 170 * 1024;  // bytes of a block's part of a row, held
+constexpr int SMP_PART = 75 * 1024;   // the same where two blocks are to fit an SM
 
 template <typename In>
-cudaError_t launch(IrisSample* a, cudaStream_t stream) {
+cudaError_t launch(IrisSample* a, int num_sms, cudaStream_t stream) {
   const int64_t bytes = (int64_t)a->vocab * (int64_t)sizeof(In) + 16;
-  // blocks on a row: as many as leave each 16 KB
+  // Blocks on a row: as many as leave each no more than SMP_PART of it, so that two fit an SM, and more where the device has room
+  // for them and each keeps 16 KB
   a->parts = 1;
-  while (a->parts < SMP_PARTS && bytes > (int64_t)a->parts * 16384) a->parts *= 2;
+  while (a->parts < SMP_PARTS &&
+         (bytes > (int64_t)a->parts * SMP_PART ||
+          (bytes > (int64_t)a->parts * 16384 && (int64_t)a->rows * a->parts * 2 <= 2 * num_sms)))
+    a->parts *= 2;
   const int64_t vecs = (bytes + 15) / 16, held = (vecs + a->parts - 1) / a->parts * 16;
   const bool fits = held <= SMP_MOST;
   a->held_bytes = fits ? (int)((held + 127) / 128 * 128) : 0;
@@ -820,6 +949,6 @@ extern "C" cudaError_t iris_sample_init(void) {
   return cudaSuccess;
 }
 
-extern "C" cudaError_t iris_launch_sample(IrisSample* a, int f32, cudaStream_t stream) {
-  return f32 ? launch<float>(a, stream) : launch<__nv_bfloat16>(a, stream);
+extern "C" cudaError_t iris_launch_sample(IrisSample* a, int f32, int num_sms, cudaStream_t stream) {
+  return f32 ? launch<float>(a, num_sms, stream) : launch<__nv_bfloat16>(a, num_sms, stream);
 }
