@@ -31,15 +31,16 @@ namespace {
 // with exact sums, until few are left, or tokens of one value, of which the id decides.
 // Weights and sums are 64-bit: a token is taken by where a sum of 100000 weights
 // ends, and with 32 bits one row in a hundred would take its neighbour.
-constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32, SMP_PARTS = 8;
-constexpr int SMP_LIST = 1024;  // tokens put in order: two a thread
+constexpr int SMP_THREADS = 256, SMP_WARPS = SMP_THREADS / 32, SMP_PARTS = 8;
+constexpr int SMP_LIST = 1024;  // tokens put in order
 constexpr int SMP_TOP = 512;    // largest top-k whose tokens are looked for through a bound
-constexpr int SMP_BINS = 2048;  // four a thread
+constexpr int SMP_BINS = 2048;
 constexpr float SMP_SPAN = 24.f;      // (m - x) / t that the bins cover; the last one holds all that is below
 constexpr int SMP_CUT = 16, SMP_CUTTERS = 64;  // bins of a closer look, threads that fill bins of their own
 constexpr int SMP_SORT = 1024;  // places of the sort by value
-static_assert(SMP_BINS == 4 * SMP_THREADS && SMP_LIST == 2 * SMP_THREADS && SMP_SORT == 2 * SMP_THREADS && SMP_CUT == SMP_WARPS,
-              "shares of a thread, and warp");
+constexpr int SMP_OWN = 128;    // vectors of a warp's list
+constexpr int SMP_MINE = SMP_BINS / SMP_THREADS, SMP_EACH = SMP_LIST / SMP_THREADS;  // of a thread
+static_assert(SMP_MINE % 4 == 0 && SMP_SORT == SMP_LIST, "shares of a thread");
 
 struct SmpSums {  // of the closer bins, from each block of the cluster
   double mass[SMP_PARTS][SMP_CUT];
@@ -74,7 +75,7 @@ struct SmpShared {
 constexpr int SMP_HIST = SMP_BINS * 4, SMP_ALONG = SMP_BINS * 4;
 constexpr int SMP_TAIL = 2 * SMP_LIST * 8;
 constexpr int SMP_WORK = SMP_HIST + SMP_ALONG + SMP_TAIL;
-static_assert(SMP_TAIL >= SMP_CUT * SMP_CUTTERS * (8 + 4) && SMP_ALONG >= SMP_SORT * 4 && SMP_ALONG >= SMP_LIST * 8 &&
+static_assert(SMP_TAIL >= SMP_CUT * SMP_CUTTERS * (8 + 4) && SMP_ALONG >= SMP_SORT * 4 && SMP_ALONG >= SMP_WARPS * SMP_OWN * 4 && SMP_ALONG >= SMP_LIST * 8 &&
               SMP_HIST >= SMP_LIST * 8, "the bins and lists fit");
 
 struct SmpWindow {  // part of the line: ranks lo .. hi, `count` tokens, with sums over what stands ahead of it
@@ -98,6 +99,7 @@ struct SmpRow {
   double top, inv_t, rate;   // rate: 64 log2(e) / t
   float inv_bin;
   float unit;                // of the histogram's weights, so that a block's tokens in one bin stay within 32 bits
+  bool plain;                // no min-p, and a temperature with which -inf weighs nothing by itself
   float near_;               // relative error of the sums along the bins, with room to spare: half a unit of rounding, 2^-17 for
                              // distances and bins' weights in 32 bits, 2^-20 for sums in 32 bits
   uint32_t turn = 0;
@@ -236,7 +238,7 @@ struct SmpRow {
   // share of k tokens reaches
   __device__ const uint2* load(int k) {
     float best = -INFINITY;
-    constexpr int FLY = 10;  // 76 KB of a row in one round
+    constexpr int FLY = 20;  // 75 KB of a row in one round
     for (int b = tid; b < nv; b += FLY * SMP_THREADS) {
       uint4 u[FLY];
 #pragma unroll
@@ -306,23 +308,30 @@ struct SmpRow {
 
   // ---- by the first block: the blocks' tokens, n in all, in order, largest first, into ordered().  (Of many, the sums along
   // the bins are lost, those of the first block)
-  __device__ void put_in_order(const uint2* from, int n, int which = 0) {
+  __device__ static int tokens_of(const uint2& v, int) { return (int)v.x; }
+  __device__ static int tokens_of(const SmpExact& v, int which) { return (int)v.n[which]; }
+  template <typename Found>
+  __device__ void put_in_order(const Found* from, int n, int which = 0, int blocks = SMP_PARTS) {
     uint64_t* l = ordered();
-    __syncthreads();
-    uint64_t mine[2];  // tokens tid and tid + SMP_THREADS of all
+    // of the tokens of all blocks in a row, this thread's: tid, tid + SMP_THREADS ..
+    uint64_t mine[SMP_EACH] = {};
+    int begin = 0;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      int i = tid + j * SMP_THREADS, p = 0;
-      mine[j] = 0;
-      if (i >= n) continue;
-      while (i >= (int)from[p].x) i -= (int)from[p++].x;
-      mine[j] = list(which)[p * quota() + i];
+    for (int p = 0; p < SMP_PARTS; p++) {
+      if (p >= parts || p >= blocks) break;
+      const int here = tokens_of(from[p], which);
+#pragma unroll
+      for (int j = 0; j < SMP_EACH; j++) {
+        const int i = tid + j * SMP_THREADS - begin;
+        if (i >= 0 && i < here) mine[j] = list(which)[p * quota() + i];
+      }
+      begin += here;
     }
     if (n <= 128) {
-      // how many are ahead of each: n^2 comparisons, 4 to 32 threads a token
+      // how many are ahead of each: n^2 comparisons, 2 to 32 threads a token
       if (tid < n) l[tid] = mine[0];
       __syncthreads();
-      int per = 4;
+      int per = 1;
       while (per < 32 && 2 * per * n <= SMP_THREADS) per *= 2;
       const int i = tid / per;
       const uint64_t p = i < n ? l[i] : 0;
@@ -340,7 +349,7 @@ struct SmpRow {
     uint64_t* sorted = list(which);
     uint32_t top_rank = 0, low_rank = 0;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < SMP_EACH; j++) {
       count[tid + j * SMP_THREADS] = 0;
       const uint32_t r = (uint32_t)(mine[j] >> 32);
       if (r) top_rank = max(top_rank, r), low_rank = max(low_rank, ~r);
@@ -350,47 +359,63 @@ struct SmpRow {
     const int shift = max(0, 22 - __clz(top_rank - low_rank));
     auto where = [&](uint64_t p) { return (top_rank - (uint32_t)(p >> 32)) >> shift; };
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int j = 0; j < SMP_EACH; j++)
       if (mine[j]) atomicAdd(count + where(mine[j]), 1u);
     __syncthreads();
-    const uint2 two = reinterpret_cast<uint2*>(count)[tid];
-    uint32_t all, before = scan_count(two.x + two.y, &all);
-    reinterpret_cast<uint2*>(count)[tid] = make_uint2(before, before + two.x);
+    uint32_t own[SMP_EACH], sum = 0, all;
+#pragma unroll
+    for (int j = 0; j < SMP_EACH; j++) own[j] = count[SMP_EACH * tid + j], sum += own[j];
+    uint32_t before = scan_count(sum, &all);
+#pragma unroll
+    for (int j = 0; j < SMP_EACH; j++) count[SMP_EACH * tid + j] = before, before += own[j];
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int j = 0; j < SMP_EACH; j++)
       if (mine[j]) sorted[atomicAdd(count + where(mine[j]), 1u)] = mine[j];  // a place's count becomes its end
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < SMP_EACH; j++) {
       if (!mine[j]) continue;
-      const uint32_t w = where(mine[j]), begin = w ? count[w - 1] : 0, end = count[w];
-      uint32_t ahead = begin;
-      for (uint32_t i = begin; i < end; i++) ahead += sorted[i] > mine[j];
+      const uint32_t w = where(mine[j]), from_here = w ? count[w - 1] : 0, end = count[w];
+      uint32_t ahead = from_here;
+      for (uint32_t i = from_here; i < end; i++) ahead += sorted[i] > mine[j];
       l[ahead] = mine[j];
     }
     __syncthreads();
   }
-  // number of tokens for which f(token's number, sum up to and with it) holds; those of `n` in order, w and c as sums_of() has it
+  // number of the n tokens in order for which f(token, weight, sum up to and with it) holds
   template <typename F>
-  __device__ uint32_t number(int n, const double c[2], F f) const {
-    uint32_t r = __syncthreads_count(tid < n && f(tid, c[0]));
-    if (n > SMP_THREADS) r += __syncthreads_count(tid + SMP_THREADS < n && f(tid + SMP_THREADS, c[1]));
+  __device__ uint32_t number(int n, const double w[SMP_EACH], const double c[SMP_EACH], F f) const {
+    uint32_t r = 0;
+#pragma unroll
+    for (int j = 0; j < SMP_EACH; j++) {
+      if (j * SMP_THREADS >= n) break;
+      const int i = tid + j * SMP_THREADS;
+      r += __syncthreads_count(i < n && f(i, w[j], c[j]));
+    }
     return r;
   }
-  // the sums of the weights up to and with tokens tid and tid + SMP_THREADS of n in order
-  __device__ void sums_of(int n, double w[2], double c[2]) {
-    auto one = [&](int i) { return i < n ? weight(rank_value((uint32_t)(ordered()[i] >> 32))) : 0.0; };
-    w[0] = one(tid);
-    double first;
-    c[0] = scan(w[0], sh.scan, &first) + w[0];
-    w[1] = c[1] = 0.0;
-    if (n > SMP_THREADS) {
-        w[1] = one(tid + SMP_THREADS);
-      c[1] = first + (scan_mass(w[1]) + w[1]);
+  // weights of the tokens tid, tid + SMP_THREADS .. of n in order, and the sums up to and with them
+  __device__ void sums_of(int n, double w[SMP_EACH], double c[SMP_EACH]) {
+    double first = 0.0;
+#pragma unroll
+    for (int j = 0; j < SMP_EACH; j++) {
+      w[j] = c[j] = 0.0;
+      if (j * SMP_THREADS >= n) continue;
+      const int i = tid + j * SMP_THREADS;
+      if (i < n) w[j] = weight(rank_value((uint32_t)(ordered()[i] >> 32)));
+      double sum;
+      c[j] = first + (scan(w[j], sh.scan, &sum) + w[j]);
+      first += sum;
     }
   }
-
+  // f(token, sum) by the thread that has token i
+  template <typename F>
+  __device__ void at_token(uint32_t i, const double c[SMP_EACH], F f) const {
+#pragma unroll
+    for (int j = 0; j < SMP_EACH; j++)
+      if (tid + j * SMP_THREADS == (int)i) f(ordered()[i], c[j]);
+  }
   __device__ void answer(int id, double logprob, uint32_t kept) const {
     const int row = blockIdx.x / parts;
     a.ids[row] = id;
@@ -405,31 +430,34 @@ struct SmpRow {
   __device__ void finish(const uint2* from, int n, int k, float p, double u) {
     put_in_order(from, n);
     if (k) n = min(n, k);
-    double w[2], c[2];
+    double w[SMP_EACH], c[SMP_EACH];
     sums_of(n, w, c);
     double* sums = line();
-    sums[tid] = c[0], sums[tid + SMP_THREADS] = c[1];
+#pragma unroll
+    for (int j = 0; j < SMP_EACH; j++) sums[tid + j * SMP_THREADS] = c[j];
     __syncthreads();
     const double mass = sums[n - 1];
     uint32_t kept = n;
     if (p < 1.f) {
       const double goal = (double)p * mass;
-      kept = max(number(n, c, [&](int i, double s) { return (i ? sums[i - 1] : 0.0) < goal; }), 1u);
+      kept = max(number(n, w, c, [&](int i, double, double) { return (i ? sums[i - 1] : 0.0) < goal; }), 1u);
     }
     const double m_kept = sums[kept - 1], goal = u * m_kept;
-    uint32_t pick = number((int)kept, c, [&](int, double s) { return s <= goal; });
+    uint32_t pick = number((int)kept, w, c, [&](int, double, double s) { return s <= goal; });
     if (pick == kept)  // by rounding: the last with a weight (the first one weighs 1)
-      pick = number((int)kept, c, [&](int i, double) { return w[i >= SMP_THREADS] > 0.0; }) - 1;
+      pick = number((int)kept, w, c, [&](int, double v, double) { return v > 0.0; }) - 1;
     if (tid == 0) answer((int)~(uint32_t)ordered()[pick], logprob(ordered()[pick], m_kept), kept);
   }
 
   // ---- how the line grows along the bins: along()[b] is the sum up to and with bin b, to near_ (or the count, a whole number)
-  __device__ float distance(float y) const { return fminf(fminf(m - y, FLT_MAX) * inv_bin, SMP_BINS - 1); }
+  __device__ float distance(float y) const {
+    return fminf((plain ? m - y : fminf(m - y, FLT_MAX)) * inv_bin, SMP_BINS - 1);
+  }
   __device__ static float nearest(float d) { return (d + 0x1.8p23f) - 0x1.8p23f; }  // whole number, ties to even
   __device__ float bin_of(float y) const { return nearest(distance(y)); }           // the bins are around whole numbers
-  // y: the sums up to and with this thread's four bins, and the bin before them
+  // y: the sums up to and with this thread's bins, and the bin before them
   template <bool COUNTS>
-  __device__ void measure(float y[5], float& last) {
+  __device__ void measure(float y[SMP_MINE + 1], float& last) {
     uint32_t* h = hist();
     for (int i = tid; i < SMP_BINS; i += SMP_THREADS) h[i] = 0;
     __syncthreads();
@@ -443,92 +471,130 @@ struct SmpRow {
         } else {
           // unit e^-r for the way r behind the bin's middle, |r| <= 12 / 2048 (the series' next term is under 2^-24), as a
           // whole number
-          const float r = (d - b) * (SMP_SPAN / SMP_BINS);
-          const float w = fmaf(unit, r * fmaf(0.5f, r, -1.f), unit + 0x1p23f);
+          constexpr float step = SMP_SPAN / SMP_BINS;
+          const float r = d - b, w = fmaf(r, fmaf(r, 0.5f * step * step * unit, -step * unit), unit + 0x1p23f);
           // (no branches around the additions: they would keep those of a vector apart)
-          atomicAdd(h + at, y[i] >= floor_ && b < SMP_BINS - 1 ? __float_as_uint(w) - 0x4B000000u : 0u);
+          atomicAdd(h + at, b < SMP_BINS - 1 && (plain || y[i] >= floor_) ? __float_as_uint(w) - 0x4B000000u : 0u);
         }
       }
     });
     all_sync();
-    uint32_t n[4] = {0, 0, 0, 0};
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t n[SMP_MINE] = {}, n_all = 0;
+    float s[SMP_MINE] = {}, s_all = 0.f;
 #pragma unroll
     for (int p = 0; p < SMP_PARTS; p++) {
       if (p >= parts) break;
-      const uint4 u = *reinterpret_cast<const uint4*>(at(h, p) + 4 * tid);
-      if (COUNTS) n[0] += u.x, n[1] += u.y, n[2] += u.z, n[3] += u.w;
-      else s[0] += (float)u.x, s[1] += (float)u.y, s[2] += (float)u.z, s[3] += (float)u.w;
+      const uint4* from = reinterpret_cast<const uint4*>(at(h, p) + SMP_MINE * tid);
+#pragma unroll
+      for (int j = 0; j < SMP_MINE; j += 4) {
+        const uint4 u = from[j / 4];
+        if (COUNTS) n[j] += u.x, n[j + 1] += u.y, n[j + 2] += u.z, n[j + 3] += u.w;
+        else s[j] += (float)u.x, s[j + 1] += (float)u.y, s[j + 2] += (float)u.z, s[j + 3] += (float)u.w;
+      }
     }
     if (COUNTS) {
-      uint32_t all, before = scan_count(n[0] + n[1] + n[2] + n[3], &all);
+#pragma unroll
+      for (int j = 0; j < SMP_MINE; j++) n_all += n[j];
+      uint32_t all, before = scan_count(n_all, &all);
       last = __uint_as_float(all);
       y[0] = __uint_as_float(before);
 #pragma unroll
-      for (int j = 0; j < 4; j++) before += n[j], y[j + 1] = __uint_as_float(before);
+      for (int j = 0; j < SMP_MINE; j++) before += n[j], y[j + 1] = __uint_as_float(before);
     } else {
-      const float one = exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * 4 * tid) / unit;
+      const float one = exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * SMP_MINE * tid) / unit;
 #pragma unroll
-      for (int j = 0; j < 4; j++) s[j] *= one * exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * j);
-      float before = scan_float((s[0] + s[1]) + (s[2] + s[3]), &last);
+      for (int j = 0; j < SMP_MINE; j++) s[j] *= one * exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * j), s_all += s[j];
+      float before = scan_float(s_all, &last);
       y[0] = before;
 #pragma unroll
-      for (int j = 0; j < 4; j++) before += s[j], y[j + 1] = before;
+      for (int j = 0; j < SMP_MINE; j++) before += s[j], y[j + 1] = before;
     }
   }
   // Most that the tokens of the last bin, which was not measured, can weigh.
   __device__ double tail() const { return (double)a.vocab * exp2_approx(-kLog2e * SMP_SPAN * (SMP_BINS - 2) / SMP_BINS); }
 
-  // ---- exact sums and counts of all tokens (all: else only the counts) and of those ahead of bin b0[i], and the tokens of bins
-  // b0[i] .. b1[i] into the first block's lists, as far as there is room, for one window or two.  n_of[i]: how many each block
-  // has; before: of the first window, in the blocks ahead of this one
+  // ---- exact sums of all tokens (if all; for one window their number too) and of those ahead of bin b0[i], and the tokens of bins
+  // b0[i] .. b1[i] into the first block's lists, as far as there is room, for one window or two.  From each block
   template <int WINDOWS>
-  __device__ SmpExact exactly(bool all, const float b0[WINDOWS], const float b1[WINDOWS], uint32_t& before,
-                              uint2 n_of[WINDOWS][SMP_PARTS]) {
+  __device__ const SmpExact* exactly(bool all, const float b0[WINDOWS], const float b1[WINDOWS]) {
     if (tid < 2) sh.n[tid] = 0;
     __syncthreads();
     SmpExact e = {};
-    float behind = b0[0], last = b1[0];
-    if (WINDOWS == 2) behind = fmaxf(behind, b0[WINDOWS - 1]), last = fmaxf(last, b1[WINDOWS - 1]);
-    vectors([&](const float* y, int id) {
-      float b[VEC], first = 2 * SMP_BINS;
+    // The vectors that have a token of a window, few, are put into a list of the warp's own and looked at by all its lanes when
+    // there are enough.
+    uint32_t* own = reinterpret_cast<uint32_t*>(along()) + tid / 32 * SMP_OWN;
+    uint32_t found = 0;
+    auto look = [&]() {
+      __syncwarp();
+      for (uint32_t j = tid % 32; j < found; j += 32) {
+        const int v = (int)own[j], id = first_id(v);
+        float y[VEC];
+        vec_values<In>(vec(v), y);
 #pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        b[i] = y[i] >= floor_ ? bin_of(y[i]) : 2 * SMP_BINS;
-        e.n_all += b[i] < SMP_BINS;
-        first = fminf(first, b[i]);
-      }
-      const bool some = __any_sync(__activemask(), first < behind);
-      if (all || some) {
-        double w[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; i++) w[i] = weight(y[i]);
-        if (all) {
-#pragma unroll
-          for (int i = 0; i < VEC; i++) e.all += b[i] < SMP_BINS ? w[i] : 0.0;
-        }
-        if (some) {
+        for (int i = 0; i < VEC; i++) {
+          const float b = bin_of(y[i]);
 #pragma unroll
           for (int k = 0; k < WINDOWS; k++)
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-              e.ahead[k] += b[i] < b0[k] ? w[i] : 0.0;
-              e.n_ahead[k] += b[i] < b0[k];
-            }
-        }
-      }
-      if (first <= last) {
-#pragma unroll
-        for (int k = 0; k < WINDOWS; k++)
-#pragma unroll
-          for (int i = 0; i < VEC; i++)
-            if (b[i] >= b0[k] && b[i] <= b1[k]) {
+            if (b >= b0[k] && b <= b1[k] && y[i] >= floor_) {
               e.n[k]++;
               const int n = (int)atomicAdd(sh.n + k, 1u);
               if (n < quota()) at(list(k), 0)[part * quota() + n] = place(rank_bits(y[i]), (uint32_t)(id + i));
             }
+        }
       }
-    });
+      __syncwarp();
+      found = 0;
+    };
+    for (int v0 = 0; v0 < nv; v0 += SMP_THREADS) {
+      const int v = v0 + tid;
+      bool hit = false;
+      if (v < nv) {
+        float y[VEC], b[VEC], first = SMP_BINS;
+        vec_values<In>(vec(v), y);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          b[i] = bin_of(y[i]);
+          if (!plain && !(y[i] >= floor_)) b[i] = 2 * SMP_BINS;
+          first = fminf(first, b[i]);
+#pragma unroll
+          for (int k = 0; k < WINDOWS; k++) hit |= b[i] >= b0[k] && b[i] <= b1[k];
+        }
+        bool ahead = first < b0[0];
+        if (WINDOWS == 2) ahead |= first < b0[WINDOWS - 1];
+        if (all || ahead) {
+          double w[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; i++) w[i] = weight(y[i]);
+          if (all) {
+            if (plain) {
+#pragma unroll
+              for (int i = 0; i < VEC; i += 2) e.all += w[i] + w[i + 1];
+            } else {
+#pragma unroll
+              for (int i = 0; i < VEC; i++) e.all += b[i] < SMP_BINS ? w[i] : 0.0;
+            }
+          }
+          if (ahead) {
+#pragma unroll
+            for (int k = 0; k < WINDOWS; k++)
+#pragma unroll
+              for (int i = 0; i < VEC; i++) {
+                e.ahead[k] += b[i] < b0[k] ? w[i] : 0.0;
+                e.n_ahead[k] += b[i] < b0[k];
+              }
+          }
+        }
+        if (WINDOWS == 1 && all) {  // (with top-p the number of all is not asked for)
+#pragma unroll
+          for (int i = 0; i < VEC; i++) e.n_all += y[i] >= floor_;
+        }
+      }
+      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+      if (hit) own[found + __popc(hits & ((1u << tid % 32) - 1))] = (uint32_t)v;
+      found += __popc(hits);
+      if (found > SMP_OWN - 32) look();
+    }
+    look();
     auto sums = [](SmpExact& v, int lanes) {
       for (int o = lanes / 2; o; o >>= 1) {
         v.all += __shfl_xor_sync(0xffffffffu, v.all, o);
@@ -553,21 +619,22 @@ struct SmpRow {
       if (tid < parts) *at(told + part, tid) = v;
     }
     all_sync();
+    return told;
+  }
+  // over the blocks
+  __device__ SmpExact sum_of(const SmpExact* told) const {
     SmpExact r = {};
-    before = 0;
-#pragma unroll
-    for (int p = 0; p < SMP_PARTS; p++) {
-      if (p >= parts) break;
+    for (int p = 0; p < parts; p++) {
       const SmpExact v = told[p];
       r.all += v.all, r.n_all += v.n_all;
-      if (p < part) before += v.n[0];
-#pragma unroll
-      for (int k = 0; k < WINDOWS; k++) {
-        r.ahead[k] += v.ahead[k], r.n_ahead[k] += v.n_ahead[k], r.n[k] += v.n[k];
-        n_of[k][p].x = v.n[k];
-      }
+      for (int k = 0; k < 2; k++) r.ahead[k] += v.ahead[k], r.n_ahead[k] += v.n_ahead[k], r.n[k] += v.n[k];
     }
     return r;
+  }
+  // whether the tokens of the windows have all found room
+  __device__ bool room(const SmpExact* told) const {
+    const SmpExact* v = told + (tid % 32 < parts ? tid % 32 : 0);
+    return __reduce_max_sync(0xffffffffu, max(v->n[0], v->n[1])) <= quota();
   }
 
   __device__ static bool crosses(SmpKind kind, double mass, uint32_t count, double goal) {
@@ -576,21 +643,18 @@ struct SmpRow {
 
   // ---- the first bin with which a sum of `from` may be reached (a count: is), and the first with which one of `to` surely is
   // passed; y as measure() gives it
-  __device__ void bins(bool counts, double from, double to, const float y[5], float& b0, float& b1) {
+  __device__ void bins(bool counts, double from, double to, const float y[SMP_MINE + 1], float& b0, float& b1) {
     if (tid == 0) sh.lo = sh.hi = SMP_BINS - 1;
     __syncthreads();
-    bool may[5], must[5];
+    bool may = false, must = false;
 #pragma unroll
-    for (int j = 0; j < 5; j++) {
-      may[j] = counts ? (double)__float_as_uint(y[j]) >= from : (double)(y[j] * (1.f + near_)) >= from;
-      must[j] = counts ? may[j] : (double)(y[j] * (1.f - near_)) > to;
-    }
-    if (tid == 0) may[0] = must[0] = false;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int b = 4 * tid + j;
-      if (b < SMP_BINS - 1 && may[j + 1] && !may[j]) sh.lo = b;
-      if (b < SMP_BINS - 1 && must[j + 1] && !must[j]) sh.hi = b;
+    for (int j = 0; j <= SMP_MINE; j++) {
+      const bool now_may = counts ? (double)__float_as_uint(y[j]) >= from : (double)(y[j] * (1.f + near_)) >= from;
+      const bool now_must = counts ? now_may : (double)(y[j] * (1.f - near_)) > to;
+      const int b = SMP_MINE * tid + j - 1;
+      if (j && b < SMP_BINS - 1 && now_may && !may) sh.lo = b;
+      if (j && b < SMP_BINS - 1 && now_must && !must) sh.hi = b;
+      may = now_may && (j || tid), must = now_must && (j || tid);
     }
     __syncthreads();
     b0 = (float)sh.lo, b1 = (float)sh.hi;
@@ -602,14 +666,16 @@ struct SmpRow {
 
   // ---- no top-k: top-p, and the token, in one pass.  How much is kept is known well enough from the bins to say where the
   // token may be.  False where the tokens there find no room; then the sum and number of all are known.
-  __device__ bool at_once(float p, double u, const float y[5], float last, double& all, uint32_t& n_all) {
+  __device__ bool at_once(float p, double u, const float y[SMP_MINE + 1], float last, double& all, uint32_t& n_all) {
     float b0[2], b1[2];
     double from = least_sum(last), to = most_sum(last);
     if (p < 1.f) {
       from *= (double)p, to *= (double)p;
       bins(false, from, to, y, b0[1], b1[1]);
       // what is kept ends in these bins
-      if (tid == (int)b1[1] / 4) sh.fscan[0] = y[(int)b1[1] % 4 + 1];
+#pragma unroll
+      for (int j = 0; j < SMP_MINE; j++)
+        if (SMP_MINE * tid + j == (int)b1[1]) sh.fscan[0] = y[j + 1];
       __syncthreads();
       to = b1[1] < SMP_BINS - 1 ? (double)sh.fscan[0] * (1.0 + near_) : most_sum(last);
       __syncthreads();
@@ -617,39 +683,32 @@ struct SmpRow {
       b0[1] = 3 * SMP_BINS, b1[1] = 2.5f * SMP_BINS;  // no window
     }
     bins(false, u * from, u * to, y, b0[0], b1[0]);
-    uint32_t before;
-    uint2 n_of[2][SMP_PARTS];
-    SmpExact r;
-    if (p < 1.f) {
-      r = exactly<2>(true, b0, b1, before, n_of);
-    } else {
-      r = exactly<1>(true, b0, b1, before, n_of);
+    const SmpExact* told = p < 1.f ? exactly<2>(true, b0, b1) : exactly<1>(true, b0, b1);
+    if (!room(told)) {
+      const SmpExact r = sum_of(told);
+      all = r.all, n_all = r.n_all;
+      return false;
     }
-    all = r.all, n_all = r.n_all;
-    bool fits = true;
-#pragma unroll
-    for (int q = 0; q < SMP_PARTS; q++)
-      if (q < parts) fits &= n_of[0][q].x <= quota() && (p >= 1.f || n_of[1][q].x <= quota());
-    if (!fits) return false;
     if (part) return true;
-    double mass = r.all, wt[2], c[2];
+    const SmpExact r = sum_of(told);
+    double mass = r.all, w[SMP_EACH], c[SMP_EACH];
     uint32_t kept = r.n_all;
     uint64_t last_place = 0;
     if (p < 1.f) {
       const uint32_t n = r.n[1];
-      put_in_order(n_of[1], (int)n, 1);
-      sums_of((int)n, wt, c);
+      put_in_order(told, (int)n, 1);
+      sums_of((int)n, w, c);
       const double goal = (double)p * mass;
-      const uint32_t ahead = min(number((int)n, c, [&](int, double s) { return r.ahead[1] + s < goal; }), n - 1);
-      if (ahead % SMP_THREADS == tid) sh.found = {ordered()[ahead], r.ahead[1] + c[ahead / SMP_THREADS], r.n_ahead[1] + ahead + 1};
+      const uint32_t ahead = min(number((int)n, w, c, [&](int, double, double s) { return r.ahead[1] + s < goal; }), n - 1);
+      at_token(ahead, c, [&](uint64_t place, double s) { sh.found = {place, r.ahead[1] + s, r.n_ahead[1] + ahead + 1}; });
       __syncthreads();
       mass = sh.found.mass, kept = sh.found.count, last_place = sh.found.place;
     }
     const uint32_t n = r.n[0];
-    put_in_order(n_of[0], (int)n, 0);
-    sums_of((int)n, wt, c);
+    put_in_order(told, (int)n, 0);
+    sums_of((int)n, w, c);
     const double goal = u * mass;
-    const uint32_t ahead = min(number((int)n, c, [&](int, double s) { return r.ahead[0] + s <= goal; }), n - 1);
+    const uint32_t ahead = min(number((int)n, w, c, [&](int, double, double s) { return r.ahead[0] + s <= goal; }), n - 1);
     if (tid == 0) {
       const uint64_t found = r.n_ahead[0] + ahead < kept ? ordered()[ahead] : last_place;  // (else by rounding alone)
       answer((int)~(uint32_t)found, logprob(found, mass), kept);
@@ -658,18 +717,15 @@ struct SmpRow {
   }
 
   // ---- the token at which the count or the sum crosses `goal`.  (kind SMP_PASS, the last one: for the first block alone)
-  __device__ SmpFound search(SmpKind kind, double goal, const float y[5]) {
+  __device__ SmpFound search(SmpKind kind, double goal, const float y[SMP_MINE + 1]) {
     float b0, b1;
     bins(kind == SMP_COUNT, goal, goal, y, b0, b1);
     SmpWindow w;
-    uint2 n_of[1][SMP_PARTS];
-    const SmpExact r = exactly<1>(false, &b0, &b1, w.before, n_of);
-    w.mass = r.ahead[0], w.ahead = r.n_ahead[0], w.count = r.n[0];
-    bool fits = true;
-#pragma unroll
-    for (int q = 0; q < SMP_PARTS; q++)
-      if (q < parts) fits &= n_of[0][q].x <= quota();
-    if (fits) return among(kind, goal, w, n_of[0]);
+    const SmpExact* told = exactly<1>(false, &b0, &b1);
+    const SmpExact r = sum_of(told);
+    w.mass = r.ahead[0], w.ahead = r.n_ahead[0], w.count = r.n[0], w.before = 0;
+    for (int q = 0; q < part; q++) w.before += told[q].n[0];
+    if (room(told)) return among(kind, goal, w, told, parts);
     // the ranks of these bins, which are monotone in the value
     const uint32_t least = rank_bits(floor_), most = rank_bits(m);
     uint32_t lo = least, hi = most;
@@ -690,18 +746,19 @@ struct SmpRow {
   }
 
   // ---- the window's tokens are in the first block's list
-  __device__ SmpFound among(SmpKind kind, double goal, const SmpWindow& w, const uint2* from) {
+  template <typename Found>
+  __device__ SmpFound among(SmpKind kind, double goal, const SmpWindow& w, const Found* from, int blocks) {
     if (part == 0) {
       const uint32_t n = w.count;
-      put_in_order(from, (int)n);
-      double wt[2], c[2];
+      put_in_order(from, (int)n, 0, blocks);
+      double wt[SMP_EACH], c[SMP_EACH];
       sums_of((int)n, wt, c);
-      uint32_t ahead = number((int)n, c, [&](int i, double s) { return !crosses(kind, w.mass + s, w.ahead + i + 1, goal); });
+      uint32_t ahead = number((int)n, wt, c, [&](int i, double, double s) { return !crosses(kind, w.mass + s, w.ahead + i + 1, goal); });
       ahead = min(ahead, n - 1);
-      if (ahead % SMP_THREADS == tid) {
-        const SmpFound f = {ordered()[ahead], w.mass + c[ahead / SMP_THREADS], w.ahead + ahead + 1};
+      at_token(ahead, c, [&](uint64_t place, double s) {
+        const SmpFound f = {place, w.mass + s, w.ahead + ahead + 1};
         for (int p = 0; p < (kind == SMP_PASS ? 1 : parts); p++) *at(&sh.found, p) = f;
-      }
+      });
       __syncthreads();
     }
     if (kind != SMP_PASS) all_sync();
@@ -723,7 +780,7 @@ struct SmpRow {
         });
         all_sync();
         const uint2 all_in_first = make_uint2(w.count, 0);
-        return among(kind, goal, w, &all_in_first);
+        return among(kind, goal, w, &all_in_first, 1);
       }
       if (w.lo == w.hi) return tied(kind, goal, w);
       const uint32_t range = w.hi - w.lo, hi = w.hi, shift = max(0, 28 - __clz(range));
@@ -753,14 +810,15 @@ struct SmpRow {
       }, SMP_CUTTERS);
     }
     __syncthreads();
-    // 32 threads a bin
-    const int b = tid / 32, i = tid % 32;
-    double s = cut_mass()[b * SMP_CUTTERS + i] + cut_mass()[b * SMP_CUTTERS + 32 + i];
-    const uint32_t n = __reduce_add_sync(0xffffffffu, cut_count()[b * SMP_CUTTERS + i] + cut_count()[b * SMP_CUTTERS + 32 + i]);
-    s = warp_sum(s);
-    if (i < parts) {
-      *at(&to.mass[part][b], i) = s;
-      *at(&to.count[part][b], i) = n;
+    // a warp a bin
+    for (int b = tid / 32; b < SMP_CUT; b += SMP_WARPS) {
+      const int i = tid % 32;
+      const double s = warp_sum(cut_mass()[b * SMP_CUTTERS + i] + cut_mass()[b * SMP_CUTTERS + 32 + i]);
+      const uint32_t n = __reduce_add_sync(0xffffffffu, cut_count()[b * SMP_CUTTERS + i] + cut_count()[b * SMP_CUTTERS + 32 + i]);
+      if (i < parts) {
+        *at(&to.mass[part][b], i) = s;
+        *at(&to.count[part][b], i) = n;
+      }
     }
     all_sync();
   }
@@ -876,11 +934,12 @@ struct SmpRow {
       }
     }
     inv_bin = fminf(SMP_BINS / (SMP_SPAN * t), FLT_MAX);
+    plain = floor_ == -FLT_MAX && lowest > -FLT_MAX && inv_bin > 0.f;
     __syncthreads();
     double mass = 0.0;
     uint32_t kept = 0;
     uint64_t end = 0;       // the last place that is kept, where that is known
-    float y[5], last;
+    float y[SMP_MINE + 1], last;
     bool known = false;     // whether mass and kept are
     if (k) {
       measure<true>(y, last);
@@ -895,7 +954,7 @@ struct SmpRow {
     if (!known && at_once(p, u, y, last, mass, kept)) return;
     if (p < 1.f) {
       const SmpFound f = search(SMP_REACH, (double)p * mass, y);
-      if (f.count < kept) mass = f.mass, kept = f.count, end = f.place;
+      if (!known || f.count < kept) mass = f.mass, kept = f.count, end = f.place;
     }
     SmpFound f = search(SMP_PASS, u * mass, y);
     if (f.count > kept) f.place = end;  // by rounding alone
