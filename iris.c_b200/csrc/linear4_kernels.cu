@@ -29,10 +29,24 @@ __device__ __forceinline__ uint32_t minus2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's nibbles, less the zero (128 + z twice)
-__device__ __forceinline__ void nibbles(uint32_t w, uint32_t zero, uint32_t p[4]) {
+// Numbers that the compiler does not see through, for the two below.
+struct Constants4 {
+  uint32_t mask, magic;
+  __device__ Constants4() {
+    asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(mask));
+    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
+  }
+};
+// Pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's nibbles, less the zero (128 + z twice).  What bounds the kernel is the pipe of
+// shifts and logic: mask and magic are in registers, so that one instruction does both (constants would take two: the head's
+// 151936 x 2560 74 us, 66 so; the shifts as high halves of products, on another pipe, 79).
+__device__ __forceinline__ void nibbles(uint32_t w, uint32_t zero, const Constants4& k, uint32_t p[4]) {
 #pragma unroll
-  for (int j = 0; j < 4; j++) p[j] = minus2((w >> 4 * j & 0x000F000Fu) | 0x43004300u, zero);
+  for (int j = 0; j < 4; j++) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> 4 * j), "r"(k.mask), "r"(k.magic));  // and, or
+    p[j] = minus2(x, zero);
+  }
 }
 
 // A warp's 16 MT rows of the weights from n0 on; what does not change from chunk to chunk is worked out once.  GS: parts of 32
@@ -40,6 +54,7 @@ __device__ __forceinline__ void nibbles(uint32_t w, uint32_t zero, uint32_t p[4]
 template <int MT, int GS, bool ZERO>
 struct Weights {
   const IrisLinear4& a;
+  Constants4 constants;
   const uint8_t* q[2 * MT];    // rows 8 j + g, at this lane's 16 bytes of a chunk
   const uint8_t* scale[2 * MT];
   const uint8_t* zero[2 * MT];
@@ -95,18 +110,13 @@ struct Weights {
     float sum[MT][NT][4];
 #pragma unroll
     for (int s = 0; s < 4; s++) {
-      if (s % GS == 0) {
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int t = 0; t < NT; t++) sum[m][t][0] = sum[m][t][1] = sum[m][t][2] = sum[m][t][3] = 0.f;
-      }
       uint32_t p[2 * MT][4];
+      const uint32_t word = base + g * 64 + ((s ^ (g >> 1 & 3)) << 4) + i4 * 4;
 #pragma unroll
       for (int j = 0; j < 2 * MT; j++) {
         uint32_t w;
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(base + (j * 8 + g) * 64 + ((s ^ (g >> 1 & 3)) << 4) + i4 * 4));
-        nibbles(w, GS == 4 || !ZERO ? z[j] : __shfl_sync(0xffffffffu, z[j], g * 4 + s), p[j]);
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(word + j * 512));
+        nibbles(w, GS == 4 || !ZERO ? z[j] : __shfl_sync(0xffffffffu, z[j], g * 4 + s), constants, p[j]);
       }
 #pragma unroll
       for (int t = 0; t < NT; t++) {
@@ -115,7 +125,8 @@ struct Weights {
         const uint32_t x2 = __byte_perm(u.y, u.w, 0x5410), x3 = __byte_perm(u.y, u.w, 0x7632);
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-          mma_bf16(sum[m][t], p[2 * m][0], p[2 * m + 1][0], p[2 * m][1], p[2 * m + 1][1], x0, x1);
+          if (s % GS == 0) mma_bf16_first(sum[m][t], p[2 * m][0], p[2 * m + 1][0], p[2 * m][1], p[2 * m + 1][1], x0, x1);
+          else mma_bf16(sum[m][t], p[2 * m][0], p[2 * m + 1][0], p[2 * m][1], p[2 * m + 1][1], x0, x1);
           mma_bf16(sum[m][t], p[2 * m][2], p[2 * m + 1][2], p[2 * m][3], p[2 * m + 1][3], x2, x3);
         }
       }
@@ -427,7 +438,7 @@ cudaError_t variant(IrisLinear4* a, int num_sms, cudaStream_t stream) {
   const bool many = a->n > 16 * 8 * num_sms;
   if (a->rows > 16) return many ? go_rows<4, 1, GS, ZERO>(a, num_sms, stream) : go_rows<4, 2, GS, ZERO>(a, num_sms, stream);
   if (a->rows > 8) return many ? go_rows<2, 1, GS, ZERO>(a, num_sms, stream) : go_rows<2, 2, GS, ZERO>(a, num_sms, stream);
-  return many ? go_few<2, 2, GS, ZERO>(a, num_sms, stream) : go_few<1, 8, GS, ZERO>(a, num_sms, stream);
+  return a->n >= 4 * 128 * num_sms ? go_few<2, 2, GS, ZERO>(a, num_sms, stream) : go_few<1, 8, GS, ZERO>(a, num_sms, stream);
 }
 
 template <int GS, bool ZERO>
