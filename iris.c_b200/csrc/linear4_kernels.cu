@@ -419,8 +419,11 @@ cudaError_t go_rows(IrisLinear4* a, int num_sms, cudaStream_t stream) {
   using Sh = L4Rows<NT, WK>;
   const int blocks = (a->rows + NT * 8 - 1) / (NT * 8), strips = (a->n + Sh::kRows - 1) / Sh::kRows;
   const int steps = ((a->k + L4_CHUNK - 1) / L4_CHUNK + WK - 1) / WK;
-  a->parts = 1;
-  while (a->parts < 8 && (int64_t)strips * blocks * a->parts * 2 <= 3 * num_sms && a->parts * 4 <= steps) a->parts *= 2;
+  // as many parts of k as let all blocks be on the device at once, two an SM, of which clusters reach seven eighths
+  const int64_t fit = num_sms * 2 * 7 / 8 / ((int64_t)strips * blocks);
+  a->parts = (int)(fit < 8 ? fit : 8);
+  if (a->parts > steps / 2) a->parts = steps / 2;
+  if (a->parts < 1) a->parts = 1;
   return go(linear4_rows_kernel<NT, WK, GS, ZERO>, dim3((unsigned)strips, blocks), Sh::kSmem, stream, *a);
 }
 
