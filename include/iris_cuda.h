@@ -835,8 +835,8 @@ typedef struct {
  * grows, the block's other slots are rounded to it.  Where the first slot is among
  * them, what the block held counts as dead: its other slots keep their bytes.  So
  * feed a sequence in order of its positions, in any number of calls; within a call
- * tokens stand in any order.  Values that are not finite are held as NaN; magnitudes past 448 * 2^60 as
- * that.  Of two tokens with one slot the later row stays. */
+ * tokens stand in any order (those of a block side by side are found soonest).
+ * Values that are not finite are held as NaN; magnitudes past 448 * 2^60 as that. */
 int iris_gpu_rope_append8(const iris_gpu_kv_cache8_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
                           const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int f32,
                           const float *q_norm, const float *k_norm, float eps, const int32_t *seq, const int32_t *pos,

@@ -74,12 +74,12 @@ __device__ __forceinline__ void norm_turn(float4& x, float4& y, const float* w, 
   }
 }
 
-// cos and sin of pair i at a position
-__device__ __forceinline__ void angle(const iris_gpu_rope_t& rope, int pos, int i, float& c, float& s) {
-  const uint64_t turn = (uint64_t)pos * rope.turns[i];
+// cos and sin of a pair at a position
+__device__ __forceinline__ void angle(uint64_t turns, float amplitude, int pos, float& c, float& s) {
+  const uint64_t turn = (uint64_t)pos * turns;
   sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
-  c *= rope.amplitude;
-  s *= rope.amplitude;
+  c *= amplitude;
+  s *= amplitude;
 }
 
 template <typename In, int HD>
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
   }
   if (seq < 0 || seq >= a.cache.num_seqs || pos < 0) return;
   const int block = iris_paged_block(a.div, pos), page = iris_paged_page(&a.cache, seq, block);
-  for (int i = threadIdx.x; i < rd / 2; i += ROPE_THREADS) angle(a.rope, pos, i, cs[i], sn[i]);
+  for (int i = threadIdx.x; i < rd / 2; i += ROPE_THREADS) angle(a.rope.turns[i], a.rope.amplitude, pos, cs[i], sn[i]);
   const int64_t slot = page < 0 ? -1 : iris_paged_offset(&a.cache, page, pos - block * a.cache.page_size);
   __nv_bfloat16* qo = (__nv_bfloat16*)a.q_out + (int64_t)t * a.ldq_out;
   __nv_bfloat16* ko = (__nv_bfloat16*)a.cache.k + slot;
@@ -135,15 +135,17 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------ keys and values into an 8-bit cache
-// The queries go the way above.  A scale is shared by a block of tokens, so the
-// tokens of a call that belong to one block of the cache (its mates) are taken
-// together, by the thread block of the first of them: it looks for the others among
-// all tokens of the call, in whatever order they stand (a token whose mate is the row
-// before leaves at once, so that a prompt's rows are searched once a block of the
-// cache).  Lanes hold columns as above; a warp has two (head, K or V), and goes over
-// the mates twice, for the largest magnitude and, behind the scale, for the values,
-// which the second time come from L1.
-constexpr int APPEND8_THREADS = 256, APPEND8_ITEMS = 2, APPEND8_SLOTS = 16;  // slots whose angles are held at a time
+// A scale is shared by a block of tokens, so the tokens of a call that belong to one
+// block of the cache (its mates) are taken together, by the thread block that meets
+// the first of them: it looks for the others among all tokens of the call, in
+// whatever order they stand (a token whose mate is the row before is left out at
+// once, so that a prompt's rows are searched once a block of the cache).  Lanes hold
+// columns as above; a warp has a (head, K or V) and APPEND8_ROUNDS mates in
+// registers, and goes over the mates twice, for the largest magnitude and, behind the
+// scale, for the values, from the registers where all fit.  Other blocks of the same
+// launch do the queries, 64 threads a token as above.
+constexpr int APPEND8_THREADS = 256, APPEND8_WARPS = APPEND8_THREADS / 32;
+constexpr int APPEND8_TOKENS = 8;  // that a block goes through where there are many
 
 // four values at a scale as e4m3, what is not finite as NaN
 __device__ __forceinline__ uint32_t to_e4m3(float4 x, float f) {
@@ -179,112 +181,187 @@ __device__ __forceinline__ int exponent8(uint32_t bits) {
   return min(max(e, IRIS_EXP8_MIN), IRIS_EXP8_MAX);
 }
 
-template <typename In, int HD>
-__global__ void __launch_bounds__(APPEND8_THREADS) rope_append8_kernel(const __grid_constant__ IrisRopeAppend a) {
-  constexpr int LPH = HD / 8, UNITS = 32 / LPH;  // lanes of a (token, head), of which a warp takes UNITS
+// grid: kv_blocks of them for keys and values, items (head, K or V) in turn, `per` tokens each; then the queries, `slices` of the
+// heads in turn
+struct Append8Plan {
+  int kv_blocks, items, per, slices;
+};
+
+// MANY: tokens.  Half as many mates in registers and twice the blocks on an SM: 8191 tokens of 32 + 8 + 8 heads of 128, f32, 94 us
+// -> 75; 64 tokens 6.4 -> 8.3.
+template <typename In, int HD, bool MANY>
+__global__ void __launch_bounds__(APPEND8_THREADS, MANY ? 4 : 2) rope_append8_kernel(const __grid_constant__ IrisRopeAppend a,
+                                                                          const __grid_constant__ Append8Plan plan) {
+  constexpr int LPH = HD / 8, UNITS = 32 / LPH;               // lanes of a (token, head), of which a warp takes UNITS
+  constexpr int MOST = MANY ? 4 : 8, ROUNDS = 16 / UNITS < MOST ? 16 / UNITS : MOST, BATCH = ROUNDS * UNITS;  // slots held at a time
   using Raw = typename Raw4<In>::T;
-  __shared__ __align__(16) float cs[APPEND8_SLOTS][HD / 2], sn[APPEND8_SLOTS][HD / 2];
+  __shared__ __align__(16) float cs[16][HD / 2], sn[16][HD / 2];
+  __shared__ uint64_t turns[HD / 2];  // (from the arguments each lane's own costs a turn of its own)
   __shared__ int rows[128];  // of the call, by the block's slots
   __shared__ int first;
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid % LPH, unit = tid % 32 / LPH;
+  const int tid = threadIdx.x, lane = tid % LPH, unit = tid % 32 / LPH;
   const int nkv = a.cache.kv_heads, rd = a.rope.rot_dim, size = a.exp.block;
   const bool turned = lane < rd / 8, halves = a.rope.layout == IRIS_ROPE_HALF && turned;
   const int ca = halves ? lane * 4 : lane * 8, cb = halves ? rd / 2 + lane * 4 : lane * 8 + 4;
+  for (int i = tid; i < rd / 2; i += APPEND8_THREADS) turns[i] = a.rope.turns[i];
+  __syncthreads();
   iris::grid_dep_wait();
   iris::grid_dep_launch();
-  const int seq = a.seq[t], pos = a.pos[t];
-  const int seq_before = t ? a.seq[t - 1] : -1, pos_before = t ? a.pos[t - 1] : -1;
-  if (seq < 0 || seq >= a.cache.num_seqs || pos < 0) return;
-  const int part = iris_paged_block(a.exp.div, pos), begin = part * size;  // the block of the sequence, its first position
-  if (seq_before == seq && pos_before >= 0 && iris_paged_block(a.exp.div, pos_before) == part) return;
-  const int block = iris_paged_block(a.div, pos), page = iris_paged_page(&a.cache, seq, block);
-  if (page < 0) return;
-  for (int i = tid; i < size; i += APPEND8_THREADS) rows[i] = -1;
-  if (tid == 0) first = t;
-  __syncthreads();
-  for (int u0 = tid; u0 < a.tokens; u0 += 4 * APPEND8_THREADS) {
-    int s[4];
+
+  if ((int)blockIdx.x >= plan.kv_blocks) {  // queries
+    constexpr int GROUPS = ROPE_THREADS / LPH, SUBS = APPEND8_THREADS / ROPE_THREADS;
+    const int b = (int)blockIdx.x - plan.kv_blocks, sub = tid / ROPE_THREADS, in = tid % ROPE_THREADS;
+    const int t = b / plan.slices * SUBS + sub, nh = a.heads;
+    if (t >= a.tokens) return;
+    const int head0 = b % plan.slices * GROUPS + in / LPH, step = plan.slices * GROUPS;
+    const In* q = (const In*)a.q + (int64_t)t * a.ldq;
+    const int seq = a.seq[t], pos = a.pos[t];
+    Raw ra[ROPE_HEADS], rb[ROPE_HEADS];
 #pragma unroll
-    for (int j = 0; j < 4; j++) s[j] = u0 + j * APPEND8_THREADS < a.tokens ? a.seq[u0 + j * APPEND8_THREADS] : -1;
+    for (int i = 0; i < ROPE_HEADS; i++) {
+      ra[i] = rb[i] = Raw();
+      if (head0 + i * step < nh) {
+        ra[i] = *reinterpret_cast<const Raw*>(q + (head0 + i * step) * HD + ca);
+        rb[i] = *reinterpret_cast<const Raw*>(q + (head0 + i * step) * HD + cb);
+      }
+    }
+    if (seq < 0 || seq >= a.cache.num_seqs || pos < 0) return;  // (all threads of the token)
+    float *c = &cs[0][0] + sub * 128, *s = &sn[0][0] + sub * 128;
+    for (int i = in; i < rd / 2; i += ROPE_THREADS) angle(turns[i], a.rope.amplitude, pos, c[i], s[i]);
+    asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "n"(ROPE_THREADS) : "memory");
+    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (turned) c4 = *reinterpret_cast<const float4*>(c + lane * 4), s4 = *reinterpret_cast<const float4*>(s + lane * 4);
+    __nv_bfloat16* out = (__nv_bfloat16*)a.q_out + (int64_t)t * a.ldq_out;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if (s[j] != seq) continue;
-      const int u = u0 + j * APPEND8_THREADS, at = a.pos[u] - begin;
-      if (a.pos[u] < 0 || at < 0 || at >= size) continue;
+    for (int i = 0; i < ROPE_HEADS; i++) {
+      if (head0 + i * step >= nh) continue;
+      float4 x = values4(ra[i]), y = values4(rb[i]);
+      norm_turn<HD>(x, y, a.q_norm, a.eps, ca, cb, halves, turned, c4, s4);
+      __nv_bfloat16* to = out + (head0 + i * step) * HD;
+      *reinterpret_cast<uint2*>(to + ca) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
+      *reinterpret_cast<uint2*>(to + cb) = make_uint2(pack2(y.x, y.y), pack2(y.z, y.w));
+    }
+    return;
+  }
+
+  const int item = (int)blockIdx.x % plan.items * APPEND8_WARPS + tid / 32, head = item < nkv ? item : item - nkv;
+  const bool works = item < 2 * nkv, is_v = item >= nkv;
+  const int t0 = (int)blockIdx.x / plan.items * plan.per, t1 = min(a.tokens, t0 + plan.per);
+  for (int t = t0; t < t1; t++) {
+    const int seq = a.seq[t], pos = a.pos[t];
+    const int seq_before = t ? a.seq[t - 1] : -1, pos_before = t ? a.pos[t - 1] : -1;
+    if (seq < 0 || seq >= a.cache.num_seqs || pos < 0) continue;
+    const int part = iris_paged_block(a.exp.div, pos), begin = part * size;  // the block of the sequence, its first position
+    if (seq_before == seq && pos_before >= 0 && iris_paged_block(a.exp.div, pos_before) == part) continue;
+    const int block = iris_paged_block(a.div, pos), page = iris_paged_page(&a.cache, seq, block);
+    if (page < 0) continue;
+    __syncthreads();  // the last token's mates are done with
+    for (int i = tid; i < size; i += APPEND8_THREADS) rows[i] = -1;
+    if (tid == 0) first = t;
+    __syncthreads();
+    auto mate = [&](int u, int its_seq) {
+      if (its_seq != seq) return;
+      const int p = a.pos[u], at = p - begin;
+      if (p < 0 || at < 0 || at >= size) return;
       atomicMax(&rows[at], u);
       atomicMin(&first, u);
+    };
+    if (size == 1) {  // none but itself
+      if (tid == 0) rows[0] = t;
+    } else if ((reinterpret_cast<uintptr_t>(a.seq) & 15) == 0) {
+      constexpr int FLY = 8;  // 8192 tokens in one round
+      const int4* four = reinterpret_cast<const int4*>(a.seq);
+      for (int i0 = tid; i0 < a.tokens / 4; i0 += FLY * APPEND8_THREADS) {
+        int4 s[FLY];
+#pragma unroll
+        for (int j = 0; j < FLY; j++)
+          s[j] = i0 + j * APPEND8_THREADS < a.tokens / 4 ? __ldg(four + i0 + j * APPEND8_THREADS) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+        for (int j = 0; j < FLY; j++) {
+          const int u = 4 * (i0 + j * APPEND8_THREADS);
+          if (s[j].x != seq && s[j].y != seq && s[j].z != seq && s[j].w != seq) continue;
+          mate(u, s[j].x), mate(u + 1, s[j].y), mate(u + 2, s[j].z), mate(u + 3, s[j].w);
+        }
+      }
+      if (tid < a.tokens % 4) mate(a.tokens / 4 * 4 + tid, a.seq[a.tokens / 4 * 4 + tid]);
+    } else {
+      for (int u = tid; u < a.tokens; u += APPEND8_THREADS) mate(u, a.seq[u]);
     }
-  }
-  __syncthreads();
-  if (first != t) return;
+    __syncthreads();
+    if (first != t) continue;
 
-  const int first_slot = begin - block * a.cache.page_size;  // of the page
-  const bool fresh = rows[0] >= 0;
-  const int item0 = (blockIdx.y * (APPEND8_THREADS / 32) + tid / 32) * APPEND8_ITEMS;
-  const int chunks = (size + APPEND8_SLOTS - 1) / APPEND8_SLOTS;
-  uint32_t top[APPEND8_ITEMS] = {};
-  int exp[APPEND8_ITEMS], old[APPEND8_ITEMS];
-  for (int pass = 0; pass < 2; pass++) {
-    for (int c = 0; c < chunks; c++) {
-      const int slot0 = c * APPEND8_SLOTS, slots = min(APPEND8_SLOTS, size - slot0);
-      if (pass == 0 || chunks > 1) {
-        __syncthreads();
-        for (int i = tid; i < slots * (rd / 2); i += APPEND8_THREADS) {
-          const int s = i / (rd / 2), p = i - s * (rd / 2);
-          if (rows[slot0 + s] >= 0) angle(a.rope, begin + slot0 + s, p, cs[s][p], sn[s][p]);
-        }
-        __syncthreads();
-      }
+    const int first_slot = begin - block * a.cache.page_size;  // of the page
+    const bool fresh = rows[0] >= 0, whole = size <= BATCH;
+    const In* from = (const In*)(is_v ? a.v : a.k) + (works ? head : 0) * HD;
+    const int64_t ld = is_v ? a.ldv : a.ldk;
+    uint8_t* to = (uint8_t*)(is_v ? a.cache.v : a.cache.k) + iris_paged_offset(&a.cache, page, first_slot) +
+                  (works ? head : 0) * a.cache.head_stride;
+    uint8_t* at_exp = (is_v ? a.exp.v : a.exp.k) + page * a.exp.page_stride +
+                      iris_paged_block(a.exp.div, first_slot) * a.exp.block_stride + (works ? head : 0) * a.exp.head_stride;
+    const int old = works ? exp8(*at_exp) : 0;
+    Raw ra[ROUNDS], rb[ROUNDS];
+    int row[ROUNDS];
+    // the values of a batch's mates, and their angles
+    auto load = [&](int slot0) {
 #pragma unroll
-      for (int k = 0; k < APPEND8_ITEMS; k++) {
-        const int item = item0 + k, head = item < nkv ? item : item - nkv;
-        if (item >= 2 * nkv) continue;
-        const bool is_v = item >= nkv;
-        const In* from = (const In*)(is_v ? a.v : a.k) + head * HD;
-        const int64_t ld = is_v ? a.ldv : a.ldk;
-        uint8_t* to = (uint8_t*)(is_v ? a.cache.v : a.cache.k) + iris_paged_offset(&a.cache, page, first_slot) +
-                      head * a.cache.head_stride;
-        for (int s = unit; s < slots; s += UNITS) {
-          const int row = rows[slot0 + s];
-          uint8_t* at = to + (slot0 + s) * a.cache.token_stride;
-          if (row >= 0) {
-            const In* r = from + row * ld;
-            float4 x = values4(*reinterpret_cast<const Raw*>(r + ca)), y = values4(*reinterpret_cast<const Raw*>(r + cb));
-            if (!is_v) {
-              float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (turned) {
-                c4 = *reinterpret_cast<const float4*>(&cs[s][lane * 4]);
-                s4 = *reinterpret_cast<const float4*>(&sn[s][lane * 4]);
-              }
-              norm_turn<HD>(x, y, a.k_norm, a.eps, ca, cb, halves, turned, c4, s4);
-            }
-            if (pass == 0) {
-              top[k] = most_bits(most_bits(top[k], x), y);
-            } else {
-              const float f = scale8(254 - exp[k]);
-              *reinterpret_cast<uint32_t*>(at + ca) = to_e4m3(x, f);
-              *reinterpret_cast<uint32_t*>(at + cb) = to_e4m3(y, f);
-            }
-          } else if (pass == 1 && !fresh && exp[k] > old[k]) {  // what was there, to the larger scale
-            uint2* w = reinterpret_cast<uint2*>(at + lane * 8);
-            const float f = scale8(127 + old[k] - exp[k]);
-            *w = make_uint2(scaled_e4m3(w->x, f), scaled_e4m3(w->y, f));
-          }
+      for (int j = 0; j < ROUNDS; j++) {
+        const int s = slot0 + j * UNITS + unit;
+        row[j] = works && s < size ? rows[s] : -1;
+        if (row[j] >= 0) {
+          const In* r = from + row[j] * ld;
+          ra[j] = *reinterpret_cast<const Raw*>(r + ca);
+          rb[j] = *reinterpret_cast<const Raw*>(r + cb);
         }
+      }
+      if ((int)blockIdx.x % plan.items * APPEND8_WARPS >= nkv) return;  // V alone in this block
+      __syncthreads();
+      for (int i = tid; i < BATCH * (rd / 2); i += APPEND8_THREADS) {
+        const int s = i / (rd / 2), p = i - s * (rd / 2);
+        if (slot0 + s < size && rows[slot0 + s] >= 0) angle(turns[p], a.rope.amplitude, begin + slot0 + s, cs[s][p], sn[s][p]);
+      }
+      __syncthreads();
+    };
+    auto value = [&](int j, float4& x, float4& y) {
+      x = values4(ra[j]), y = values4(rb[j]);
+      if (is_v) return;
+      float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (turned) {
+        c4 = *reinterpret_cast<const float4*>(&cs[j * UNITS + unit][lane * 4]);
+        s4 = *reinterpret_cast<const float4*>(&sn[j * UNITS + unit][lane * 4]);
+      }
+      norm_turn<HD>(x, y, a.k_norm, a.eps, ca, cb, halves, turned, c4, s4);
+    };
+    uint32_t top = 0;
+    for (int slot0 = 0; slot0 < size; slot0 += BATCH) {
+      load(slot0);
+#pragma unroll
+      for (int j = 0; j < ROUNDS; j++) {
+        if (row[j] < 0) continue;
+        float4 x, y;
+        value(j, x, y);
+        top = most_bits(most_bits(top, x), y);
       }
     }
-    if (pass) break;
+    int exp = exponent8(__reduce_max_sync(0xffffffffu, top));
+    if (!fresh) exp = max(exp, old);
+    if (works && tid % 32 == 0) *at_exp = (uint8_t)exp;
+    const float f = scale8(254 - exp), down = scale8(127 + min(0, old - exp));
+    for (int slot0 = 0; slot0 < size; slot0 += BATCH) {
+      if (!whole) load(slot0);
 #pragma unroll
-    for (int k = 0; k < APPEND8_ITEMS; k++) {
-      const int item = item0 + k;
-      if (item >= 2 * nkv) continue;
-      uint8_t* at = (item < nkv ? a.exp.k + item * a.exp.head_stride : a.exp.v + (item - nkv) * a.exp.head_stride) +
-                    page * a.exp.page_stride + iris_paged_block(a.exp.div, first_slot) * a.exp.block_stride;
-      exp[k] = exponent8(__reduce_max_sync(0xffffffffu, top[k]));
-      old[k] = exp8(*at);
-      if (!fresh) exp[k] = max(exp[k], old[k]);
-      __syncwarp();
-      if (tid % 32 == 0) *at = (uint8_t)exp[k];
+      for (int j = 0; j < ROUNDS; j++) {
+        const int s = slot0 + j * UNITS + unit;
+        uint8_t* at = to + s * a.cache.token_stride;
+        if (row[j] >= 0) {
+          float4 x, y;
+          value(j, x, y);
+          *reinterpret_cast<uint32_t*>(at + ca) = to_e4m3(x, f);
+          *reinterpret_cast<uint32_t*>(at + cb) = to_e4m3(y, f);
+        } else if (works && s < size && !fresh && exp > old) {  // what was there, to the larger scale
+          uint2* w = reinterpret_cast<uint2*>(at + lane * 8);
+          *w = make_uint2(scaled_e4m3(w->x, down), scaled_e4m3(w->y, down));
+        }
+      }
     }
   }
 }
@@ -2022,23 +2099,31 @@ extern "C" cudaError_t iris_launch_rope_append(IrisRopeAppend* a, int f32, int n
 extern "C" cudaError_t iris_launch_rope_append8(IrisRopeAppend* a, int f32, int num_sms, cudaStream_t stream) {
   a->div = iris_paged_div(a->cache.page_size);
   a->exp.div = iris_paged_div(a->exp.block);
-  if (a->heads) {
-    IrisRopeAppend q = *a;
-    q.cache.kv_heads = 0;
-    const cudaError_t e = iris_launch_rope_append(&q, f32, num_sms, stream);
-    if (e != cudaSuccess) return e;
-  }
-  constexpr int items = APPEND8_THREADS / 32 * APPEND8_ITEMS;
-  const dim3 grid(a->tokens, (2 * a->cache.kv_heads + items - 1) / items);
-  auto go = [&](auto kernel) { return iris::launch_overlapped(kernel, grid, dim3(APPEND8_THREADS), 0, stream, *a); };
-  if (f32) {
-    if (a->cache.head_dim == 64) return go(rope_append8_kernel<float, 64>);
-    if (a->cache.head_dim == 128) return go(rope_append8_kernel<float, 128>);
-    return go(rope_append8_kernel<float, 256>);
-  }
-  if (a->cache.head_dim == 64) return go(rope_append8_kernel<__nv_bfloat16, 64>);
-  if (a->cache.head_dim == 128) return go(rope_append8_kernel<__nv_bfloat16, 128>);
-  return go(rope_append8_kernel<__nv_bfloat16, 256>);
+  Append8Plan plan;
+  plan.items = (2 * a->cache.kv_heads + APPEND8_WARPS - 1) / APPEND8_WARPS;
+  const bool many = a->tokens > 8 * num_sms;
+  plan.per = many && a->exp.block >= APPEND8_TOKENS ? APPEND8_TOKENS : 1;
+  const int64_t kv = ((int64_t)a->tokens + plan.per - 1) / plan.per * plan.items;
+  const int groups = ROPE_THREADS / (a->cache.head_dim / 8), all = (a->heads + groups - 1) / groups;
+  // as for iris_launch_rope_append
+  const bool few = (int64_t)a->tokens * all * ROPE_THREADS <= 1024 * num_sms;
+  plan.slices = few ? all : (all + ROPE_HEADS - 1) / ROPE_HEADS;
+  constexpr int subs = APPEND8_THREADS / ROPE_THREADS;
+  const int64_t blocks = kv + ((int64_t)a->tokens + subs - 1) / subs * plan.slices;
+  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  plan.kv_blocks = (int)kv;
+  auto go = [&](auto kernel) {
+    return iris::launch_overlapped(kernel, dim3((unsigned)blocks), dim3(APPEND8_THREADS), 0, stream, *a, plan);
+  };
+  auto of = [&](auto in, auto is_many) {
+    using In = decltype(in);
+    constexpr bool M = decltype(is_many)::value;
+    if (a->cache.head_dim == 64) return go(rope_append8_kernel<In, 64, M>);
+    if (a->cache.head_dim == 128) return go(rope_append8_kernel<In, 128, M>);
+    return go(rope_append8_kernel<In, 256, M>);
+  };
+  if (f32) return many ? of(0.f, std::true_type()) : of(0.f, std::false_type());
+  return many ? of(__nv_bfloat16(), std::true_type()) : of(__nv_bfloat16(), std::false_type());
 }
 
 // CTAs of an attention launch: as many as the device holds at once, no more than the tables have room for tiles

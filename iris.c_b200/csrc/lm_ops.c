@@ -202,7 +202,7 @@ static int append_to(const char *what, const iris_gpu_kv_cache_t *cache, const i
     a.heads = heads;
     if (!cache8) return lm_leave(&d, iris_launch_rope_append(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, 1);
     a.exp = exp_of(cache8);
-    return lm_leave(&d, iris_launch_rope_append8(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, heads ? 2 : 1);
+    return lm_leave(&d, iris_launch_rope_append8(&a, f32 != 0, g_rt.num_sms, (cudaStream_t)stream), what, 1);
 }
 
 int iris_gpu_rope_append(const iris_gpu_kv_cache_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
