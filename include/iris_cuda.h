@@ -444,6 +444,14 @@ size_t iris_cuda_qwen3_lm_cache_bytes(const iris_cuda_qwen3_lm_t *lm);
 int iris_cuda_qwen3_lm_step(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos,
                             const int *targets, int tokens, int top_k, float *logprob, float *entropy, int *top_ids,
                             float *top_logprobs);
+/* The same, and draws a next token behind each of the step's tokens, as
+ * iris_gpu_sample_tokens does, with the caller's random numbers: uniform [tokens];
+ * temperature, top_k, top_p, min_p [tokens], each optional (host arrays).  next
+ * [tokens] gets the tokens, logprobs [tokens] (optional) their log probabilities
+ * among what the settings keep. */
+int iris_cuda_qwen3_lm_sample(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos, int tokens,
+                              const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+                              const double *uniform, int *next, float *logprobs);
 /* Tokens a sequence holds, or a negative status. */
 int iris_cuda_qwen3_lm_length(const iris_cuda_qwen3_lm_t *lm, int seq);
 

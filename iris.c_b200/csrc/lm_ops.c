@@ -81,10 +81,11 @@ static int cache8_check(const iris_gpu_kv_cache8_t *c, const char *what) {
     if (c->block < 1 || c->block > 128 || c->pages.page_size % c->block)
         return LM_FAIL("%s: blocks of %d tokens in pages of %d (a divisor, at most 128)", what, c->block, c->pages.page_size);
     /* the kernels count places in 16 bytes, in 32 bits */
-    if (((c->pages.num_pages - 1) * c->pages.page_stride >> 36) || ((c->pages.page_size - 1) * c->pages.token_stride >> 36) ||
-        ((c->pages.kv_heads - 1) * c->pages.head_stride >> 36) ||
-        (c->pages.num_pages - 1) * c->pages.page_stride + (c->pages.page_size - 1) * c->pages.token_stride +
-                (c->pages.kv_heads - 1) * c->pages.head_stride + c->pages.head_dim > (int64_t)1 << 36)
+    int64_t a, b, d;
+    if (__builtin_mul_overflow(c->pages.num_pages - 1, c->pages.page_stride, &a) ||
+        __builtin_mul_overflow(c->pages.page_size - 1, c->pages.token_stride, &b) ||
+        __builtin_mul_overflow(c->pages.kv_heads - 1, c->pages.head_stride, &d) || __builtin_add_overflow(a, b, &a) ||
+        __builtin_add_overflow(a, d, &a) || a > ((int64_t)1 << 36) - c->pages.head_dim)
         return LM_FAIL("%s: pools of more than 64 GiB", what);
     if (c->exp_page_stride < 0 || c->exp_block_stride < 0 || c->exp_head_stride < 0 ||
         (c->pages.num_pages > 1 && !c->exp_page_stride) || (c->pages.page_size > c->block && !c->exp_block_stride) ||
@@ -366,7 +367,7 @@ int iris_gpu_sample_tokens(const void *logits, int f32, int64_t ld, int rows, in
 /* ------------------------------------------------------------------ weights of 4 bits */
 static int weights4_check(const iris_gpu_weights4_t *w, const char *what) {
     if (!w || !w->q || !w->scale) return LM_FAIL("%s: null weights or scales", what);
-    if (w->n < 1 || w->k < 1 || (w->group != 32 && w->group != 64 && (w->group < 128 || w->group % 128)) || w->k % w->group)
+    if (w->n < 1 || w->k < 1 || w->n > 1 << 30 || w->k > 1 << 30 || (w->group != 32 && w->group != 64 && (w->group < 128 || w->group % 128)) || w->k % w->group)
         return LM_FAIL("%s: weights [%d, %d] in groups of %d (32, 64 or a multiple of 128, and of it a whole number in a row)",
                        what, w->n, w->k, w->group);
     const int groups = w->k / w->group;

@@ -17,10 +17,11 @@
 #define LM_PAGE 16          /* tokens of a page */
 #define LM_MAX_TOKENS 8192  /* of a step: the logits are f32 [tokens, vocab] */
 #define LM_SIZES 16         /* of steps, remembered */
+#define LM_DRAW (-1)
 
 /* a size of step: its graph, once captured */
 typedef struct {
-    int tokens, top_k;      /* tokens 0: none */
+    int tokens, top_k;      /* tokens 0: none; top_k LM_DRAW: a token is drawn behind each */
     uint64_t used;          /* the step that last had it */
     cudaGraph_t graph;
     cudaGraphExec_t gexec;  /* NULL before its second step */
@@ -44,6 +45,8 @@ struct iris_cuda_qwen3_lm {
     void *attn_ws, *lp_ws;
     float *out;             /* logprob, entropy, top_logprobs: [2 + 32][max_tokens] */
     int32_t *out_ids;       /* [max_tokens, 32] */
+    double *draw, *h_draw;  /* a step's settings of draws: uniform [tokens], then f32 temperature, top_p, min_p and int32 top_k
+                               [4][tokens]; the same on the host */
     CUtensorMap tm_xn, tm_attn, tm_mlp;
     iris_gpu_rope_t rope;
     lm_size_t sizes[LM_SIZES];
@@ -62,9 +65,10 @@ void iris_cuda_qwen3_lm_free(iris_cuda_qwen3_lm_t *lm) {
     if (g_rt.initialized) cudaStreamSynchronize(g_rt.stream);
     for (int i = 0; i < LM_SIZES; i++) lm_size_free(&lm->sizes[i]);
     void *b[] = {lm->table, lm->pools, lm->in, lm->x, lm->qkv, lm->logits, lm->ws, lm->xn, lm->q, lm->attn, lm->mlp,
-                 lm->attn_ws, lm->lp_ws, lm->out, lm->out_ids};
+                 lm->attn_ws, lm->lp_ws, lm->out, lm->out_ids, lm->draw};
     for (size_t i = 0; i < sizeof(b) / sizeof(b[0]); i++) iris_dfree(b[i]);
     free(lm->h_in);
+    free(lm->h_draw);
     free(lm->len);
     free(lm->next);
     free(lm->named);
@@ -119,7 +123,8 @@ iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_se
     lm->next = (int *)calloc((size_t)num_seqs, sizeof(int));
     lm->named = (uint64_t *)calloc((size_t)num_seqs, sizeof(uint64_t));
     lm->h_in = (int32_t *)malloc(4 * T * 4);
-    if (!lm->len || !lm->next || !lm->named || !lm->h_in) rc = iris_fail(IRIS_CUDA_ERR_OOM, "language model session");
+    lm->h_draw = (double *)malloc(24 * T);
+    if (!lm->len || !lm->next || !lm->named || !lm->h_in || !lm->h_draw) rc = iris_fail(IRIS_CUDA_ERR_OOM, "language model session");
 #define ALLOC(dst, bytes) \
     do { if (!rc && !((dst) = iris_dmalloc(bytes))) rc = iris_fail(IRIS_CUDA_ERR_OOM, "language model session"); } while (0)
     ALLOC(lm->table, pages * 4);
@@ -138,6 +143,7 @@ iris_cuda_qwen3_lm_t *iris_cuda_qwen3_lm_create(iris_cuda_qwen3_t *m, int num_se
     ALLOC(lm->lp_ws, iris_logprobs_ws_bytes(max_tokens, c->vocab));
     ALLOC(lm->out, (2 + 32) * T * 4);
     ALLOC(lm->out_ids, 32 * T * 4);
+    ALLOC(lm->draw, 24 * T);
 #undef ALLOC
     if (!rc) {
         /* sequence s has the pages [s * blocks, (s + 1) * blocks) */
@@ -216,6 +222,13 @@ static int lm_enqueue(iris_cuda_qwen3_lm_t *lm, int T, int top_k, q3_enq_t *E) {
     iris_q3_done(E, iris_launch_rmsnorm(lm->x, H, m->norm, NULL, lm->xn, H, T, H, Q3_EPS, NULL, st), "rmsnorm", 1);
     iris_q3_gemm(E, "head", &lm->tm_xn, &m->tm_head, T, m->head_rows, H, IRIS_EPI_F32, lm->logits, m->head_rows, NULL, NULL, 0,
                  NULL, 0);
+    if (top_k == LM_DRAW) {
+        const float *set = (const float *)(lm->draw + T);
+        IrisSample d = {lm->logits, m->head_rows, T, c->vocab, set, set + T, set + 2 * T, (const int32_t *)(set + 3 * T), lm->draw,
+                        lm->out_ids, NULL, lm->out, 0, 0};
+        if (!E->rc) iris_q3_done(E, iris_launch_sample(&d, 1, g_rt.num_sms, st), "draw", 1);
+        return E->rc;
+    }
     IrisLogprobs p = {lm->logits, m->head_rows, T, c->vocab, top_k, targets, lm->out, lm->out + lm->max_tokens,
                       lm->out + 2 * lm->max_tokens, lm->out_ids, lm->lp_ws};
     if (!E->rc) {
@@ -284,29 +297,28 @@ static int lm_check(iris_cuda_qwen3_lm_t *lm, const int *seq, const int *pos, in
     return 0;
 }
 
-int iris_cuda_qwen3_lm_step(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos,
-                            const int *targets, int tokens, int top_k, float *logprob, float *entropy, int *top_ids,
-                            float *top_logprobs) {
+/* what every step's arguments have to be */
+static int lm_args(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos, int tokens) {
     if (!lm || !ids || !seq || !pos) return iris_fail(IRIS_CUDA_ERR_ARG, "null argument");
     if (tokens < 1 || tokens > lm->max_tokens)
         return iris_fail(IRIS_CUDA_ERR_ARG, "step of %d tokens (1..%d)", tokens, lm->max_tokens);
-    if (top_k < 0 || top_k > 32 || top_k > lm->m->cfg.vocab)
-        return iris_fail(IRIS_CUDA_ERR_ARG, "top_k %d (0..min(32, vocabulary))", top_k);
-    int rc = lm_check(lm, seq, pos, tokens);
-    if (rc) return rc;
-    const size_t n = (size_t)tokens, T = (size_t)lm->max_tokens;
+    return lm_check(lm, seq, pos, tokens);
+}
+
+typedef struct { void *to; const void *from; size_t bytes; } lm_out_t;
+
+/* the step itself; its outputs back to the host */
+static int lm_feed(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos, const int *targets, int tokens,
+                   int top_k, const lm_out_t *outs, int n_outs) {
+    const size_t n = (size_t)tokens;
     memcpy(lm->h_in, ids, n * 4);
     memcpy(lm->h_in + n, seq, n * 4);
     memcpy(lm->h_in + 2 * n, pos, n * 4);
     if (targets) memcpy(lm->h_in + 3 * n, targets, n * 4);
     else memset(lm->h_in + 3 * n, 0xFF, n * 4);  /* -1 */
-    rc = iris_h2d(lm->in, lm->h_in, 4 * n * 4);
+    int rc = iris_h2d(lm->in, lm->h_in, 4 * n * 4);
     if (!rc) rc = lm_run(lm, tokens, top_k);
-    const size_t k = (size_t)top_k;
-    struct { void *to; const void *from; size_t bytes; } outs[] = {
-        {logprob, lm->out, n * 4}, {entropy, lm->out + T, n * 4}, {top_logprobs, lm->out + 2 * T, n * k * 4},
-        {top_ids, lm->out_ids, n * k * 4}};
-    for (int i = 0; !rc && i < 4; i++)
+    for (int i = 0; !rc && i < n_outs; i++)
         if (outs[i].to && outs[i].bytes)
             rc = iris_cuda_check(cudaMemcpyAsync(outs[i].to, outs[i].from, outs[i].bytes, cudaMemcpyDeviceToHost, g_rt.stream),
                                  "outputs");
@@ -315,4 +327,39 @@ int iris_cuda_qwen3_lm_step(iris_cuda_qwen3_lm_t *lm, const int *ids, const int 
     if (!rc)
         for (int t = 0; t < tokens; t++) lm->len[seq[t]] = lm->next[seq[t]];
     return rc;
+}
+
+int iris_cuda_qwen3_lm_step(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos,
+                            const int *targets, int tokens, int top_k, float *logprob, float *entropy, int *top_ids,
+                            float *top_logprobs) {
+    if (lm && (top_k < 0 || top_k > 32 || top_k > lm->m->cfg.vocab))
+        return iris_fail(IRIS_CUDA_ERR_ARG, "top_k %d (0..min(32, vocabulary))", top_k);
+    const int rc = lm_args(lm, ids, seq, pos, tokens);
+    if (rc) return rc;
+    const size_t n = (size_t)tokens, T = (size_t)lm->max_tokens, k = (size_t)top_k;
+    const lm_out_t outs[] = {{logprob, lm->out, n * 4}, {entropy, lm->out + T, n * 4}, {top_logprobs, lm->out + 2 * T, n * k * 4},
+                             {top_ids, lm->out_ids, n * k * 4}};
+    return lm_feed(lm, ids, seq, pos, targets, tokens, top_k, outs, 4);
+}
+
+int iris_cuda_qwen3_lm_sample(iris_cuda_qwen3_lm_t *lm, const int *ids, const int *seq, const int *pos, int tokens,
+                              const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+                              const double *uniform, int *next, float *logprobs) {
+    if (!uniform || !next) return iris_fail(IRIS_CUDA_ERR_ARG, "null argument");
+    int rc = lm_args(lm, ids, seq, pos, tokens);
+    if (rc) return rc;
+    const size_t n = (size_t)tokens;
+    float *set = (float *)(lm->h_draw + n);
+    int32_t *k = (int32_t *)(set + 3 * n);
+    memcpy(lm->h_draw, uniform, n * 8);
+    for (size_t t = 0; t < n; t++) {
+        set[t] = temperature ? temperature[t] : 1.0f;
+        set[n + t] = top_p ? top_p[t] : 1.0f;
+        set[2 * n + t] = min_p ? min_p[t] : 0.0f;
+        k[t] = top_k ? top_k[t] : 0;
+    }
+    rc = iris_h2d(lm->draw, lm->h_draw, 24 * n);
+    if (rc) return rc;
+    const lm_out_t outs[] = {{next, lm->out_ids, n * 4}, {logprobs, lm->out, n * 4}};
+    return lm_feed(lm, ids, seq, pos, NULL, tokens, LM_DRAW, outs, 2);
 }

@@ -295,6 +295,8 @@ SIGNATURES = {
     "iris_cuda_qwen3_lm_cache_bytes": (C.c_size_t, [C.c_void_p]),
     "iris_cuda_qwen3_lm_step": (C.c_int, [C.c_void_p] + [C.POINTER(C.c_int)] * 4 + [C.c_int, C.c_int, _fp, _fp,
                                                                                   C.POINTER(C.c_int), _fp]),
+    "iris_cuda_qwen3_lm_sample": (C.c_int, [C.c_void_p] + [C.POINTER(C.c_int)] * 3 + [C.c_int, _fp, C.POINTER(C.c_int), _fp, _fp,
+                                            C.POINTER(C.c_double), C.POINTER(C.c_int), _fp]),
     "iris_cuda_qwen3_lm_length": (C.c_int, [C.c_void_p, C.c_int]),
     "iris_cuda_qwen3_graph_kernels": (C.c_uint64, [C.c_void_p]),
     "iris_cuda_qwen3_profile": (C.c_int, [C.c_void_p, C.POINTER(KernelTime), C.c_int]),
@@ -926,6 +928,28 @@ class Qwen3Lm:
             self.h, *[None if a is None else a.ctypes.data_as(ip) for a in arrs], n, top_k, _f(out["logprob"]),
             _f(out["entropy"]), out["top_ids"].ctypes.data_as(ip), _f(out["top_logprobs"]))
         if rc:
+            raise IrisCudaError(last_error())
+        return out
+
+
+    def sample(self, ids, seq, pos, uniform, temperature=None, top_k=None, top_p=None, min_p=None) -> dict:
+        """Feed tokens and draw the next one behind each (iris_gpu_sample_tokens): next, logprobs.  The settings are
+        one number for all tokens, a list of them, or None."""
+        ip, n = C.POINTER(C.c_int), len(ids)
+        ints = [np.ascontiguousarray(a, np.int32) for a in (ids, seq, pos)]
+        u = np.ascontiguousarray(uniform, np.float64)
+        of = lambda a, ty: None if a is None else np.array(np.broadcast_to(np.asarray(a, ty), (n,)))  # noqa: E731
+        try:
+            t, k, p, m = of(temperature, np.float32), of(top_k, np.int32), of(top_p, np.float32), of(min_p, np.float32)
+        except ValueError:
+            raise IrisCudaError("sample: the settings are one number or as many as tokens") from None
+        if any(a.shape != (n,) for a in (*ints, u)):
+            raise IrisCudaError("sample: ids, seq, pos and uniform are lists of one length")
+        out = dict(next=np.zeros(n, np.int32), logprobs=np.zeros(n, np.float32))
+        opt = lambda a, ty: None if a is None else a.ctypes.data_as(C.POINTER(ty))  # noqa: E731
+        if lib().iris_cuda_qwen3_lm_sample(self.h, *[a.ctypes.data_as(ip) for a in ints], n, opt(t, C.c_float), opt(k, C.c_int),
+                                           opt(p, C.c_float), opt(m, C.c_float), opt(u, C.c_double),
+                                           out["next"].ctypes.data_as(ip), _f(out["logprobs"])):
             raise IrisCudaError(last_error())
         return out
 

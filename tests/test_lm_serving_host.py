@@ -63,7 +63,8 @@ def test_bad_pages_are_refused(bad):
     dict(k_exp=None), dict(v_exp=None), dict(block=0), dict(block=-1), dict(block=5), dict(block=32), dict(exp_page_stride=0),
     dict(exp_page_stride=-4), dict(exp_block_stride=0), dict(exp_block_stride=-1), dict(exp_head_stride=0), dict(exp_head_stride=-1),
     dict(pages=cache(page_size=256, page_stride=256 * 256), block=256), dict(pages=cache(token_stride=264)),
-    dict(pages=cache(head_stride=136)), dict(pages=cache(page_stride=4104))])
+    dict(pages=cache(head_stride=136)), dict(pages=cache(page_stride=4104)), dict(pages=cache(page_stride=1 << 34)),
+    dict(pages=cache(page_stride=1 << 60)), dict(pages=cache(token_stride=1 << 62))])
 def test_bad_8_bit_caches_are_refused(bad):
     c = cache8(**bad)
     refused(append8(c), "rope_append8")
@@ -106,7 +107,7 @@ def test_sample_tokens_refusals(bad):
     refused(sample(**bad), "sample_tokens")
 
 
-BAD_WEIGHTS = [dict(q=None), dict(scale=None), dict(n=0), dict(k=0), dict(group=0), dict(group=16), dict(group=96), dict(group=192),
+BAD_WEIGHTS = [dict(n=(1 << 30) + 1), dict(k=(1 << 30) + 64, q_stride=1 << 30, scale_stride=1 << 30), dict(q=None), dict(scale=None), dict(n=0), dict(k=0), dict(group=0), dict(group=16), dict(group=96), dict(group=192),
                dict(group=512), dict(k=288), dict(q_stride=120), dict(q_stride=136), dict(q_stride=-128), dict(scale_stride=3),
                dict(q=A + 8), dict(scale=A + 1), dict(scale_f32=1, scale=A + 2)]
 
