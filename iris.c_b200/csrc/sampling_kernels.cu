@@ -22,9 +22,9 @@ namespace {
 // With top-k of up to SMP_TOP, or where min-p leaves few, the tokens above a bound
 // (which k of the threads' own largest reach) are few: one block puts them in order
 // and has the answer.  Else a histogram over the distance from m, in parts of
-// SMP_SPAN / SMP_BINS of t, says to 2^-14 (large vocabularies: less closely) how the sum grows along the line
-// (each value adds its weight relative to its bin's, a whole number of 16 bits, so
-// that no order of additions shows); a pass over the row adds up exactly what
+// SMP_SPAN / SMP_BINS of t, says to 2^-14 (large vocabularies: less closely) how the
+// sum grows along the line (each value adds its weight relative to its bin's, a whole
+// number of 16 bits, so that no order of additions shows); a pass over the row adds up exactly what
 // stands ahead of the bins in which the number is crossed and collects their
 // tokens, some hundreds, which one block puts in order.  Where they are too many
 // (equal logits, high temperatures) the bins are cut further, each time into 16,
@@ -71,12 +71,14 @@ struct SmpShared {
   uint32_t n[2], lo, hi;
 };
 
-// shared memory besides the row: the histogram, the sums along the bins, and two lists, in whose place the closer bins stand
+// shared memory besides the row: the histogram, in whose place tokens are put in order; lists of the warps, places of the sort or
+// sums along a line; and two lists, in whose place the closer bins stand
 constexpr int SMP_HIST = SMP_BINS * 4, SMP_ALONG = SMP_BINS * 4;
 constexpr int SMP_TAIL = 2 * SMP_LIST * 8;
 constexpr int SMP_WORK = SMP_HIST + SMP_ALONG + SMP_TAIL;
-static_assert(SMP_TAIL >= SMP_CUT * SMP_CUTTERS * (8 + 4) && SMP_ALONG >= SMP_SORT * 4 && SMP_ALONG >= SMP_WARPS * SMP_OWN * 4 && SMP_ALONG >= SMP_LIST * 8 &&
-              SMP_HIST >= SMP_LIST * 8, "the bins and lists fit");
+static_assert(SMP_TAIL >= SMP_CUT * SMP_CUTTERS * (8 + 4) && SMP_ALONG >= SMP_SORT * 4 &&
+                  SMP_ALONG >= SMP_WARPS * SMP_OWN * 4 && SMP_ALONG >= SMP_LIST * 8 && SMP_HIST >= SMP_LIST * 8,
+              "the bins and lists fit");
 
 struct SmpWindow {  // part of the line: ranks lo .. hi, `count` tokens, with sums over what stands ahead of it
   uint32_t lo, hi;
@@ -119,11 +121,11 @@ struct SmpRow {
   }
   __device__ uint8_t* work() const { return smem + (HELD ? a.held_bytes : 0); }
   __device__ uint32_t* hist() const { return reinterpret_cast<uint32_t*>(work()); }
-  __device__ float* along() const { return reinterpret_cast<float*>(work() + SMP_HIST); }  // sums up to and with a bin, or counts
+  __device__ uint32_t* along() const { return reinterpret_cast<uint32_t*>(work() + SMP_HIST); }
   // the tokens that the blocks have found, each in a part of its own of the first one's lists
   __device__ uint64_t* list(int i = 0) const { return reinterpret_cast<uint64_t*>(work() + SMP_HIST + SMP_ALONG) + i * SMP_LIST; }
   __device__ int quota() const { return SMP_LIST / parts; }
-  // by the first block, when there is no histogram: the tokens in order; when there are no sums along the bins: sums along them
+  // by the first block, behind the histogram: the tokens in order, and sums along them
   __device__ uint64_t* ordered() const { return reinterpret_cast<uint64_t*>(hist()); }
   __device__ double* line() const { return reinterpret_cast<double*>(along()); }
   __device__ double* cut_mass() const { return reinterpret_cast<double*>(list()); }
@@ -306,8 +308,7 @@ struct SmpRow {
     return most_of(&n->x) <= quota();
   }
 
-  // ---- by the first block: the blocks' tokens, n in all, in order, largest first, into ordered().  (Of many, the sums along
-  // the bins are lost, those of the first block)
+  // ---- by the first block: the blocks' tokens, n in all, in order, largest first, into ordered().  
   __device__ static int tokens_of(const uint2& v, int) { return (int)v.x; }
   __device__ static int tokens_of(const SmpExact& v, int which) { return (int)v.n[which]; }
   template <typename Found>
@@ -345,7 +346,7 @@ struct SmpRow {
       return;
     }
     // by value into SMP_SORT places, then by comparison within a place
-    uint32_t* count = reinterpret_cast<uint32_t*>(along());
+    uint32_t* count = along();
     uint64_t* sorted = list(which);
     uint32_t top_rank = 0, low_rank = 0;
 #pragma unroll
@@ -449,15 +450,15 @@ struct SmpRow {
     if (tid == 0) answer((int)~(uint32_t)ordered()[pick], logprob(ordered()[pick], m_kept), kept);
   }
 
-  // ---- how the line grows along the bins: along()[b] is the sum up to and with bin b, to near_ (or the count, a whole number)
+  // ---- how the line grows along the bins: the sum up to and with each bin, to near_ (or the count, a whole number)
   __device__ float distance(float y) const {
     return fminf((plain ? m - y : fminf(m - y, FLT_MAX)) * inv_bin, SMP_BINS - 1);
   }
   __device__ static float nearest(float d) { return (d + 0x1.8p23f) - 0x1.8p23f; }  // whole number, ties to even
   __device__ float bin_of(float y) const { return nearest(distance(y)); }           // the bins are around whole numbers
-  // y: the sums up to and with this thread's bins, and the bin before them
+  // y: the sums up to and with this thread's bins
   template <bool COUNTS>
-  __device__ void measure(float y[SMP_MINE + 1], float& last) {
+  __device__ void measure(float y[SMP_MINE], float& last) {
     uint32_t* h = hist();
     for (int i = tid; i < SMP_BINS; i += SMP_THREADS) h[i] = 0;
     __syncthreads();
@@ -497,17 +498,15 @@ struct SmpRow {
       for (int j = 0; j < SMP_MINE; j++) n_all += n[j];
       uint32_t all, before = scan_count(n_all, &all);
       last = __uint_as_float(all);
-      y[0] = __uint_as_float(before);
 #pragma unroll
-      for (int j = 0; j < SMP_MINE; j++) before += n[j], y[j + 1] = __uint_as_float(before);
+      for (int j = 0; j < SMP_MINE; j++) before += n[j], y[j] = __uint_as_float(before);
     } else {
       const float one = exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * SMP_MINE * tid) / unit;
 #pragma unroll
       for (int j = 0; j < SMP_MINE; j++) s[j] *= one * exp2_approx(-kLog2e * SMP_SPAN / SMP_BINS * j), s_all += s[j];
       float before = scan_float(s_all, &last);
-      y[0] = before;
 #pragma unroll
-      for (int j = 0; j < SMP_MINE; j++) before += s[j], y[j + 1] = before;
+      for (int j = 0; j < SMP_MINE; j++) before += s[j], y[j] = before;
     }
   }
   // Most that the tokens of the last bin, which was not measured, can weigh.
@@ -522,7 +521,7 @@ struct SmpRow {
     SmpExact e = {};
     // The vectors that have a token of a window, few, are put into a list of the warp's own and looked at by all its lanes when
     // there are enough.
-    uint32_t* own = reinterpret_cast<uint32_t*>(along()) + tid / 32 * SMP_OWN;
+    uint32_t* own = along() + tid / 32 * SMP_OWN;
     uint32_t found = 0;
     auto look = [&]() {
       __syncwarp();
@@ -643,18 +642,24 @@ struct SmpRow {
 
   // ---- the first bin with which a sum of `from` may be reached (a count: is), and the first with which one of `to` surely is
   // passed; y as measure() gives it
-  __device__ void bins(bool counts, double from, double to, const float y[SMP_MINE + 1], float& b0, float& b1) {
+  __device__ void bins(bool counts, double from, double to, const float y[SMP_MINE], float& b0, float& b1) {
     if (tid == 0) sh.lo = sh.hi = SMP_BINS - 1;
     __syncthreads();
-    bool may = false, must = false;
+    // the least of the threads' first bins: a thread's sums and the next one's are rounded apart, so that where they meet neither
+    // may see a step
+    uint32_t lo = SMP_BINS - 1, hi = SMP_BINS - 1;
 #pragma unroll
-    for (int j = 0; j <= SMP_MINE; j++) {
-      const bool now_may = counts ? (double)__float_as_uint(y[j]) >= from : (double)(y[j] * (1.f + near_)) >= from;
-      const bool now_must = counts ? now_may : (double)(y[j] * (1.f - near_)) > to;
-      const int b = SMP_MINE * tid + j - 1;
-      if (j && b < SMP_BINS - 1 && now_may && !may) sh.lo = b;
-      if (j && b < SMP_BINS - 1 && now_must && !must) sh.hi = b;
-      may = now_may && (j || tid), must = now_must && (j || tid);
+    for (int j = SMP_MINE - 1; j >= 0; j--) {
+      const uint32_t b = SMP_MINE * tid + j;
+      if (b >= SMP_BINS - 1) continue;
+      const bool may = counts ? (double)__float_as_uint(y[j]) >= from : (double)(y[j] * (1.f + near_)) >= from;
+      if (may) lo = b;
+      if (counts ? may : (double)(y[j] * (1.f - near_)) > to) hi = b;
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_min_sync(0xffffffffu, hi);
+    if (tid % 32 == 0) {
+      if (lo < SMP_BINS - 1) atomicMin(&sh.lo, lo);
+      if (hi < SMP_BINS - 1) atomicMin(&sh.hi, hi);
     }
     __syncthreads();
     b0 = (float)sh.lo, b1 = (float)sh.hi;
@@ -666,7 +671,7 @@ struct SmpRow {
 
   // ---- no top-k: top-p, and the token, in one pass.  How much is kept is known well enough from the bins to say where the
   // token may be.  False where the tokens there find no room; then the sum and number of all are known.
-  __device__ bool at_once(float p, double u, const float y[SMP_MINE + 1], float last, double& all, uint32_t& n_all) {
+  __device__ bool at_once(float p, double u, const float y[SMP_MINE], float last, double& all, uint32_t& n_all) {
     float b0[2], b1[2];
     double from = least_sum(last), to = most_sum(last);
     if (p < 1.f) {
@@ -675,7 +680,7 @@ struct SmpRow {
       // what is kept ends in these bins
 #pragma unroll
       for (int j = 0; j < SMP_MINE; j++)
-        if (SMP_MINE * tid + j == (int)b1[1]) sh.fscan[0] = y[j + 1];
+        if (SMP_MINE * tid + j == (int)b1[1]) sh.fscan[0] = y[j];
       __syncthreads();
       to = b1[1] < SMP_BINS - 1 ? (double)sh.fscan[0] * (1.0 + near_) : most_sum(last);
       __syncthreads();
@@ -717,7 +722,7 @@ struct SmpRow {
   }
 
   // ---- the token at which the count or the sum crosses `goal`.  (kind SMP_PASS, the last one: for the first block alone)
-  __device__ SmpFound search(SmpKind kind, double goal, const float y[SMP_MINE + 1]) {
+  __device__ SmpFound search(SmpKind kind, double goal, const float y[SMP_MINE]) {
     float b0, b1;
     bins(kind == SMP_COUNT, goal, goal, y, b0, b1);
     SmpWindow w;
@@ -939,7 +944,7 @@ struct SmpRow {
     double mass = 0.0;
     uint32_t kept = 0;
     uint64_t end = 0;       // the last place that is kept, where that is known
-    float y[SMP_MINE + 1], last;
+    float y[SMP_MINE], last;
     bool known = false;     // whether mass and kept are
     if (k) {
       measure<true>(y, last);

@@ -189,6 +189,30 @@ def test_sample_tokens_follows_the_distribution(ops):
     assert ((count - n * torch.softmax(x[0].double().cpu(), 0)).abs() <= 1.0).all()
 
 
+@pytest.mark.parametrize("top_p", (None, 0.75))
+def test_sample_tokens_a_million_draws(ops, top_p):
+    """Draws all along one row's line, against a search in its 64-bit sums.  A random number within 2^-30 of a token's end (the
+    two sums are within 5000 * 2^-52 of each other) may go either way."""
+    vocab, rows = 5000, 8192
+    x = torch.randn(vocab, generator=torch.Generator().manual_seed(41)).cuda() * 2
+    line = torch.argsort(x.double(), descending=True, stable=True)
+    w = torch.exp(x.double() - x.double().max())[line]
+    if top_p:
+        w = w[:int((torch.cumsum(w, 0) - w < np.float64(np.float32(top_p)) * w.sum()).sum())]
+    end = torch.cumsum(w, 0) / w.sum()
+    logits, ids = x.repeat(rows, 1), torch.empty(rows, dtype=torch.int32, device="cuda")
+    p = None if top_p is None else torch.full((rows,), top_p, device="cuda")
+    wrong = 0
+    for i in range(128):
+        u = torch.rand(rows, generator=torch.Generator().manual_seed(i), dtype=torch.float64).cuda()
+        ops.sample_tokens(logits, u, ids, top_p=p)
+        at = torch.searchsorted(end, u, right=True).clamp(max=w.numel() - 1)
+        near = torch.minimum((end[at] - u).abs(), (end[(at - 1).clamp(min=0)] - u).abs()) < 2.0 ** -30
+        wrong += int(((ids.long() != line[at]) & ~near).sum())
+    assert wrong == 0
+
+
+
 # ------------------------------------------------------------------ the 8-bit cache
 def pool8(pages, page, heads, d, hm, seed, block):
     """A pool with earlier values and their exponents."""
