@@ -11,7 +11,8 @@ namespace {
 
 // ------------------------------------------------------------------ products
 //   y[r][n] = sum over groups g of  s[n][g] sum over k in g of (q[n][k] - z[n][g]) x[r][k]   (+ add[r][n])
-// Bound by the weights' bytes.  The products are mma m16n8k16 with 16 rows of the
+// Should be bound by the weights' bytes; the pipe of shifts and logic that unpacks them is (below).  151936 x 2560 in groups of 32,
+// one row: 65 us, 34 for the bytes; 6144 x 2560 in groups of 128: 5.5 us, of which 1.3.  The products are mma m16n8k16 with 16 rows of the
 // weights as m and 8 rows of x as n.  q - z is a whole number of at most 8 bits,
 // exact in bf16, and so is x; the scale multiplies a group's f32 sum.
 // A 32-bit word holds eight columns k .. k + 7 of a row; its halves' nibble j give
@@ -414,19 +415,39 @@ cudaError_t go(Kernel kernel, dim3 grid, size_t smem, cudaStream_t stream, const
   return iris::launch_cluster_overlapped(kernel, grid, dim3(L4_THREADS), smem, a.parts, stream, a);
 }
 
-template <int NT, int WK, int GS, bool ZERO>
-cudaError_t go_rows(IrisLinear4* a, int num_sms, cudaStream_t stream) {
-  using Sh = L4Rows<NT, WK>;
-  const int blocks = (a->rows + NT * 8 - 1) / (NT * 8), strips = (a->n + Sh::kRows - 1) / Sh::kRows;
-  const int steps = ((a->k + L4_CHUNK - 1) / L4_CHUNK + WK - 1) / WK;
-  // as many parts of k as let all blocks be on the device at once, two an SM, of which clusters reach seven eighths
-  const int64_t fit = num_sms * 2 * 7 / 8 / ((int64_t)strips * blocks);
-  a->parts = (int)(fit < 8 ? fit : 8);
-  if (a->parts > steps / 2) a->parts = steps / 2;
-  if (a->parts < 1) a->parts = 1;
-  return go(linear4_rows_kernel<NT, WK, GS, ZERO>, dim3((unsigned)strips, blocks), Sh::kSmem, stream, *a);
+// Parts of k for blocks of 128 / wk rows of the weights and 8 nt of x: as many as let all blocks be on the device at once, two an
+// SM, of which clusters reach seven eighths (16 rows of 9728 -> 2560 28 -> 11 us, of 4096 -> 2560 13 -> 6.8)
+int rows_parts(const IrisLinear4* a, int nt, int wk, int num_sms, int64_t* blocks) {
+  const int64_t base = (int64_t)((a->n + 128 / wk - 1) / (128 / wk)) * ((a->rows + nt * 8 - 1) / (nt * 8));
+  const int steps = ((a->k + L4_CHUNK - 1) / L4_CHUNK + wk - 1) / wk;
+  int64_t parts = num_sms * 2 * 7 / 8 / base;
+  if (parts > 8) parts = 8;
+  if (parts > steps / 2) parts = steps / 2;
+  if (parts < 1) parts = 1;
+  *blocks = base * parts;
+  return (int)parts;
 }
 
+template <int NT, int WK, int GS, bool ZERO>
+cudaError_t go_rows(IrisLinear4* a, int parts, cudaStream_t stream) {
+  using Sh = L4Rows<NT, WK>;
+  a->parts = parts;
+  const dim3 grid((unsigned)((a->n + Sh::kRows - 1) / Sh::kRows), (a->rows + NT * 8 - 1) / (NT * 8));
+  return go(linear4_rows_kernel<NT, WK, GS, ZERO>, grid, Sh::kSmem, stream, *a);
+}
+
+// Warps that share 16 rows of the weights: one where the weights have many rows (16 rows of x, n 75776 of k 2560 46 us, 51 with
+// two; 151936 97 and 103) or where that lets more blocks be on the device at once (n 6144 8.0 and 8.8, 9728 11.4 and 13.2); else
+// two (n 38912 33 us, 36 with one; 25600 21 and 23; 2560 of k 9728 11 and 13).
+template <int NT, int GS, bool ZERO>
+cudaError_t rows_variant(IrisLinear4* a, int num_sms, cudaStream_t stream) {
+  int64_t one, two;
+  const int parts1 = rows_parts(a, NT, 1, num_sms, &one), parts2 = rows_parts(a, NT, 2, num_sms, &two);
+  if (a->n >= 4 * 128 * num_sms || one > two) return go_rows<NT, 1, GS, ZERO>(a, parts1, stream);
+  return go_rows<NT, 2, GS, ZERO>(a, parts2, stream);
+}
+
+// parts: while that adds blocks for which there is room (one row of 9728 -> 2560 11.0 -> 9.6 us)
 template <int MT, int WK, int GS, bool ZERO>
 cudaError_t go_few(IrisLinear4* a, int num_sms, cudaStream_t stream) {
   constexpr int rows = L4_WARPS / WK * MT * 16;
@@ -436,11 +457,12 @@ cudaError_t go_few(IrisLinear4* a, int num_sms, cudaStream_t stream) {
   return go(linear4_kernel<MT, WK, GS, ZERO>, dim3((unsigned)strips), L4_WARPS * L4_RING * MT * L4_STAGE, stream, *a);
 }
 
+// Up to 8 rows: all of a block's warps on 16 rows of the weights (one row of x, n 9728 of k 2560 8.1 us, 11.8 with two; 38912 22.5
+// and 24.8), or, of many rows, two on 32 (75776 32 us, 41 with all; 151936 63 and 79).
 template <int GS, bool ZERO>
 cudaError_t variant(IrisLinear4* a, int num_sms, cudaStream_t stream) {
-  const bool many = a->n > 16 * 8 * num_sms;
-  if (a->rows > 16) return many ? go_rows<4, 1, GS, ZERO>(a, num_sms, stream) : go_rows<4, 2, GS, ZERO>(a, num_sms, stream);
-  if (a->rows > 8) return many ? go_rows<2, 1, GS, ZERO>(a, num_sms, stream) : go_rows<2, 2, GS, ZERO>(a, num_sms, stream);
+  if (a->rows > 16) return rows_variant<4, GS, ZERO>(a, num_sms, stream);
+  if (a->rows > 8) return rows_variant<2, GS, ZERO>(a, num_sms, stream);
   return a->n >= 4 * 128 * num_sms ? go_few<2, 2, GS, ZERO>(a, num_sms, stream) : go_few<1, 8, GS, ZERO>(a, num_sms, stream);
 }
 

@@ -984,12 +984,16 @@ constexpr int SMP_PART = 75 * 1024;   // the same where two blocks are to fit an
 template <typename In>
 cudaError_t launch(IrisSample* a, int num_sms, cudaStream_t stream) {
   const int64_t bytes = (int64_t)a->vocab * (int64_t)sizeof(In) + 16;
-  // Blocks on a row: as many as leave each no more than SMP_PART of it, so that two fit an SM, and more where the device has room
-  // for them and each keeps 16 KB
+  // Blocks on a row: as many as leave each no more than SMP_PART of it, so that two fit an SM (512 f32 rows of 151936, usual
+  // settings 167 us, 201 with twice that; top-p alone 594 and 581), and more where each keeps 16 KB and the device has room
+  // for them: for two blocks an SM up to four a row (48 bf16 rows of 32000 with top-p 24 us, 28 with one), for eight, of which
+  // clusters reach seven eighths of the SMs, one (16 bf16 rows of 151936, usual settings 9.7 us, 11.4 with four; 32 rows 15.4 with
+  // eight and two an SM, 12.2 with four).
   a->parts = 1;
   while (a->parts < SMP_PARTS &&
          (bytes > (int64_t)a->parts * SMP_PART ||
-          (bytes > (int64_t)a->parts * 16384 && (int64_t)a->rows * a->parts * 2 <= 2 * num_sms)))
+          (bytes > (int64_t)a->parts * 16384 &&
+           (int64_t)a->rows * a->parts * 2 <= (a->parts < 4 ? 2 * num_sms : num_sms * 7 / 8))))
     a->parts *= 2;
   const int64_t vecs = (bytes + 15) / 16, held = (vecs + a->parts - 1) / a->parts * 16;
   const bool fits = held <= SMP_MOST;
