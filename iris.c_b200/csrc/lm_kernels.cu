@@ -475,13 +475,13 @@ __device__ __forceinline__ float queries8(const __nv_bfloat16* q, bool live, int
 // of four e4m3, all bits of each one that is NaN
 __device__ __forceinline__ uint32_t nan4(uint32_t x) { return __vcmpeq4(x & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
 
-// HD: head_dim.  MH: query heads of a unit (8 or 16).  CLUSTER: few rows (see the kernel).
-template <typename E, int HD, int MH, bool CLUSTER>
+// HD: head_dim.  MH: query heads of a unit (8 or 16).
+template <typename E, int HD, int MH>
 struct PagedShape {
   // Keys of a tile that a warp takes.  Over 8 bits 32 have half the steps' shuffles, page numbers and scales (64 rows of 1 to
-  // 8192 keys, 32 heads on 8 of 128: 357 instructions for 16 keys instead of 500, 100.3 us instead of 102.6); few rows want
-  // more warps (one of 512 keys: 6.6 us with 32, 5.6 with 16).
-  static constexpr int kKeys = kEight<E> && (!CLUSTER || MH == 16) ? 32 : 16;
+  // 8192 keys, 32 heads on 8 of 128: 357 instructions for 16 keys instead of 500, 100.3 us instead of 102.6; of few rows, one
+  // of 512 keys 6.5 us either way, 8 of 512 9.2 and 10.1, one of 2048 10.5 and 10.3).
+  static constexpr int kKeys = kEight<E> ? 32 : 16;
   static constexpr int kGroups = IRIS_PAGED_TILE / kKeys;        // of them
   static constexpr int kPair = HD / 128 ? HD / 128 : 1;          // warps on the same keys, 128 columns of o each
   static constexpr int kThreads = 32 * kGroups * kPair;
@@ -492,7 +492,7 @@ struct PagedShape {
   static constexpr int kRow = HD * (int)sizeof(E);               // bytes of a row
   // Over 8 bits (64 rows of 1 to 8192 keys, 32 heads on 8 of 128) 4 CTAs of two warps with 3 stages 100.3 us, 5 x 2 103.7, 6 x 2
   // 109, 3 x 4 168: loads in flight as much as warps.
-  static constexpr int kCtas = kEight<E> ? (HD == 64 ? (kKeys == 16 ? 5 : MH == 16 ? 6 : 8) : HD == 128 ? 4 : 2)
+  static constexpr int kCtas = kEight<E> ? (HD == 64 ? (MH == 16 ? 6 : 8) : HD == 128 ? 4 : 2)
                                          : HD == 64 ? 4 : HD == 128 ? 2 : 1;
   static constexpr int kStages = kEight<E> ? 3 : HD == 64 || MH == 16 ? 2 : 3;
   static constexpr int kStageBytes = kKeys * kRow;               // a warp's rows of K or of V
@@ -592,9 +592,9 @@ __device__ __forceinline__ bool paged_begin(const IrisPagedAttention& a, int uni
 // equal part of its tiles each, and joins the parts in distributed shared
 // memory: one launch, and no round through the workspace.
 template <typename E, int HD, int MH, bool CLUSTER>
-__global__ void __launch_bounds__(PagedShape<E, HD, MH, CLUSTER>::kThreads, PagedShape<E, HD, MH, CLUSTER>::kCtas)
+__global__ void __launch_bounds__(PagedShape<E, HD, MH>::kThreads, PagedShape<E, HD, MH>::kCtas)
 paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
-  using Sh = PagedShape<E, HD, MH, CLUSTER>;
+  using Sh = PagedShape<E, HD, MH>;
   constexpr bool EIGHT = kEight<E>;
   constexpr int D = Sh::kStages, CH = Sh::kRow / 16;  // CH: 16-byte chunks of a row
   constexpr int PAIR = Sh::kPair, T = Sh::kThreads, OC = HD / PAIR;  // OC: columns of o a warp holds
@@ -679,7 +679,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
   auto issue = [&](int stage) {
     if constexpr (EIGHT) {
       // the exponents of the stage before: read a round ago, needed in the next one at the earliest
-      if (exps_to >= 0 && half == 0 && lane < KEYS) put_scales(scales[kg][exps_to], lane, exp8(ke), exp8(ve));
+      if (exps_to >= 0 && half == 0) put_scales(scales[kg][exps_to], lane, exp8(ke), exp8(ve));
       exps_to = loads ? stage : -1;
     }
     if (loads) {
@@ -1506,7 +1506,7 @@ constexpr int JOIN_THREADS = 512;
 template <int HD, int MH, bool FEW>
 __global__ void __launch_bounds__(JOIN_THREADS)
 paged_join_kernel(const __grid_constant__ IrisPagedAttention a, int ctas, int per_block) {
-  using Sh = PagedShape<__nv_bfloat16, HD, MH, false>;  // pieces are f32, alike for both
+  using Sh = PagedShape<__nv_bfloat16, HD, MH>;  // pieces are f32, alike for both
   constexpr int COLS = HD / 4;
   __shared__ float4 acc[JOIN_THREADS];
   __shared__ float2 ml[JOIN_THREADS / COLS];
@@ -2137,8 +2137,7 @@ constexpr int CLUSTER_TILES = 4;
 
 template <typename E, int HD, int MH>
 struct PagedLaunch {
-  using Sh = PagedShape<E, HD, MH, false>;
-  using Few = PagedShape<E, HD, MH, true>;
+  using Sh = PagedShape<E, HD, MH>;
   using Runs = RunShape<E, HD>;
   static size_t ws_bytes(int num_sms) {
     const int ctas = num_sms * Sh::kCtas, runs = num_sms * Runs::kCtas;
@@ -2152,7 +2151,7 @@ struct PagedLaunch {
     e = cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                Sh::kSmem);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few::kSmem);
+    return cudaFuncSetAttribute(paged_attention_kernel<E, HD, MH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
   }
   static cudaError_t launch(const IrisPagedAttention* a, int num_sms, cudaStream_t stream, int* launches) {
     // few rows: a block, or a cluster of up to 8, on each unit, all on the device at once (clusters of 4 and 8 do not fill
@@ -2165,13 +2164,13 @@ struct PagedLaunch {
     const int64_t units = (int64_t)a->rows * iris_paged_units(&a->cache, a->heads);
     const int room = iris_paged_tiles(iris_paged_len(&a->cache, 0x7FFFFFFF));
     unsigned parts = 8;
-    const int64_t slots = (int64_t)num_sms * Few::kCtas;
+    const int64_t slots = (int64_t)num_sms * Sh::kCtas;
     while (parts > 1 && units * parts > (parts > 2 ? slots * 7 / 8 : slots)) parts /= 2;
     const int64_t tiles = 2 * CLUSTER_TILES * units * parts / slots + 1;  // 2 CLUSTER_TILES with every slot taken
     if (units * parts <= slots && room <= (tiles < CLUSTER_TILES ? CLUSTER_TILES : tiles) * parts) {
       *launches = 1;
       return iris::launch_cluster_overlapped(paged_attention_kernel<E, HD, MH, true>, dim3((unsigned)units * parts),
-                                             dim3(Few::kThreads), Few::kSmem, parts, stream, *a);
+                                             dim3(Sh::kThreads), Sh::kSmem, parts, stream, *a);
     }
     // four times as many rows as sequences: runs of rows.  On the device, 32 heads on 8 of 128, rows by themselves -> runs:
     // a prompt of 128 15.3 -> 15.8 us, 512 83 -> 31, 2048 934 -> 196, 8192 13.7 -> 2.6 ms; 64 tokens behind 32704 855 ->

@@ -224,10 +224,6 @@ struct SmpRow {
   }
   __device__ uint32_t scan_count(uint32_t v, uint32_t* total) { return scan(v, sh.iscan, total); }
   __device__ float scan_float(float v, float* total) { return scan(v, sh.fscan, total); }
-  __device__ double scan_mass(double v) {
-    double total;
-    return scan(v, sh.scan, &total);
-  }
   // over the blocks' numbers
   __device__ uint32_t most_of(const uint32_t* first_of_pairs) const {
     return __reduce_max_sync(0xffffffffu, tid % 32 < parts ? first_of_pairs[tid % 32 * 2] : 0u);

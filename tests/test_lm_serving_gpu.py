@@ -348,6 +348,30 @@ def test_rope_append8_one_token_at_a_time(ops):
             assert (err <= 2.0 ** -3 * pn[i].float().abs() + 2.0 ** -9).all()
 
 
+@pytest.mark.parametrize("n", (7, 1203))
+def test_rope_append8_numbers_at_any_address(ops, n):
+    """Sequence numbers that do not start at 16 bytes, tokens in any order: the same bytes."""
+    d, nkv, page, block, seqs = 64, 3, 32, 16, 5
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, nkv * d, device="cuda", generator=gen(n))
+    blocks = (n + seqs - 1) // seqs // page + 1
+    order = torch.randperm(n, generator=g)
+    seq, pos = (order % seqs).int(), (order // seqs).int()
+    got = []
+    for at in (0, 1, 3):
+        pools = [torch.zeros(seqs * blocks, page, nkv, d, device="cuda", dtype=torch.uint8).view(E4) for _ in range(2)]
+        exps = [torch.zeros(seqs * blocks, page // block, nkv, device="cuda", dtype=torch.uint8) for _ in range(2)]
+        cache = ops.KvCache8.of(*pools, *exps, torch.arange(seqs * blocks, dtype=torch.int32).view(seqs, blocks).cuda())
+        s = torch.full((n + 4,), -1, dtype=torch.int32, device="cuda")
+        s[at:at + n] = seq.cuda()
+        ops.rope_append8(cache, None, None, None, x, x, s[at:at + n], pos.cuda(), heads=0, stream=stream())
+        torch.cuda.synchronize()
+        got.append([p.view(torch.uint8) for p in pools] + exps)
+    assert got[0][0].any()
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
 def test_rope_append8_odd_values(ops):
     """Infinities and NaN are held as NaN and do not move the scale; zeros; magnitudes past the range."""
     d, page = 64, 8
