@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
 // the first of them: it looks for the others among all tokens of the call, in
 // whatever order they stand (a token whose mate is the row before is left out at
 // once, so that a prompt's rows are searched once a block of the cache).  Lanes hold
-// columns as above; a warp has a (head, K or V) and APPEND8_ROUNDS mates in
+// columns as above; a warp has a (head, K or V) and BATCH of its mates in
 // registers, and goes over the mates twice, for the largest magnitude and, behind the
 // scale, for the values, from the registers where all fit.  Other blocks of the same
 // launch do the queries, 64 threads a token as above.
