@@ -852,8 +852,9 @@ int iris_gpu_rope_append8(const iris_gpu_kv_cache8_t *cache, const iris_gpu_rope
 
 /* iris_gpu_attention_paged over an 8-bit cache.  Keys and values are the numbers
  * that they stand for, and NaN shows as there (a value of NaN makes its column NaN).
- * The softmax weight of a key times its value's scale counts with 11 bits, and as 0
- * under 2^-25 of the row's largest. */
+ * The softmax weight of a key times its value's scale counts with 22 bits, or in
+ * steps of 2^-39 of the row's largest where these are wider; a query's column in
+ * steps of 2^-38 of the head's largest where these are wider than its own bits. */
 size_t iris_gpu_attention_paged8_workspace(const iris_gpu_kv_cache8_t *cache, int heads);
 int iris_gpu_attention_paged8(const iris_gpu_kv_cache8_t *cache, void *out, const void *q, int64_t ldo, int64_t ldq,
                               const int32_t *seq, const int32_t *pos, int rows, int heads, float scale,

@@ -405,13 +405,24 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_
 // A cache's elements: bf16, or e4m3 with exponents (an 8-bit cache).
 //
 // Over 8 bits the products are of f16, which holds every e4m3 value; the queries of
-// a head are scaled by a power of two to fill f16's range (what is under 2^-29 of the
-// largest loses bits).  A key's scale multiplies its score.  The value's scale 2^ve
+// a head are scaled by a power of two to fill f16's range (steps of 2^-38 of the
+// largest, where these are wider than a column's own bits).  A key's scale multiplies its score.  The value's scale 2^ve
 // joins the weight instead: with t = s c + ve the running maximum is that of t, p =
-// 2^(t - m) is at most 1 and rounded to f16, 11 bits, and l adds up p 2^-ve in f32.
-// So one product of p and the values as they lie does where bf16 takes two.
+// 2^(t - m + 15), in the upper part of f16's range, and l adds up p 2^-ve in f32.  p
+// comes in two parts of f16, the second what the first one's rounding left: 22
+// bits, or steps of 2^-39 of the largest where that is more.  (One part, 11 bits and
+// steps of 2^-24, took 200 us instead of 207 for a prompt of 2047, 104 and 104 for 64
+// rows of up to 8192 keys, 32.5 and 34.9 for 64 with 32 heads on 2 of 64.)
 typedef __nv_fp8_storage_t e4m3;
 template <typename E> constexpr bool kEight = sizeof(E) == 1;
+constexpr float UP8 = 15.f;  // (added to t - m, not taken from m: of a large m it would be rounded away)
+
+__device__ __forceinline__ void split8(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(p0, p1);
+  const float2 first = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = pack2h(p0 - first.x, p1 - first.y);
+}
 
 // bytes of a row of K or V lie in 16-byte chunks; chunk ch of row r is at place swz(ch, r), so that ldmatrix meets no bank
 // conflict
@@ -872,7 +883,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
         float kx[2 * KS], vx[2 * KS], vi[2 * KS];  // of keys 8 i + g
 #pragma unroll
         for (int i = 0; i < 2 * KS; i++) kx[i] = sc.k[8 * i + g], vx[i] = sc.v[8 * i + g], vi[i] = sc.v_inv[8 * i + g];
-        uint32_t pt[KS][R][2];
+        uint32_t pt[KS][R][2], rest[KS][R][2];
         float f[S];
         bool moved = false;
 #pragma unroll
@@ -899,15 +910,19 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 #pragma unroll
             for (int i = 0; i < 2 * KS; i++) {
               float& y = x[i / 2][r][i % 2 * 2 + h];
-              y = exp2_approx(y - base);
+              y = exp2_approx((y - base) + UP8);
               sum += y * vi[i];
             }
             l[e] = l[e] * f[e] + sum;
           }
 #pragma unroll
           for (int k = 0; k < KS; k++) {
-            pt[k][r][0] = transposed(pack2h(x[k][r][0], x[k][r][1]));
-            pt[k][r][1] = transposed(pack2h(x[k][r][2], x[k][r][3]));
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              uint32_t hi, lo;
+              split8(x[k][r][2 * i], x[k][r][2 * i + 1], hi, lo);
+              pt[k][r][i] = transposed(hi), rest[k][r][i] = transposed(lo);
+            }
           }
         }
         if (__any_sync(0xffffffffu, moved)) {
@@ -934,7 +949,10 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
               e4m3_to_f16(__byte_perm(b[2 * n], 0u, 0x3120), a0, a1);
               e4m3_to_f16(__byte_perm(b[2 * n + 1], 0u, 0x3120), a2, a3);
 #pragma unroll
-              for (int r = 0; r < R; r++) mma_f16(o[(2 * j + n) * R + r], a0, a1, a2, a3, pt[k][r][0], pt[k][r][1]);
+              for (int r = 0; r < R; r++) {
+                mma_f16(o[(2 * j + n) * R + r], a0, a1, a2, a3, pt[k][r][0], pt[k][r][1]);
+                mma_f16(o[(2 * j + n) * R + r], a0, a1, a2, a3, rest[k][r][0], rest[k][r][1]);
+              }
             }
           }
       }
@@ -1307,10 +1325,12 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
 #pragma unroll
           for (int k = 0; k < 4; k++) {  // rows g, g + 8, g, g + 8; keys 0-7, 0-7, 8-15, 8-15
             const int h = k & 1, b = 2 * n + k / 2;
-            const float p0 = exp2_approx(s[b][2 * h] - base[h]), p1 = exp2_approx(s[b][2 * h + 1] - base[h]);
+            float t0 = s[b][2 * h] - base[h], t1 = s[b][2 * h + 1] - base[h];
+            if constexpr (EIGHT) t0 += UP8, t1 += UP8;
+            const float p0 = exp2_approx(t0), p1 = exp2_approx(t1);
             if constexpr (EIGHT) {
               l[h] += p0 * vi[k / 2].x + p1 * vi[k / 2].y;
-              hi[k] = pack2h(p0, p1);
+              split8(p0, p1, hi[k], lo[k]);
             } else {
               l[h] += p0 + p1;
               split2(p0, p1, hi[k], lo[k]);
@@ -1329,6 +1349,8 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
                 e4m3_to_f16(__byte_perm(b[2 * i + 1], 0u, 0x3120), e1, d1);
                 mma_f16(o[4 * j + 2 * i], hi[0], hi[1], hi[2], hi[3], e0, e1);
                 mma_f16(o[4 * j + 2 * i + 1], hi[0], hi[1], hi[2], hi[3], d0, d1);
+                mma_f16(o[4 * j + 2 * i], lo[0], lo[1], lo[2], lo[3], e0, e1);
+                mma_f16(o[4 * j + 2 * i + 1], lo[0], lo[1], lo[2], lo[3], d0, d1);
               }
             }
           }

@@ -1,0 +1,86 @@
+"""Sampling, the 8-bit cache and 4-bit weights on the GPU against plain 64-bit forms: small weights, the kernels that
+large calls get, magnitudes at the ends of the range.
+
+Tolerances (u = 2^-24, half an f32 step; 2^-8 half a bf16 step, relative):
+
+attention_paged8: 2^-8 of the value and, times A = sum p |v|: 4 hd u S for the scores (S the largest sum of scale |q k|), len u
+  for the sums, 8 u (T + 15) for the rounding of the exponent, which has five roundings of numbers up to T + 15 (T the largest
+  magnitude of a key's score and scale in powers of two, 15 what they are raised by; numerator and denominator see them) times
+  ln 2, and 2^-21 for the exponential (2^-22) and weights of 22 bits.  Weights under 2^-25 of the largest weight times scale W
+  come in steps of 2^-39 of it (their second part is a multiple of 2^-24 where the largest is 2^15), rounded: 2^-40 448 W a
+  key.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from test_lm_ops_gpu import BF, U, gen, i32, stream
+from test_lm_serving_gpu import E4, one_sequence8, ops, values8  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def attention8_fine64(q, k, v, vs, scale):
+    """q [heads, d], k / v [len, d], vs [len] scales of the values -> (out, tolerance) [heads, d]."""
+    n, d = k.shape
+    q = q.double().cpu()
+    s = scale * q @ k.t()
+    p = torch.softmax(s, -1)
+    size = abs(scale) * (q.abs() @ k.abs().t()).amax(-1)
+    t = (s * math.log2(math.e) + torch.log2(vs)).abs().amax(-1)
+    out, a = p @ v, p @ v.abs()
+    slack = (4 * d * U * size + n * U + 8 * U * (t + 15) + 2.0 ** -21)[:, None] * a
+    return out, BF * out.abs() + slack + (n * 2.0 ** -40 * 448 * (p * vs).amax(-1))[:, None]
+
+
+def check_one_sequence8(ops, n, new, q, k, v, ke, ve, table, block, scale):  # noqa: F811
+    """The newest `new` rows of a sequence of n keys, all heads on one."""
+    cache = ops.KvCache8.of(k, v, ke, ve, table)
+    heads, d = q.shape[1:]
+    out = torch.zeros_like(q)
+    ws = torch.empty(ops.attention_paged8_workspace(cache, heads), device="cuda", dtype=torch.uint8)
+    ops.attention_paged8(cache, out, q, i32([0] * new), i32(range(n - new, n)), scale=scale, workspace=ws, stream=stream())
+    torch.cuda.synchronize()
+    kv, vv = (values8(p, e, block).flatten(0, 2) for p, e in ((k, ke), (v, ve)))
+    vs = 2.0 ** (ve.cpu().double().repeat_interleave(block, 1).flatten() - 127)
+    scale = float(np.float32(scale))
+    for r in range(new):
+        at = n - new + r + 1
+        want, tol = attention8_fine64(q[r], kv[:at], vv[:at], vs[:at], scale)
+        err = (out[r].double().cpu() - want).abs()
+        assert (err <= tol).all(), (r, float(err.max()), float(want.abs().max()), float((err / tol).max()))
+
+
+@pytest.mark.parametrize("d", (64, 128, 256))
+@pytest.mark.parametrize("n,new,heads", [(300, 1, 4), (5000, 1, 16), (300, 90, 4), (200, 130, 16)])
+@pytest.mark.parametrize("kind", ("cancel", "steps", "many", "scales"))
+def test_attention_paged8_small_weights(ops, kind, n, new, heads, d):  # noqa: F811
+    """Weights that differ in their 13th bit and cancel; light ones beside a key of weight 1 that is 0 in half the columns:
+    between two steps of an f16 at 2^-20, all under 2^-28, and as light by the values' scales alone."""
+    block = 16
+    k, v, ke, ve, table = one_sequence8(ops, n, d, block)
+    pages, page = k.shape[:2]
+    k.zero_()
+    flat_k, flat_v = k.view(pages * page, d), v.view(pages * page, d)
+    q = torch.randn(new, heads, d, device="cuda", generator=gen(7)).bfloat16()
+    q[..., 0] = 1.0
+    one = torch.ones(d, device="cuda")
+    scale = 1.0
+    if kind == "cancel":
+        flat_k[1::2, 0] = (-one[:1]).to(E4)
+        flat_v[0::2], flat_v[1::2] = one.to(E4), (-one).to(E4)
+        scale = 2.0 ** -13
+    else:
+        flat_v.copy_(one.expand(pages * page, d).to(E4))
+        flat_v[0, :d // 2] = torch.zeros(d // 2, device="cuda").to(E4)
+        flat_k[0, 0] = (one[0] * {"steps": 14.0, "many": 20.0, "scales": 1.0}[kind]).to(E4)
+        if kind == "steps":
+            scale = math.log(2) * (24 - math.log2(10.5)) / 14  # the others weigh 10.5 * 2^-24
+        if kind == "scales":
+            scale = 0.3
+            ve[1:] = 127 - 25
+            flat_v[1:block] = torch.zeros(d, device="cuda").to(E4)
+    check_one_sequence8(ops, n, new, q, k, v, ke, ve, table, block, scale)
