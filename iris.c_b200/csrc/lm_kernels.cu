@@ -895,7 +895,7 @@ paged_attention_kernel(const __grid_constant__ IrisPagedAttention a) {
 #pragma unroll
             for (int i = 0; i < 2 * KS; i++) {
               float& y = x[i / 2][r][i % 2 * 2 + h];
-              y = y * (cq[e] * kx[i]) + vx[i];
+              y = (y * kx[i]) * cq[e] + vx[i];  // (cq kx may be past f32, where y is not)
               if (have != (0xffffffffu >> (32 - KEYS)) && !(have >> g & 1u << 8 * i)) y = -INFINITY;
               mn = fmaxf(mn, y);
             }
@@ -1285,7 +1285,7 @@ paged_runs_kernel(const __grid_constant__ IrisPagedAttention a) {
         for (int e = 0; e < 8; e++) {
           const int h = e / 2 % 2, key = e / 4 * 8 + 2 * i4 + e % 2;
           float& x = s[2 * n + e / 4][e % 4];
-          if constexpr (EIGHT) x = x * (cq[h] * (e % 2 ? kx[e / 4].y : kx[e / 4].x)) + (e % 2 ? vx[e / 4].y : vx[e / 4].x);
+          if constexpr (EIGHT) x = (x * (e % 2 ? kx[e / 4].y : kx[e / 4].x)) * cq[h] + (e % 2 ? vx[e / 4].y : vx[e / 4].x);
           else x *= c;
           if (!all && (n * 16 + key >= len[h] - first - k0 || !(have >> key & 1))) x = -INFINITY;
           mx[h] = fmaxf(mx[h], x);

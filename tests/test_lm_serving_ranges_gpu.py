@@ -84,3 +84,15 @@ def test_attention_paged8_small_weights(ops, kind, n, new, heads, d):  # noqa: F
             ve[1:] = 127 - 25
             flat_v[1:block] = torch.zeros(d, device="cuda").to(E4)
     check_one_sequence8(ops, n, new, q, k, v, ke, ve, table, block, scale)
+
+
+@pytest.mark.parametrize("d", (64, 128, 256))
+@pytest.mark.parametrize("n,new,heads", [(300, 1, 4), (200, 130, 16)])
+def test_attention_paged8_large_queries_on_columns_of_zeros(ops, n, new, heads, d):  # noqa: F811
+    """A query of 2^120 on a column in which keys of scale 2^33 are 0: scores of 0, all keys weigh alike."""
+    k, v, ke, ve, table = one_sequence8(ops, n, d, 16)
+    k.view(-1, d)[:, 0] = torch.zeros(1, device="cuda").to(E4)
+    ke.fill_(127 + 33)
+    q = torch.zeros(new, heads, d, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 2.0 ** 120
+    check_one_sequence8(ops, n, new, q, k, v, ke, ve, table, 16, 1 / math.sqrt(d))
