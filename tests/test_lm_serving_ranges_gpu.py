@@ -9,12 +9,15 @@ attention_paged8: 2^-8 of the value and, times A = sum p |v|: 4 hd u S for the s
   ln 2, and 2^-21 for the exponential (2^-22) and weights of 22 bits.  Weights under 2^-25 of the largest weight times scale W
   come in steps of 2^-39 of it (their second part is a multiple of 2^-24 where the largest is 2^15), rounded: 2^-40 448 W a
   key.
+Products with 4-bit weights and appends: as in test_lm_serving_gpu, whose checks they go through.
 """
+import ctypes
 import math
 
 import numpy as np
 import pytest
 
+import test_lm_serving_gpu as serving
 from test_lm_ops_gpu import BF, U, gen, i32, stream
 from test_lm_serving_gpu import E4, one_sequence8, ops, values8  # noqa: F401
 
@@ -96,3 +99,71 @@ def test_attention_paged8_large_queries_on_columns_of_zeros(ops, n, new, heads, 
     q = torch.zeros(new, heads, d, device="cuda", dtype=torch.bfloat16)
     q[..., 0] = 2.0 ** 120
     check_one_sequence8(ops, n, new, q, k, v, ke, ve, table, 16, 1 / math.sqrt(d))
+
+
+def kernels_of(call):
+    """Names of the kernels that a call launches, from the graph that it is captured into (and that is not run)."""
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    cu, raw, n = ctypes.CDLL("libcuda.so.1"), ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t()
+    assert cu.cuGraphGetNodes(raw, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert cu.cuGraphGetNodes(raw, nodes, ctypes.byref(n)) == 0
+    names = []
+    for node in nodes:
+        params, name = (ctypes.c_void_p * 32)(), ctypes.c_char_p()  # the first member is the function
+        assert cu.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(node), params) == 0
+        assert cu.cuFuncGetName(ctypes.byref(name), ctypes.c_void_p(params[0])) == 0
+        names.append(name.value.decode())
+    return names
+
+
+class Named:
+    """The binding, each call `what` of which has to launch one kernel with `kernel` in its mangled name."""
+
+    def __init__(self, ops, what, kernel):  # noqa: F811
+        self.ops, self.what, self.kernel = ops, what, kernel
+
+    def __getattr__(self, name):
+        call = getattr(self.ops, name)
+        if name != self.what:
+            return call
+
+        def checked(*args, **kw):
+            names = kernels_of(lambda: call(*args, **{**kw, "stream": stream()}))
+            assert len(names) == 1 and self.kernel in names[0], (names, self.kernel)
+            call(*args, **kw)
+        return checked
+
+
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+# Every kernel of the products: rows of x, then n of the weights by the number of SMs, so that each rule of the launch is met: many
+# rows of the weights; five and three parts of k in a cluster where one warp a strip lets more blocks be there at once; few.
+LINEAR_WAYS = {
+    "few": ("linear4_kernelILi1ELi8E", (1, 5, 8), lambda: 300, 1),
+    "few_head": ("linear4_kernelILi2ELi2E", (1, 3, 8), lambda: 512 * sms() + 1, 0),
+    "rows16_one": ("linear4_rows_kernelILi2ELi1E", (9, 12, 16), lambda: 128 * (sms() * 7 // 4 // 5) - 126, 1),
+    "rows16_one_3": ("linear4_rows_kernelILi2ELi1E", (16,), lambda: 128 * (sms() * 7 // 4 // 3) - 127, 1),
+    "rows16_head": ("linear4_rows_kernelILi2ELi1E", (10,), lambda: 512 * sms() + 77, 0),
+    "rows16_two": ("linear4_rows_kernelILi2ELi2E", (9, 13, 16), lambda: 250, 2),
+    "rows32_one": ("linear4_rows_kernelILi4ELi1E", (17, 31, 33), lambda: 128 * (sms() * 7 // 4 // 5) - 126, 1),
+    "rows32_one_3": ("linear4_rows_kernelILi4ELi1E", (32,), lambda: 128 * (sms() * 7 // 4 // 3) - 127, 1),
+    "rows32_head": ("linear4_rows_kernelILi4ELi1E", (32,), lambda: 512 * sms() + 77, 0),
+    "rows32_two": ("linear4_rows_kernelILi4ELi2E", (17, 32, 70), lambda: 250, 2),
+}
+
+
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("group", (32, 64, 384))
+@pytest.mark.parametrize("way", LINEAR_WAYS)
+def test_linear4_each_kernel(ops, way, group, zeros):  # noqa: F811
+    kernel, rows, n, deep = LINEAR_WAYS[way]
+    k = {32: (160, 1440, 4128), 64: (192, 1472, 4160), 384: (384, 1536, 4224)}[group][deep]
+    kernel += f"Li{ {32: 1, 64: 2, 384: 4}[group] }ELb{int(zeros)}E"
+    for i, r in enumerate(rows):
+        f32, add = (i + zeros) % 2 == 0, (None, "same", "other")[(i + group // 32) % 3]
+        serving.test_linear4(Named(ops, "linear4", kernel), (r, n(), k, group, zeros, i % 2 == 0, f32, add, 8 * (i % 2)))
