@@ -167,3 +167,25 @@ def test_linear4_each_kernel(ops, way, group, zeros):  # noqa: F811
     for i, r in enumerate(rows):
         f32, add = (i + zeros) % 2 == 0, (None, "same", "other")[(i + group // 32) % 3]
         serving.test_linear4(Named(ops, "linear4", kernel), (r, n(), k, group, zeros, i % 2 == 0, f32, add, 8 * (i % 2)))
+
+
+# rows beyond 8 an SM, then as test_lm_serving_gpu's: heads, kv heads, d, rot, interleaved, page, block, head major, f32, norm,
+# sequences, shuffled
+APPEND_MANY = [
+    (17, 4, 2, 128, 128, False, 16, 16, False, True, True, 3, False),
+    (1, 2, 1, 128, 128, True, 16, 16, True, False, True, 3, True),
+    (30, 1, 3, 128, 64, True, 20, 4, False, False, False, 4, True),
+    (5, 3, 1, 128, 128, False, 8, 1, True, False, True, 2, False),
+    (60, 0, 2, 128, 32, False, 64, 64, False, True, False, 3, True),
+    (9, 2, 2, 64, 64, False, 64, 32, False, False, True, 3, True),
+    (44, 7, 1, 64, 32, True, 48, 16, True, True, False, 5, False),
+    (21, 2, 1, 256, 256, False, 24, 24, False, False, True, 2, False),
+    (12, 1, 2, 256, 64, True, 7, 7, True, True, True, 3, True),
+]
+
+
+@pytest.mark.parametrize("case", APPEND_MANY, ids=lambda c: "-".join(map(str, c[:8])))
+def test_rope_append8_of_many_tokens(ops, case):  # noqa: F811
+    more, nh, nkv, d, f32 = *case[:4], case[9]
+    kernel = f"rope_append8_kernelI{'f' if f32 else '13__nv_bfloat16'}Li{d}ELb1E"
+    serving.test_rope_append8(Named(ops, "rope_append8", kernel), (8 * sms() + more, *case[1:]))
