@@ -19,9 +19,9 @@ namespace {
 // all of it is: where in the line does a count, or a sum, cross a number?
 //
 // The row is read once, by a cluster of blocks that hold it in shared memory.
-// With top-k of up to SMP_TOP, or where min-p leaves few, the tokens above a bound
-// (which k of the threads' own largest reach) are few: one block puts them in order
-// and has the answer.  Else a histogram over the distance from m, in parts of
+// With top-k of up to SMP_TOP, in shares of up to SMP_SHARE a block, the tokens above
+// a bound (which k of the threads' own largest reach) are few, and so they are where
+// min-p leaves few: one block puts them in order and has the answer.  Else a histogram over the distance from m, in parts of
 // SMP_SPAN / SMP_BINS of t, says to 2^-14 (large vocabularies: less closely) how the
 // sum grows along the line (each value adds its weight relative to its bin's, a whole
 // number of 16 bits, so that no order of additions shows); a pass over the row adds up exactly what
@@ -37,7 +37,9 @@ namespace {
 // in shared memory; 52 % of the issue slots) for many.
 constexpr int SMP_THREADS = 256, SMP_WARPS = SMP_THREADS / 32, SMP_PARTS = 8;
 constexpr int SMP_LIST = 1024;  // tokens put in order
-constexpr int SMP_TOP = 512;    // largest top-k whose tokens are looked for through a bound
+constexpr int SMP_TOP = 512;    // largest top-k whose tokens are looked for through a bound, and the largest share of a block in it:
+constexpr int SMP_SHARE = 200;  // some 390 tokens reach the 200th of 256 threads' largest, 1570 the last one, more than the lists hold
+                                // (512 bf16 rows of 32000, top-k 200 37 us, 256 120 through a bound and then without, 95 without)
 constexpr int SMP_BINS = 2048;
 constexpr float SMP_SPAN = 24.f;      // (m - x) / t that the bins cover; the last one holds all that is below
 constexpr int SMP_CUT = 16, SMP_CUTTERS = 64;  // bins of a closer look, threads that fill bins of their own
@@ -236,7 +238,9 @@ struct SmpRow {
     return __reduce_min_sync(0xffffffffu, tid % 32 < parts ? first_of_pairs[tid % 32 * 2] : 0xffffffffu);
   }
 
-  // ---- the row.  From each block its largest value (NaN if there is one), and with top_k = k of 1 to SMP_TOP a value that its
+  __device__ bool bounded(int k) const { return k > 0 && k <= min(SMP_TOP, SMP_SHARE * parts); }
+
+  // ---- the row.  From each block its largest value (NaN if there is one), and with top_k = k through a bound a value that its
   // share of k tokens reaches
   __device__ const uint2* load(int k) {
     float best = -INFINITY;
@@ -262,7 +266,7 @@ struct SmpRow {
     if (tid % 32 == 0) sh.iscan[tid / 32] = w;
     __syncthreads();
     const uint32_t most = __reduce_max_sync(0xffffffffu, sh.iscan[tid % SMP_WARPS]);
-    return tell(most, k > 0 && k <= SMP_TOP ? reached((k + parts - 1) / parts, own) : 0u);
+    return tell(most, bounded(k) ? reached((k + parts - 1) / parts, own) : 0u);
   }
 
   // a value that `share` of this block's tokens reach, 0 if it may have fewer; sh.iscan: the warps' largest
@@ -924,9 +928,9 @@ struct SmpRow {
     floor_ = -FLT_MAX;
     if (min_p >= 1.f) floor_ = m;
     else if (min_p > 0.f) floor_ = fmaxf(floor_, __double2float_ru(top + (double)t * log((double)min_p)));
-    if ((k && k <= SMP_TOP) || min_p > 0.f) {
+    if (bounded(k) || (k && k <= SMP_TOP && a.vocab <= SMP_LIST) || min_p > 0.f) {
       float from = floor_;
-      if (k && k <= SMP_TOP) {
+      if (bounded(k)) {
         const uint32_t least = least_of(&told->y);
         from = fmaxf(from, rank_value(max(least, rank_bits(-FLT_MAX))));
       }

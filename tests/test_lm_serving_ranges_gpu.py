@@ -189,3 +189,16 @@ def test_rope_append8_of_many_tokens(ops, case):  # noqa: F811
     more, nh, nkv, d, f32 = *case[:4], case[9]
     kernel = f"rope_append8_kernelI{'f' if f32 else '13__nv_bfloat16'}Li{d}ELb1E"
     serving.test_rope_append8(Named(ops, "rope_append8", kernel), (8 * sms() + more, *case[1:]))
+
+
+@pytest.mark.parametrize("rows,vocab,f32", [(3, 1024, True), (3, 1025, False), (500, 1500, False), (450, 16001, True), (200, 40001, False),
+                                            (40, 40000, True)])
+@pytest.mark.parametrize("steps", (0, 2))
+def test_sample_tokens_top_k_in_shares(ops, rows, vocab, f32, steps):  # noqa: F811
+    """Top-k around the largest share of a block, with one to eight blocks a row; with steps many tokens are equal."""
+    ks = (1, 128, 199, 200, 201, 255, 256, 257, 400, 401, 511, 512, 513)
+    x = torch.randn(rows, vocab, device="cuda", generator=gen(vocab)) * 2.5
+    if steps:
+        x = torch.round(x * steps) / steps
+    settings = [(1.0, ks[r % len(ks)], (1.0, 0.97)[r // len(ks) % 2], (0.0, 0.0, 1e-3)[r % 3]) for r in range(rows)]
+    serving.check_samples(ops, x if f32 else x.bfloat16(), settings, np.random.default_rng(rows).random(rows).tolist())
