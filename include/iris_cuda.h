@@ -843,7 +843,10 @@ typedef struct {
  * grows, the block's other slots are rounded to it.  Where the first slot is among
  * them, what the block held counts as dead: its other slots keep their bytes.  So
  * feed a sequence in order of its positions, in any number of calls; within a call
- * tokens stand in any order (those of a block side by side are found soonest).
+ * tokens stand in any order.  Two sequences whose tables share a page must not
+ * both have tokens for a block of it in one call.  Each block that is written looks
+ * for its tokens among all of the call's: beyond some ten thousand, several calls
+ * are faster.
  * Values that are not finite are held as NaN; magnitudes past 448 * 2^60 as that. */
 int iris_gpu_rope_append8(const iris_gpu_kv_cache8_t *cache, const iris_gpu_rope_t *rope, void *q_out, int64_t ldq_out,
                           const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int f32,
@@ -893,7 +896,8 @@ int iris_gpu_token_logprobs(const void *logits, int f32, int64_t ld, int rows, i
  *                 among its logits, or a temperature of NaN
  *   logprobs      (optional) log of its weight's share of what is kept; with -1 -inf
  *   kept          (optional) tokens kept; with -1 0
- * Weights and sums are 64-bit.  The same call gives the same bits every time. */
+ * Weights and sums are 64-bit, weights good to 2^-44.  The same call gives the same
+ * bits every time. */
 int iris_gpu_sample_tokens(const void *logits, int f32, int64_t ld, int rows, int vocab, const float *temperature,
                            const int32_t *top_k, const float *top_p, const float *min_p, const double *uniform,
                            int32_t *ids, float *logprobs, int32_t *kept, void *stream);

@@ -11,8 +11,9 @@ namespace {
 
 // ------------------------------------------------------------------ products
 //   y[r][n] = sum over groups g of  s[n][g] sum over k in g of (q[n][k] - z[n][g]) x[r][k]   (+ add[r][n])
-// Should be bound by the weights' bytes; the pipe of shifts and logic that unpacks them is (below).  151936 x 2560 in groups of 32,
-// one row: 65 us, 34 for the bytes; 6144 x 2560 in groups of 128: 5.5 us, of which 1.3.  The products are mma m16n8k16 with 16 rows of the
+// Should be bound by the weights' bytes; instructions are.  151936 x 2560 in groups of 32,
+// one row: 65 us, 34 for the bytes, 27 instructions for a word of eight weights, 65 % of the issue slots, the pipe of shifts and logic
+// 58 % active; 6144 x 2560 in groups of 128: 5.5 us, of which 1.3 for the bytes (one round, latency).  The products are mma m16n8k16 with 16 rows of the
 // weights as m and 8 rows of x as n.  q - z is a whole number of at most 8 bits,
 // exact in bf16, and so is x; the scale multiplies a group's f32 sum.
 // A 32-bit word holds eight columns k .. k + 7 of a row; its halves' nibble j give
@@ -38,7 +39,7 @@ struct Constants4 {
     asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
   }
 };
-// Pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's nibbles, less the zero (128 + z twice).  What bounds the kernel is the pipe of
+// Pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's nibbles, less the zero (128 + z twice).  The busiest pipe is that of
 // shifts and logic: mask and magic are in registers, so that one instruction does both (constants would take two: the head's
 // 151936 x 2560 74 us, 66 so; the shifts as high halves of products, on another pipe, 79).
 __device__ __forceinline__ void nibbles(uint32_t w, uint32_t zero, const Constants4& k, uint32_t p[4]) {

@@ -144,6 +144,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(const __grid_
 // registers, and goes over the mates twice, for the largest magnitude and, behind the
 // scale, for the values, from the registers where all fit.  Other blocks of the same
 // launch do the queries, 64 threads a token as above.
+// The search goes with the product of the call's tokens and the cache's blocks that
+// they fill.  bf16, 32 + 8 + 8 heads of 128, blocks of 16, beside rope_append: a prompt
+// of 8192 63 us (36), of 32768 320 (138), of 131072 2500 (542); single tokens of 1024
+// sequences 37 (7.5), of 8192 240 (37).
 constexpr int APPEND8_THREADS = 256, APPEND8_WARPS = APPEND8_THREADS / 32;
 constexpr int APPEND8_TOKENS = 8;  // that a block goes through where there are many
 
@@ -188,7 +192,8 @@ struct Append8Plan {
 };
 
 // MANY: tokens.  Half as many mates in registers and twice the blocks on an SM: 8191 tokens of 32 + 8 + 8 heads of 128, f32, 94 us
-// -> 75; 64 tokens 6.4 -> 8.3.
+// -> 75; 64 tokens 6.4 -> 8.3.  At 128 columns a block of 16 tokens is more than the 8 held then, so that its rows are read, and
+// their angles worked out, twice; and f32 at 64 registers spills (some 310 bytes of stores and 450 of loads a thread).
 template <typename In, int HD, bool MANY>
 __global__ void __launch_bounds__(APPEND8_THREADS, MANY ? 4 : 2) rope_append8_kernel(const __grid_constant__ IrisRopeAppend a,
                                                                           const __grid_constant__ Append8Plan plan) {
@@ -490,8 +495,8 @@ __device__ __forceinline__ uint32_t nan4(uint32_t x) { return __vcmpeq4(x & 0x7F
 template <typename E, int HD, int MH>
 struct PagedShape {
   // Keys of a tile that a warp takes.  Over 8 bits 32 have half the steps' shuffles, page numbers and scales (64 rows of 1 to
-  // 8192 keys, 32 heads on 8 of 128: 357 instructions for 16 keys instead of 500, 100.3 us instead of 102.6; of few rows, one
-  // of 512 keys 6.5 us either way, 8 of 512 9.2 and 10.1, one of 2048 10.5 and 10.3).
+  // 8192 keys, 32 heads on 8 of 128: 100.3 us instead of 102.6; of few rows, one of 512 keys 6.5 us either way, 8 of 512 9.2
+  // and 10.1, one of 2048 10.5 and 10.3; 319 instructions for 16 keys and 4 heads).
   static constexpr int kKeys = kEight<E> ? 32 : 16;
   static constexpr int kGroups = IRIS_PAGED_TILE / kKeys;        // of them
   static constexpr int kPair = HD / 128 ? HD / 128 : 1;          // warps on the same keys, 128 columns of o each

@@ -33,8 +33,8 @@ namespace {
 // ends, and with 32 bits one row in a hundred would take its neighbour.
 // Rows of 151936 f32: one with the usual settings 9.3 us, greedy 4.5, top-p alone 30;
 // 512 with the usual settings 167 us, top-p alone 595 (bf16 381), of which 49 for the
-// bytes: barriers of the cluster for few rows, instructions (64-bit weights, additions
-// in shared memory; 52 % of the issue slots) for many.
+// bytes: barriers of the cluster for few rows; for many, latency: 16 warps an SM (registers)
+// with 64-bit weights and additions in shared memory, 41 % of the issue slots.
 constexpr int SMP_THREADS = 256, SMP_WARPS = SMP_THREADS / 32, SMP_PARTS = 8;
 constexpr int SMP_LIST = 1024;  // tokens put in order
 constexpr int SMP_TOP = 512;    // largest top-k whose tokens are looked for through a bound, and the largest share of a block in it:
