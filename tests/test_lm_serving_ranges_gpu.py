@@ -202,3 +202,27 @@ def test_sample_tokens_top_k_in_shares(ops, rows, vocab, f32, steps):  # noqa: F
         x = torch.round(x * steps) / steps
     settings = [(1.0, ks[r % len(ks)], (1.0, 0.97)[r // len(ks) % 2], (0.0, 0.0, 1e-3)[r % 3]) for r in range(rows)]
     serving.check_samples(ops, x if f32 else x.bfloat16(), settings, np.random.default_rng(rows).random(rows).tolist())
+
+
+@pytest.mark.parametrize("d", (64, 128, 256))
+@pytest.mark.parametrize("new,heads", [(1, 4), (80, 4), (80, 16)])
+def test_attention_paged8_pages_outside_the_pool(ops, new, heads, d):  # noqa: F811
+    """Pages that the pool does not have, in the middle of a sequence and at its ends: their keys are not seen."""
+    n, block = 300, 8
+    k, v, ke, ve, table = one_sequence8(ops, n, d, block)
+    pages, page = k.shape[:2]
+    table[0, 0], table[0, 3], table[0, 9], table[0, 18] = -1, pages, 2 ** 31 - 1, -2 ** 31
+    q = torch.randn(new, heads, d, device="cuda", generator=gen(3)).bfloat16()
+    out = torch.zeros_like(q)
+    cache = ops.KvCache8.of(k, v, ke, ve, table)
+    ws = torch.empty(ops.attention_paged8_workspace(cache, heads), device="cuda", dtype=torch.uint8)
+    scale = 2.0 ** -4
+    ops.attention_paged8(cache, out, q, i32([0] * new), i32(range(n - new, n)), scale=scale, workspace=ws, stream=stream())
+    torch.cuda.synchronize()
+    kv, vv = (values8(p, e, block).flatten(0, 2) for p, e in ((k, ke), (v, ve)))
+    held = ((table[0] >= 0) & (table[0] < pages)).cpu().repeat_interleave(page)
+    for r in range(new):
+        seen = held.clone()
+        seen[n - new + r + 1:] = False
+        want, tol = attention8_fine64(q[r], kv[seen], vv[seen], torch.ones(int(seen.sum()), dtype=torch.float64), scale)
+        assert ((out[r].double().cpu() - want).abs() <= tol).all(), r
